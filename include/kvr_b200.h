@@ -428,6 +428,85 @@ KVR_API int kvr_peer_merge_candidates(void *const *bufs, int n_ranks, int rank, 
 KVR_API int kvr_peer_lse_merge(void *const *bufs, int n_ranks, int rank, const float *partials, int n_rows, int d,
                                void *out, int out_dtype, kvr_stream_t stream);
 
+/* ------------------------------------------------- paged exact cache ----
+ * Serving of many requests of different lengths (no reference counterpart:
+ * the reference serves one sequence).  A layer's cache is a pool of pages,
+ * K and V (n_pages, page, n_kv, d) of fp16 or bf16 with explicit strides in
+ * elements (heads of a token contiguous; rows 16-byte aligned); request b's
+ * token p lies in page block_table[b, p / page], row p % page.  A step
+ * appends the new tokens of all requests, packed in request order: those of
+ * request b are [cu_q[b], cu_q[b+1]).  Lengths, offsets and tables are int32
+ * on the device, so no call reads them on the host and a step can be captured.
+ * d = 128; at most 128 query heads per KV head, 4096 requests, 2^24 tokens. */
+
+/* The attention plan: the work list kvr_paged_attn and kvr_prompt_attn run,
+ * built on the device from the lengths; one plan serves every layer of a
+ * step.  Queries of request b are cu_q[b] .. cu_q[b+1] (tokens past
+ * cu_q[batch] up to n_tokens are padding: output rows 0).  Keys: kv_len[b]
+ * keys in pages; or packed keys cu_k[b] .. cu_k[b+1]; or, with both NULL,
+ * the queries' own tokens.  The queries are the LAST tokens of their request:
+ * with `causal` query i of q_len sees keys j <= kv_len - q_len + i, and with
+ * window > 0 only the last `window` of those.  A query that sees no key gets
+ * output 0 and log-sum-exp -inf. */
+KVR_API size_t kvr_attn_plan_bytes(int64_t n_tokens, int batch, int n_q, int n_kv);
+KVR_API int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const int32_t *cu_k, int batch,
+                          int64_t n_tokens, int n_q, int n_kv, int causal, int64_t window, void *plan,
+                          size_t plan_bytes, kvr_stream_t stream);
+
+/* Block tables and slot maps of a step: request b has ctx_len[b] tokens in
+ * the cache and gets new_len[b] more; pages come off the end of the free list
+ * in request order (the k-th fresh page of the step is
+ * free_pages[*n_free - 1 - k]) and are entered into block_table (batch,
+ * table_width; row stride table_stride) behind the ceil(ctx/page) pages that
+ * the request holds.  Writes cu_q (batch + 1), kv_len (batch) = ctx + new,
+ * positions (n_tokens), slots (n_tokens) = page id * page + row, the free
+ * count left, and info (4): pages missing, requests whose new tokens did not
+ * fit n_tokens (the last ones are cut), requests longer than their table row,
+ * 0.  Tokens without a page and padding tokens get slot -1; a missing page's
+ * table entry is -1.  ctx_len, new_len and n_free are not changed, so
+ * repeating a call repeats its result.  With `plan`, the causal attention
+ * plan of the step (n_q, n_kv, window as kvr_attn_plan) is built in the same
+ * launch. */
+KVR_API int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int batch, int64_t n_tokens, int page,
+                          int32_t *block_table, int64_t table_stride, int table_width, const int32_t *free_pages,
+                          int64_t n_free_cap, const int32_t *n_free, int32_t *cu_q, int32_t *kv_len,
+                          int32_t *positions, int64_t *slots, int32_t *n_free_out, int32_t *info, int n_q, int n_kv,
+                          int64_t window, void *plan, size_t plan_bytes, kvr_stream_t stream);
+
+/* RoPE (rotate_half, fp32, rounded once) of q and k at positions[t], and the
+ * write of k and v into cache slot slots[t] of the pool.  q (n_tokens, n_q, d),
+ * k and v (n_tokens, n_kv, d) with token strides in elements; tables (max_pos,
+ * d) fp32, NULL: no rotation; q and q_out (contiguous) may both be NULL.
+ * A token whose slot is outside the pool (or position outside the tables)
+ * writes nothing to the cache and its q_out rows are 0. */
+KVR_API int kvr_paged_write(const void *q, const void *k, const void *v, int dtype, int64_t n_tokens, int n_q,
+                            int n_kv, int d, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                            const float *cos_tbl, const float *sin_tbl, int64_t rope_stride, int64_t max_pos,
+                            const int32_t *positions, const int64_t *slots, void *q_out, void *k_pages,
+                            void *v_pages, int64_t n_pages, int page, int64_t page_stride, int64_t tok_stride,
+                            kvr_stream_t stream);
+
+/* Attention of a step's query tokens over their requests' pages (a plan with
+ * kv_len) or over packed prompts (a plan without, or with cu_k): q (n_tokens,
+ * n_q, d) with token stride q_stride, out (n_tokens, n_q, d) contiguous of the
+ * same type, lse (n_tokens, n_q) fp32 natural log or NULL.  scale <= 0 means
+ * sqrt(d) (scores are divided by it).  The page size must be a multiple of 8.
+ * Missing pages (entries outside [0, n_pages)) read as zeros.  Keys beyond a
+ * request's length never reach its output, whatever the pool holds there.
+ * The workspace (kvr_attn_workspace_bytes) must not be shared by calls that
+ * overlap; its error word (kvr_workspace_status) reports a bounded wait that
+ * gave up, or a plan that was not built for this call's shapes. */
+KVR_API size_t kvr_attn_workspace_bytes(int n_q, int n_kv);
+KVR_API int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int batch, int n_q, int n_kv, int d,
+                           int64_t q_stride, const void *k_pages, const void *v_pages, int64_t n_pages, int page,
+                           int64_t page_stride, int64_t tok_stride, const int32_t *block_table,
+                           int64_t table_stride, int table_width, const void *plan, size_t plan_bytes, float scale,
+                           void *out, float *lse, void *workspace, size_t workspace_bytes, kvr_stream_t stream);
+KVR_API int kvr_prompt_attn(const void *q, const void *k, const void *v, int dtype, int64_t n_tokens,
+                            int64_t n_keys, int batch, int n_q, int n_kv, int d, int64_t q_stride, int64_t k_stride,
+                            int64_t v_stride, const void *plan, size_t plan_bytes, float scale, void *out,
+                            float *lse, void *workspace, size_t workspace_bytes, kvr_stream_t stream);
+
 /* Allocation-free variant of kvr_decode_attn (no counterpart in the
  * reference).  For callers that cannot allocate device memory — a plugin
  * inside a host that owns the GPU heap, or a path where cudaMalloc would
@@ -452,7 +531,8 @@ KVR_API int kvr_decode_attn_noalloc(const void *q, int q_dtype, int n_q, int n_k
 
 /* Synchronises `stream`, then reads and clears the error word every workspace
  * starts with: KVR_ETIMEOUT if a bounded device-side wait of an earlier call
- * using this workspace gave up, else KVR_OK. */
+ * using this workspace gave up, KVR_EINVAL if an attention call met a plan of
+ * other shapes, else KVR_OK. */
 KVR_API int kvr_workspace_status(const void *workspace, kvr_stream_t stream);
 
 /* Test of the failure path above (no reference counterpart): one kernel

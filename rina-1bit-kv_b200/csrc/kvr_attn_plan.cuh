@@ -1,0 +1,63 @@
+// The work list of an attention call over requests of different lengths
+// (kvr_paged_attn, kvr_prompt_attn), built on the device from the lengths.
+//
+// The query rows of a request and KV head are its (token, head of the group)
+// pairs, row = token * g + j, g = n_q / n_kv.  An item is the rows of up to
+// 2 * tpt consecutive tokens, tpt = floor(128 / g): two 128-row tiles that
+// share every K/V tile of 128 keys they read.  A piece is a range of an
+// item's K/V tiles; the list holds the pieces of ONE head, longest first, and
+// serves every KV head: entry p stands for pieces p * n_kv + h.
+#pragma once
+
+#include "kvr_common.cuh"
+
+namespace kvr {
+
+constexpr int kPlanMagic = 0x4b565031;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxBatch = 4096;
+constexpr int kPlanMaxTokens = 1 << 24;  // query tokens of a call
+constexpr int kPlanMaxLen = 1 << 29;     // keys of a request: leaves room for sums in 32 bits
+constexpr int kD = 128;          // head_dim
+constexpr int kPlanRows = 128;   // rows of a query tile
+constexpr int kPlanKeys = 128;   // keys of a K/V tile
+constexpr int kPlanCtas = 148;   // SMs the work is spread over
+
+struct PlanHeader {  // 64 words
+  int magic, n_tokens, batch, n_q, n_kv, causal, window;
+  int n_pieces;      // per head
+  int dropped;       // 1: items did not fit the list (offsets that overlap)
+  int pad[55];
+};
+
+struct PlanPiece {   // 8 words
+  int q_start;       // first token of the item, in the packed batch
+  int n_tok;         // its tokens
+  int first_end;     // keys its first token may see: kv_len - q_len + offset + 1 (causal), can be <= 0
+  int kv_len;        // keys of the request
+  int k_start;       // first key of the request in packed K/V (prompt), or the request's index (pages)
+  int kt0, kt1;      // K/V tiles [kt0, kt1) of the piece
+  int part;          // row base of its partial results, -1: the piece is the whole item
+};
+static_assert(sizeof(PlanPiece) == 32, "piece record");
+
+__host__ __device__ inline int plan_tpt(int n_q, int n_kv) { return kPlanRows / (n_q / n_kv); }
+__host__ __device__ inline int64_t plan_max_items(int64_t n_tokens, int batch, int n_q, int n_kv) {
+  return n_tokens / (2 * plan_tpt(n_q, n_kv)) + batch + 2;
+}
+
+struct PlanArgs {
+  const int *cu_q;    // (batch + 1)
+  const int *kv_len;  // (batch) or NULL
+  const int *cu_k;    // (batch + 1) or NULL; both NULL: the keys are the queries' tokens
+  int batch, n_tokens, n_q, n_kv, causal, window;
+  PlanHeader *hdr;
+  PlanPiece *pieces;
+  int max_items;
+};
+
+// Checks of the arguments every plan-building entry point shares; fills the
+// pointers into the plan buffer.  Returns a status.
+int plan_check(const char *fn, PlanArgs &a, int64_t n_tokens, int64_t window, void *plan, size_t plan_bytes);
+
+}  // namespace kvr

@@ -1,0 +1,373 @@
+// Block tables, slot maps and attention plans from request lengths.
+//
+// A serving step appends new_len[b] tokens to request b, which has ctx_len[b]
+// in the cache.  With pages of P tokens the request holds ceil(ctx/P) pages
+// and needs ceil((ctx+new)/P); the fresh ones come off the end of the free
+// list in request order, so page k of the step (exclusive sum of the needs
+// plus its index) is free[n_free - 1 - k] and no page needs an atomic.  Token
+// i lies at position p = ctx + i - cu[b] and in slot table[b][p/P] * P + p%P.
+//
+// One launch does all of it.  Every CTA forms the two prefix sums (tokens,
+// fresh pages) of all requests in shared memory by itself: two words per
+// request from L2 are cheaper than a second kernel that waits for a first.
+// CTA 0 then writes the per-request outputs and the attention plan, the others
+// take the tokens and fresh pages.  Tokens in fresh pages read the free list,
+// not the table that other CTAs are filling.  The work is a few hundred bytes
+// to a few MB: launch and dependent-load latency bound it.
+#include "kvr_attn_plan.cuh"
+
+namespace kvr {
+
+// Exclusive sum over the CTA of one value per thread; `total` is the sum.
+__device__ __forceinline__ int64_t block_exclusive(int64_t v, int64_t *warp_sums, int64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t s = lane < nw ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  total = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+// Largest i in [0, n) with a[i] <= x (a ascending, a[0] <= x).
+__device__ __forceinline__ int last_not_above(const int *a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// One request as the plan sees it; b == batch stands for the tokens past the
+// last request (padding: no keys, their rows come out as zeros).
+struct PlanRequest {
+  int q0, q_len, kv_len, k_start;
+};
+__device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, int b) {
+  PlanRequest r;
+  const int lo = min(max(a.cu_q[b], 0), a.n_tokens);
+  const int hi = b < a.batch ? min(max(a.cu_q[b + 1], lo), a.n_tokens) : a.n_tokens;
+  r.q0 = lo;
+  r.q_len = hi - lo;
+  if (b == a.batch) {
+    r.kv_len = 0;
+    r.k_start = 0;
+  } else if (a.kv_len) {
+    r.kv_len = min(max(a.kv_len[b], 0), 2 * kPlanMaxLen);
+    r.k_start = b;
+  } else if (a.cu_k) {
+    r.k_start = max(a.cu_k[b], 0);
+    r.kv_len = max(a.cu_k[b + 1] - r.k_start, 0);
+  } else {
+    r.k_start = lo;
+    r.kv_len = r.q_len;
+  }
+  return r;
+}
+
+// Item i of request r: its piece record over all the K/V tiles it needs.
+__device__ __forceinline__ PlanPiece plan_item(const PlanArgs &a, const PlanRequest &r, int i) {
+  const int per = 2 * plan_tpt(a.n_q, a.n_kv);
+  PlanPiece p;
+  p.q_start = r.q0 + i * per;
+  p.n_tok = min(per, r.q_len - i * per);
+  p.kv_len = r.kv_len;
+  p.k_start = r.k_start;
+  p.part = -1;
+  p.first_end = a.causal ? r.kv_len - r.q_len + i * per + 1 : r.kv_len;
+  const int64_t end = a.causal ? min((int64_t)r.kv_len, (int64_t)p.first_end + p.n_tok - 1) : r.kv_len;
+  const int64_t begin = a.window > 0 ? max((int64_t)0, (int64_t)p.first_end - a.window) : 0;
+  p.kt0 = (int)(begin / kPlanKeys);
+  p.kt1 = end > begin ? (int)((end + kPlanKeys - 1) / kPlanKeys) : p.kt0;
+  return p;
+}
+
+constexpr int kPlanBins = 1024;
+
+struct PlanShared {
+  int first[kPlanMaxBatch + 2];  // exclusive sum of the requests' items
+  int hist[kPlanBins];
+  int64_t warp_sums[32];
+  int longest;
+};
+
+__device__ void plan_build(const PlanArgs &a, PlanShared &s) {
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const int per = 2 * plan_tpt(a.n_q, a.n_kv);
+  const int nb = a.batch + 1;
+  // requests -> first item of each (a contiguous run of requests per thread)
+  const int each = (nb + nt - 1) / nt;
+  int64_t sum = 0, total;  // 64 bits: offsets that overlap can add up to more than 2^31 items
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < nb) sum += (plan_request(a, b).q_len + per - 1) / per;
+  }
+  int64_t at = block_exclusive(sum, s.warp_sums, total);
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < nb) {
+      s.first[b] = (int)min(at, (int64_t)INT_MAX);
+      at += (plan_request(a, b).q_len + per - 1) / per;
+    }
+  }
+  const int n = (int)min(total, (int64_t)a.max_items);
+  const int dropped = total > n ? 1 : 0;
+  for (int i = tid; i < kPlanBins; i += nt) s.hist[i] = 0;
+  if (tid == 0) s.longest = 0;
+  __syncthreads();
+  // longest first: counting sort by length, `shift` keeps the lengths inside the bins
+  for (int i = tid; i < n; i += nt) {
+    const int b = last_not_above(s.first, nb, i);
+    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+    atomicMax(&s.longest, p.kt1 - p.kt0);
+  }
+  __syncthreads();
+  int shift = 0;
+  while ((s.longest >> shift) >= kPlanBins) ++shift;
+  for (int i = tid; i < n; i += nt) {
+    const int b = last_not_above(s.first, nb, i);
+    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+    atomicAdd(&s.hist[kPlanBins - 1 - ((p.kt1 - p.kt0) >> shift)], 1);
+  }
+  __syncthreads();
+  const int start = (int)block_exclusive(s.hist[tid], s.warp_sums, total);
+  s.hist[tid] = start;
+  __syncthreads();
+  for (int i = tid; i < n; i += nt) {
+    const int b = last_not_above(s.first, nb, i);
+    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+    a.pieces[atomicAdd(&s.hist[kPlanBins - 1 - ((p.kt1 - p.kt0) >> shift)], 1)] = p;
+  }
+  if (tid == 0) {
+    PlanHeader &h = *a.hdr;
+    h.magic = kPlanMagic;
+    h.n_tokens = a.n_tokens;
+    h.batch = a.batch;
+    h.n_q = a.n_q;
+    h.n_kv = a.n_kv;
+    h.causal = a.causal;
+    h.window = a.window;
+    h.n_pieces = n;
+    h.dropped = dropped;
+  }
+}
+static_assert(kPlanBins == kPlanThreads, "one bin per thread in the scan");
+
+__global__ void __launch_bounds__(kPlanThreads, 1) attn_plan_kernel(PlanArgs a) {
+  __shared__ PlanShared s;
+  plan_build(a, s);
+}
+
+struct MapArgs {
+  const int *ctx_len, *new_len;
+  int batch, n_tokens, page;
+  int *table;
+  int64_t table_stride;
+  int table_width;
+  const int *free_pages, *n_free;
+  int n_free_cap;  // entries of free_pages
+  int *cu, *kv_len, *positions;
+  int64_t *slots;
+  int *n_free_out, *info;
+  PlanArgs plan;
+  int with_plan;
+};
+
+// Cached tokens of request b (a length that no cache can have counts as its bound).
+__device__ __forceinline__ int map_ctx(const MapArgs &a, int b) { return min(max(a.ctx_len[b], 0), kPlanMaxLen); }
+
+__global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
+  __shared__ int cu[kPlanMaxBatch + 1];
+  __shared__ union {
+    int fresh[kPlanMaxBatch + 1];  // exclusive sum of the fresh pages
+    PlanShared plan;
+  } s;
+  __shared__ int64_t warp_sums[32];
+  __shared__ int n_cut, n_over;
+  int *fresh = s.fresh;
+  const int tid = threadIdx.x, nt = blockDim.x, P = a.page;
+  if (tid == 0) n_cut = n_over = 0;
+  const int each = (a.batch + nt - 1) / nt;
+  // tokens first: requests are cut where the step's n_tokens end
+  int64_t sum = 0, total;
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < a.batch) sum += max(a.new_len[b], 0);
+  }
+  int64_t at = block_exclusive(sum, warp_sums, total);
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < a.batch) {
+      cu[b] = (int)min(at, (int64_t)a.n_tokens);
+      at += max(a.new_len[b], 0);
+    }
+  }
+  if (tid == 0) cu[a.batch] = (int)min(total, (int64_t)a.n_tokens);
+  __syncthreads();
+  sum = 0;
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < a.batch) {
+      const int ctx = map_ctx(a, b), kv = ctx + cu[b + 1] - cu[b];
+      sum += (kv + P - 1) / P - (ctx + P - 1) / P;
+    }
+  }
+  at = block_exclusive(sum, warp_sums, total);
+  const int need = (int)total;
+  for (int k = 0; k < each; ++k) {
+    const int b = tid * each + k;
+    if (b < a.batch) {
+      const int ctx = map_ctx(a, b), kv = ctx + cu[b + 1] - cu[b];
+      fresh[b] = (int)at;
+      at += (kv + P - 1) / P - (ctx + P - 1) / P;
+    }
+  }
+  if (tid == 0) fresh[a.batch] = need;
+  __syncthreads();
+  const int n_free = min(max(*a.n_free, 0), a.n_free_cap);
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < a.batch; b += nt) {
+      const int ctx = map_ctx(a, b), now = cu[b + 1] - cu[b];
+      a.cu[b] = cu[b];
+      a.kv_len[b] = ctx + now;
+      if (max(a.new_len[b], 0) > now) atomicAdd(&n_cut, 1);
+      if ((ctx + now + P - 1) / P > a.table_width) atomicAdd(&n_over, 1);
+    }
+    __syncthreads();  // cu and kv_len are in place for the plan as well
+    if (tid == 0) {
+      a.cu[a.batch] = cu[a.batch];
+      *a.n_free_out = max(n_free - need, 0);
+      a.info[0] = max(need - n_free, 0);
+      a.info[1] = n_cut;
+      a.info[2] = n_over;
+      a.info[3] = 0;
+    }
+    __syncthreads();
+    if (a.with_plan) plan_build(a.plan, s.plan);
+    return;
+  }
+  const int64_t step = (int64_t)(gridDim.x - 1) * nt, me = (int64_t)(blockIdx.x - 1) * nt + tid;
+  for (int64_t i = me; i < a.n_tokens; i += step) {
+    int pos = 0;
+    int64_t slot = -1;
+    if (i < cu[a.batch]) {
+      // the last request that starts at or before token i and is not empty owns it
+      const int b = last_not_above(cu, a.batch, (int)i);
+      const int ctx = map_ctx(a, b), had = (ctx + P - 1) / P;
+      pos = ctx + (int)i - cu[b];
+      const int j = pos / P;
+      if (j < a.table_width) {
+        int page = -1;
+        if (j < had) {
+          page = a.table[b * a.table_stride + j];
+        } else {
+          const int k = fresh[b] + j - had;
+          if (k < n_free) page = a.free_pages[n_free - 1 - k];
+        }
+        if (page >= 0) slot = (int64_t)page * P + pos % P;
+      }
+    }
+    a.positions[i] = pos;
+    a.slots[i] = slot;
+  }
+  for (int64_t k = me; k < need; k += step) {
+    const int b = last_not_above(fresh, a.batch, (int)k);
+    const int ctx = map_ctx(a, b);
+    const int j = (ctx + P - 1) / P + (int)k - fresh[b];
+    if (j < a.table_width) a.table[b * a.table_stride + j] = k < n_free ? a.free_pages[n_free - 1 - k] : -1;
+  }
+}
+
+int plan_check(const char *fn, PlanArgs &a, int64_t n_tokens, int64_t window, void *plan, size_t plan_bytes) {
+  KVR_REQUIRE(a.batch >= 1 && a.batch <= kPlanMaxBatch, "%s: batch must be in [1, %d]", fn, kPlanMaxBatch);
+  KVR_REQUIRE(n_tokens >= 0 && n_tokens <= kPlanMaxTokens, "%s: bad token count", fn);
+  KVR_REQUIRE(a.n_kv > 0 && a.n_q > 0 && a.n_q % a.n_kv == 0, "%s: n_q must be a multiple of n_kv", fn);
+  if (a.n_q / a.n_kv > kPlanRows)
+    return set_error(KVR_ENOTSUP, "%s: more than %d query heads per KV head", fn, kPlanRows);
+  KVR_REQUIRE(window >= 0, "%s: window must be >= 0 (0: none)", fn);
+  KVR_REQUIRE(a.causal || window == 0, "%s: a window needs causal", fn);
+  KVR_REQUIRE(plan && (reinterpret_cast<uintptr_t>(plan) & 15) == 0, "%s: plan must be 16-byte aligned", fn);
+  const size_t want = kvr_attn_plan_bytes(n_tokens, a.batch, a.n_q, a.n_kv);
+  KVR_REQUIRE(plan_bytes >= want, "%s: plan %zu < %zu bytes", fn, plan_bytes, want);
+  a.n_tokens = (int)n_tokens;
+  a.window = (int)(window > INT_MAX / 2 ? 0 : window);
+  a.hdr = reinterpret_cast<PlanHeader *>(plan);
+  a.pieces = reinterpret_cast<PlanPiece *>(a.hdr + 1);
+  a.max_items = (int)plan_max_items(n_tokens, a.batch, a.n_q, a.n_kv);
+  return KVR_OK;
+}
+
+}  // namespace kvr
+
+using namespace kvr;
+
+extern "C" size_t kvr_attn_plan_bytes(int64_t n_tokens, int batch, int n_q, int n_kv) {
+  if (n_tokens < 0 || batch < 1 || n_kv < 1 || n_q < n_kv || n_q / n_kv > kPlanRows) return 0;
+  return sizeof(PlanHeader) + (size_t)plan_max_items(n_tokens, batch, n_q, n_kv) * sizeof(PlanPiece);
+}
+
+extern "C" int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const int32_t *cu_k, int batch,
+                             int64_t n_tokens, int n_q, int n_kv, int causal, int64_t window, void *plan,
+                             size_t plan_bytes, kvr_stream_t stream) {
+  clear_error();
+  KVR_REQUIRE(cu_q, "kvr_attn_plan: null pointer");
+  KVR_REQUIRE(!(kv_len && cu_k), "kvr_attn_plan: give kv_len (pages) or cu_k (packed keys), not both");
+  PlanArgs a{cu_q, kv_len, cu_k, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, 0};
+  const int rc = plan_check("kvr_attn_plan", a, n_tokens, window, plan, plan_bytes);
+  if (rc) return rc;
+  attn_plan_kernel<<<1, kPlanThreads, 0, as_cuda(stream)>>>(a);
+  return check_launch("kvr_attn_plan");
+}
+
+extern "C" int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int batch, int64_t n_tokens, int page,
+                             int32_t *block_table, int64_t table_stride, int table_width, const int32_t *free_pages,
+                             int64_t n_free_cap, const int32_t *n_free, int32_t *cu_q, int32_t *kv_len,
+                             int32_t *positions, int64_t *slots, int32_t *n_free_out, int32_t *info, int n_q, int n_kv,
+                             int64_t window, void *plan, size_t plan_bytes, kvr_stream_t stream) {
+  clear_error();
+  KVR_REQUIRE(ctx_len && new_len && block_table && n_free && cu_q && kv_len && n_free_out && info,
+              "kvr_paged_map: null pointer");
+  KVR_REQUIRE(n_tokens == 0 || (positions && slots), "kvr_paged_map: null pointer");
+  KVR_REQUIRE(n_free_cap >= 0 && n_free_cap <= INT_MAX / 2 && (n_free_cap == 0 || free_pages),
+              "kvr_paged_map: bad free list");
+  KVR_REQUIRE(batch >= 1 && batch <= kPlanMaxBatch, "kvr_paged_map: batch must be in [1, %d]", kPlanMaxBatch);
+  KVR_REQUIRE(n_tokens >= 0 && n_tokens <= kPlanMaxTokens, "kvr_paged_map: bad token count");
+  KVR_REQUIRE(page >= 1 && page <= (1 << 20), "kvr_paged_map: bad page size");
+  KVR_REQUIRE(table_width >= 1 && table_stride >= table_width, "kvr_paged_map: bad block table shape");
+  KVR_REQUIRE(n_free != n_free_out, "kvr_paged_map: n_free_out must not be n_free");
+  MapArgs m{};
+  if (plan) {
+    m.plan = PlanArgs{cu_q, kv_len, nullptr, batch, 0, n_q, n_kv, 1, 0, nullptr, nullptr, 0};
+    const int rc = plan_check("kvr_paged_map", m.plan, n_tokens, window, plan, plan_bytes);
+    if (rc) return rc;
+    m.with_plan = 1;
+  }
+  m.ctx_len = ctx_len; m.new_len = new_len;
+  m.batch = batch; m.n_tokens = (int)n_tokens; m.page = page;
+  m.table = block_table; m.table_stride = table_stride; m.table_width = table_width;
+  m.free_pages = free_pages; m.n_free = n_free; m.n_free_cap = (int)n_free_cap;
+  m.cu = cu_q; m.kv_len = kv_len; m.positions = positions; m.slots = slots;
+  m.n_free_out = n_free_out; m.info = info;
+  // CTA 0 and one CTA per 1024 tokens, at most one per SM
+  int64_t ctas = (n_tokens + kPlanThreads - 1) / kPlanThreads;
+  ctas = ctas < 1 ? 1 : (ctas > kPlanCtas - 1 ? kPlanCtas - 1 : ctas);
+  paged_map_kernel<<<(unsigned)ctas + 1, kPlanThreads, 0, as_cuda(stream)>>>(m);
+  return check_launch("kvr_paged_map");
+}

@@ -4,8 +4,9 @@
 
 from .kvr_window import WindowBuffer
 from .kvr_retrieval import RetrievalIndex
+from .kvr_paged import PagedKVCache
 
-__all__ = ["WindowBuffer", "RetrievalIndex", "KVRHook", "KVRGenerator"]
+__all__ = ["WindowBuffer", "RetrievalIndex", "PagedKVCache", "KVRHook", "KVRGenerator"]
 
 
 def __getattr__(name):

@@ -92,6 +92,14 @@ SIGNATURES = {
     "kvr_int4w_vpredict_status": (I, [P]),
     "kvr_workspace_status": (I, [P, P]),
     "kvr_selftest_bounded_wait": (I, [P, C.c_uint32, P]),
+    "kvr_attn_plan_bytes": (SZ, [I64, I, I, I]),
+    "kvr_attn_plan": (I, [P, P, P, I, I64, I, I, I, I64, P, SZ, P]),
+    "kvr_paged_map": (I, [P, P, I, I64, I, P, I64, I, P, I64, P, P, P, P, P, P, P, I, I, I64, P, SZ, P]),
+    "kvr_paged_write": (I, [P, P, P, I, I64, I, I, I, I64, I64, I64, P, P, I64, I64, P, P, P, P, P, I64, I, I64, I64,
+                            P]),
+    "kvr_attn_workspace_bytes": (SZ, [I, I]),
+    "kvr_paged_attn": (I, [P, I, I64, I, I, I, I, I64, P, P, I64, I, I64, I64, P, I64, I, P, SZ, F, P, P, P, SZ, P]),
+    "kvr_prompt_attn": (I, [P, P, P, I, I64, I64, I, I, I, I, I64, I64, I64, P, SZ, F, P, P, P, SZ, P]),
     "kvr_decode_attn_noalloc_max_scratch_bytes": (SZ, []),
     "kvr_decode_attn_noalloc": (I, [P, I, I, I, I, P, P, I, I, I64, I64, P, P, I, I, I64, I64, F, P, I, P]),
 }

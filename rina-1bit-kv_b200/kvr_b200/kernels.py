@@ -527,6 +527,228 @@ def sd1_prefill_scores(store: Sd1Store, q):
     return out
 
 
+# ----------------------------------------------------- paged exact cache --
+
+
+def _tokens(x, name):
+    """(n, heads, 128) with contiguous heads and 16-byte aligned rows, and its
+    token stride in elements; views that are not laid out so are copied."""
+    if x.dim() != 3 or x.shape[2] != D:
+        raise ValueError(f"{name} must be (tokens, heads, {D}), got {tuple(x.shape)}")
+    n, heads, _ = x.shape
+    ok = (x.stride(2) == 1 and (heads == 1 or x.stride(1) == D) and x.data_ptr() % 16 == 0
+          and (n <= 1 or (x.stride(0) >= heads * D and x.stride(0) % 8 == 0)))
+    if not ok:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.stride(0) if n > 1 else heads * D
+
+
+def _pool(k_pages, v_pages):
+    """(n_pages, page, n_kv, 128) pools, e.g. views of one (n_pages, 2, page,
+    n_kv, 128) tensor; never copied, since they are the caller's cache."""
+    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if x.dim() != 4 or x.shape[3] != D:
+            raise ValueError(f"{name} must be (pages, page, heads, {D}), got {tuple(x.shape)}")
+        if x.stride(3) != 1 or (x.shape[2] > 1 and x.stride(2) != D):
+            raise ValueError(f"{name}: a token's heads must be contiguous")
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+        raise ValueError("k_pages and v_pages must have one shape, type and layout")
+    return k_pages.shape[0], k_pages.shape[1], k_pages.stride(0), k_pages.stride(1)
+
+
+def _i32(x, name, numel=None):
+    if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous int32 vector")
+    if numel is not None and x.numel() != numel:
+        raise ValueError(f"{name} must have {numel} entries, got {x.numel()}")
+    return x
+
+
+class AttnPlan:
+    """The work list of an attention call (kvr_attn_plan), on the device, and
+    the shapes it was built for."""
+
+    def __init__(self, n_tokens, batch, n_q, n_kv, paged, device):
+        self.n_tokens, self.batch, self.n_q, self.n_kv, self.paged = n_tokens, batch, n_q, n_kv, paged
+        nbytes = call("kvr_attn_plan_bytes", n_tokens, batch, n_q, n_kv)
+        self.buf = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def _match(self, n_tokens, n_q, paged):
+        if (self.n_tokens, self.n_q, self.paged) != (n_tokens, n_q, paged):
+            raise ValueError(f"the plan is for {self.n_tokens} tokens of {self.n_q} heads"
+                             f"{' over pages' if self.paged else ''}, not {n_tokens} of {n_q}"
+                             f"{' over pages' if paged else ''}")
+
+
+def attn_plan(cu_q, n_tokens, n_q, n_kv, kv_len=None, cu_k=None, causal=True, window=0):
+    """Plan of the attention of packed queries: those of request b are
+    [cu_q[b], cu_q[b+1]) of n_tokens and are the last tokens of kv_len[b] keys
+    in pages (paged_attn), or of the packed keys [cu_k[b], cu_k[b+1])
+    (prompt_attn; cu_k None: the queries' own tokens).  window > 0: a query
+    sees the last `window` keys up to itself.  All lengths int32 on the device;
+    one plan serves every layer."""
+    _i32(cu_q, "cu_q")
+    batch = cu_q.numel() - 1
+    if batch < 1:
+        raise ValueError("cu_q must have at least two entries")
+    if kv_len is not None:
+        _i32(kv_len, "kv_len", batch)
+    if cu_k is not None:
+        _i32(cu_k, "cu_k", batch + 1)
+    plan = AttnPlan(n_tokens, batch, n_q, n_kv, kv_len is not None, cu_q.device)
+    call("kvr_attn_plan", ptr(cu_q), ptr(kv_len), ptr(cu_k), batch, n_tokens, n_q, n_kv, int(causal), window,
+         ptr(plan.buf), plan.buf.numel(), stream())
+    return plan
+
+
+class PagedStep:
+    """What paged_map makes of a step's lengths (int32 on the device unless
+    noted): cu_q (B + 1), kv_len (B), positions (T), slots (T) int64, n_free
+    (1) left, info (4) = [pages missing, requests cut, requests longer than
+    their table row, 0], and the attention plan (None without n_q)."""
+
+    __slots__ = ("cu_q", "kv_len", "positions", "slots", "n_free", "info", "plan", "n_tokens")
+
+
+def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens, n_q=0, n_kv=0, window=0):
+    """Block tables, slot maps and the attention plan of a step in one launch:
+    request b has ctx_len[b] tokens cached and gets new_len[b]; pages come off
+    the end of free_pages[:n_free] and are entered into block_table (B, width)
+    in place.  n_tokens: the step's packed length (>= the sum of new_len; the
+    rest is padding).  ctx_len, new_len and n_free are left as they are."""
+    batch = ctx_len.numel()
+    _i32(ctx_len, "ctx_len")
+    _i32(new_len, "new_len", batch)
+    _i32(free_pages, "free_pages")
+    _i32(n_free, "n_free", 1)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise TypeError("block_table must be an int32 matrix with contiguous rows")
+    if block_table.shape[0] < batch:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {batch} requests")
+    dev = ctx_len.device
+    width = block_table.shape[1]
+    # one allocation: cu_q, kv_len, n_free, info, positions, then slots on an 8-byte boundary
+    head = (2 * batch + 6 + n_tokens + 1) // 2 * 2
+    buf = torch.empty(head + 2 * n_tokens, dtype=torch.int32, device=dev)
+    st = PagedStep()
+    st.cu_q, st.kv_len = buf[:batch + 1], buf[batch + 1:2 * batch + 1]
+    st.n_free, st.info = buf[2 * batch + 1:2 * batch + 2], buf[2 * batch + 2:2 * batch + 6]
+    st.positions = buf[2 * batch + 6:2 * batch + 6 + n_tokens]
+    st.slots = buf[head:].view(torch.int64)
+    st.n_tokens = n_tokens
+    st.plan = AttnPlan(n_tokens, batch, n_q, n_kv, True, dev) if n_q else None
+    call("kvr_paged_map", ptr(ctx_len), ptr(new_len), batch, n_tokens, page, ptr(block_table),
+         max(block_table.stride(0), width), width, ptr(free_pages), free_pages.numel(), ptr(n_free), ptr(st.cu_q),
+         ptr(st.kv_len), ptr(st.positions), ptr(st.slots), ptr(st.n_free), ptr(st.info), n_q, n_kv, window,
+         ptr(st.plan.buf) if st.plan else None, st.plan.buf.numel() if st.plan else 0, stream())
+    return st
+
+
+def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=None, q_out=None):
+    """RoPE of q (T, n_q, d) and k (T, n_kv, d) at `positions` (cos None: no
+    rotation) and the write of k and v into cache slots `slots` (T) int64 of
+    the pools (n_pages, page, n_kv, d).  Returns the rotated q (None if q is);
+    rows of tokens with slot -1 are 0."""
+    n_pages, page, ps, ts = _pool(k_pages, v_pages)
+    n_tokens = k.shape[0]
+    k, ks = _tokens(k, "k")
+    v, vs = _tokens(v, "v")
+    if k.dtype != k_pages.dtype or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError("q, k, v and the pools must share a dtype")
+    if k.shape != v.shape or k.shape[1] != k_pages.shape[2] or (q is not None and q.shape[0] != n_tokens):
+        raise ValueError("q, k, v and the pools do not fit together")
+    if slots.dtype != torch.int64 or not slots.is_contiguous() or slots.numel() != n_tokens:
+        raise TypeError("slots must be a contiguous int64 vector, one per token")
+    qs, n_q, rs, max_pos = 0, 0, 0, 0
+    if q is not None:
+        q, qs = _tokens(q, "q")
+        n_q = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(n_tokens, n_q, D, dtype=q.dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous and of q's shape and dtype")
+    if cos is not None:
+        _i32(positions, "positions", n_tokens)
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise TypeError("the RoPE tables must be fp32")
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D:
+            raise ValueError(f"the RoPE tables must be (max_pos, {D})")
+        cos, sin, rs = _rope_args(cos, sin)
+        max_pos = cos.shape[0]
+    call("kvr_paged_write", ptr(q), ptr(k), ptr(v), dtype_code(k), n_tokens, n_q, k.shape[1], D, qs, ks, vs, ptr(cos),
+         ptr(sin), rs, max_pos, ptr(positions) if cos is not None else None, ptr(slots), ptr(q_out), ptr(k_pages),
+         ptr(v_pages), n_pages, page, ps, ts, stream())
+    return q_out
+
+
+def _attn_workspace(n_q, n_kv, device):
+    """The attention workspace of the current stream (calls on one stream do
+    not overlap; each stream has its own)."""
+    s = stream()
+    return N.workspace(f"attn_work_{s}", call("kvr_attn_workspace_bytes", n_q, n_kv), device), s
+
+
+def _attn_out(q, out, return_lse):
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous and of q's shape and dtype")
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    return out, lse
+
+
+def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, return_lse=False):
+    """Attention of a step's query tokens q (T, n_q, d) over their requests'
+    pages; `plan` from paged_map or attn_plan(kv_len=...).  Returns out of q's
+    shape and dtype, or (out, lse (T, n_q) fp32)."""
+    n_pages, page, ps, ts = _pool(k_pages, v_pages)
+    q, qs = _tokens(q, "q")
+    n_tokens, n_q, _ = q.shape
+    plan._match(n_tokens, n_q, True)
+    if q.dtype != k_pages.dtype:
+        raise TypeError("q and the pools must share a dtype")
+    if k_pages.shape[2] != plan.n_kv:
+        raise ValueError(f"the plan is for {plan.n_kv} KV heads, the pool has {k_pages.shape[2]}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise TypeError("block_table must be an int32 matrix with contiguous rows")
+    if block_table.shape[0] < plan.batch:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {plan.batch} requests")
+    out, lse = _attn_out(q, out, return_lse)
+    ws, s = _attn_workspace(n_q, plan.n_kv, q.device)
+    width = block_table.shape[1]
+    call("kvr_paged_attn", ptr(q), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, ptr(k_pages),
+         ptr(v_pages), n_pages, page, ps, ts, ptr(block_table), max(block_table.stride(0), width), width,
+         ptr(plan.buf), plan.buf.numel(), float(scale or 0.0), ptr(out), ptr(lse), ptr(ws), ws.numel(), s)
+    return (out, lse) if return_lse else out
+
+
+def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
+    """Attention over whole packed prompts: q (T, n_q, d), k and v (T_k, n_kv,
+    d), possibly strided views of one projection; `plan` from attn_plan.
+    Returns out of q's shape and dtype, or (out, lse (T, n_q) fp32)."""
+    q, qs = _tokens(q, "q")
+    k, ks = _tokens(k, "k")
+    v, vs = _tokens(v, "v")
+    n_tokens, n_q, _ = q.shape
+    plan._match(n_tokens, n_q, False)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share a dtype")
+    if k.shape != v.shape or k.shape[1] != plan.n_kv:
+        raise ValueError("k and v must be (tokens, n_kv, d) with the plan's n_kv")
+    out, lse = _attn_out(q, out, return_lse)
+    ws, s = _attn_workspace(n_q, plan.n_kv, q.device)
+    call("kvr_prompt_attn", ptr(q), ptr(k), ptr(v), dtype_code(q), n_tokens, k.shape[0], plan.batch, n_q, plan.n_kv, D,
+         qs, ks, vs, ptr(plan.buf), plan.buf.numel(), float(scale or 0.0), ptr(out), ptr(lse), ptr(ws), ws.numel(), s)
+    return (out, lse) if return_lse else out
+
+
+def attn_status(device=None):
+    """Raises if an attention call on the current stream gave up or met a plan
+    of other shapes (synchronises the stream)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    workspace_status(_attn_workspace(1, 1, device)[0])
+
+
 def kmeans(x, k=128, iters=10):
     """Deterministic Lloyd k-means on the device: x (n, 128) -> (labels (n,)
     int32, centroids (k, 128) fp32)."""
