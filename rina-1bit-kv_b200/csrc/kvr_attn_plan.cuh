@@ -6,7 +6,15 @@
 // 2 * tpt consecutive tokens, tpt = floor(128 / g): two 128-row tiles that
 // share every K/V tile of 128 keys they read.  A piece is a range of an
 // item's K/V tiles; the list holds the pieces of ONE head, longest first, and
-// serves every KV head: entry p stands for pieces p * n_kv + h.
+// serves every KV head: entry p stands for pieces p * n_kv + h.  CTA c of G
+// takes pieces c, 2G-1-c, 2G+c, 4G-1-c, ...: with the list sorted the long and
+// the short ones even out, and no counter has to be shared or reset.
+//
+// Items are cut into pieces only where whole items would leave SMs idle: the
+// length of the longest piece is the one of 32 candidates for which the
+// estimated time is least (plan_estimate).  The pieces of a cut item leave
+// unnormalised partial rows in the workspace, which a second kernel joins in
+// the order of the pieces.
 #pragma once
 
 #include "kvr_common.cuh"
@@ -26,8 +34,10 @@ constexpr int kPlanCtas = 148;   // SMs the work is spread over
 struct PlanHeader {  // 64 words
   int magic, n_tokens, batch, n_q, n_kv, causal, window;
   int n_pieces;      // per head
+  int n_splits;      // items cut into pieces, per head
+  int part_rows;     // rows of partial results, per head
   int dropped;       // 1: items did not fit the list (offsets that overlap)
-  int pad[55];
+  int pad[53];
 };
 
 struct PlanPiece {   // 8 words
@@ -41,6 +51,15 @@ struct PlanPiece {   // 8 words
 };
 static_assert(sizeof(PlanPiece) == 32, "piece record");
 
+struct PlanSplit {   // an item cut into pieces
+  int q_start, n_tok;
+  int part;          // row base of its first piece; the others follow, n_tok * g rows each
+  int n_pieces;
+};
+
+constexpr int kPlanExtra = 1024;                  // pieces per head beyond one per item
+constexpr int kPartRows = 2 * kPlanCtas * 2 * kPlanRows;  // partial rows the workspace holds
+
 __host__ __device__ inline int plan_tpt(int n_q, int n_kv) { return kPlanRows / (n_q / n_kv); }
 __host__ __device__ inline int64_t plan_max_items(int64_t n_tokens, int batch, int n_q, int n_kv) {
   return n_tokens / (2 * plan_tpt(n_q, n_kv)) + batch + 2;
@@ -53,8 +72,15 @@ struct PlanArgs {
   int batch, n_tokens, n_q, n_kv, causal, window;
   PlanHeader *hdr;
   PlanPiece *pieces;
+  PlanSplit *splits;
   int max_items;
 };
+
+__host__ __device__ inline const PlanSplit *plan_splits(const PlanHeader *h, int64_t n_tokens, int batch, int n_q,
+                                                        int n_kv) {
+  const PlanPiece *p = reinterpret_cast<const PlanPiece *>(h + 1);
+  return reinterpret_cast<const PlanSplit *>(p + plan_max_items(n_tokens, batch, n_q, n_kv) + kPlanExtra);
+}
 
 // Checks of the arguments every plan-building entry point shares; fills the
 // pointers into the plan buffer.  Returns a status.

@@ -5,88 +5,666 @@
 // out = softmax(q k^T / scale) v over the keys a row sees, and lse =
 // log(sum exp(q k^T / scale)); a row that sees no key gives zeros and -inf.
 //
-// A warp per query row walks the row's keys once with a running maximum and
-// sum; lane l holds channels 4l .. 4l+3 of q, k, v and the output.
+// One pass over the keys with a running maximum and sum.  A CTA (one per SM)
+// walks the plan's pieces: up to two 128-row query tiles against K/V tiles of
+// 128 keys.  Packing the g query heads of a KV head into the rows (row = token
+// * g + j) lets one K/V tile serve all of them, for one token as for many.
+//   warp 9   copies: Q tiles, then K, V, K, V, ... by TMA (128-byte swizzle)
+//            into a ring of five 32 KB stages; a paged tile is a box per page
+//            (or per gcd(page, 128) rows), a missing page an out-of-range box,
+//            which the TMA fills with zeros;
+//   warp 8   one lane issues tcgen05.mma: S_t = Q_t K^T (128 x 128 x 128,
+//            operands in shared memory), later O_t += P_t V with P_t in tensor
+//            memory and V read column-wise from shared memory;
+//   warps 0-3 and 4-7   a warpgroup per query tile, a row per thread: S_t
+//            from tensor memory, mask, maximum, exp2, sum; P_t, rounded to the
+//            tensors' 16-bit type, goes back over S_t.
+// While one tile's rows are in their softmax the tensor core works for the
+// other tile; S of the next K/V tile follows P V in the issue order, which is
+// also what makes the reuse of S_t's columns for P_t safe: MMAs of one thread
+// execute in order.  Tensor memory: S_0, S_1, O_0, O_1, 128 columns each.
+//
+// The output accumulator is rescaled only when a row's maximum has grown by
+// more than 2^kLazy since its last rescale (the weights stay below 2^(kLazy +
+// kShift), the sums are exact either way), so the read-modify-write of O is
+// rare after the first tiles.  Weights carry a factor 2^kShift that cancels in
+// the division: it keeps fp16 weights of 2^-18 out of the subnormals.
+//
+// Keys past a request's end, or before every row's window, are masked in S,
+// and their V rows are zeroed in shared memory, because 0 times a NaN of a
+// neighbour would still be a NaN.
+//
+// Every wait is bounded; one that gives up sets the error word, lets the
+// copies and MMAs in flight drain and frees the tensor memory.
+#include <cuda.h>
+
 #include "kvr_attn_plan.cuh"
 
 namespace kvr {
 
+constexpr int kCaThreads = 384;  // two softmax warpgroups; MMA, copies and two idle warps
+constexpr int kCaStages = 5;
+constexpr uint32_t kCaTile = 128 * kD * 2;      // 32 KB: 128 rows of K, V or Q
+constexpr uint32_t kCaHalf = kCaTile / 2;       // 64 channels of them
+constexpr uint32_t kCaOffKv = 2 * kCaTile;
+constexpr uint32_t kCaOffBar = kCaOffKv + kCaStages * kCaTile;
+constexpr int kCaBars = 2 * kCaStages + 11;
+constexpr uint32_t kCaSmem = kCaOffBar + kCaBars * 8 + 16;
+constexpr uint32_t kCaTmemCols = 512;
+constexpr float kLazy = 6.0f, kShift = 4.0f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
 struct ChunkArgs {
-  const void *q, *k, *v;
-  int64_t q_stride;
-  int64_t n_tokens, n_keys;         // packed K/V: tokens; pages: unused
-  int64_t tok_stride, page_stride;  // elements
-  int64_t k_tok_stride, v_tok_stride;
+  int64_t n_tokens;
   int n_q, n_kv, batch;
-  int paged, page;
-  int64_t n_pages;
+  int page, box;                // paged: tokens per page, rows per copy (gcd(page, 128))
+  int n_pages;
   const int *table;
   int64_t table_stride;
   int table_width;
   const PlanHeader *hdr;
-  float inv_scale;
+  float to_log2;                // log2(e) / scale
   void *out;
   float *lse;
+  float *part_o, *part_ml;      // partial rows: 128 values; maximum (log2 units) and sum
   unsigned *err;
 };
 
+// ------------------------------------------------------- tcgen05 and TMA ----
+
+// K-major operand, 128-byte swizzle: 8-row atoms of 1 KB, 1 KB apart.
+__device__ __forceinline__ uint64_t ca_desc_k(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// V read as the N x K operand with N (channels) contiguous, 128-byte swizzle:
+// atoms of 64 channels x 8 keys; 16 KB to the other 64 channels, 1 KB to the next 8 keys.
+__device__ __forceinline__ uint64_t ca_desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(kCaHalf >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16, fp32 accumulator, M 128, N 128.
 template <int DT>
-__global__ void __launch_bounds__(256) chunk_attn_kernel(ChunkArgs a) {
-  const PlanHeader &h = *a.hdr;
-  if (h.magic != kPlanMagic || h.n_tokens != a.n_tokens || h.n_q != a.n_q || h.n_kv != a.n_kv || h.batch != a.batch) {
-    if (threadIdx.x == 0) atomicOr(a.err, kWsErrPlan);
-    return;
+__host__ __device__ constexpr uint32_t ca_idesc(bool b_mn) {
+  return (1u << 4) | ((DT == KVR_BF16 ? 1u : 0u) << 7) | ((DT == KVR_BF16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
+         ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void ca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void ca_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void ca_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void ca_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ca_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ca_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void ca_ld32(uint32_t taddr, float *f) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ca_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void ca_tma4(uint32_t dst, const CUtensorMap *m, int c1, int c2, int c3, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(m), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void ca_tma5(uint32_t dst, const CUtensorMap *m, int c1, int c2, int c3, int c4,
+                                        uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(dst),
+      "l"(m), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ---------------------------------------------------------------- waiting ----
+
+__device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile int *abort_s) {
+  if (mbar_try_wait(bar, phase)) return true;
+  for (uint32_t it = 0; it < kSpinLimit; ++it) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((it & 255u) == 255u && *abort_s) return false;
   }
-  const PlanPiece *pieces = reinterpret_cast<const PlanPiece *>(a.hdr + 1);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = a.n_q / a.n_kv;
-  for (int64_t w = blockIdx.x; w < (int64_t)h.n_pieces * a.n_kv; w += gridDim.x) {
-    const PlanPiece p = pieces[w / a.n_kv];
-    const int head = (int)(w % a.n_kv);
-    for (int r = warp; r < p.n_tok * g; r += 8) {
-      const int64_t t = p.q_start + r / g;
-      const int hq = head * g + r % g;
-      if (t < 0 || t >= a.n_tokens) continue;
-      const int end = h.causal ? min(p.kv_len, p.first_end + r / g) : p.kv_len;
-      const int begin = h.window > 0 ? max(0, p.first_end + r / g - h.window) : 0;
-      float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.0f;
-      load4<DT>(a.q, t * a.q_stride + (int64_t)hq * kD + lane * 4, q);
-      for (int j = begin; j < end; ++j) {
-        int64_t ki, vi;
-        float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        bool there;
-        if (a.paged) {
-          const int pj = j / a.page;
-          const int page = pj < a.table_width ? a.table[p.k_start * a.table_stride + pj] : -1;
-          there = page >= 0 && page < a.n_pages;
-          ki = vi = page * a.page_stride + (int64_t)(j % a.page) * a.tok_stride;
-        } else {
-          there = (int64_t)p.k_start + j < a.n_keys;
-          ki = ((int64_t)p.k_start + j) * a.k_tok_stride;
-          vi = ((int64_t)p.k_start + j) * a.v_tok_stride;
-        }
-        if (there) {
-          load4<DT>(a.k, ki + (int64_t)head * kD + lane * 4, k);
-          load4<DT>(a.v, vi + (int64_t)head * kD + lane * 4, v);
-        }
-        const float s = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]) * a.inv_scale;
-        const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn), e = expf(s - mn);
-        l = l * f + e;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = o[c] * f + e * v[c];
-        m = mn;
-      }
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-      const int64_t oi = (t * a.n_q + hq) * kD + lane * 4;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) store_elem<DT>(a.out, oi + c, l == 0.0f ? 0.0f : o[c] * inv);
-      if (a.lse && lane == 0) a.lse[t * a.n_q + hq] = l == 0.0f ? -INFINITY : m + logf(l);
+  return false;
+}
+__device__ __forceinline__ void ca_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ------------------------------------------------------------ the pieces ----
+
+// Piece number r of CTA c (see kvr_attn_plan.cuh), or false past the last.
+struct CaPiece {
+  PlanPiece p;
+  int head, n, two;  // KV head, K/V tiles, whether the second query tile has rows
+};
+__device__ __forceinline__ bool ca_piece(const ChunkArgs &a, int64_t total, int per, int r, CaPiece &o) {
+  const int64_t G = gridDim.x, c = blockIdx.x;
+  const int64_t i = (int64_t)r * G + ((r & 1) ? G - 1 - c : c);
+  if (i >= total) return false;
+  o.p = reinterpret_cast<const PlanPiece *>(a.hdr + 1)[i / a.n_kv];
+  o.head = (int)(i % a.n_kv);
+  o.p.n_tok = min(max(o.p.n_tok, 0), per);
+  o.n = o.p.n_tok > 0 ? max(o.p.kt1 - o.p.kt0, 0) : 0;
+  o.two = o.p.n_tok > (per >> 1);
+  return true;
+}
+
+__device__ __forceinline__ float ca_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT == KVR_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int DT, bool PAGED>
+__global__ void __launch_bounds__(kCaThreads, 1)
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                      const __grid_constant__ CUtensorMap mv, const ChunkArgs a) {
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t *kv_full = reinterpret_cast<uint64_t *>(sm + kCaOffBar);
+  uint64_t *kv_empty = kv_full + kCaStages;
+  uint64_t *q_full = kv_empty + kCaStages;
+  uint64_t *q_empty = q_full + 2;
+  uint64_t *s_full = q_empty + 2;
+  uint64_t *p_full = s_full + 2;
+  uint64_t *o_full = p_full + 2;
+  uint64_t *drained = o_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+  volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kCaTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 9 * 32) {
+    *abort_s = 0;
+    for (int s = 0; s < kCaStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
     }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(drained, 1);
+  }
+  ca_fence_before();
+  __syncthreads();
+  ca_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();  // what follows reads the plan, q and the cache
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel waits for this grid's end
+
+  const PlanHeader &h = *a.hdr;
+  const bool fits = h.magic == kPlanMagic && h.n_tokens == a.n_tokens && h.n_q == a.n_q && h.n_kv == a.n_kv &&
+                    h.batch == a.batch;
+  if (!fits && tid == 0) atomicOr(a.err, kWsErrPlan);
+  const int64_t total = fits ? (int64_t)h.n_pieces * a.n_kv : 0;
+  const int causal = h.causal, window = h.window;
+  const int g = a.n_q / a.n_kv, tpt = kPlanRows / g, per = 2 * tpt;
+
+  // registers: 384 threads x 168 at launch = (208 + 208 + 88) x 128
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp >= 10) {
+    __syncthreads();
+  } else if (warp == 9) {
+    // ---- copies
+    int j = 0, uses[2] = {0, 0};  // ring stages and Q tiles filled so far
+    CaPiece c;
+    bool ok = true;
+    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+      const int64_t row = PAGED ? (int64_t)c.p.k_start * a.table_stride : 0;
+      const bool known = PAGED && c.p.k_start >= 0 && c.p.k_start < a.batch;
+      int id = 0, off = 0;  // paged: this lane's page and row in it, of the next K/V tile
+      auto look = [&](int kt) {
+        if (PAGED && lane * a.box < 128) {
+          const int key = kt * 128 + lane * a.box, pj = key / a.page;
+          off = key - pj * a.page;
+          id = known && key < c.p.kv_len && pj < a.table_width ? a.table[row + pj] : -1;
+          if (id < 0 || id >= a.n_pages) id = a.n_pages;  // out of range: zeros
+        }
+      };
+      auto load = [&](const CUtensorMap *m, int kt) {
+        const int s = j % kCaStages;
+        if (j >= kCaStages && !ca_wait(&kv_empty[s], (unsigned)((j / kCaStages - 1) & 1), abort_s)) return false;
+        const uint32_t dst = smem_u32(sm) + kCaOffKv + s * kCaTile;
+        if (lane == 0) mbar_expect_tx(&kv_full[s], kCaTile);
+        __syncwarp();
+        if (PAGED) {
+          if (lane * a.box < 128) {
+            const uint32_t d = dst + lane * a.box * 128;
+            ca_tma5(d, m, off, 0, c.head, id, &kv_full[s]);
+            ca_tma5(d + kCaHalf, m, off, 1, c.head, id, &kv_full[s]);
+          }
+        } else if (lane == 0) {
+          ca_tma4(dst, m, c.p.k_start + kt * 128, 0, c.head, &kv_full[s]);
+        }
+        ++j;
+        return true;
+      };
+      auto load_q = [&](int t) {
+        if (uses[t] > 0 && !ca_wait(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
+        if (lane == 0) {
+          const uint32_t dst = smem_u32(sm) + t * kCaTile;
+          mbar_expect_tx(&q_full[t], 2u * 128u * tpt * g);
+          ca_tma5(dst, &mq, 0, c.p.q_start + t * tpt, 0, c.head, &q_full[t]);
+          ca_tma5(dst + kCaHalf, &mq, 0, c.p.q_start + t * tpt, 1, c.head, &q_full[t]);
+        }
+        ++uses[t];
+        return true;
+      };
+      if (c.n == 0) continue;
+      look(c.p.kt0);
+      ok = load_q(0) && load(&mk, c.p.kt0) && (!c.two || load_q(1));
+      for (int i = 0; ok && i < c.n; ++i) {
+        ok = load(&mv, c.p.kt0 + i);
+        if (ok && i + 1 < c.n) {
+          look(c.p.kt0 + i + 1);
+          ok = load(&mk, c.p.kt0 + i + 1);
+        }
+      }
+      if (*abort_s) ok = false;
+    }
+    if (!__all_sync(~0u, ok)) {
+      if (lane == 0) {
+        if (!*abort_s) atomicOr(a.err, 1u);
+        *abort_s = 1;
+      }
+    }
+    __syncthreads();  // end of work
+    if (*abort_s) {   // copies in flight must land before the CTA exits
+      for (int k = max(0, j - kCaStages); k < j; ++k)
+        for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(&kv_full[k % kCaStages], (unsigned)((k / kCaStages) & 1));)
+          ++it;
+      for (int t = 0; t < 2; ++t)
+        for (uint32_t it = 0; uses[t] && it < kSpinLimit && !mbar_try_wait(&q_full[t], (unsigned)((uses[t] - 1) & 1));)
+          ++it;
+    }
+  } else {
+    // ---- MMAs
+    const uint32_t q_base = smem_u32(sm), kv_base = q_base + kCaOffKv;
+    constexpr uint32_t kQk = ca_idesc<DT>(false), kPv = ca_idesc<DT>(true);
+    int j = 0, qn[2] = {0, 0}, pn[2] = {0, 0};  // ring stages, Q tiles and P tiles consumed so far
+    CaPiece c, nx;
+    int r = 0;
+    bool ok = true;
+    auto next_piece = [&](CaPiece &o) {  // the next piece that has K/V tiles
+      while (ca_piece(a, total, per, r, o)) {
+        ++r;
+        if (o.n > 0) return true;
+      }
+      return false;
+    };
+    auto wait_stage = [&](int k) { return ca_wait(&kv_full[k % kCaStages], (unsigned)((k / kCaStages) & 1), abort_s); };
+    // S_t of K stage k; `fresh`: the piece's first use of its Q tile, `last`: its last
+    auto issue_s = [&](int t, int k, bool fresh, bool last) {
+      if (fresh) {
+        if (!ca_wait(&q_full[t], (unsigned)(qn[t] & 1), abort_s)) return false;
+        ++qn[t];
+      }
+      ca_fence_after();
+      if (lane == 0) {
+        const uint32_t qa = q_base + t * kCaTile, kb = kv_base + (k % kCaStages) * kCaTile;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const uint32_t o = (s >> 2) * kCaHalf + (s & 3) * 32;
+          ca_mma_ss(tmem + t * 128, ca_desc_k(qa + o), ca_desc_k(kb + o), kQk, s > 0);
+        }
+        ca_commit(&s_full[t]);
+        if (last) ca_commit(&q_empty[t]);
+      }
+      return true;
+    };
+    auto issue_pv = [&](int t, int k, bool first, bool last) {
+      if (!ca_wait(&p_full[t], (unsigned)(pn[t] & 1), abort_s)) return false;
+      ++pn[t];
+      ca_fence_after();
+      if (lane == 0) {
+        const uint32_t vb = kv_base + (k % kCaStages) * kCaTile;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          ca_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, ca_desc_mn(vb + s * 2048), kPv, !(first && s == 0));
+        if (last) ca_commit(&o_full[t]);
+      }
+      return true;
+    };
+    bool have = next_piece(c);
+    if (have) {
+      ok = wait_stage(j) && issue_s(0, j, true, c.n == 1) && (!c.two || issue_s(1, j, true, c.n == 1));
+      if (ok && lane == 0) ca_commit(&kv_empty[j % kCaStages]);
+    }
+    while (ok && have) {
+      bool more = false;
+      // rows of V that no query row of the piece may see
+      const int before = window > 0 ? c.p.first_end - window : 0;
+      for (int i = 0; ok && i < c.n; ++i) {
+        const int v = j + 1, kn = j + 2;
+        const bool tail = i + 1 == c.n;
+        if (tail) more = next_piece(nx);
+        const bool s_next = !tail || more;
+        const bool n_two = tail ? nx.two : c.two;
+        const bool n_last = tail ? nx.n == 1 : i + 2 == c.n;
+        ok = wait_stage(v);
+        if (!ok) break;
+        const int key0 = (c.p.kt0 + i) * 128, hi = min(128, c.p.kv_len - key0), lo = min(128, max(0, before - key0));
+        if (hi < 128 || lo > 0) {
+          unsigned char *vs = sm + kCaOffKv + (v % kCaStages) * kCaTile;
+          for (int e = lane; e < 128 * 16; e += 32) {
+            const int row = e >> 4;
+            if (row < lo || row >= hi)
+              *reinterpret_cast<uint4 *>(vs + (e & 8 ? kCaHalf : 0) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        ok = issue_pv(0, v, i == 0, tail);
+        if (ok && s_next) ok = wait_stage(kn) && issue_s(0, kn, tail, n_last);
+        if (ok && c.two) ok = issue_pv(1, v, i == 0, tail);
+        if (ok && lane == 0) ca_commit(&kv_empty[v % kCaStages]);
+        if (ok && s_next) {
+          if (n_two) ok = issue_s(1, kn, tail, n_last);
+          if (ok && lane == 0) ca_commit(&kv_empty[kn % kCaStages]);
+        }
+        j += 2;
+      }
+      have = more;
+      c = nx;
+    }
+    if (!__all_sync(~0u, ok)) {
+      if (lane == 0) {
+        if (!*abort_s) atomicOr(a.err, 1u);
+        *abort_s = 1;
+        ca_commit(drained);  // MMAs in flight must finish before the tensor memory is freed
+      }
+      __syncwarp();
+      for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(drained, 0);) ++it;
+    }
+    __syncthreads();
+  }
+  } else {
+    // ---- softmax: warpgroup t, a row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane;
+    const uint32_t s_addr = tmem + ((uint32_t)wrow << 16) + t * 128, o_addr = s_addr + 256;
+    const int tok_in = row / g;               // token of the row within its tile
+    const int tok = t * tpt + tok_in;         // ... within the item
+    const int tok_a = t * tpt + wrow / g, tok_b = t * tpt + min(tpt - 1, (wrow + 31) / g);
+    int sn = 0, on = 0;                       // S tiles and outputs consumed so far
+    bool ok = true;
+    CaPiece c;
+    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+      const int n_tok = min(tpt, c.p.n_tok - t * tpt);  // tokens of this tile
+      if (n_tok <= 0) continue;
+      const bool live = tok_in < n_tok, busy = wrow < n_tok * g;  // the row / the warp has something to do
+      const int end = causal ? min(c.p.kv_len, c.p.first_end + tok) : c.p.kv_len;
+      const int begin = window > 0 ? max(0, c.p.first_end + tok - window) : 0;
+      const int end_a = causal ? min(c.p.kv_len, c.p.first_end + tok_a) : c.p.kv_len;
+      const int begin_b = window > 0 ? max(0, c.p.first_end + tok_b - window) : 0;
+      float m = -INFINITY, mc = 0.0f, l = 0.0f;  // running maximum (raw score units), its log2 multiple, sum
+      for (int i = 0; i < c.n; ++i, ++sn) {
+        ok = __all_sync(~0u, ca_wait(&s_full[t], (unsigned)(sn & 1), abort_s));
+        if (!ok) break;
+        if (busy) {
+          ca_fence_after();
+          float s[128];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ca_ld32(s_addr + k * 32, s + k * 32);
+          ca_wait_ld();
+          const int k0 = (c.p.kt0 + i) * 128;
+          if (k0 + 128 > end_a || k0 < begin_b) {
+            const int e = end - k0, b = begin - k0;
+#pragma unroll
+            for (int k = 0; k < 128; ++k) s[k] = k < e && k >= b ? s[k] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < 128; k += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float x = s[k + u], y = k + 4 + u < 128 ? s[k + 4 + u] : -INFINITY;
+              mx[u] = fmaxf(mx[u], fmaxf(x, y));
+            }
+          }
+          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          // the first tile sets the maximum; later it moves only in steps above 2^kLazy
+          const bool grow = i == 0 || !((m_new - m) * a.to_log2 <= kLazy);
+          if (i > 0 && __any_sync(~0u, grow && m_new != m)) {
+            const float f = grow ? (m == -INFINITY ? 0.0f : ca_exp2((m - m_new) * a.to_log2)) : 1.0f;
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float o[32];
+              ca_ld32(o_addr + k * 32, o);
+              ca_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = f == 0.0f ? 0.0f : o[e] * f;
+              ca_st16(o_addr + k * 32, reinterpret_cast<const uint32_t *>(o));
+              ca_st16(o_addr + k * 32 + 16, reinterpret_cast<const uint32_t *>(o + 16));
+            }
+          }
+          if (grow) {
+            m = m_new;
+            mc = m == -INFINITY ? 0.0f : m * a.to_log2;
+          }
+          const float add = kShift - mc;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = ca_exp2(fmaf(s[k * 32 + 2 * e], a.to_log2, add));
+              const float y = ca_exp2(fmaf(s[k * 32 + 2 * e + 1], a.to_log2, add));
+              sum[e & 3] += x + y;
+              pk[e] = ca_pack<DT>(x, y);
+            }
+            ca_st16(s_addr + k * 16, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          ca_wait_st();
+          ca_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) ca_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // ---- the piece's rows
+      if (c.n > 0) {
+        ok = __all_sync(~0u, ca_wait(&o_full[t], (unsigned)(on & 1), abort_s));
+        if (!ok) break;
+        ++on;
+      }
+      if (!busy) continue;
+      ca_fence_after();
+      const int64_t token = (int64_t)c.p.q_start + tok;
+      const int hq = c.head * g + row - tok_in * g;
+      const bool store = live && token >= 0 && token < a.n_tokens;
+      if (c.p.part >= 0) {
+        const int64_t pr = (int64_t)c.head * h.part_rows + c.p.part + t * tpt * g + row;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float o[32];
+          ca_ld32(o_addr + k * 32, o);
+          ca_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<float4 *>(a.part_o + pr * kD + k * 32)[e] =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (live) *reinterpret_cast<float2 *>(a.part_ml + pr * 2) = make_float2(m == -INFINITY ? -INFINITY : mc - kShift, l);
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t *dst = static_cast<uint16_t *>(a.out) + (token * a.n_q + hq) * kD;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float o[32];
+          if (c.n > 0) {
+            ca_ld32(o_addr + k * 32, o);
+            ca_wait_ld();
+          }
+          if (store) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const float x = o[e * 8 + 2 * u], y = o[e * 8 + 2 * u + 1];
+                w[u] = l == 0.0f ? 0u : ca_pack<DT>(x * inv, y * inv);
+              }
+              reinterpret_cast<uint4 *>(dst + k * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (store && a.lse) a.lse[token * a.n_q + hq] = l == 0.0f ? -INFINITY : (mc - kShift + log2f(l)) * kLn2;
+      }
+      // the next piece's first P V overwrites O: it waits for p_full, which this warp arrives at later
+      ca_fence_before();
+    }
+    if (!ok && lane == 0) {
+      if (!*abort_s) atomicOr(a.err, 1u);
+      *abort_s = 1;
+    }
+    __syncthreads();
+  }
+  // every role is past its last access to the tensor memory (or drained after an abort)
+  ca_fence_after();
+  if (warp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCaTmemCols));
+}
+
+// Joins the partial rows of cut items in the order of their pieces: a warp per
+// row, lane l channels 4l .. 4l+3.
+template <int DT>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
+  griddep_wait();
+  const PlanHeader &h = *a.hdr;
+  if (h.magic != kPlanMagic || h.n_tokens != a.n_tokens || h.n_q != a.n_q || h.n_kv != a.n_kv || h.batch != a.batch) return;
+  const PlanSplit *splits = plan_splits(a.hdr, a.n_tokens, a.batch, a.n_q, a.n_kv);
+  const int lane = threadIdx.x & 31, g = a.n_q / a.n_kv, rows = 2 * (kPlanRows / g) * g;
+  const int64_t units = (int64_t)h.n_splits * a.n_kv * rows;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
+    const int row = (int)(u % rows);
+    const int64_t sh = u / rows;
+    const PlanSplit sp = splits[sh / a.n_kv];
+    if (row >= sp.n_tok * g) continue;
+    const int head = (int)(sh % a.n_kv);
+    const int64_t r0 = (int64_t)head * h.part_rows + sp.part + row, step = (int64_t)sp.n_tok * g;
+    float m = -INFINITY;
+    for (int k = lane; k < sp.n_pieces; k += 32) {
+      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r0 + k * step) * 2);
+      if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+    }
+    m = warp_max(m);
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < sp.n_pieces; ++k) {
+      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r0 + k * step) * 2);
+      if (ml.y == 0.0f) continue;  // a piece in which the row sees nothing
+      const float4 x = *reinterpret_cast<const float4 *>(a.part_o + (r0 + k * step) * kD + lane * 4);
+      const float f = exp2f(ml.x - m);
+      l += f * ml.y;
+      o[0] += f * x.x;
+      o[1] += f * x.y;
+      o[2] += f * x.z;
+      o[3] += f * x.w;
+    }
+    const int64_t token = (int64_t)sp.q_start + row / g;
+    const int hq = head * g + row % g;
+    if (token < 0 || token >= a.n_tokens) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint2 w = make_uint2(ca_pack<DT>(o[0] * inv, o[1] * inv), ca_pack<DT>(o[2] * inv, o[3] * inv));
+    if (l == 0.0f) w = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (token * a.n_q + hq) * kD + lane * 4) = w;
+    if (a.lse && lane == 0) a.lse[token * a.n_q + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
 }
 
-static int chunk_check(const char *fn, ChunkArgs &a, int dtype, int d, float scale, const void *plan,
+// ------------------------------------------------------------------- host ----
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// A tensor of 16-bit values with dims[0] = 64 channels (one swizzle row);
+// strides (bytes) and boxes of the other dimensions follow.
+static bool make_map(CUtensorMap *m, int dtype, const void *base, int rank, const cuuint64_t *dims,
+                     const cuuint64_t *strides, const cuuint32_t *box) {
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  return encode_tiled()(m, dtype == KVR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct ChunkCall {
+  const void *q, *k, *v;
+  int64_t q_stride;
+  ChunkArgs a;
+  CUtensorMap mq, mk, mv;
+};
+
+static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float scale, const void *plan,
                        size_t plan_bytes, void *workspace, size_t workspace_bytes) {
-  KVR_REQUIRE(a.q && a.k && a.v && a.out && plan && workspace, "%s: null pointer", fn);
+  ChunkArgs &a = c.a;
+  KVR_REQUIRE(c.q && c.k && c.v && a.out && plan && workspace, "%s: null pointer", fn);
   if (d != kD) return set_error(KVR_ENOTSUP, "%s: head_dim must be 128", fn);
   if (dtype != KVR_F16 && dtype != KVR_BF16) return set_error(KVR_ENOTSUP, "%s: fp16 or bf16", fn);
   KVR_REQUIRE(a.n_kv > 0 && a.n_q > 0 && a.n_q % a.n_kv == 0, "%s: n_q must be a multiple of n_kv", fn);
@@ -94,10 +672,10 @@ static int chunk_check(const char *fn, ChunkArgs &a, int dtype, int d, float sca
     return set_error(KVR_ENOTSUP, "%s: more than %d query heads per KV head", fn, kPlanRows);
   KVR_REQUIRE(a.batch >= 1 && a.batch <= kPlanMaxBatch, "%s: batch must be in [1, %d]", fn, kPlanMaxBatch);
   KVR_REQUIRE(a.n_tokens >= 0 && a.n_tokens <= kPlanMaxTokens, "%s: bad token count", fn);
-  KVR_REQUIRE(a.q_stride >= (int64_t)a.n_q * d && a.q_stride % 8 == 0,
+  KVR_REQUIRE(c.q_stride >= (int64_t)a.n_q * d && c.q_stride % 8 == 0,
               "%s: a token's heads must be contiguous, rows 16-byte aligned", fn);
-  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
-                         reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out) |
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k) |
+                         reinterpret_cast<uintptr_t>(c.v) | reinterpret_cast<uintptr_t>(a.out) |
                          reinterpret_cast<uintptr_t>(plan);
   KVR_REQUIRE((ptrs & 15) == 0, "%s: pointers must be 16-byte aligned", fn);
   KVR_REQUIRE(plan_bytes >= kvr_attn_plan_bytes(a.n_tokens, a.batch, a.n_q, a.n_kv), "%s: plan too small", fn);
@@ -105,15 +683,57 @@ static int chunk_check(const char *fn, ChunkArgs &a, int dtype, int d, float sca
   const size_t need = kvr_attn_workspace_bytes(a.n_q, a.n_kv);
   KVR_REQUIRE(workspace_bytes >= need, "%s: workspace %zu < %zu bytes", fn, workspace_bytes, need);
   KVR_REQUIRE(scale == scale && scale <= 3.0e38f, "%s: bad scale", fn);
-  a.inv_scale = 1.0f / (scale > 0.0f ? scale : sqrtf((float)d));
+  a.to_log2 = kLog2e / (scale > 0.0f ? scale : sqrtf((float)d));
   a.hdr = static_cast<const PlanHeader *>(plan);
   a.err = static_cast<unsigned *>(workspace);
+  a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWsHeader);
+  a.part_o = a.part_ml + 2 * (size_t)kPartRows;
   return KVR_OK;
 }
 
-static int chunk_launch(const char *fn, const ChunkArgs &a, int dtype, kvr_stream_t stream) {
-  if (dtype == KVR_F16) chunk_attn_kernel<KVR_F16><<<148 * 8, 256, 0, as_cuda(stream)>>>(a);
-  else chunk_attn_kernel<KVR_BF16><<<148 * 8, 256, 0, as_cuda(stream)>>>(a);
+template <int DT, bool PAGED>
+static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
+  static thread_local int set_dev = -1;
+  if (set_dev != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_kernel<DT, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kCaSmem);
+    if (e != cudaSuccess) return e;
+    set_dev = dev;
+  }
+  cudaLaunchAttribute dep[1];
+  dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  dep[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = dep;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(kPlanCtas);
+  cfg.blockDim = dim3(kCaThreads);
+  cfg.dynamicSmemBytes = kCaSmem;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel<DT, PAGED>, c.mq, c.mk, c.mv, c.a);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(kPlanCtas * 4);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, chunk_join_kernel<DT>, c.a);
+}
+
+static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr_stream_t stream) {
+  const ChunkArgs &a = c.a;
+  if (!encode_tiled()) return set_error(KVR_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", fn);
+  const int g = a.n_q / a.n_kv, tpt = kPlanRows / g;
+  // q as (64 channels, head of the group, token, channel half, KV head)
+  const cuuint64_t qd[5] = {64, (cuuint64_t)g, (cuuint64_t)a.n_tokens, 2, (cuuint64_t)a.n_kv};
+  const cuuint64_t qs[4] = {kD * 2, (cuuint64_t)c.q_stride * 2, 128, (cuuint64_t)g * kD * 2};
+  const cuuint32_t qb[5] = {64, (cuuint32_t)g, (cuuint32_t)tpt, 1, 1};
+  if (!make_map(&c.mq, dtype, c.q, 5, qd, qs, qb)) return set_error(KVR_EINVAL, "%s: q has a layout TMA cannot read", fn);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e;
+  cudaStream_t st = as_cuda(stream);
+  if (dtype == KVR_F16) e = paged ? chunk_kernels<KVR_F16, true>(c, dev, st) : chunk_kernels<KVR_F16, false>(c, dev, st);
+  else e = paged ? chunk_kernels<KVR_BF16, true>(c, dev, st) : chunk_kernels<KVR_BF16, false>(c, dev, st);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "%s: %s", fn, cudaGetErrorString(e));
   return check_launch(fn);
 }
 
@@ -124,7 +744,7 @@ using namespace kvr;
 extern "C" size_t kvr_attn_workspace_bytes(int n_q, int n_kv) {
   (void)n_q;
   (void)n_kv;
-  return kWsHeader;
+  return kWsHeader + (size_t)kPartRows * (kD + 2) * sizeof(float);
 }
 
 extern "C" int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int batch, int n_q, int n_kv, int d,
@@ -134,24 +754,32 @@ extern "C" int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int ba
                               void *out, float *lse, void *workspace, size_t workspace_bytes, kvr_stream_t stream) {
   clear_error();
   if (n_tokens == 0) return KVR_OK;
-  ChunkArgs a{};
-  a.q = q; a.k = k_pages; a.v = v_pages;
-  a.q_stride = q_stride;
+  ChunkCall c{};
+  c.q = q; c.k = k_pages; c.v = v_pages;
+  c.q_stride = q_stride;
+  ChunkArgs &a = c.a;
   a.n_tokens = n_tokens;
-  a.tok_stride = tok_stride; a.page_stride = page_stride;
   a.n_q = n_q; a.n_kv = n_kv; a.batch = batch;
-  a.paged = 1; a.page = page; a.n_pages = n_pages;
+  a.page = page; a.n_pages = (int)n_pages;
   a.table = block_table; a.table_stride = table_stride; a.table_width = table_width;
   a.out = out; a.lse = lse;
-  const int rc = chunk_check("kvr_paged_attn", a, dtype, d, scale, plan, plan_bytes, workspace, workspace_bytes);
+  const int rc = chunk_check("kvr_paged_attn", c, dtype, d, scale, plan, plan_bytes, workspace, workspace_bytes);
   if (rc) return rc;
   KVR_REQUIRE(block_table && table_width >= 1 && table_stride >= table_width, "kvr_paged_attn: bad block table");
-  KVR_REQUIRE(n_pages > 0 && n_pages <= INT_MAX, "kvr_paged_attn: bad page pool");
+  KVR_REQUIRE(n_pages > 0 && n_pages < INT_MAX, "kvr_paged_attn: bad page pool");
   if (page < 8 || page % 8 != 0 || page > (1 << 20))
     return set_error(KVR_ENOTSUP, "kvr_paged_attn: the page size must be a multiple of 8 tokens");
   KVR_REQUIRE(tok_stride >= (int64_t)n_kv * d && tok_stride % 8 == 0 && page_stride >= 0 && page_stride % 8 == 0,
               "kvr_paged_attn: a token's heads must be contiguous, rows 16-byte aligned");
-  return chunk_launch("kvr_paged_attn", a, dtype, stream);
+  a.box = 128;
+  while (page % a.box) a.box /= 2;
+  // the pool as (64 channels, row of the page, channel half, KV head, page)
+  const cuuint64_t kd[5] = {64, (cuuint64_t)page, 2, (cuuint64_t)n_kv, (cuuint64_t)n_pages};
+  const cuuint64_t ks[4] = {(cuuint64_t)tok_stride * 2, 128, kD * 2, (cuuint64_t)page_stride * 2};
+  const cuuint32_t kb[5] = {64, (cuuint32_t)a.box, 1, 1, 1};
+  if (!encode_tiled() || !make_map(&c.mk, dtype, k_pages, 5, kd, ks, kb) || !make_map(&c.mv, dtype, v_pages, 5, kd, ks, kb))
+    return set_error(KVR_EINVAL, "kvr_paged_attn: the pool has a layout TMA cannot read");
+  return chunk_launch("kvr_paged_attn", c, dtype, true, stream);
 }
 
 extern "C" int kvr_prompt_attn(const void *q, const void *k, const void *v, int dtype, int64_t n_tokens,
@@ -160,17 +788,23 @@ extern "C" int kvr_prompt_attn(const void *q, const void *k, const void *v, int 
                                float *lse, void *workspace, size_t workspace_bytes, kvr_stream_t stream) {
   clear_error();
   if (n_tokens == 0) return KVR_OK;
-  ChunkArgs a{};
-  a.q = q; a.k = k; a.v = v;
-  a.q_stride = q_stride;
-  a.n_tokens = n_tokens; a.n_keys = n_keys;
-  a.k_tok_stride = k_stride; a.v_tok_stride = v_stride;
+  ChunkCall c{};
+  c.q = q; c.k = k; c.v = v;
+  c.q_stride = q_stride;
+  ChunkArgs &a = c.a;
+  a.n_tokens = n_tokens;
   a.n_q = n_q; a.n_kv = n_kv; a.batch = batch;
   a.out = out; a.lse = lse;
-  const int rc = chunk_check("kvr_prompt_attn", a, dtype, d, scale, plan, plan_bytes, workspace, workspace_bytes);
+  const int rc = chunk_check("kvr_prompt_attn", c, dtype, d, scale, plan, plan_bytes, workspace, workspace_bytes);
   if (rc) return rc;
   KVR_REQUIRE(n_keys > 0 && n_keys <= kPlanMaxLen, "kvr_prompt_attn: bad key count");
   KVR_REQUIRE(k_stride >= (int64_t)n_kv * d && v_stride >= (int64_t)n_kv * d && (k_stride | v_stride) % 8 == 0,
               "kvr_prompt_attn: a token's heads must be contiguous, rows 16-byte aligned");
-  return chunk_launch("kvr_prompt_attn", a, dtype, stream);
+  // k and v as (64 channels, token, channel half, KV head)
+  const cuuint64_t kd[4] = {64, (cuuint64_t)n_keys, 2, (cuuint64_t)n_kv};
+  const cuuint64_t ks[3] = {(cuuint64_t)k_stride * 2, 128, kD * 2}, vs[3] = {(cuuint64_t)v_stride * 2, 128, kD * 2};
+  const cuuint32_t kb[4] = {64, 128, 2, 1};
+  if (!encode_tiled() || !make_map(&c.mk, dtype, k, 4, kd, ks, kb) || !make_map(&c.mv, dtype, v, 4, kd, vs, kb))
+    return set_error(KVR_EINVAL, "kvr_prompt_attn: k or v has a layout TMA cannot read");
+  return chunk_launch("kvr_prompt_attn", c, dtype, false, stream);
 }

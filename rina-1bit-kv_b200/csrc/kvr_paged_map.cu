@@ -87,7 +87,7 @@ __device__ __forceinline__ PlanPiece plan_item(const PlanArgs &a, const PlanRequ
   const int per = 2 * plan_tpt(a.n_q, a.n_kv);
   PlanPiece p;
   p.q_start = r.q0 + i * per;
-  p.n_tok = min(per, r.q_len - i * per);
+  p.n_tok = max(0, min(per, r.q_len - i * per));
   p.kv_len = r.kv_len;
   p.k_start = r.k_start;
   p.part = -1;
@@ -100,17 +100,41 @@ __device__ __forceinline__ PlanPiece plan_item(const PlanArgs &a, const PlanRequ
 }
 
 constexpr int kPlanBins = 1024;
+constexpr int kPlanCands = 32;
+constexpr int kPlanCutItems = 16384;
 
 struct PlanShared {
   int first[kPlanMaxBatch + 2];  // exclusive sum of the requests' items
   int hist[kPlanBins];
   int64_t warp_sums[32];
+  unsigned long long work;       // K/V tiles of all items, one head
   int longest;
+  int count[kPlanCands], rows[kPlanCands];  // pieces and partial rows with each candidate length
+  int piece_len, n_splits, n_rows;
 };
 
+// Candidate lengths of the longest piece: the longest item in k parts.
+__device__ __constant__ short kPlanParts[kPlanCands] = {1,  2,  3,  4,  5,  6,  7,  8,  9,  10, 11, 12, 14, 16, 18, 20,
+                                                        22, 24, 28, 32, 36, 42, 48, 56, 64, 74, 84, 96, 112, 128, 148, 296};
+
+// Estimated time, in K/V tiles, with `count` pieces of at most `len` tiles per
+// head and `rows` partial rows: a piece costs about one tile to fill and drain,
+// a partial tile of 256 rows about two more to write and join, joining at all
+// about three (a second launch).  Pieces beyond a full round of the SMs leave
+// the last round partly empty; the more unequal the pieces are, the better the
+// short ones fill it, which the fourth power of mean / longest stands for.
+__device__ __forceinline__ float plan_estimate(float work, int count, int rows, int len, int n_kv) {
+  const float pieces = (float)count * n_kv, top = len + 1.0f;
+  const float total = (work + count + rows * (2.0f / 256.0f)) * n_kv;
+  const float joined = rows ? 3.0f : 0.0f;
+  if (pieces <= kPlanCtas) return top + joined + (rows ? 2.0f * fminf(1.0f, rows / (256.0f * count)) : 0.0f);
+  const float rounds = pieces / kPlanCtas, mean = total / pieces, u = fminf(1.0f, mean / top);
+  return joined + fmaxf(top, total / kPlanCtas + (ceilf(rounds) - rounds) * mean * u * u * u * u);
+}
+
 __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
-  const int tid = threadIdx.x, nt = blockDim.x;
-  const int per = 2 * plan_tpt(a.n_q, a.n_kv);
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
+  const int g = a.n_q / a.n_kv, per = 2 * plan_tpt(a.n_q, a.n_kv);
   const int nb = a.batch + 1;
   // requests -> first item of each (a contiguous run of requests per thread)
   const int each = (nb + nt - 1) / nt;
@@ -130,31 +154,88 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
   const int n = (int)min(total, (int64_t)a.max_items);
   const int dropped = total > n ? 1 : 0;
   for (int i = tid; i < kPlanBins; i += nt) s.hist[i] = 0;
-  if (tid == 0) s.longest = 0;
+  if (tid < kPlanCands) s.count[tid] = s.rows[tid] = 0;
+  if (tid == 0) {
+    s.longest = s.n_splits = s.n_rows = 0;
+    s.work = 0;
+  }
   __syncthreads();
-  // longest first: counting sort by length, `shift` keeps the lengths inside the bins
   for (int i = tid; i < n; i += nt) {
     const int b = last_not_above(s.first, nb, i);
     const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
     atomicMax(&s.longest, p.kt1 - p.kt0);
+    atomicAdd(&s.work, (unsigned long long)(p.kt1 - p.kt0));
   }
   __syncthreads();
+  const int longest = s.longest;
+  // (with more items than this the rounds even out by themselves)
+  const bool may_cut = n <= kPlanCutItems;
+  for (int i0 = 0; may_cut && i0 < n; i0 += nt) {
+    const int i = i0 + tid;
+    int len = 0, rows = 0;
+    if (i < n) {
+      const int b = last_not_above(s.first, nb, i);
+      const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+      len = p.kt1 - p.kt0;
+      rows = p.n_tok * g;
+    }
+    for (int c = 0; c < kPlanCands; ++c) {
+      const int top = max(1, (longest + kPlanParts[c] - 1) / kPlanParts[c]);
+      const int np = i < n ? max(1, (len + top - 1) / top) : 0;
+      // saturated: a candidate with that many pieces or rows is refused below
+      const int cnt = (int)__reduce_add_sync(0xffffffffu, (unsigned)min(np, 1 << 16));
+      const int r = (int)__reduce_add_sync(0xffffffffu, (unsigned)(np > 1 ? min(np, 1 << 10) * rows : 0));
+      if (lane == 0) {
+        atomicAdd(&s.count[c], cnt);
+        if (r) atomicAdd(&s.rows[c], min(r, 1 << 18));
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < 32) {
+    const int c = lane, top = max(1, (longest + kPlanParts[c] - 1) / kPlanParts[c]);
+    float t = INFINITY;
+    if (c == 0 || (may_cut && s.count[c] - n <= kPlanExtra && (int64_t)s.rows[c] * a.n_kv <= kPartRows))
+      t = plan_estimate((float)s.work, s.count[c], s.rows[c], top, a.n_kv);
+    float best = t;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    const unsigned who = __ballot_sync(0xffffffffu, t == best);
+    if (lane == __ffs(who) - 1) s.piece_len = top;
+  }
+  __syncthreads();
+  // longest first: counting sort by length, `shift` keeps the lengths inside the bins
+  const int top = s.piece_len;
   int shift = 0;
-  while ((s.longest >> shift) >= kPlanBins) ++shift;
+  while ((top >> shift) >= kPlanBins) ++shift;
   for (int i = tid; i < n; i += nt) {
     const int b = last_not_above(s.first, nb, i);
     const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
-    atomicAdd(&s.hist[kPlanBins - 1 - ((p.kt1 - p.kt0) >> shift)], 1);
+    const int len = p.kt1 - p.kt0, np = max(1, (len + top - 1) / top);
+    atomicAdd(&s.hist[kPlanBins - 1 - (((len + np - 1) / np) >> shift)], np);
   }
   __syncthreads();
-  const int start = (int)block_exclusive(s.hist[tid], s.warp_sums, total);
-  s.hist[tid] = start;
+  const int64_t start = block_exclusive(s.hist[tid], s.warp_sums, total);
+  s.hist[tid] = (int)start;
   __syncthreads();
   for (int i = tid; i < n; i += nt) {
     const int b = last_not_above(s.first, nb, i);
-    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
-    a.pieces[atomicAdd(&s.hist[kPlanBins - 1 - ((p.kt1 - p.kt0) >> shift)], 1)] = p;
+    PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+    const int len = p.kt1 - p.kt0, np = max(1, (len + top - 1) / top), kt0 = p.kt0;
+    const int to = atomicAdd(&s.hist[kPlanBins - 1 - (((len + np - 1) / np) >> shift)], np);
+    int part = -1;
+    if (np > 1) {
+      part = atomicAdd(&s.n_rows, np * p.n_tok * g);
+      a.splits[atomicAdd(&s.n_splits, 1)] = PlanSplit{p.q_start, p.n_tok, part, np};
+    }
+    for (int k = 0; k < np; ++k) {
+      p.kt0 = kt0 + (int)((int64_t)len * k / np);
+      p.kt1 = kt0 + (int)((int64_t)len * (k + 1) / np);
+      p.part = part < 0 ? -1 : part + k * p.n_tok * g;
+      a.pieces[to + k] = p;
+    }
   }
+  __syncthreads();
   if (tid == 0) {
     PlanHeader &h = *a.hdr;
     h.magic = kPlanMagic;
@@ -164,7 +245,9 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
     h.n_kv = a.n_kv;
     h.causal = a.causal;
     h.window = a.window;
-    h.n_pieces = n;
+    h.n_pieces = (int)total;
+    h.n_splits = s.n_splits;
+    h.part_rows = s.n_rows;
     h.dropped = dropped;
   }
 }
@@ -311,6 +394,7 @@ int plan_check(const char *fn, PlanArgs &a, int64_t n_tokens, int64_t window, vo
   a.hdr = reinterpret_cast<PlanHeader *>(plan);
   a.pieces = reinterpret_cast<PlanPiece *>(a.hdr + 1);
   a.max_items = (int)plan_max_items(n_tokens, a.batch, a.n_q, a.n_kv);
+  a.splits = const_cast<PlanSplit *>(plan_splits(a.hdr, n_tokens, a.batch, a.n_q, a.n_kv));
   return KVR_OK;
 }
 
@@ -320,7 +404,8 @@ using namespace kvr;
 
 extern "C" size_t kvr_attn_plan_bytes(int64_t n_tokens, int batch, int n_q, int n_kv) {
   if (n_tokens < 0 || batch < 1 || n_kv < 1 || n_q < n_kv || n_q / n_kv > kPlanRows) return 0;
-  return sizeof(PlanHeader) + (size_t)plan_max_items(n_tokens, batch, n_q, n_kv) * sizeof(PlanPiece);
+  return sizeof(PlanHeader) + (size_t)(plan_max_items(n_tokens, batch, n_q, n_kv) + kPlanExtra) * sizeof(PlanPiece) +
+         kPlanExtra * sizeof(PlanSplit);
 }
 
 extern "C" int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const int32_t *cu_k, int batch,
@@ -329,7 +414,7 @@ extern "C" int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const i
   clear_error();
   KVR_REQUIRE(cu_q, "kvr_attn_plan: null pointer");
   KVR_REQUIRE(!(kv_len && cu_k), "kvr_attn_plan: give kv_len (pages) or cu_k (packed keys), not both");
-  PlanArgs a{cu_q, kv_len, cu_k, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, 0};
+  PlanArgs a{cu_q, kv_len, cu_k, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, nullptr, 0};
   const int rc = plan_check("kvr_attn_plan", a, n_tokens, window, plan, plan_bytes);
   if (rc) return rc;
   attn_plan_kernel<<<1, kPlanThreads, 0, as_cuda(stream)>>>(a);
@@ -354,7 +439,7 @@ extern "C" int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int
   KVR_REQUIRE(n_free != n_free_out, "kvr_paged_map: n_free_out must not be n_free");
   MapArgs m{};
   if (plan) {
-    m.plan = PlanArgs{cu_q, kv_len, nullptr, batch, 0, n_q, n_kv, 1, 0, nullptr, nullptr, 0};
+    m.plan = PlanArgs{cu_q, kv_len, nullptr, batch, 0, n_q, n_kv, 1, 0, nullptr, nullptr, nullptr, 0};
     const int rc = plan_check("kvr_paged_map", m.plan, n_tokens, window, plan, plan_bytes);
     if (rc) return rc;
     m.with_plan = 1;
