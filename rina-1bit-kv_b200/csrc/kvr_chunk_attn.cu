@@ -13,16 +13,27 @@
 //            into a ring of five 32 KB stages; a paged tile is a box per page
 //            (or per gcd(page, 128) rows), a missing page an out-of-range box,
 //            which the TMA fills with zeros;
-//   warp 8   one lane issues tcgen05.mma: S_t = Q_t K^T (128 x 128 x 128,
-//            operands in shared memory), later O_t += P_t V with P_t in tensor
-//            memory and V read column-wise from shared memory;
-//   warps 0-3 and 4-7   a warpgroup per query tile, a row per thread: S_t
-//            from tensor memory, mask, maximum, exp2, sum; P_t, rounded to the
-//            tensors' 16-bit type, goes back over S_t.
-// While one tile's rows are in their softmax the tensor core works for the
-// other tile; S of the next K/V tile follows P V in the issue order, which is
-// also what makes the reuse of S_t's columns for P_t safe: MMAs of one thread
-// execute in order.  Tensor memory: S_0, S_1, O_0, O_1, 128 columns each.
+//   warp 8   one lane issues tcgen05.mma: S = Q_t K^T (128 x 128 x 128,
+//            operands in shared memory);
+//   warp 10  likewise O_t += P_t V, P_t in tensor memory, V read column-wise
+//            from shared memory; a warp of its own, so that neither kind waits
+//            in the other's issue order;
+//   warps 0-3 and 4-7   a warpgroup per query tile, a row per thread: S from
+//            tensor memory into registers, mask, maximum, exp2, sum; the
+//            weights P_t, rounded to the tensors' 16-bit type, back to tensor
+//            memory.
+// Tensor memory: S, P_0 | P_1 (64 columns each), O_0, O_1, 128 columns each.
+// One S serves both tiles: a warpgroup copies it to registers at once and
+// frees it, so the tensor core computes the next S while the weights of this
+// one are formed, and each tile's chain is its softmax alone, not softmax + two
+// MMAs (an S per tile with P over it, and S of the next keys after P V:
+// 2.20 ms instead of 1.79 for a prompt of 16384, 32/8 heads).
+//
+// The exponentials bind next: 16 a cycle from the special function unit against
+// 2 x 128 x 128 per 2048 cycles of MMA.  kEmul of 32 go to the FMA pipe
+// instead: x = n + r with |r| <= 1/2 by rounding, 2^r by a degree-4 polynomial
+// (minimax in relative error, 2.6e-6, fitted by iteratively reweighted least
+// squares), n added to the exponent.
 //
 // The output accumulator is rescaled only when a row's maximum has grown by
 // more than 2^kLazy since its last rescale (the weights stay below 2^(kLazy +
@@ -48,10 +59,11 @@ constexpr uint32_t kCaTile = 128 * kD * 2;      // 32 KB: 128 rows of K, V or Q
 constexpr uint32_t kCaHalf = kCaTile / 2;       // 64 channels of them
 constexpr uint32_t kCaOffKv = 2 * kCaTile;
 constexpr uint32_t kCaOffBar = kCaOffKv + kCaStages * kCaTile;
-constexpr int kCaBars = 2 * kCaStages + 11;
+constexpr int kCaBars = 2 * kCaStages + 15;
 constexpr uint32_t kCaSmem = kCaOffBar + kCaBars * 8 + 16;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr float kLazy = 6.0f, kShift = 4.0f;
+constexpr int kEmul = 0;         // of 32 exponentials on the FMA pipe (a multiple of 2)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct ChunkArgs {
@@ -72,17 +84,16 @@ struct ChunkArgs {
 
 // ------------------------------------------------------- tcgen05 and TMA ----
 
-// K-major operand, 128-byte swizzle: 8-row atoms of 1 KB, 1 KB apart.
-__device__ __forceinline__ uint64_t ca_desc_k(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// V read as the N x K operand with N (channels) contiguous, 128-byte swizzle:
-// atoms of 64 channels x 8 keys; 16 KB to the other 64 channels, 1 KB to the next 8 keys.
-__device__ __forceinline__ uint64_t ca_desc_mn(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(kCaHalf >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory matrix descriptors with 128-byte swizzle, as a low word to
+// which an address step >> 4 can be added (addresses stay below 2^18) and a
+// constant high word.
+// K-major (Q, K): 8-row atoms of 1 KB, 1 KB apart.
+// N x K with N contiguous (V, N = channels): atoms of 64 channels x 8 keys; 16
+// KB to the other 64 channels (low word), 1 KB to the next 8 keys.
+constexpr uint32_t kCaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t ca_desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t ca_desc_mn(uint32_t saddr) { return (saddr >> 4) | ((kCaHalf >> 4) << 16); }
+__device__ __forceinline__ uint64_t ca_desc(uint32_t lo) { return ((uint64_t)kCaDescHi << 32) | lo; }
 // kind::f16, fp32 accumulator, M 128, N 128.
 template <int DT>
 __host__ __device__ constexpr uint32_t ca_idesc(bool b_mn) {
@@ -104,9 +115,18 @@ __device__ __forceinline__ void ca_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void ca_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// One lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool ca_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+// A value that is the same in all lanes, in a form the compiler knows to be:
+// MMA descriptors live in uniform registers, and moving each one there from
+// per-lane registers made an MMA cost 95 to 160 cycles to issue instead of 64.
+__device__ __forceinline__ uint32_t ca_uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void ca_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void ca_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ca_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -122,6 +142,15 @@ __device__ __forceinline__ void ca_ld32(uint32_t taddr, float *f) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ca_ld16(uint32_t taddr, float *f) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 __device__ __forceinline__ void ca_st16(uint32_t taddr, const uint32_t *r) {
@@ -187,6 +216,43 @@ __device__ __forceinline__ float ca_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float ca_max3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+// Pairs of floats for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t ca_pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float ca_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float ca_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t ca_fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t ca_add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t ca_both(float x) { return ca_pair(x, x); }
+__device__ __forceinline__ uint64_t ca_exp2_sfu(uint64_t x) { return ca_pair(ca_exp2(ca_lo(x)), ca_exp2(ca_hi(x))); }
+// 2^x for x <= kLazy + kShift on the FMA pipe; below 2^-126 it ends at 2^-126.
+__device__ __forceinline__ uint64_t ca_exp2_fma(uint64_t x) {
+  x = ca_pair(fmaxf(ca_lo(x), -126.0f), fmaxf(ca_hi(x), -126.0f));
+  const uint64_t n = ca_add2(x, ca_both(12582912.0f));  // 1.5 * 2^23: the integer part lands in the low bits
+  const uint64_t r = ca_fma2(ca_add2(n, ca_both(-12582912.0f)), ca_both(-1.0f), x);
+  uint64_t p = ca_fma2(r, ca_both(0.009570102207362652f), ca_both(0.05591785907745361f));
+  p = ca_fma2(p, r, ca_both(0.240247443318367f));
+  p = ca_fma2(p, r, ca_both(0.6931217908859253f));
+  p = ca_fma2(p, r, ca_both(0.9999992847442627f));
+  return ca_pair(__uint_as_float(__float_as_uint(ca_lo(p)) + (__float_as_uint(ca_lo(n)) << 23)),
+                 __uint_as_float(__float_as_uint(ca_hi(p)) + (__float_as_uint(ca_hi(n)) << 23)));
+}
 template <int DT>
 __device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
   uint32_t r;
@@ -206,9 +272,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   uint64_t *q_empty = q_full + 2;
   uint64_t *s_full = q_empty + 2;
   uint64_t *p_full = s_full + 2;
-  uint64_t *o_full = p_full + 2;
-  uint64_t *drained = o_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+  uint64_t *pv_done = p_full + 4;  // p_full: two halves per tile
+  uint64_t *s_free = pv_done + 2;
+  uint64_t *drained = s_free + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 2);
   volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -227,10 +294,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&o_full[t], 1);
+      mbar_init(&p_full[2 * t], 4);
+      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&drained[t], 1);
+      mbar_init(&pv_done[t], 1);
     }
-    mbar_init(drained, 1);
+    mbar_init(s_free, 4);
   }
   ca_fence_before();
   __syncthreads();
@@ -250,7 +319,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   // registers: 384 threads x 168 at launch = (208 + 208 + 88) x 128
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp >= 10) {
+  if (warp == 11) {
     __syncthreads();
   } else if (warp == 9) {
     // ---- copies
@@ -326,103 +395,89 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           ++it;
     }
   } else {
-    // ---- MMAs
+    // ---- MMAs: warp 8 the products S, warp 10 the products P V
     const uint32_t q_base = smem_u32(sm), kv_base = q_base + kCaOffKv;
-    constexpr uint32_t kQk = ca_idesc<DT>(false), kPv = ca_idesc<DT>(true);
-    int j = 0, qn[2] = {0, 0}, pn[2] = {0, 0};  // ring stages, Q tiles and P tiles consumed so far
-    CaPiece c, nx;
-    int r = 0;
+    const bool scores = warp == 8;
+    const uint32_t tmem_u = ca_uniform(tmem);
+    int j = scores ? 0 : 1;  // ring stage: K and V take turns
+    int seen[2] = {0, 0};    // warp 8: Q tiles, warp 10: P tiles consumed so far
+    int si = 0;
     bool ok = true;
-    auto next_piece = [&](CaPiece &o) {  // the next piece that has K/V tiles
-      while (ca_piece(a, total, per, r, o)) {
-        ++r;
-        if (o.n > 0) return true;
-      }
-      return false;
-    };
-    auto wait_stage = [&](int k) { return ca_wait(&kv_full[k % kCaStages], (unsigned)((k / kCaStages) & 1), abort_s); };
-    // S_t of K stage k; `fresh`: the piece's first use of its Q tile, `last`: its last
-    auto issue_s = [&](int t, int k, bool fresh, bool last) {
-      if (fresh) {
-        if (!ca_wait(&q_full[t], (unsigned)(qn[t] & 1), abort_s)) return false;
-        ++qn[t];
-      }
-      ca_fence_after();
-      if (lane == 0) {
-        const uint32_t qa = q_base + t * kCaTile, kb = kv_base + (k % kCaStages) * kCaTile;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const uint32_t o = (s >> 2) * kCaHalf + (s & 3) * 32;
-          ca_mma_ss(tmem + t * 128, ca_desc_k(qa + o), ca_desc_k(kb + o), kQk, s > 0);
-        }
-        ca_commit(&s_full[t]);
-        if (last) ca_commit(&q_empty[t]);
-      }
-      return true;
-    };
-    auto issue_pv = [&](int t, int k, bool first, bool last) {
-      if (!ca_wait(&p_full[t], (unsigned)(pn[t] & 1), abort_s)) return false;
-      ++pn[t];
-      ca_fence_after();
-      if (lane == 0) {
-        const uint32_t vb = kv_base + (k % kCaStages) * kCaTile;
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          ca_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, ca_desc_mn(vb + s * 2048), kPv, !(first && s == 0));
-        if (last) ca_commit(&o_full[t]);
-      }
-      return true;
-    };
-    bool have = next_piece(c);
-    if (have) {
-      ok = wait_stage(j) && issue_s(0, j, true, c.n == 1) && (!c.two || issue_s(1, j, true, c.n == 1));
-      if (ok && lane == 0) ca_commit(&kv_empty[j % kCaStages]);
-    }
-    while (ok && have) {
-      bool more = false;
+    CaPiece c;
+    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+      const int tiles = c.two ? 2 : 1;
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
-      for (int i = 0; ok && i < c.n; ++i) {
-        const int v = j + 1, kn = j + 2;
-        const bool tail = i + 1 == c.n;
-        if (tail) more = next_piece(nx);
-        const bool s_next = !tail || more;
-        const bool n_two = tail ? nx.two : c.two;
-        const bool n_last = tail ? nx.n == 1 : i + 2 == c.n;
-        ok = wait_stage(v);
+      for (int i = 0; ok && i < c.n; ++i, j += 2) {
+        const int s = j % kCaStages;
+        ok = ca_wait(&kv_full[s], (unsigned)((j / kCaStages) & 1), abort_s);
         if (!ok) break;
-        const int key0 = (c.p.kt0 + i) * 128, hi = min(128, c.p.kv_len - key0), lo = min(128, max(0, before - key0));
-        if (hi < 128 || lo > 0) {
-          unsigned char *vs = sm + kCaOffKv + (v % kCaStages) * kCaTile;
-          for (int e = lane; e < 128 * 16; e += 32) {
-            const int row = e >> 4;
-            if (row < lo || row >= hi)
-              *reinterpret_cast<uint4 *>(vs + (e & 8 ? kCaHalf : 0) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+        if (scores) {
+          for (int t = 0; ok && t < tiles; ++t) {
+            if (i == 0) ok = ca_wait(&q_full[t], (unsigned)(seen[t]++ & 1), abort_s);
+            if (ok && si > 0) ok = ca_wait(s_free, (unsigned)((si - 1) & 1), abort_s);
+            if (!ok) break;
+            ++si;
+            ca_fence_after();
+            const uint32_t qa = ca_uniform(ca_desc_k(q_base + t * kCaTile));
+            const uint32_t kb = ca_uniform(ca_desc_k(kv_base + s * kCaTile));
+            const uint32_t full = ca_uniform(smem_u32(&s_full[t]));
+            if (ca_elect()) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t o = ((k >> 2) * kCaHalf + (k & 3) * 32) >> 4;
+                ca_mma_ss(tmem_u, ca_desc(qa + o), ca_desc(kb + o), ca_idesc<DT>(false), k > 0);
+              }
+              ca_commit(full);
+              if (i + 1 == c.n) ca_commit(smem_u32(&q_empty[t]));
+            }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
+        } else {
+          const int key0 = (c.p.kt0 + i) * 128, hi = min(128, c.p.kv_len - key0), lo = min(128, max(0, before - key0));
+          if (hi < 128 || lo > 0) {
+            unsigned char *vs = sm + kCaOffKv + s * kCaTile;
+            for (int e = lane; e < 128 * 16; e += 32) {
+              const int row = e >> 4;
+              if (row < lo || row >= hi)
+                *reinterpret_cast<uint4 *>(vs + (e & 8 ? kCaHalf : 0) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          for (int t = 0; ok && t < tiles; ++t) {
+            const uint32_t vb = ca_uniform(ca_desc_mn(kv_base + s * kCaTile)), add = ca_uniform(i > 0 ? 1u : 0u);
+            const uint32_t pa = ca_uniform(tmem + 128 + t * 64), oa = ca_uniform(tmem + 256 + t * 128);
+            const uint32_t done = ca_uniform(smem_u32(&pv_done[t]));
+            // in two halves of the keys: the first weights are multiplied while the others are formed
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ca_wait(&p_full[2 * t + half], (unsigned)(seen[t] & 1), abort_s);
+              if (!ok) break;
+              ca_fence_after();
+              if (ca_elect()) {
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                  ca_mma_ts(oa, pa + k * 8, ca_desc(vb + k * (2048 >> 4)), ca_idesc<DT>(true), k > 0 ? 1u : add);
+                if (half) ca_commit(done);
+              }
+            }
+            ++seen[t];
+          }
         }
-        ok = issue_pv(0, v, i == 0, tail);
-        if (ok && s_next) ok = wait_stage(kn) && issue_s(0, kn, tail, n_last);
-        if (ok && c.two) ok = issue_pv(1, v, i == 0, tail);
-        if (ok && lane == 0) ca_commit(&kv_empty[v % kCaStages]);
-        if (ok && s_next) {
-          if (n_two) ok = issue_s(1, kn, tail, n_last);
-          if (ok && lane == 0) ca_commit(&kv_empty[kn % kCaStages]);
-        }
-        j += 2;
+        __syncwarp();
+        if (ok && ca_elect()) ca_commit(smem_u32(&kv_empty[s]));
       }
-      have = more;
-      c = nx;
     }
     if (!__all_sync(~0u, ok)) {
       if (lane == 0) {
         if (!*abort_s) atomicOr(a.err, 1u);
         *abort_s = 1;
-        ca_commit(drained);  // MMAs in flight must finish before the tensor memory is freed
       }
       __syncwarp();
-      for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(drained, 0);) ++it;
+      // MMAs in flight must finish before the tensor memory is freed
+      uint64_t *bar = &drained[scores ? 0 : 1];
+      if (ca_elect()) ca_commit(smem_u32(bar));
+      for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(bar, 0);) ++it;
     }
     __syncthreads();
   }
@@ -430,11 +485,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     // ---- softmax: warpgroup t, a row per thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane;
-    const uint32_t s_addr = tmem + ((uint32_t)wrow << 16) + t * 128, o_addr = s_addr + 256;
+    const uint32_t s_addr = tmem + ((uint32_t)wrow << 16), p_addr = s_addr + 128 + t * 64, o_addr = s_addr + 256 + t * 128;
     const int tok_in = row / g;               // token of the row within its tile
     const int tok = t * tpt + tok_in;         // ... within the item
     const int tok_a = t * tpt + wrow / g, tok_b = t * tpt + min(tpt - 1, (wrow + 31) / g);
-    int sn = 0, on = 0;                       // S tiles and outputs consumed so far
+    int sn = 0, on = 0;                       // S tiles and P V products seen so far
+    const uint64_t to2 = ca_pair(a.to_log2, a.to_log2);
     bool ok = true;
     CaPiece c;
     for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
@@ -455,71 +511,119 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) ca_ld32(s_addr + k * 32, s + k * 32);
           ca_wait_ld();
+          ca_fence_before();
+          __syncwarp();
+          if (lane == 0) ca_arrive(s_free);
           const int k0 = (c.p.kt0 + i) * 128;
           if (k0 + 128 > end_a || k0 < begin_b) {
             const int e = end - k0, b = begin - k0;
 #pragma unroll
             for (int k = 0; k < 128; ++k) s[k] = k < e && k >= b ? s[k] : -INFINITY;
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          float mx[8];
 #pragma unroll
-          for (int k = 4; k < 128; k += 8) {
+          for (int u = 0; u < 8; ++u) mx[u] = ca_max3(s[u], s[8 + u], s[16 + u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float x = s[k + u], y = k + 4 + u < 128 ? s[k + 4 + u] : -INFINITY;
-              mx[u] = fmaxf(mx[u], fmaxf(x, y));
-            }
+          for (int k = 24; k < 120; k += 16) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) mx[u] = ca_max3(mx[u], s[k + u], s[k + 8 + u]);
           }
-          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = ca_max3(mx[u], s[120 + u], s[124 + u]);
+          mx[0] = ca_max3(mx[0], mx[4], mx[5]);
+          mx[1] = ca_max3(mx[1], mx[6], mx[7]);
+          // a NaN score makes the row's maximum NaN and with it the whole row; so does one of +inf
+          float m_new = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], m);
+          if (m_new == INFINITY) m_new = NAN;
           // the first tile sets the maximum; later it moves only in steps above 2^kLazy
           const bool grow = i == 0 || !((m_new - m) * a.to_log2 <= kLazy);
+          bool before = i > 0;  // P V of the tile before still has to be waited for
           if (i > 0 && __any_sync(~0u, grow && m_new != m)) {
+            ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+            if (!ok) break;
+            ++on;
+            before = false;
+            ca_fence_after();
             const float f = grow ? (m == -INFINITY ? 0.0f : ca_exp2((m - m_new) * a.to_log2)) : 1.0f;
             l *= f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float o[32];
-              ca_ld32(o_addr + k * 32, o);
+            for (int k = 0; k < 8; ++k) {
+              float o[16];
+              ca_ld16(o_addr + k * 16, o);
               ca_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = f == 0.0f ? 0.0f : o[e] * f;
-              ca_st16(o_addr + k * 32, reinterpret_cast<const uint32_t *>(o));
-              ca_st16(o_addr + k * 32 + 16, reinterpret_cast<const uint32_t *>(o + 16));
+              for (int e = 0; e < 16; ++e) o[e] = f == 0.0f ? 0.0f : o[e] * f;
+              ca_st16(o_addr + k * 16, reinterpret_cast<const uint32_t *>(o));
             }
           }
           if (grow) {
             m = m_new;
             mc = m == -INFINITY ? 0.0f : m * a.to_log2;
           }
-          const float add = kShift - mc;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint64_t add2 = ca_pair(kShift - mc, kShift - mc);
+          uint64_t sum = 0;
+          uint32_t pk[64];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            uint32_t pk[16];
+            uint64_t y[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = ca_exp2(fmaf(s[k * 32 + 2 * e], a.to_log2, add));
-              const float y = ca_exp2(fmaf(s[k * 32 + 2 * e + 1], a.to_log2, add));
-              sum[e & 3] += x + y;
-              pk[e] = ca_pack<DT>(x, y);
+            for (int e = 0; e < 16; ++e) y[e] = ca_fma2(ca_pair(s[k * 32 + 2 * e], s[k * 32 + 2 * e + 1]), to2, add2);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              y[e] = kEmul && e % (32 / max(kEmul, 1)) == 32 / max(kEmul, 1) - 1 ? ca_exp2_fma(y[e]) : ca_exp2_sfu(y[e]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[k * 16 + e] = ca_pack<DT>(ca_lo(y[e]), ca_hi(y[e]));
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) {
+#pragma unroll
+              for (int e = 0; e < w; ++e) y[e] = ca_add2(y[e], y[e + w]);
             }
-            ca_st16(s_addr + k * 16, pk);
+            sum = ca_add2(sum, y[0]);
+            if (k == 1) {
+              if (before) {  // P is free once P V of the tile before has read it
+                ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+                if (!ok) break;
+                ++on;
+                ca_fence_after();
+              }
+              ca_st16(p_addr, pk);
+              ca_st16(p_addr + 16, pk + 16);
+            }
+            if (k == 2) {  // the first half's stores have had chunk 2 to land
+              ca_wait_st();
+              ca_fence_before();
+              __syncwarp();
+              if (lane == 0) ca_arrive(&p_full[2 * t]);
+            }
+            if (k >= 2) ca_st16(p_addr + k * 16, pk + k * 16);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if (!ok) break;
+          l += ca_lo(sum) + ca_hi(sum);
           ca_wait_st();
           ca_fence_before();
+        } else {
+          if (lane == 0) ca_arrive(s_free);
+          if (i > 0) {
+            ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+            if (!ok) break;
+            ++on;
+          }
+          if (lane == 0) ca_arrive(&p_full[2 * t]);
         }
         __syncwarp();
-        if (lane == 0) ca_arrive(&p_full[t]);
+        if (lane == 0) ca_arrive(&p_full[2 * t + 1]);
       }
       if (!ok) break;
       // ---- the piece's rows
       if (c.n > 0) {
-        ok = __all_sync(~0u, ca_wait(&o_full[t], (unsigned)(on & 1), abort_s));
+        ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
         if (!ok) break;
         ++on;
       }
       if (!busy) continue;
+      // a row that saw a key has a weight of 2^kShift at least; without one, the sum is 0 or the
+      // smallest normal numbers that the FMA pipe's 2^x ends at
+      const bool none = l < 1.0f;
       ca_fence_after();
       const int64_t token = (int64_t)c.p.q_start + tok;
       const int hq = c.head * g + row - tok_in * g;
@@ -538,9 +642,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                   make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
-        if (live) *reinterpret_cast<float2 *>(a.part_ml + pr * 2) = make_float2(m == -INFINITY ? -INFINITY : mc - kShift, l);
+        if (live) *reinterpret_cast<float2 *>(a.part_ml + pr * 2) = make_float2(mc - kShift, none ? 0.0f : l);
       } else {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = 1.0f / l;
         uint16_t *dst = static_cast<uint16_t *>(a.out) + (token * a.n_q + hq) * kD;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -556,13 +660,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
                 const float x = o[e * 8 + 2 * u], y = o[e * 8 + 2 * u + 1];
-                w[u] = l == 0.0f ? 0u : ca_pack<DT>(x * inv, y * inv);
+                w[u] = none ? 0u : ca_pack<DT>(x * inv, y * inv);
               }
               reinterpret_cast<uint4 *>(dst + k * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
-        if (store && a.lse) a.lse[token * a.n_q + hq] = l == 0.0f ? -INFINITY : (mc - kShift + log2f(l)) * kLn2;
+        if (store && a.lse) a.lse[token * a.n_q + hq] = none ? -INFINITY : (mc - kShift + log2f(l)) * kLn2;
       }
       // the next piece's first P V overwrites O: it waits for p_full, which this warp arrives at later
       ca_fence_before();
