@@ -25,15 +25,16 @@
 // Tensor memory: S, P_0 | P_1 (64 columns each), O_0, O_1, 128 columns each.
 // One S serves both tiles: a warpgroup copies it to registers at once and
 // frees it, so the tensor core computes the next S while the weights of this
-// one are formed, and each tile's chain is its softmax alone, not softmax + two
-// MMAs (an S per tile with P over it, and S of the next keys after P V:
-// 2.20 ms instead of 1.79 for a prompt of 16384, 32/8 heads).
+// one are formed, and a tile's chain is its softmax, not softmax + two MMAs.
+// (An S per tile with P over it and S of the next keys after P V, one issuing
+// warp: 328 us for a chunk of 512 at 32256, 32/8 heads; this way 234 us.)
 //
-// The exponentials bind next: 16 a cycle from the special function unit against
-// 2 x 128 x 128 per 2048 cycles of MMA.  kEmul of 32 go to the FMA pipe
-// instead: x = n + r with |r| <= 1/2 by rounding, 2^r by a degree-4 polynomial
-// (minimax in relative error, 2.6e-6, fitted by iteratively reweighted least
-// squares), n added to the exponent.
+// What binds a long prompt: the chain S (512 cycles, with P V of the other
+// tile in between) -> warpgroup -> registers -> free -> next S, twice per 128
+// keys, about 3300 cycles against 2048 of MMA.  Tensor pipe 61 % active, special
+// function unit (16 exponentials a cycle) 61 %.  Exponentials on the FMA pipe
+// instead (a polynomial for 1/8 to 1/2 of them) lost 3 to 30 %: the instructions
+// they add lengthen the chain more than the special function unit shortens it.
 //
 // The output accumulator is rescaled only when a row's maximum has grown by
 // more than 2^kLazy since its last rescale (the weights stay below 2^(kLazy +
@@ -63,8 +64,8 @@ constexpr int kCaBars = 2 * kCaStages + 15;
 constexpr uint32_t kCaSmem = kCaOffBar + kCaBars * 8 + 16;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr float kLazy = 6.0f, kShift = 4.0f;
-constexpr int kEmul = 0;         // of 32 exponentials on the FMA pipe (a multiple of 2)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
 
 struct ChunkArgs {
   int64_t n_tokens;
@@ -181,7 +182,7 @@ __device__ __forceinline__ void ca_tma5(uint32_t dst, const CUtensorMap *m, int 
 // ---------------------------------------------------------------- waiting ----
 
 __device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile int *abort_s) {
-  if (mbar_try_wait(bar, phase)) return true;
+  if (__builtin_expect(mbar_try_wait(bar, phase), 1)) return true;
   for (uint32_t it = 0; it < kSpinLimit; ++it) {
     if (mbar_try_wait(bar, phase)) return true;
     if ((it & 255u) == 255u && *abort_s) return false;
@@ -239,20 +240,7 @@ __device__ __forceinline__ uint64_t ca_add2(uint64_t x, uint64_t y) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
-__device__ __forceinline__ uint64_t ca_both(float x) { return ca_pair(x, x); }
 __device__ __forceinline__ uint64_t ca_exp2_sfu(uint64_t x) { return ca_pair(ca_exp2(ca_lo(x)), ca_exp2(ca_hi(x))); }
-// 2^x for x <= kLazy + kShift on the FMA pipe; below 2^-126 it ends at 2^-126.
-__device__ __forceinline__ uint64_t ca_exp2_fma(uint64_t x) {
-  x = ca_pair(fmaxf(ca_lo(x), -126.0f), fmaxf(ca_hi(x), -126.0f));
-  const uint64_t n = ca_add2(x, ca_both(12582912.0f));  // 1.5 * 2^23: the integer part lands in the low bits
-  const uint64_t r = ca_fma2(ca_add2(n, ca_both(-12582912.0f)), ca_both(-1.0f), x);
-  uint64_t p = ca_fma2(r, ca_both(0.009570102207362652f), ca_both(0.05591785907745361f));
-  p = ca_fma2(p, r, ca_both(0.240247443318367f));
-  p = ca_fma2(p, r, ca_both(0.6931217908859253f));
-  p = ca_fma2(p, r, ca_both(0.9999992847442627f));
-  return ca_pair(__uint_as_float(__float_as_uint(ca_lo(p)) + (__float_as_uint(ca_lo(n)) << 23)),
-                 __uint_as_float(__float_as_uint(ca_hi(p)) + (__float_as_uint(ca_hi(n)) << 23)));
-}
 template <int DT>
 __device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
   uint32_t r;
@@ -468,17 +456,15 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         if (ok && ca_elect()) ca_commit(smem_u32(&kv_empty[s]));
       }
     }
-    if (!__all_sync(~0u, ok)) {
-      if (lane == 0) {
-        if (!*abort_s) atomicOr(a.err, 1u);
-        *abort_s = 1;
-      }
-      __syncwarp();
-      // MMAs in flight must finish before the tensor memory is freed
-      uint64_t *bar = &drained[scores ? 0 : 1];
-      if (ca_elect()) ca_commit(smem_u32(bar));
-      for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(bar, 0);) ++it;
+    if (!__all_sync(~0u, ok) && lane == 0) {
+      if (!*abort_s) atomicOr(a.err, 1u);
+      *abort_s = 1;
     }
+    // every MMA, and the arrivals that its commits owe, before the tensor memory is freed and the CTA ends
+    uint64_t *bar = &drained[scores ? 0 : 1];
+    __syncwarp();
+    if (ca_elect()) ca_commit(smem_u32(bar));
+    for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(bar, 0);) ++it;
     __syncthreads();
   }
   } else {
@@ -515,7 +501,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           __syncwarp();
           if (lane == 0) ca_arrive(s_free);
           const int k0 = (c.p.kt0 + i) * 128;
-          if (k0 + 128 > end_a || k0 < begin_b) {
+          if (__builtin_expect(k0 + 128 > end_a || k0 < begin_b, 0)) {
             const int e = end - k0, b = begin - k0;
 #pragma unroll
             for (int k = 0; k < 128; ++k) s[k] = k < e && k >= b ? s[k] : -INFINITY;
@@ -538,7 +524,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           // the first tile sets the maximum; later it moves only in steps above 2^kLazy
           const bool grow = i == 0 || !((m_new - m) * a.to_log2 <= kLazy);
           bool before = i > 0;  // P V of the tile before still has to be waited for
-          if (i > 0 && __any_sync(~0u, grow && m_new != m)) {
+          if (__builtin_expect(i > 0 && __any_sync(~0u, grow && m_new != m), 0)) {
             ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
             if (!ok) break;
             ++on;
@@ -561,25 +547,22 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             mc = m == -INFINITY ? 0.0f : m * a.to_log2;
           }
           const uint64_t add2 = ca_pair(kShift - mc, kShift - mc);
-          uint64_t sum = 0;
+          // A pair of weights per step: scale and shift kAhead pairs ahead of the exponentials, rounding
+          // and sum kBehind pairs after them, so that the special function unit is fed without a pause.
+          constexpr int kAhead = 4, kBehind = 4;
+          uint64_t x[64];
+          uint64_t sums[4] = {0, 0, 0, 0};
           uint32_t pk[64];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint64_t y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = ca_fma2(ca_pair(s[k * 32 + 2 * e], s[k * 32 + 2 * e + 1]), to2, add2);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              y[e] = kEmul && e % (32 / max(kEmul, 1)) == 32 / max(kEmul, 1) - 1 ? ca_exp2_fma(y[e]) : ca_exp2_sfu(y[e]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[k * 16 + e] = ca_pack<DT>(ca_lo(y[e]), ca_hi(y[e]));
-#pragma unroll
-            for (int w = 8; w > 0; w >>= 1) {
-#pragma unroll
-              for (int e = 0; e < w; ++e) y[e] = ca_add2(y[e], y[e + w]);
+          for (int e = -kAhead; e < 64 + kBehind; ++e) {
+            const int f = e + kAhead, b = e - kBehind;
+            if (f >= 0 && f < 64) x[f] = ca_fma2(ca_pair(s[2 * f], s[2 * f + 1]), to2, add2);
+            if (e >= 0 && e < 64) x[e] = ca_exp2_sfu(x[e]);
+            if (b >= 0) {
+              pk[b] = ca_pack<DT>(ca_lo(x[b]), ca_hi(x[b]));
+              sums[b & 3] = ca_add2(sums[b & 3], x[b]);
             }
-            sum = ca_add2(sum, y[0]);
-            if (k == 1) {
+            if (b == 31) {
               if (before) {  // P is free once P V of the tile before has read it
                 ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
                 if (!ok) break;
@@ -589,15 +572,17 @@ __global__ void __launch_bounds__(kCaThreads, 1)
               ca_st16(p_addr, pk);
               ca_st16(p_addr + 16, pk + 16);
             }
-            if (k == 2) {  // the first half's stores have had chunk 2 to land
+            if (b == 47) {  // the first half's stores have had 16 pairs to land
               ca_wait_st();
               ca_fence_before();
               __syncwarp();
               if (lane == 0) ca_arrive(&p_full[2 * t]);
+              ca_st16(p_addr + 32, pk + 32);
             }
-            if (k >= 2) ca_st16(p_addr + k * 16, pk + k * 16);
+            if (b == 63) ca_st16(p_addr + 48, pk + 48);
           }
           if (!ok) break;
+          const uint64_t sum = ca_add2(ca_add2(sums[0], sums[1]), ca_add2(sums[2], sums[3]));
           l += ca_lo(sum) + ca_hi(sum);
           ca_wait_st();
           ca_fence_before();
@@ -621,8 +606,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         ++on;
       }
       if (!busy) continue;
-      // a row that saw a key has a weight of 2^kShift at least; without one, the sum is 0 or the
-      // smallest normal numbers that the FMA pipe's 2^x ends at
+      // a row that saw a key has a weight of 2^kShift at least
       const bool none = l < 1.0f;
       ca_fence_after();
       const int64_t token = (int64_t)c.p.q_start + tok;
