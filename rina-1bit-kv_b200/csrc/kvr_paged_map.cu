@@ -101,16 +101,15 @@ __device__ __forceinline__ PlanPiece plan_item(const PlanArgs &a, const PlanRequ
 
 constexpr int kPlanBins = 1024;
 constexpr int kPlanCands = 32;
-constexpr int kPlanCutItems = 16384;
 
 struct PlanShared {
   int first[kPlanMaxBatch + 2];  // exclusive sum of the requests' items
-  int hist[kPlanBins];
+  int hist[kPlanBins];           // items of each length
+  int rows[kPlanBins];           // their query rows
+  int place[kPlanBins];          // next list entry of each piece length
   int64_t warp_sums[32];
-  unsigned long long work;       // K/V tiles of all items, one head
-  int longest;
-  int count[kPlanCands], rows[kPlanCands];  // pieces and partial rows with each candidate length
-  int piece_len, n_splits, n_rows;
+  float time[kPlanCands];        // estimate of each candidate
+  int longest_kv, longest, n_splits, n_rows;
 };
 
 // Candidate lengths of the longest piece: the longest item in k parts.
@@ -123,106 +122,124 @@ __device__ __constant__ short kPlanParts[kPlanCands] = {1,  2,  3,  4,  5,  6,  
 // about three (a second launch).  Pieces beyond a full round of the SMs leave
 // the last round partly empty; the more unequal the pieces are, the better the
 // short ones fill it, which the fourth power of mean / longest stands for.
-__device__ __forceinline__ float plan_estimate(float work, int count, int rows, int len, int n_kv) {
-  const float pieces = (float)count * n_kv, top = len + 1.0f;
+__device__ __forceinline__ float plan_estimate(float work, float count, float rows, int len, int n_kv) {
+  const float pieces = count * n_kv, top = len + 1.0f;
   const float total = (work + count + rows * (2.0f / 256.0f)) * n_kv;
-  const float joined = rows ? 3.0f : 0.0f;
-  if (pieces <= kPlanCtas) return top + joined + (rows ? 2.0f * fminf(1.0f, rows / (256.0f * count)) : 0.0f);
+  const float joined = rows > 0.0f ? 3.0f : 0.0f;
+  if (pieces <= kPlanCtas) return top + joined + (rows > 0.0f ? 2.0f * fminf(1.0f, rows / (256.0f * count)) : 0.0f);
   const float rounds = pieces / kPlanCtas, mean = total / pieces, u = fminf(1.0f, mean / top);
   return joined + fmaxf(top, total / kPlanCtas + (ceilf(rounds) - rounds) * mean * u * u * u * u);
 }
 
+// One CTA.  Two passes over the items (their lengths; their places), an item
+// per thread; in between a warp per candidate length goes over the histogram of
+// lengths, not over the items.  Atomics on shared counters are made once per
+// warp and value: 700 items of one length on one counter cost more than all of
+// the rest (map of 48 prompts: 50 us with an atomic per item and candidate
+// sums over the items, PLACEHOLDER us this way).
 __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.n_q / a.n_kv, per = 2 * plan_tpt(a.n_q, a.n_kv);
   const int nb = a.batch + 1;
+  s.hist[tid] = s.rows[tid] = s.place[tid] = 0;
+  if (tid == 0) s.longest_kv = s.longest = s.n_splits = s.n_rows = 0;
   // requests -> first item of each (a contiguous run of requests per thread)
   const int each = (nb + nt - 1) / nt;
   int64_t sum = 0, total;  // 64 bits: offsets that overlap can add up to more than 2^31 items
+  int most = 0;
   for (int k = 0; k < each; ++k) {
     const int b = tid * each + k;
-    if (b < nb) sum += (plan_request(a, b).q_len + per - 1) / per;
+    if (b < nb) {
+      const PlanRequest r = plan_request(a, b);
+      sum += (r.q_len + per - 1) / per;
+      if (r.q_len > 0) most = max(most, r.kv_len);
+    }
   }
   int64_t at = block_exclusive(sum, s.warp_sums, total);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) atomicMax(&s.longest_kv, most);
   for (int k = 0; k < each; ++k) {
     const int b = tid * each + k;
     if (b < nb) {
       s.first[b] = (int)min(at, (int64_t)INT_MAX);
-      at += (plan_request(a, b).q_len + per - 1) / per;
+      if (each > 1) at += (plan_request(a, b).q_len + per - 1) / per;
     }
   }
+  __syncthreads();
   const int n = (int)min(total, (int64_t)a.max_items);
   const int dropped = total > n ? 1 : 0;
-  for (int i = tid; i < kPlanBins; i += nt) s.hist[i] = 0;
-  if (tid < kPlanCands) s.count[tid] = s.rows[tid] = 0;
-  if (tid == 0) {
-    s.longest = s.n_splits = s.n_rows = 0;
-    s.work = 0;
-  }
-  __syncthreads();
-  for (int i = tid; i < n; i += nt) {
+  int shift = 0;  // lengths of 2^shift share a bin and count as the longest of them
+  while (((s.longest_kv / kPlanKeys + 1) >> shift) >= kPlanBins) ++shift;
+  auto item = [&](int i) {
     const int b = last_not_above(s.first, nb, i);
-    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
-    atomicMax(&s.longest, p.kt1 - p.kt0);
-    atomicAdd(&s.work, (unsigned long long)(p.kt1 - p.kt0));
-  }
-  __syncthreads();
-  const int longest = s.longest;
-  // (with more items than this the rounds even out by themselves)
-  const bool may_cut = n <= kPlanCutItems;
-  for (int i0 = 0; may_cut && i0 < n; i0 += nt) {
+    return plan_item(a, plan_request(a, b), i - s.first[b]);
+  };
+  const PlanPiece mine = tid < n ? item(tid) : PlanPiece{};
+  for (int i0 = 0; i0 < n; i0 += nt) {
     const int i = i0 + tid;
-    int len = 0, rows = 0;
+    int len = 0;
     if (i < n) {
-      const int b = last_not_above(s.first, nb, i);
-      const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
+      const PlanPiece p = i0 ? item(i) : mine;
       len = p.kt1 - p.kt0;
-      rows = p.n_tok * g;
-    }
-    for (int c = 0; c < kPlanCands; ++c) {
-      const int top = max(1, (longest + kPlanParts[c] - 1) / kPlanParts[c]);
-      const int np = i < n ? max(1, (len + top - 1) / top) : 0;
-      // saturated: a candidate with that many pieces or rows is refused below
-      const int cnt = (int)__reduce_add_sync(0xffffffffu, (unsigned)min(np, 1 << 16));
-      const int r = (int)__reduce_add_sync(0xffffffffu, (unsigned)(np > 1 ? min(np, 1 << 10) * rows : 0));
-      if (lane == 0) {
-        atomicAdd(&s.count[c], cnt);
-        if (r) atomicAdd(&s.rows[c], min(r, 1 << 18));
+      const unsigned same = __match_any_sync(__activemask(), len >> shift);
+      const int rows = (int)__reduce_add_sync(same, (unsigned)(p.n_tok * g));
+      if (lane == __ffs(same) - 1) {
+        atomicAdd(&s.hist[len >> shift], __popc(same));
+        atomicAdd(&s.rows[len >> shift], rows);
       }
     }
+    len = __reduce_max_sync(0xffffffffu, len);
+    if (lane == 0) atomicMax(&s.longest, len);
   }
   __syncthreads();
-  if (tid < 32) {
-    const int c = lane, top = max(1, (longest + kPlanParts[c] - 1) / kPlanParts[c]);
-    float t = INFINITY;
-    if (c == 0 || (may_cut && s.count[c] - n <= kPlanExtra && (int64_t)s.rows[c] * a.n_kv <= kPartRows))
-      t = plan_estimate((float)s.work, s.count[c], s.rows[c], top, a.n_kv);
-    float best = t;
+  const int longest = s.longest, low = (1 << shift) - 1;
+  {  // warp c: candidate c
+    const int top = max(1, (longest + kPlanParts[warp] - 1) / kPlanParts[warp]);
+    float work = 0.0f, count = 0.0f, rows = 0.0f;
+    for (int bin = lane; bin <= longest >> shift; bin += 32) {
+      const int items = s.hist[bin], len = shift ? (bin << shift) | low : bin;
+      if (items == 0) continue;
+      const int np = max(1, (len + top - 1) / top);
+      work += (float)items * len;
+      count += (float)items * np;
+      if (np > 1) rows += (float)s.rows[bin] * np;
+    }
+    work = warp_sum(work);
+    count = warp_sum(count);
+    rows = warp_sum(rows);
+    // a list too long for the plan or rows too many for the workspace (with a margin for the fp32 sums) are refused
+    const bool fits = warp == 0 || (count - n <= kPlanExtra - 1 && rows * a.n_kv <= kPartRows * 0.999f);
+    if (lane == 0) s.time[warp] = fits ? plan_estimate(work, count, rows, top, a.n_kv) : INFINITY;
+  }
+  __syncthreads();
+  float best = s.time[lane];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    const unsigned who = __ballot_sync(0xffffffffu, t == best);
-    if (lane == __ffs(who) - 1) s.piece_len = top;
+  for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  const int parts = kPlanParts[__ffs(__ballot_sync(0xffffffffu, s.time[lane] == best)) - 1];
+  const int top = max(1, (longest + parts - 1) / parts);
+  // longest pieces first: counting sort by the pieces' length (thread = bin of item lengths here)
+  auto pieces_of = [&](int len) { return max(1, ((shift ? len | low : len) + top - 1) / top); };
+  auto place_of = [&](int len, int np) { return kPlanBins - 1 - ((((shift ? len | low : len) + np - 1) / np) >> shift); };
+  if (s.hist[tid]) {
+    const int len = tid << shift, np = pieces_of(len);
+    atomicAdd(&s.place[place_of(len, np)], s.hist[tid] * np);
   }
   __syncthreads();
-  // longest first: counting sort by length, `shift` keeps the lengths inside the bins
-  const int top = s.piece_len;
-  int shift = 0;
-  while ((top >> shift) >= kPlanBins) ++shift;
-  for (int i = tid; i < n; i += nt) {
-    const int b = last_not_above(s.first, nb, i);
-    const PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
-    const int len = p.kt1 - p.kt0, np = max(1, (len + top - 1) / top);
-    atomicAdd(&s.hist[kPlanBins - 1 - (((len + np - 1) / np) >> shift)], np);
-  }
-  __syncthreads();
-  const int64_t start = block_exclusive(s.hist[tid], s.warp_sums, total);
-  s.hist[tid] = (int)start;
+  const int start = (int)block_exclusive(s.place[tid], s.warp_sums, total);
+  s.place[tid] = start;
   __syncthreads();
   for (int i = tid; i < n; i += nt) {
-    const int b = last_not_above(s.first, nb, i);
-    PlanPiece p = plan_item(a, plan_request(a, b), i - s.first[b]);
-    const int len = p.kt1 - p.kt0, np = max(1, (len + top - 1) / top), kt0 = p.kt0;
-    const int to = atomicAdd(&s.hist[kPlanBins - 1 - (((len + np - 1) / np) >> shift)], np);
+    PlanPiece p = i == tid ? mine : item(i);
+    const int len = p.kt1 - p.kt0, np = pieces_of(len), to_bin = place_of(len, np), kt0 = p.kt0;
+    if (np == 1 && parts == 1) {
+      const unsigned same = __match_any_sync(__activemask(), to_bin);
+      int to = 0;
+      if (lane == __ffs(same) - 1) to = atomicAdd(&s.place[to_bin], __popc(same));
+      to = __shfl_sync(same, to, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
+      a.pieces[to] = p;
+      continue;
+    }
+    const int to = atomicAdd(&s.place[to_bin], np);
     int part = -1;
     if (np > 1) {
       part = atomicAdd(&s.n_rows, np * p.n_tok * g);
@@ -251,6 +268,7 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
     h.dropped = dropped;
   }
 }
+static_assert(kPlanCands == kPlanThreads / 32, "one candidate per warp");
 static_assert(kPlanBins == kPlanThreads, "one bin per thread in the scan");
 
 __global__ void __launch_bounds__(kPlanThreads, 1) attn_plan_kernel(PlanArgs a) {
