@@ -496,7 +496,7 @@ KVR_API int kvr_paged_write(const void *q, const void *k, const void *v, int dty
  * The workspace (kvr_attn_workspace_bytes) must not be shared by calls that
  * overlap; its error word (kvr_workspace_status) reports a bounded wait that
  * gave up, or a plan that was not built for this call's shapes. */
-KVR_API size_t kvr_attn_workspace_bytes(int n_q, int n_kv);
+KVR_API size_t kvr_attn_workspace_bytes(void);
 KVR_API int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int batch, int n_q, int n_kv, int d,
                            int64_t q_stride, const void *k_pages, const void *v_pages, int64_t n_pages, int page,
                            int64_t page_stride, int64_t tok_stride, const int32_t *block_table,

@@ -57,7 +57,7 @@ struct PlanSplit {   // an item cut into pieces
   int n_pieces;
 };
 
-constexpr int kPlanExtra = 1024;                  // pieces per head beyond one per item
+constexpr int kPlanExtra = 512;                   // pieces per head beyond one per item
 constexpr int kPartRows = 2 * kPlanCtas * 2 * kPlanRows;  // partial rows the workspace holds
 
 __host__ __device__ inline int plan_tpt(int n_q, int n_kv) { return kPlanRows / (n_q / n_kv); }

@@ -768,7 +768,7 @@ static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float sca
   KVR_REQUIRE((ptrs & 15) == 0, "%s: pointers must be 16-byte aligned", fn);
   KVR_REQUIRE(plan_bytes >= kvr_attn_plan_bytes(a.n_tokens, a.batch, a.n_q, a.n_kv), "%s: plan too small", fn);
   KVR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "%s: workspace alignment", fn);
-  const size_t need = kvr_attn_workspace_bytes(a.n_q, a.n_kv);
+  const size_t need = kvr_attn_workspace_bytes();
   KVR_REQUIRE(workspace_bytes >= need, "%s: workspace %zu < %zu bytes", fn, workspace_bytes, need);
   KVR_REQUIRE(scale == scale && scale <= 3.0e38f, "%s: bad scale", fn);
   a.to_log2 = kLog2e / (scale > 0.0f ? scale : sqrtf((float)d));
@@ -829,9 +829,7 @@ static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr
 
 using namespace kvr;
 
-extern "C" size_t kvr_attn_workspace_bytes(int n_q, int n_kv) {
-  (void)n_q;
-  (void)n_kv;
+extern "C" size_t kvr_attn_workspace_bytes(void) {
   return kWsHeader + (size_t)kPartRows * (kD + 2) * sizeof(float);
 }
 

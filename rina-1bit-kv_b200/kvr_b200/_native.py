@@ -97,7 +97,7 @@ SIGNATURES = {
     "kvr_paged_map": (I, [P, P, I, I64, I, P, I64, I, P, I64, P, P, P, P, P, P, P, I, I, I64, P, SZ, P]),
     "kvr_paged_write": (I, [P, P, P, I, I64, I, I, I, I64, I64, I64, P, P, I64, I64, P, P, P, P, P, I64, I, I64, I64,
                             P]),
-    "kvr_attn_workspace_bytes": (SZ, [I, I]),
+    "kvr_attn_workspace_bytes": (SZ, []),
     "kvr_paged_attn": (I, [P, I, I64, I, I, I, I, I64, P, P, I64, I, I64, I64, P, I64, I, P, SZ, F, P, P, P, SZ, P]),
     "kvr_prompt_attn": (I, [P, P, P, I, I64, I64, I, I, I, I, I64, I64, I64, P, SZ, F, P, P, P, SZ, P]),
     "kvr_decode_attn_noalloc_max_scratch_bytes": (SZ, []),
@@ -156,7 +156,14 @@ def dtype_code(t) -> int:
         raise TypeError(f"unsupported dtype {t.dtype}") from e
 
 
+# The current stream's handle without building a Stream object (0.4 us in place
+# of 3.3 us on every operator call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream() -> int:
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

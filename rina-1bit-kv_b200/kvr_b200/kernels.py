@@ -533,27 +533,29 @@ def sd1_prefill_scores(store: Sd1Store, q):
 def _tokens(x, name):
     """(n, heads, 128) with contiguous heads and 16-byte aligned rows, and its
     token stride in elements; views that are not laid out so are copied."""
-    if x.dim() != 3 or x.shape[2] != D:
-        raise ValueError(f"{name} must be (tokens, heads, {D}), got {tuple(x.shape)}")
-    n, heads, _ = x.shape
-    ok = (x.stride(2) == 1 and (heads == 1 or x.stride(1) == D) and x.data_ptr() % 16 == 0
-          and (n <= 1 or (x.stride(0) >= heads * D and x.stride(0) % 8 == 0)))
-    if not ok:
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"{name} must be (tokens, heads, {D}), got {tuple(shape)}")
+    n, heads, _ = shape
+    st, sh, sd = x.stride()
+    if not (sd == 1 and (heads == 1 or sh == D) and x.data_ptr() % 16 == 0
+            and (n <= 1 or (st >= heads * D and st % 8 == 0))):
         x = x.clone(memory_format=torch.contiguous_format)
-    return x, x.stride(0) if n > 1 else heads * D
+        st = heads * D
+    return x, st if n > 1 else heads * D
 
 
 def _pool(k_pages, v_pages):
     """(n_pages, page, n_kv, 128) pools, e.g. views of one (n_pages, 2, page,
     n_kv, 128) tensor; never copied, since they are the caller's cache."""
-    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if x.dim() != 4 or x.shape[3] != D:
-            raise ValueError(f"{name} must be (pages, page, heads, {D}), got {tuple(x.shape)}")
-        if x.stride(3) != 1 or (x.shape[2] > 1 and x.stride(2) != D):
-            raise ValueError(f"{name}: a token's heads must be contiguous")
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape[3] != D:
+        raise ValueError(f"k_pages must be (pages, page, heads, {D}), got {tuple(shape)}")
+    if strides[3] != 1 or (shape[2] > 1 and strides[2] != D):
+        raise ValueError("k_pages: a token's heads must be contiguous")
+    if v_pages.shape != shape or v_pages.dtype != k_pages.dtype or v_pages.stride() != strides:
         raise ValueError("k_pages and v_pages must have one shape, type and layout")
-    return k_pages.shape[0], k_pages.shape[1], k_pages.stride(0), k_pages.stride(1)
+    return shape[0], shape[1], strides[0], strides[1]
 
 
 def _i32(x, name, numel=None):
@@ -570,8 +572,8 @@ class AttnPlan:
 
     def __init__(self, n_tokens, batch, n_q, n_kv, paged, device):
         self.n_tokens, self.batch, self.n_q, self.n_kv, self.paged = n_tokens, batch, n_q, n_kv, paged
-        nbytes = call("kvr_attn_plan_bytes", n_tokens, batch, n_q, n_kv)
-        self.buf = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self.nbytes = max(call("kvr_attn_plan_bytes", n_tokens, batch, n_q, n_kv), 16)
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
 
     def _match(self, n_tokens, n_q, paged):
         if (self.n_tokens, self.n_q, self.paged) != (n_tokens, n_q, paged):
@@ -597,7 +599,7 @@ def attn_plan(cu_q, n_tokens, n_q, n_kv, kv_len=None, cu_k=None, causal=True, wi
         _i32(cu_k, "cu_k", batch + 1)
     plan = AttnPlan(n_tokens, batch, n_q, n_kv, kv_len is not None, cu_q.device)
     call("kvr_attn_plan", ptr(cu_q), ptr(kv_len), ptr(cu_k), batch, n_tokens, n_q, n_kv, int(causal), window,
-         ptr(plan.buf), plan.buf.numel(), stream())
+         ptr(plan.buf), plan.nbytes, stream())
     return plan
 
 
@@ -627,20 +629,19 @@ def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens,
         raise ValueError(f"block_table has {block_table.shape[0]} rows for {batch} requests")
     dev = ctx_len.device
     width = block_table.shape[1]
-    # one allocation: cu_q, kv_len, n_free, info, positions, then slots on an 8-byte boundary
-    head = (2 * batch + 6 + n_tokens + 1) // 2 * 2
-    buf = torch.empty(head + 2 * n_tokens, dtype=torch.int32, device=dev)
+    buf = torch.empty(2 * batch + 6 + n_tokens, dtype=torch.int32, device=dev)
     st = PagedStep()
-    st.cu_q, st.kv_len = buf[:batch + 1], buf[batch + 1:2 * batch + 1]
-    st.n_free, st.info = buf[2 * batch + 1:2 * batch + 2], buf[2 * batch + 2:2 * batch + 6]
-    st.positions = buf[2 * batch + 6:2 * batch + 6 + n_tokens]
-    st.slots = buf[head:].view(torch.int64)
+    st.cu_q, st.kv_len, st.n_free, st.info, st.positions = torch.split_with_sizes(buf, (batch + 1, batch, 1, 4, n_tokens))
+    st.slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
     st.n_tokens = n_tokens
     st.plan = AttnPlan(n_tokens, batch, n_q, n_kv, True, dev) if n_q else None
+    at = buf.data_ptr()
+    plan = st.plan
     call("kvr_paged_map", ptr(ctx_len), ptr(new_len), batch, n_tokens, page, ptr(block_table),
-         max(block_table.stride(0), width), width, ptr(free_pages), free_pages.numel(), ptr(n_free), ptr(st.cu_q),
-         ptr(st.kv_len), ptr(st.positions), ptr(st.slots), ptr(st.n_free), ptr(st.info), n_q, n_kv, window,
-         ptr(st.plan.buf) if st.plan else None, st.plan.buf.numel() if st.plan else 0, stream())
+         max(block_table.stride(0), width), width, ptr(free_pages), free_pages.numel(), ptr(n_free), at,
+         at + 4 * (batch + 1), at + 4 * (2 * batch + 6), st.slots.data_ptr(), at + 4 * (2 * batch + 1),
+         at + 4 * (2 * batch + 2), n_q, n_kv, window, plan.buf.data_ptr() if plan else None,
+         plan.nbytes if plan else 0, stream())
     return st
 
 
@@ -681,16 +682,24 @@ def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=
     return q_out
 
 
-def _attn_workspace(n_q, n_kv, device):
-    """The attention workspace of the current stream (calls on one stream do
-    not overlap; each stream has its own)."""
+_ATTN_WS: dict = {}
+
+
+def _attn_workspace(device):
+    """The attention workspace of the current stream and its bytes (calls on
+    one stream do not overlap; each stream has its own).  Its size does not
+    depend on the call."""
     s = stream()
-    return N.workspace(f"attn_work_{s}", call("kvr_attn_workspace_bytes", n_q, n_kv), device), s
+    ws = _ATTN_WS.get((s, device))
+    if ws is None:
+        nbytes = call("kvr_attn_workspace_bytes")
+        ws = _ATTN_WS[s, device] = (N.workspace(f"attn_work_{s}", nbytes, device), nbytes)
+    return ws[0].data_ptr(), ws[1], s
 
 
 def _attn_out(q, out, return_lse):
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous and of q's shape and dtype")
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
@@ -714,11 +723,11 @@ def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, ret
     if block_table.shape[0] < plan.batch:
         raise ValueError(f"block_table has {block_table.shape[0]} rows for {plan.batch} requests")
     out, lse = _attn_out(q, out, return_lse)
-    ws, s = _attn_workspace(n_q, plan.n_kv, q.device)
+    ws, ws_bytes, s = _attn_workspace(q.device)
     width = block_table.shape[1]
     call("kvr_paged_attn", ptr(q), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, ptr(k_pages),
          ptr(v_pages), n_pages, page, ps, ts, ptr(block_table), max(block_table.stride(0), width), width,
-         ptr(plan.buf), plan.buf.numel(), float(scale or 0.0), ptr(out), ptr(lse), ptr(ws), ws.numel(), s)
+         ptr(plan.buf), plan.nbytes, float(scale or 0.0), ptr(out), ptr(lse), ws, ws_bytes, s)
     return (out, lse) if return_lse else out
 
 
@@ -736,9 +745,9 @@ def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
     if k.shape != v.shape or k.shape[1] != plan.n_kv:
         raise ValueError("k and v must be (tokens, n_kv, d) with the plan's n_kv")
     out, lse = _attn_out(q, out, return_lse)
-    ws, s = _attn_workspace(n_q, plan.n_kv, q.device)
+    ws, ws_bytes, s = _attn_workspace(q.device)
     call("kvr_prompt_attn", ptr(q), ptr(k), ptr(v), dtype_code(q), n_tokens, k.shape[0], plan.batch, n_q, plan.n_kv, D,
-         qs, ks, vs, ptr(plan.buf), plan.buf.numel(), float(scale or 0.0), ptr(out), ptr(lse), ptr(ws), ws.numel(), s)
+         qs, ks, vs, ptr(plan.buf), plan.nbytes, float(scale or 0.0), ptr(out), ptr(lse), ws, ws_bytes, s)
     return (out, lse) if return_lse else out
 
 
@@ -746,7 +755,8 @@ def attn_status(device=None):
     """Raises if an attention call on the current stream gave up or met a plan
     of other shapes (synchronises the stream)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    workspace_status(_attn_workspace(1, 1, device)[0])
+    ws, _, s = _attn_workspace(device)
+    call("kvr_workspace_status", ws, s)
 
 
 def kmeans(x, k=128, iters=10):
