@@ -61,7 +61,9 @@ constexpr uint32_t kCaHalf = kCaTile / 2;       // 64 channels of them
 constexpr uint32_t kCaOffKv = 2 * kCaTile;
 constexpr uint32_t kCaOffBar = kCaOffKv + kCaStages * kCaTile;
 constexpr int kCaBars = 2 * kCaStages + 15;
-constexpr uint32_t kCaSmem = kCaOffBar + kCaBars * 8 + 16;
+constexpr int kCaRecords = 64;                  // pieces of a CTA kept in shared memory
+constexpr uint32_t kCaOffRec = (kCaOffBar + kCaBars * 8 + 16 + 31) / 32 * 32;
+constexpr uint32_t kCaSmem = kCaOffRec + kCaRecords * 32;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr float kLazy = 6.0f, kShift = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -76,6 +78,7 @@ struct ChunkArgs {
   int64_t table_stride;
   int table_width;
   const PlanHeader *hdr;
+  int max_pieces;               // entries the plan has room for
   float to_log2;                // log2(e) / scale
   void *out;
   float *lse;
@@ -163,6 +166,14 @@ __device__ __forceinline__ void ca_st16(uint32_t taddr, const uint32_t *r) {
       : "memory");
 }
 
+// 32 bytes to global memory: a whole sector per lane (a row per lane makes
+// 16-byte stores write half sectors, twice as many).
+__device__ __forceinline__ void ca_store32(void *p, const uint32_t *w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 __device__ __forceinline__ void ca_tma4(uint32_t dst, const CUtensorMap *m, int c1, int c2, int c3, uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
@@ -180,6 +191,10 @@ __device__ __forceinline__ void ca_tma5(uint32_t dst, const CUtensorMap *m, int 
 }
 
 // ---------------------------------------------------------------- waiting ----
+
+__device__ __forceinline__ void ca_bar_init(uint64_t *bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
 
 __device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile int *abort_s) {
   if (__builtin_expect(mbar_try_wait(bar, phase), 1)) return true;
@@ -200,12 +215,17 @@ struct CaPiece {
   PlanPiece p;
   int head, n, two;  // KV head, K/V tiles, whether the second query tile has rows
 };
-__device__ __forceinline__ bool ca_piece(const ChunkArgs &a, int64_t total, int per, int r, CaPiece &o) {
-  const int64_t G = gridDim.x, c = blockIdx.x;
-  const int64_t i = (int64_t)r * G + ((r & 1) ? G - 1 - c : c);
+// (a call's pieces number less than 2^31: 2^24 tokens in items of 256 rows)
+__device__ __forceinline__ unsigned ca_index(int r) {
+  return r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+__device__ __forceinline__ bool ca_piece(const ChunkArgs &a, const unsigned char *rec, unsigned total, int per, int r,
+                                         CaPiece &o) {
+  const unsigned i = ca_index(r);
   if (i >= total) return false;
-  o.p = reinterpret_cast<const PlanPiece *>(a.hdr + 1)[i / a.n_kv];
-  o.head = (int)(i % a.n_kv);
+  const unsigned e = i / (unsigned)a.n_kv;
+  o.p = r < kCaRecords ? reinterpret_cast<const PlanPiece *>(rec)[r] : reinterpret_cast<const PlanPiece *>(a.hdr + 1)[e];
+  o.head = (int)(i - e * a.n_kv);
   o.p.n_tok = min(max(o.p.n_tok, 0), per);
   o.n = o.p.n_tok > 0 ? max(o.p.kt1 - o.p.kt0, 0) : 0;
   o.two = o.p.n_tok > (per >> 1);
@@ -275,33 +295,40 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   if (tid == 9 * 32) {
     *abort_s = 0;
     for (int s = 0; s < kCaStages; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      ca_bar_init(&kv_full[s], 1);
+      ca_bar_init(&kv_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 1);
-      mbar_init(&q_empty[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[2 * t], 4);
-      mbar_init(&p_full[2 * t + 1], 4);
-      mbar_init(&drained[t], 1);
-      mbar_init(&pv_done[t], 1);
+      ca_bar_init(&q_full[t], 1);
+      ca_bar_init(&q_empty[t], 1);
+      ca_bar_init(&s_full[t], 1);
+      ca_bar_init(&p_full[2 * t], 4);
+      ca_bar_init(&p_full[2 * t + 1], 4);
+      ca_bar_init(&drained[t], 1);
+      ca_bar_init(&pv_done[t], 1);
     }
-    mbar_init(s_free, 4);
+    ca_bar_init(s_free, 4);
   }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // barriers: for the copies and commits
   ca_fence_before();
   __syncthreads();
   ca_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_wait();  // what follows reads the plan, q and the cache
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel waits for this grid's end
+  griddep_launch();  // the joining kernel waits for this grid's end
 
+  // The CTA's first pieces: every role reads each of them, and a record from L2 would cost each the round
+  // trip.  They are fetched beside the header, before it is known how many of them the plan has.
   const PlanHeader &h = *a.hdr;
+  if (tid < kCaRecords && ca_index(tid) / a.n_kv < (unsigned)a.max_pieces)
+    reinterpret_cast<PlanPiece *>(sm + kCaOffRec)[tid] =
+        reinterpret_cast<const PlanPiece *>(a.hdr + 1)[ca_index(tid) / a.n_kv];
   const bool fits = h.magic == kPlanMagic && h.n_tokens == a.n_tokens && h.n_q == a.n_q && h.n_kv == a.n_kv &&
                     h.batch == a.batch;
   if (!fits && tid == 0) atomicOr(a.err, kWsErrPlan);
-  const int64_t total = fits ? (int64_t)h.n_pieces * a.n_kv : 0;
+  const unsigned total = fits ? (unsigned)h.n_pieces * a.n_kv : 0;
   const int causal = h.causal, window = h.window;
+  __syncthreads();
   const int g = a.n_q / a.n_kv, tpt = kPlanRows / g, per = 2 * tpt;
 
   // registers: 384 threads x 168 at launch = (208 + 208 + 88) x 128
@@ -314,7 +341,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     int j = 0, uses[2] = {0, 0};  // ring stages and Q tiles filled so far
     CaPiece c;
     bool ok = true;
-    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
       const int64_t row = PAGED ? (int64_t)c.p.k_start * a.table_stride : 0;
       const bool known = PAGED && c.p.k_start >= 0 && c.p.k_start < a.batch;
       int id = 0, off = 0;  // paged: this lane's page and row in it, of the next K/V tile
@@ -392,7 +419,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     int si = 0;
     bool ok = true;
     CaPiece c;
-    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
       const int tiles = c.two ? 2 : 1;
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
@@ -479,7 +506,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     const uint64_t to2 = ca_pair(a.to_log2, a.to_log2);
     bool ok = true;
     CaPiece c;
-    for (int r = 0; ok && ca_piece(a, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
       const int n_tok = min(tpt, c.p.n_tok - t * tpt);  // tokens of this tile
       if (n_tok <= 0) continue;
       const bool live = tok_in < n_tok, busy = wrow < n_tok * g;  // the row / the warp has something to do
@@ -621,9 +648,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           ca_wait_ld();
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              reinterpret_cast<float4 *>(a.part_o + pr * kD + k * 32)[e] =
-                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e)
+              ca_store32(a.part_o + pr * kD + k * 32 + e * 8, reinterpret_cast<const uint32_t *>(o + e * 8));
           }
         }
         if (live) *reinterpret_cast<float2 *>(a.part_ml + pr * 2) = make_float2(mc - kShift, none ? 0.0f : l);
@@ -639,14 +665,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           }
           if (store) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4];
+            for (int e = 0; e < 2; ++e) {
+              uint32_t w[8];
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                const float x = o[e * 8 + 2 * u], y = o[e * 8 + 2 * u + 1];
+              for (int u = 0; u < 8; ++u) {
+                const float x = o[e * 16 + 2 * u], y = o[e * 16 + 2 * u + 1];
                 w[u] = none ? 0u : ca_pack<DT>(x * inv, y * inv);
               }
-              reinterpret_cast<uint4 *>(dst + k * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+              ca_store32(dst + k * 32 + e * 16, w);
             }
           }
         }
@@ -672,6 +698,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 template <int DT>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
   griddep_wait();
+  griddep_launch();
   const PlanHeader &h = *a.hdr;
   if (h.magic != kPlanMagic || h.n_tokens != a.n_tokens || h.n_q != a.n_q || h.n_kv != a.n_kv || h.batch != a.batch) return;
   const PlanSplit *splits = plan_splits(a.hdr, a.n_tokens, a.batch, a.n_q, a.n_kv);
@@ -766,6 +793,7 @@ static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float sca
                          reinterpret_cast<uintptr_t>(c.v) | reinterpret_cast<uintptr_t>(a.out) |
                          reinterpret_cast<uintptr_t>(plan);
   KVR_REQUIRE((ptrs & 15) == 0, "%s: pointers must be 16-byte aligned", fn);
+  KVR_REQUIRE((reinterpret_cast<uintptr_t>(a.out) & 31) == 0, "%s: out must be 32-byte aligned", fn);
   KVR_REQUIRE(plan_bytes >= kvr_attn_plan_bytes(a.n_tokens, a.batch, a.n_q, a.n_kv), "%s: plan too small", fn);
   KVR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "%s: workspace alignment", fn);
   const size_t need = kvr_attn_workspace_bytes();
@@ -773,9 +801,10 @@ static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float sca
   KVR_REQUIRE(scale == scale && scale <= 3.0e38f, "%s: bad scale", fn);
   a.to_log2 = kLog2e / (scale > 0.0f ? scale : sqrtf((float)d));
   a.hdr = static_cast<const PlanHeader *>(plan);
+  a.max_pieces = (int)(plan_max_items(a.n_tokens, a.batch, a.n_q, a.n_kv) + kPlanExtra);
   a.err = static_cast<unsigned *>(workspace);
-  a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWsHeader);
-  a.part_o = a.part_ml + 2 * (size_t)kPartRows;
+  a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWsHeader);
+  a.part_ml = a.part_o + kD * (size_t)kPartRows;
   return KVR_OK;
 }
 
@@ -788,22 +817,10 @@ static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  cudaLaunchAttribute dep[1];
-  dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  dep[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = st;
-  cfg.attrs = dep;
-  cfg.numAttrs = 1;
-  cfg.gridDim = dim3(kPlanCtas);
-  cfg.blockDim = dim3(kCaThreads);
-  cfg.dynamicSmemBytes = kCaSmem;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel<DT, PAGED>, c.mq, c.mk, c.mv, c.a);
+  const cudaError_t e = launch_dependent(chunk_attn_kernel<DT, PAGED>, kPlanCtas, kCaThreads, kCaSmem, st, c.mq, c.mk,
+                                         c.mv, c.a);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(kPlanCtas * 4);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, chunk_join_kernel<DT>, c.a);
+  return launch_dependent(chunk_join_kernel<DT>, kPlanCtas * 2, 256, 0, st, c.a);
 }
 
 static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr_stream_t stream) {

@@ -273,6 +273,8 @@ static_assert(kPlanBins == kPlanThreads, "one bin per thread in the scan");
 
 __global__ void __launch_bounds__(kPlanThreads, 1) attn_plan_kernel(PlanArgs a) {
   __shared__ PlanShared s;
+  griddep_wait();
+  griddep_launch();
   plan_build(a, s);
 }
 
@@ -304,6 +306,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
   __shared__ int n_cut, n_over;
   int *fresh = s.fresh;
   const int tid = threadIdx.x, nt = blockDim.x, P = a.page;
+  griddep_wait();
+  griddep_launch();
   if (tid == 0) n_cut = n_over = 0;
   const int each = (a.batch + nt - 1) / nt;
   // tokens first: requests are cut where the step's n_tokens end
@@ -435,7 +439,8 @@ extern "C" int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const i
   PlanArgs a{cu_q, kv_len, cu_k, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, nullptr, 0};
   const int rc = plan_check("kvr_attn_plan", a, n_tokens, window, plan, plan_bytes);
   if (rc) return rc;
-  attn_plan_kernel<<<1, kPlanThreads, 0, as_cuda(stream)>>>(a);
+  const cudaError_t e = launch_dependent(attn_plan_kernel, 1, kPlanThreads, 0, as_cuda(stream), a);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_attn_plan: %s", cudaGetErrorString(e));
   return check_launch("kvr_attn_plan");
 }
 
@@ -471,6 +476,7 @@ extern "C" int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int
   // CTA 0 and one CTA per 1024 tokens, at most one per SM
   int64_t ctas = (n_tokens + kPlanThreads - 1) / kPlanThreads;
   ctas = ctas < 1 ? 1 : (ctas > kPlanCtas - 1 ? kPlanCtas - 1 : ctas);
-  paged_map_kernel<<<(unsigned)ctas + 1, kPlanThreads, 0, as_cuda(stream)>>>(m);
+  const cudaError_t e = launch_dependent(paged_map_kernel, (unsigned)ctas + 1, kPlanThreads, 0, as_cuda(stream), m);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_paged_map: %s", cudaGetErrorString(e));
   return check_launch("kvr_paged_map");
 }

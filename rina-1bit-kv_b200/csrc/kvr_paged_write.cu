@@ -35,6 +35,8 @@ struct PagedWriteArgs {
 
 template <int DT>
 __global__ void __launch_bounds__(kPwThreads) paged_write_kernel(PagedWriteArgs a) {
+  griddep_wait();
+  griddep_launch();
   const int lane = threadIdx.x & 31;
   const int64_t unit = ((int64_t)blockIdx.x * kPwThreads + threadIdx.x) >> 5;
   const int64_t t = unit / a.parts;
@@ -141,7 +143,8 @@ extern "C" int kvr_paged_write(const void *q, const void *k, const void *v, int 
   while (a.parts * 4 < rows && n_tokens * a.parts < 148 * 16) a.parts *= 2;
   const int64_t ctas = (n_tokens * a.parts * 32 + kPwThreads - 1) / kPwThreads;
   KVR_REQUIRE(ctas <= INT_MAX, "kvr_paged_write: too many tokens");
-  if (dtype == KVR_F16) paged_write_kernel<KVR_F16><<<(unsigned)ctas, kPwThreads, 0, as_cuda(stream)>>>(a);
-  else paged_write_kernel<KVR_BF16><<<(unsigned)ctas, kPwThreads, 0, as_cuda(stream)>>>(a);
+  const cudaError_t e = launch_dependent(dtype == KVR_F16 ? paged_write_kernel<KVR_F16> : paged_write_kernel<KVR_BF16>,
+                                         (unsigned)ctas, kPwThreads, 0, as_cuda(stream), a);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_paged_write: %s", cudaGetErrorString(e));
   return check_launch("kvr_paged_write");
 }
