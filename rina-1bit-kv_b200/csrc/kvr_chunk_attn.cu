@@ -10,7 +10,7 @@
 // 128 keys.  Packing the g query heads of a KV head into the rows (row = token
 // * g + j) lets one K/V tile serve all of them, for one token as for many.
 //   warp 9   copies: Q tiles, then K, V, K, V, ... by TMA (128-byte swizzle)
-//            into a ring of five 32 KB stages; a paged tile is a box per page
+//            into rings of two and three 32 KB stages; a paged tile is a box per page
 //            (or per gcd(page, 128) rows), a missing page an out-of-range box,
 //            which the TMA fills with zeros;
 //   warp 8   one lane issues tcgen05.mma: S = Q_t K^T (128 x 128 x 128,
@@ -55,7 +55,9 @@
 namespace kvr {
 
 constexpr int kCaThreads = 384;  // two softmax warpgroups; MMA, copies and two idle warps
-constexpr int kCaStages = 5;
+// A ring of K tiles and one of V tiles.  (One ring for both would not do: K and V have different consumers,
+// and a stage's barrier tells its phases apart by parity only, so each phase must be seen by the same waiter.)
+constexpr int kCaStagesK = 2, kCaStagesV = 3, kCaStages = kCaStagesK + kCaStagesV;
 constexpr uint32_t kCaTile = 128 * kD * 2;      // 32 KB: 128 rows of K, V or Q
 constexpr uint32_t kCaHalf = kCaTile / 2;       // 64 channels of them
 constexpr uint32_t kCaOffKv = 2 * kCaTile;
@@ -208,6 +210,9 @@ __device__ __forceinline__ void ca_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Stage of the n-th K (or V) tile.
+__device__ __forceinline__ int ca_stage(bool v, int n) { return v ? kCaStagesK + n % kCaStagesV : n % kCaStagesK; }
+
 // ------------------------------------------------------------ the pieces ----
 
 // Piece number r of CTA c (see kvr_attn_plan.cuh), or false past the last.
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     __syncthreads();
   } else if (warp == 9) {
     // ---- copies
-    int j = 0, uses[2] = {0, 0};  // ring stages and Q tiles filled so far
+    int fill[2] = {0, 0}, uses[2] = {0, 0};  // K and V stages, Q tiles filled so far
     CaPiece c;
     bool ok = true;
     for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
@@ -353,9 +358,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           if (id < 0 || id >= a.n_pages) id = a.n_pages;  // out of range: zeros
         }
       };
-      auto load = [&](const CUtensorMap *m, int kt) {
-        const int s = j % kCaStages;
-        if (j >= kCaStages && !ca_wait(&kv_empty[s], (unsigned)((j / kCaStages - 1) & 1), abort_s)) return false;
+      auto load = [&](const CUtensorMap *m, bool v, int kt) {
+        const int n = fill[v], depth = v ? kCaStagesV : kCaStagesK, s = ca_stage(v, n);
+        if (n >= depth && !ca_wait(&kv_empty[s], (unsigned)((n / depth - 1) & 1), abort_s)) return false;
+        ++fill[v];
         const uint32_t dst = smem_u32(sm) + kCaOffKv + s * kCaTile;
         if (lane == 0) mbar_expect_tx(&kv_full[s], kCaTile);
         __syncwarp();
@@ -368,7 +374,6 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         } else if (lane == 0) {
           ca_tma4(dst, m, c.p.k_start + kt * 128, 0, c.head, &kv_full[s]);
         }
-        ++j;
         return true;
       };
       auto load_q = [&](int t) {
@@ -384,12 +389,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       };
       if (c.n == 0) continue;
       look(c.p.kt0);
-      ok = load_q(0) && load(&mk, c.p.kt0) && (!c.two || load_q(1));
+      ok = load_q(0) && load(&mk, false, c.p.kt0) && (!c.two || load_q(1));
       for (int i = 0; ok && i < c.n; ++i) {
-        ok = load(&mv, c.p.kt0 + i);
+        ok = load(&mv, true, c.p.kt0 + i);
         if (ok && i + 1 < c.n) {
           look(c.p.kt0 + i + 1);
-          ok = load(&mk, c.p.kt0 + i + 1);
+          ok = load(&mk, false, c.p.kt0 + i + 1);
         }
       }
       if (*abort_s) ok = false;
@@ -402,9 +407,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     }
     __syncthreads();  // end of work
     if (*abort_s) {   // copies in flight must land before the CTA exits
-      for (int k = max(0, j - kCaStages); k < j; ++k)
-        for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(&kv_full[k % kCaStages], (unsigned)((k / kCaStages) & 1));)
-          ++it;
+      for (int v = 0; v < 2; ++v) {
+        const int depth = v ? kCaStagesV : kCaStagesK;
+        for (int k = max(0, fill[v] - depth); k < fill[v]; ++k)
+          for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(&kv_full[ca_stage(v, k)], (unsigned)((k / depth) & 1));)
+            ++it;
+      }
       for (int t = 0; t < 2; ++t)
         for (uint32_t it = 0; uses[t] && it < kSpinLimit && !mbar_try_wait(&q_full[t], (unsigned)((uses[t] - 1) & 1));)
           ++it;
@@ -414,7 +422,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     const uint32_t q_base = smem_u32(sm), kv_base = q_base + kCaOffKv;
     const bool scores = warp == 8;
     const uint32_t tmem_u = ca_uniform(tmem);
-    int j = scores ? 0 : 1;  // ring stage: K and V take turns
+    const int depth = scores ? kCaStagesK : kCaStagesV;
+    int j = 0;               // K or V tiles consumed so far
     int seen[2] = {0, 0};    // warp 8: Q tiles, warp 10: P tiles consumed so far
     int si = 0;
     bool ok = true;
@@ -423,9 +432,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int tiles = c.two ? 2 : 1;
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
-      for (int i = 0; ok && i < c.n; ++i, j += 2) {
-        const int s = j % kCaStages;
-        ok = ca_wait(&kv_full[s], (unsigned)((j / kCaStages) & 1), abort_s);
+      for (int i = 0; ok && i < c.n; ++i, ++j) {
+        const int s = ca_stage(!scores, j);
+        ok = ca_wait(&kv_full[s], (unsigned)((j / depth) & 1), abort_s);
         if (!ok) break;
         if (scores) {
           for (int t = 0; ok && t < tiles; ++t) {

@@ -418,6 +418,30 @@ def test_other_stream_and_graph():
     torch.cuda.current_stream().wait_stream(side)
 
 
+@pytest.mark.parametrize("kind", ["decode", "prompt"])
+def test_repeated_calls_give_the_same_bits(kind):
+    """Copies that land in another order must not show: 60 calls, the inputs out of cache before each."""
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(12)
+    flush = torch.empty(160 << 20, dtype=torch.uint8, device=DEV)
+    if kind == "decode":
+        kv, new = [3000 + 37 * b for b in range(24)], [1] * 24
+        kp, vp, table, _ = make_pages(g, kv, 8, 16, BF16)
+        q = torch.randn(24, 32, 128, device=DEV, generator=g).bfloat16()
+        plan = K.attn_plan(offsets(new), 24, 32, 8, kv_len=i32(kv))
+        call = lambda: K.paged_attn(q, kp, vp, table, plan)  # noqa: E731
+    else:
+        lens = [1500, 700, 1, 350]
+        q, k, v = torch.randn(sum(lens), 48, 128, device=DEV, generator=g).half().split([32, 8, 8], 1)
+        plan = K.attn_plan(offsets(lens), sum(lens), 32, 8)
+        call = lambda: K.prompt_attn(q, k, v, plan)  # noqa: E731
+    first = call()
+    for _ in range(60):
+        flush.zero_()
+        assert torch.equal(call(), first)
+    K.attn_status()
+
+
 def test_plan_of_another_call_is_reported():
     from kvr_b200 import _native as N
     from kvr_b200 import kernels as K
