@@ -4,9 +4,9 @@
 
 from .kvr_window import WindowBuffer
 from .kvr_retrieval import RetrievalIndex
-from .kvr_paged import PagedKVCache
+from .kvr_paged import PagedGenerator, PagedKVCache
 
-__all__ = ["WindowBuffer", "RetrievalIndex", "PagedKVCache", "KVRHook", "KVRGenerator"]
+__all__ = ["WindowBuffer", "RetrievalIndex", "PagedKVCache", "PagedGenerator", "KVRHook", "KVRGenerator"]
 
 
 def __getattr__(name):

@@ -1,4 +1,5 @@
-"""PagedKVCache — the exact K/V of many requests of different lengths in pages.
+"""PagedKVCache — the exact K/V of many requests of different lengths in pages —
+and PagedGenerator, which serves them on a HF decoder model.
 
 No reference counterpart (the reference keeps one sequence's window,
 modules/kvr_window.py).  A step appends the new tokens of every request (whole
@@ -99,3 +100,114 @@ class PagedKVCache:
     def __repr__(self):
         return (f"PagedKVCache(layers={self.n_layers}, heads={self.n_q}/{self.n_kv}, pages={self.n_pages}x{self.page}, "
                 f"requests={self.max_requests})")
+
+
+class PagedGenerator:
+    """Many requests on one HF decoder model with an exact paged cache.
+
+        gen = PagedGenerator(model, n_pages=4096, max_requests=32)
+        rows = gen.add([prompt_a, prompt_b])          # prompts in chunks of `chunk` tokens
+        tokens = gen.generate(rows, max_new_tokens=64)
+        gen.drop(rows)                                # their pages are free again
+
+    A step takes any mix of chunks and single tokens (``step``); ``score``
+    gives the logits of whole packed prompts without a cache."""
+
+    def __init__(self, model, n_pages, page=64, max_requests=32, max_len=None, window=0, chunk=2048):
+        from .kvr_hook import rope_tables
+
+        cfg = model.config
+        self.model, self.device, self.chunk = model, model.device, chunk
+        self.n_q, self.n_kv = cfg.num_attention_heads, cfg.num_key_value_heads
+        d = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.n_q
+        if d != K.D:
+            raise ValueError(f"head_dim must be {K.D}, the model has {d}")
+        max_len = max_len or cfg.max_position_embeddings
+        self.cache = PagedKVCache(cfg.num_hidden_layers, self.n_q, self.n_kv, n_pages, page, max_requests, max_len, window,
+                                  dtype=model.dtype, device=self.device)
+        self.cos_tbl, self.sin_tbl = rope_tables(model, max_len, self.device)
+        self.last = {}  # row -> logits (vocab,) fp32 after its last token
+
+    def _layers(self, h, attend):
+        """The decoder layers over packed rows h (T, hidden); attend(layer index, q, k, v) -> (T, n_q, d)."""
+        for li, layer in enumerate(self.model.model.layers):
+            at = layer.self_attn
+            x = layer.input_layernorm(h)
+            q, k, v = (p(x).view(x.shape[0], -1, K.D) for p in (at.q_proj, at.k_proj, at.v_proj))
+            h = h + at.o_proj(attend(li, q, k, v).reshape(x.shape[0], -1))
+            h = h + layer.mlp(layer.post_attention_layernorm(h))
+        return self.model.model.norm(h)
+
+    @torch.no_grad()
+    def step(self, new):
+        """One pass: new maps rows to the token ids they get (a chunk or one).
+        Returns {row: logits (vocab,) fp32 after its last new token}."""
+        rows = sorted(new)
+        lens = [len(new.get(b, ())) for b in range(self.cache.max_requests)]
+        if not rows or min(lens[b] for b in rows) < 1:
+            raise ValueError("every row of a step needs at least one token")
+        ids = torch.tensor([t for b in rows for t in new[b]], device=self.device)
+        st = self.cache.begin(lens, ids.numel())
+        try:
+            self.cache.check()
+        except RuntimeError:
+            self.cache.step = None  # nothing was written: the step can be tried again after a drop
+            raise
+        h = self._layers(self.model.model.embed_tokens(ids), lambda li, q, k, v: self.cache.attend(
+            li, self.cache.write(li, q, k, v, self.cos_tbl, self.sin_tbl)))
+        ends = st.cu_q[1:].long()[torch.tensor(rows, device=self.device)] - 1
+        logits = self.model.lm_head(h[ends]).float()
+        self.cache.commit()
+        out = {b: logits[i] for i, b in enumerate(rows)}
+        self.last.update(out)
+        return out
+
+    @torch.no_grad()
+    def add(self, prompts):
+        """Takes prompts (lists of token ids) into free rows, `chunk` tokens a
+        step and prompt; returns the rows."""
+        free = [b for b in range(self.cache.max_requests) if b not in self.last]
+        if len(free) < len(prompts):
+            raise RuntimeError(f"{len(prompts)} prompts for {len(free)} free rows")
+        rows, left = free[:len(prompts)], [list(p) for p in prompts]
+        while any(left):
+            self.step({b: left[i][:self.chunk] for i, b in enumerate(rows) if left[i]})
+            left = [p[self.chunk:] for p in left]
+        return rows
+
+    @torch.no_grad()
+    def generate(self, rows, max_new_tokens):
+        """Greedy decoding of all rows together; returns {row: new token ids}."""
+        out = {b: [] for b in rows}
+        for _ in range(max_new_tokens):
+            for b in rows:
+                out[b].append(int(self.last[b].argmax()))
+            self.step({b: out[b][-1:] for b in rows})
+        return out
+
+    def drop(self, rows):
+        """Ends requests: their pages and rows are free again."""
+        self.cache.release(rows)
+        for b in rows:
+            self.last.pop(b, None)
+
+    @torch.no_grad()
+    def score(self, prompts):
+        """Logits (T, vocab) fp32 of each whole prompt, packed into one pass and
+        kept nowhere."""
+        lens = [len(p) for p in prompts]
+        if not lens or min(lens) < 1:
+            raise ValueError("every prompt needs at least one token")
+        cu = torch.tensor([0] + lens, device=self.device).cumsum(0).to(torch.int32)
+        n = sum(lens)
+        plan = K.attn_plan(cu, n, self.n_q, self.n_kv, window=self.cache.window)
+        pos = torch.cat([torch.arange(m, device=self.device) for m in lens])
+        c, s = self.cos_tbl[pos][:, None], self.sin_tbl[pos][:, None]
+
+        def rope(x):
+            y = x.float()
+            return (y * c + torch.cat([-y[..., K.D // 2:], y[..., :K.D // 2]], -1) * s).to(x.dtype)
+
+        h = self._layers(self.model.model.embed_tokens(torch.tensor([t for p in prompts for t in p], device=self.device)),
+                         lambda li, q, k, v: K.prompt_attn(rope(q), rope(k), v, plan))
+        return list(self.model.lm_head(h).float().split(lens))
