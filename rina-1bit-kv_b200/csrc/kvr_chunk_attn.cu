@@ -29,12 +29,18 @@
 // (An S per tile with P over it and S of the next keys after P V, one issuing
 // warp: 328 us for a chunk of 512 at 32256, 32/8 heads; this way 234 us.)
 //
-// What binds a long prompt: the chain S (512 cycles, with P V of the other
-// tile in between) -> warpgroup -> registers -> free -> next S, twice per 128
-// keys, about 3300 cycles against 2048 of MMA.  Tensor pipe 61 % active, special
-// function unit (16 exponentials a cycle) 61 %.  Exponentials on the FMA pipe
-// instead (a polynomial for 1/8 to 1/2 of them) lost 3 to 30 %: the instructions
-// they add lengthen the chain more than the special function unit shortens it.
+// What binds a long prompt: a warpgroup's chain of a K/V tile, about 2900
+// cycles beside the other warpgroup's, and 500 more until the next S is seen,
+// against 2048 cycles of MMA for both tiles.  Tensor pipe and special function
+// unit (16 exponentials a cycle) are 61 % active each.  With the MMAs reduced to
+// one step in eight a chunk of 512 at 32256 takes 3 % less, without the
+// exponentials 7 %, without both 33 %: what is left is the issue of some 560
+// instructions a tile by one warp per scheduler and tile.  So the slow paths
+// (a wait that has to poll, the rescaling, the masks) are kept small and out of
+// the way: 72 KB of code to 54 KB gained 10 % on windowed and packed prompts.
+// Exponentials on the FMA pipe (a polynomial for 1/8 to 1/2 of them) lost 3 to
+// 30 % by their instructions; four warpgroups with half of a tile's keys each
+// lost 60 % (104 registers a thread, maxima met through shared memory).
 //
 // The output accumulator is rescaled only when a row's maximum has grown by
 // more than 2^kLazy since its last rescale (the weights stay below 2^(kLazy +
@@ -68,6 +74,7 @@ constexpr uint32_t kCaOffRec = (kCaOffBar + kCaBars * 8 + 16 + 31) / 32 * 32;
 constexpr uint32_t kCaSmem = kCaOffRec + kCaRecords * 32;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr float kLazy = 6.0f, kShift = 4.0f;
+constexpr float kLowest = -1e30f;  // maximum of a row that has seen nothing: finite, so that -inf - it is -inf
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 
@@ -199,12 +206,20 @@ __device__ __forceinline__ void ca_bar_init(uint64_t *bar, unsigned count) {
 }
 
 __device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile int *abort_s) {
-  if (__builtin_expect(mbar_try_wait(bar, phase), 1)) return true;
-  for (uint32_t it = 0; it < kSpinLimit; ++it) {
-    if (mbar_try_wait(bar, phase)) return true;
-    if ((it & 255u) == 255u && *abort_s) return false;
-  }
-  return false;
+#pragma unroll 1
+  for (uint32_t it = 0; !mbar_try_wait(bar, phase); ++it)
+    if (it >= kSpinLimit || *abort_s) return false;
+  return true;
+}
+// Whether the phase is complete by now (never waits).
+__device__ __forceinline__ bool ca_test(uint64_t *bar, unsigned phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  return done != 0;
 }
 __device__ __forceinline__ void ca_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -266,6 +281,8 @@ __device__ __forceinline__ uint64_t ca_add2(uint64_t x, uint64_t y) {
   return r;
 }
 __device__ __forceinline__ uint64_t ca_exp2_sfu(uint64_t x) { return ca_pair(ca_exp2(ca_lo(x)), ca_exp2(ca_hi(x))); }
+// Bits 0 .. n - 1 (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t ca_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 template <int DT>
 __device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
   uint32_t r;
@@ -523,7 +540,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int begin = window > 0 ? max(0, c.p.first_end + tok - window) : 0;
       const int end_a = causal ? min(c.p.kv_len, c.p.first_end + tok_a) : c.p.kv_len;
       const int begin_b = window > 0 ? max(0, c.p.first_end + tok_b - window) : 0;
-      float m = -INFINITY, mc = 0.0f, l = 0.0f;  // running maximum (raw score units), its log2 multiple, sum
+      float mc = kLowest, l = 0.0f;  // running maximum in log2 units, sum
       for (int i = 0; i < c.n; ++i, ++sn) {
         ok = __all_sync(~0u, ca_wait(&s_full[t], (unsigned)(sn & 1), abort_s));
         if (!ok) break;
@@ -538,9 +555,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           if (lane == 0) ca_arrive(s_free);
           const int k0 = (c.p.kt0 + i) * 128;
           if (__builtin_expect(k0 + 128 > end_a || k0 < begin_b, 0)) {
-            const int e = end - k0, b = begin - k0;
 #pragma unroll
-            for (int k = 0; k < 128; ++k) s[k] = k < e && k >= b ? s[k] : -INFINITY;
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t sees = ca_below(end - k0 - 32 * w) & ~ca_below(begin - k0 - 32 * w);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[w * 32 + k] = sees & (1u << k) ? s[w * 32 + k] : -INFINITY;
+            }
           }
           float mx[8];
 #pragma unroll
@@ -554,21 +574,22 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           for (int u = 0; u < 4; ++u) mx[u] = ca_max3(mx[u], s[120 + u], s[124 + u]);
           mx[0] = ca_max3(mx[0], mx[4], mx[5]);
           mx[1] = ca_max3(mx[1], mx[6], mx[7]);
-          // a NaN score makes the row's maximum NaN and with it the whole row; so does one of +inf
-          float m_new = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], m);
-          if (m_new == INFINITY) m_new = NAN;
-          // the first tile sets the maximum; later it moves only in steps above 2^kLazy
-          const bool grow = i == 0 || !((m_new - m) * a.to_log2 <= kLazy);
-          bool before = i > 0;  // P V of the tile before still has to be waited for
-          if (__builtin_expect(i > 0 && __any_sync(~0u, grow && m_new != m), 0)) {
+          // The maximum moves only in steps above 2^kLazy (and at the first key the row sees).  A NaN score makes
+          // it NaN and with it the whole row; so does a score of +inf, by inf - inf.
+          const float top = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.to_log2;
+          const bool grow = !(top <= mc + kLazy);
+          // P V of the tile before: whether it is through is asked ahead of the place that needs to know
+          bool before = i > 0, seen_pv = !before || ca_test(&pv_done[t], (unsigned)(on & 1));
+          if (__builtin_expect(i > 0 && __any_sync(~0u, grow), 0)) {
             ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
             if (!ok) break;
             ++on;
             before = false;
+            seen_pv = true;
             ca_fence_after();
-            const float f = grow ? (m == -INFINITY ? 0.0f : ca_exp2((m - m_new) * a.to_log2)) : 1.0f;
+            const float f = grow ? ca_exp2(mc - top) : 1.0f;
             l *= f;
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 8; ++k) {
               float o[16];
               ca_ld16(o_addr + k * 16, o);
@@ -578,10 +599,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
               ca_st16(o_addr + k * 16, reinterpret_cast<const uint32_t *>(o));
             }
           }
-          if (grow) {
-            m = m_new;
-            mc = m == -INFINITY ? 0.0f : m * a.to_log2;
-          }
+          if (grow) mc = top;
           const uint64_t add2 = ca_pair(kShift - mc, kShift - mc);
           // A pair of weights per step: scale and shift kAhead pairs ahead of the exponentials, rounding
           // and sum kBehind pairs after them, so that the special function unit is fed without a pause.
@@ -599,12 +617,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
               sums[b & 3] = ca_add2(sums[b & 3], x[b]);
             }
             if (b == 31) {
-              if (before) {  // P is free once P V of the tile before has read it
+              // P is free once P V of the tile before has read it
+              if (!__all_sync(~0u, seen_pv)) {
                 ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
                 if (!ok) break;
-                ++on;
-                ca_fence_after();
               }
+              on += before;
+              ca_fence_after();
               ca_st16(p_addr, pk);
               ca_st16(p_addr + 16, pk + 16);
             }
@@ -650,7 +669,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const bool store = live && token >= 0 && token < a.n_tokens;
       if (c.p.part >= 0) {
         const int64_t pr = (int64_t)c.head * h.part_rows + c.p.part + t * tpt * g + row;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 4; ++k) {
           float o[32];
           ca_ld32(o_addr + k * 32, o);
@@ -665,7 +684,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       } else {
         const float inv = 1.0f / l;
         uint16_t *dst = static_cast<uint16_t *>(a.out) + (token * a.n_q + hq) * kD;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 4; ++k) {
           float o[32];
           if (c.n > 0) {
