@@ -12,9 +12,14 @@
 //
 // Items are cut into pieces only where whole items would leave SMs idle: the
 // length of the longest piece is the one of 32 candidates for which the
-// estimated time is least (plan_estimate).  The pieces of a cut item leave
-// unnormalised partial rows in the workspace, which a second kernel joins in
-// the order of the pieces.
+// estimated time is least (plan_estimate).  Where there are fewer items than
+// SMs, a second way to cut is weighed against these: all items of all heads in
+// a row, and every CTA takes the same number of K/V tiles of that row (an
+// `even` plan; its list holds the pieces of all heads, round by round).  A
+// chunk of 512 at 32256 (64 items of about 254 tiles) has 110 tiles for each of
+// 148 CTAs then; equal pieces give 127 to 128 of them.  The pieces of a cut item
+// leave unnormalised partial rows in the workspace, which a second kernel joins
+// in the order of the pieces.
 #pragma once
 
 #include "kvr_common.cuh"
@@ -37,12 +42,13 @@ struct PlanHeader {  // 64 words
   int n_splits;      // items cut into pieces, per head
   int part_rows;     // rows of partial results, per head
   int dropped;       // 1: items did not fit the list (offsets that overlap)
-  int pad[53];
+  int even;          // 1: pieces and splits name their head
+  int pad[52];
 };
 
 struct PlanPiece {   // 8 words
   int q_start;       // first token of the item, in the packed batch
-  int n_tok;         // its tokens
+  int n_tok;         // its tokens (in an even plan: head << 16 | tokens; 0: no piece)
   int first_end;     // keys its first token may see: kv_len - q_len + offset + 1 (causal), can be <= 0
   int kv_len;        // keys of the request
   int k_start;       // first key of the request in packed K/V (prompt), or the request's index (pages)
@@ -52,8 +58,8 @@ struct PlanPiece {   // 8 words
 static_assert(sizeof(PlanPiece) == 32, "piece record");
 
 struct PlanSplit {   // an item cut into pieces
-  int q_start, n_tok;
-  int part;          // row base of its first piece; the others follow, n_tok * g rows each
+  int q_start, n_tok;  // as in its pieces
+  int part;          // row base of its first piece; the others follow, n_tok * g rows each (even: see plan_even_row)
   int n_pieces;
 };
 
@@ -63,6 +69,14 @@ constexpr int kPartRows = 2 * kPlanCtas * 2 * kPlanRows;  // partial rows the wo
 __host__ __device__ inline int plan_tpt(int n_q, int n_kv) { return kPlanRows / (n_q / n_kv); }
 __host__ __device__ inline int64_t plan_max_items(int64_t n_tokens, int batch, int n_q, int n_kv) {
   return n_tokens / (2 * plan_tpt(n_q, n_kv)) + batch + 2;
+}
+
+// Rows of partial results in an even plan: CTA c has room for two pieces, its
+// first and its last, at 2c and 2c + 1; an item's pieces after its first are
+// the first ones of the CTAs that follow.
+__host__ __device__ inline int plan_even_row(int part, int k) {
+  const int slot = 2 * kPlanRows;
+  return k == 0 ? part : (part / (2 * slot) + k) * 2 * slot;
 }
 
 struct PlanArgs {

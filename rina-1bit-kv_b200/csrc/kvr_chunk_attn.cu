@@ -87,7 +87,6 @@ struct ChunkArgs {
   int64_t table_stride;
   int table_width;
   const PlanHeader *hdr;
-  int max_pieces;               // entries the plan has room for
   float to_log2;                // log2(e) / scale
   void *out;
   float *lse;
@@ -239,13 +238,14 @@ struct CaPiece {
 __device__ __forceinline__ unsigned ca_index(int r) {
   return r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
-__device__ __forceinline__ bool ca_piece(const ChunkArgs &a, const unsigned char *rec, unsigned total, int per, int r,
-                                         CaPiece &o) {
+__device__ __forceinline__ bool ca_piece(const ChunkArgs &a, const unsigned char *rec, unsigned total, unsigned heads,
+                                         int per, int r, CaPiece &o) {
   const unsigned i = ca_index(r);
   if (i >= total) return false;
-  const unsigned e = i / (unsigned)a.n_kv;
+  const unsigned e = i / heads;
   o.p = r < kCaRecords ? reinterpret_cast<const PlanPiece *>(rec)[r] : reinterpret_cast<const PlanPiece *>(a.hdr + 1)[e];
-  o.head = (int)(i - e * a.n_kv);
+  o.head = (int)(i - e * heads) + (o.p.n_tok >> 16);
+  o.p.n_tok &= 0xffff;
   o.p.n_tok = min(max(o.p.n_tok, 0), per);
   o.n = o.p.n_tok > 0 ? max(o.p.kt1 - o.p.kt0, 0) : 0;
   o.two = o.p.n_tok > (per >> 1);
@@ -339,17 +339,17 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   griddep_wait();  // what follows reads the plan, q and the cache
   griddep_launch();  // the joining kernel waits for this grid's end
 
-  // The CTA's first pieces: every role reads each of them, and a record from L2 would cost each the round
-  // trip.  They are fetched beside the header, before it is known how many of them the plan has.
+  // (the CTA's first pieces go to shared memory: every role reads each of them)
   const PlanHeader &h = *a.hdr;
-  if (tid < kCaRecords && ca_index(tid) / a.n_kv < (unsigned)a.max_pieces)
-    reinterpret_cast<PlanPiece *>(sm + kCaOffRec)[tid] =
-        reinterpret_cast<const PlanPiece *>(a.hdr + 1)[ca_index(tid) / a.n_kv];
   const bool fits = h.magic == kPlanMagic && h.n_tokens == a.n_tokens && h.n_q == a.n_q && h.n_kv == a.n_kv &&
                     h.batch == a.batch;
   if (!fits && tid == 0) atomicOr(a.err, kWsErrPlan);
-  const unsigned total = fits ? (unsigned)h.n_pieces * a.n_kv : 0;
+  const unsigned heads = h.even ? 1u : (unsigned)a.n_kv;  // KV heads that a list entry stands for
+  const unsigned total = fits ? (unsigned)h.n_pieces * heads : 0;
   const int causal = h.causal, window = h.window;
+  if (tid < kCaRecords && ca_index(tid) < total)
+    reinterpret_cast<PlanPiece *>(sm + kCaOffRec)[tid] =
+        reinterpret_cast<const PlanPiece *>(a.hdr + 1)[ca_index(tid) / heads];
   __syncthreads();
   const int g = a.n_q / a.n_kv, tpt = kPlanRows / g, per = 2 * tpt;
 
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     int fill[2] = {0, 0}, uses[2] = {0, 0};  // K and V stages, Q tiles filled so far
     CaPiece c;
     bool ok = true;
-    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
       const int64_t row = PAGED ? (int64_t)c.p.k_start * a.table_stride : 0;
       const bool known = PAGED && c.p.k_start >= 0 && c.p.k_start < a.batch;
       int id = 0, off = 0;  // paged: this lane's page and row in it, of the next K/V tile
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     int si = 0;
     bool ok = true;
     CaPiece c;
-    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
       const int tiles = c.two ? 2 : 1;
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     const uint64_t to2 = ca_pair(a.to_log2, a.to_log2);
     bool ok = true;
     CaPiece c;
-    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, per, r, c); ++r) {
+    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
       const int n_tok = min(tpt, c.p.n_tok - t * tpt);  // tokens of this tile
       if (n_tok <= 0) continue;
       const bool live = tok_in < n_tok, busy = wrow < n_tok * g;  // the row / the warp has something to do
@@ -722,7 +722,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 }
 
 // Joins the partial rows of cut items in the order of their pieces: a warp per
-// row, lane l channels 4l .. 4l+3.
+// row.  Lane k first fetches maximum and sum of piece k (and k + 32, ...), so
+// that all weights exist before a value is needed; then lane l adds up channels
+// 4l .. 4l + 3, eight pieces' loads at a time.  (One piece after the other, each
+// waiting for its maximum and then its values: 15 us for 8 rows x 16 pieces.)
 template <int DT>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
   griddep_wait();
@@ -731,36 +734,46 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
   if (h.magic != kPlanMagic || h.n_tokens != a.n_tokens || h.n_q != a.n_q || h.n_kv != a.n_kv || h.batch != a.batch) return;
   const PlanSplit *splits = plan_splits(a.hdr, a.n_tokens, a.batch, a.n_q, a.n_kv);
   const int lane = threadIdx.x & 31, g = a.n_q / a.n_kv, rows = 2 * (kPlanRows / g) * g;
-  const int64_t units = (int64_t)h.n_splits * a.n_kv * rows;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
-    const int row = (int)(u % rows);
-    const int64_t sh = u / rows;
-    const PlanSplit sp = splits[sh / a.n_kv];
+  const int heads = h.even ? 1 : a.n_kv;  // KV heads that a split stands for
+  const int units = h.n_splits * heads * rows;  // (splits have workspace rows each, of which there are 75776)
+  for (int u = blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += gridDim.x * 8) {
+    const int sh = u / rows, row = u - sh * rows, e = sh / heads;
+    PlanSplit sp = splits[e];
+    const int head = sh - e * heads + (sp.n_tok >> 16);
+    sp.n_tok &= 0xffff;
     if (row >= sp.n_tok * g) continue;
-    const int head = (int)(sh % a.n_kv);
-    const int64_t r0 = (int64_t)head * h.part_rows + sp.part + row, step = (int64_t)sp.n_tok * g;
-    float m = -INFINITY;
-    for (int k = lane; k < sp.n_pieces; k += 32) {
-      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r0 + k * step) * 2);
-      if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    }
-    m = warp_max(m);
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < sp.n_pieces; ++k) {
-      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r0 + k * step) * 2);
-      if (ml.y == 0.0f) continue;  // a piece in which the row sees nothing
-      const float4 x = *reinterpret_cast<const float4 *>(a.part_o + (r0 + k * step) * kD + lane * 4);
-      const float f = exp2f(ml.x - m);
-      l += f * ml.y;
-      o[0] += f * x.x;
-      o[1] += f * x.y;
-      o[2] += f * x.z;
-      o[3] += f * x.w;
+    const int64_t r0 = h.even ? sp.part + row : (int64_t)head * h.part_rows + sp.part + row;
+    const int64_t r1 = (h.even ? plan_even_row(sp.part, 1) + row : r0 + sp.n_tok * g);  // piece 1; then equal steps
+    const int64_t step = h.even ? 4 * kPlanRows : sp.n_tok * g;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < sp.n_pieces; k0 += 32) {
+      const int k = k0 + lane;
+      const int64_t r = k == 0 ? r0 : r1 + (k - 1) * step;
+      const float2 ml = k < sp.n_pieces ? *reinterpret_cast<const float2 *>(a.part_ml + r * 2) : make_float2(0.0f, 0.0f);
+      // (a piece in which the row sees nothing has the sum 0)
+      const float mn = fmaxf(m, warp_max(ml.y != 0.0f ? ml.x : -INFINITY));
+      const float f = ml.y != 0.0f ? exp2f(ml.x - mn) : 0.0f;
+      const float old = m == -INFINITY ? 0.0f : exp2f(m - mn);
+      m = mn;
+      l = l * old + warp_sum(f * ml.y);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] *= old;
+      const int n = min(32, sp.n_pieces - k0);
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const float w = __shfl_sync(0xffffffffu, f, j);
+        const int64_t rj = k0 + j == 0 ? r0 : r1 + (k0 + j - 1) * step;
+        const float4 x = *reinterpret_cast<const float4 *>(a.part_o + rj * kD + lane * 4);
+        o[0] += w != 0.0f ? w * x.x : 0.0f;
+        o[1] += w != 0.0f ? w * x.y : 0.0f;
+        o[2] += w != 0.0f ? w * x.z : 0.0f;
+        o[3] += w != 0.0f ? w * x.w : 0.0f;
+      }
     }
     const int64_t token = (int64_t)sp.q_start + row / g;
     const int hq = head * g + row % g;
     if (token < 0 || token >= a.n_tokens) continue;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     uint2 w = make_uint2(ca_pack<DT>(o[0] * inv, o[1] * inv), ca_pack<DT>(o[2] * inv, o[3] * inv));
     if (l == 0.0f) w = make_uint2(0u, 0u);
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (token * a.n_q + hq) * kD + lane * 4) = w;
@@ -829,7 +842,6 @@ static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float sca
   KVR_REQUIRE(scale == scale && scale <= 3.0e38f, "%s: bad scale", fn);
   a.to_log2 = kLog2e / (scale > 0.0f ? scale : sqrtf((float)d));
   a.hdr = static_cast<const PlanHeader *>(plan);
-  a.max_pieces = (int)(plan_max_items(a.n_tokens, a.batch, a.n_q, a.n_kv) + kPlanExtra);
   a.err = static_cast<unsigned *>(workspace);
   a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWsHeader);
   a.part_ml = a.part_o + kD * (size_t)kPartRows;
@@ -848,7 +860,7 @@ static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
   const cudaError_t e = launch_dependent(chunk_attn_kernel<DT, PAGED>, kPlanCtas, kCaThreads, kCaSmem, st, c.mq, c.mk,
                                          c.mv, c.a);
   if (e != cudaSuccess) return e;
-  return launch_dependent(chunk_join_kernel<DT>, kPlanCtas * 2, 256, 0, st, c.a);
+  return launch_dependent(chunk_join_kernel<DT>, kPlanCtas * 4, 256, 0, st, c.a);
 }
 
 static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr_stream_t stream) {

@@ -110,6 +110,7 @@ struct PlanShared {
   int64_t warp_sums[32];
   float time[kPlanCands];        // estimate of each candidate
   int longest_kv, longest, n_splits, n_rows;
+  int ahead[kPlanCtas + 1];      // even plan: exclusive sum of the items' K/V tiles
 };
 
 // Candidate lengths of the longest piece: the longest item in k parts.
@@ -129,6 +130,115 @@ __device__ __forceinline__ float plan_estimate(float work, float count, float ro
   if (pieces <= kPlanCtas) return top + joined + (rows > 0.0f ? 2.0f * fminf(1.0f, rows / (256.0f * count)) : 0.0f);
   const float rounds = pieces / kPlanCtas, mean = total / pieces, u = fminf(1.0f, mean / top);
   return joined + fmaxf(top, total / kPlanCtas + (ceilf(rounds) - rounds) * mean * u * u * u * u);
+}
+
+__device__ __forceinline__ void plan_header(const PlanArgs &a, int n_pieces, int n_splits, int part_rows, int dropped,
+                                            int even) {
+  PlanHeader &h = *a.hdr;
+  h.magic = kPlanMagic;
+  h.n_tokens = a.n_tokens;
+  h.batch = a.batch;
+  h.n_q = a.n_q;
+  h.n_kv = a.n_kv;
+  h.causal = a.causal;
+  h.window = a.window;
+  h.n_pieces = n_pieces;
+  h.n_splits = n_splits;
+  h.part_rows = part_rows;
+  h.dropped = dropped;
+  h.even = even;
+}
+
+// The even plan for n items (at most one per CTA and head, item tid in `mine`);
+// false, with nothing written, where the best of the candidates is as good.
+__device__ bool plan_even(const PlanArgs &a, PlanShared &s, int n, const PlanPiece &mine, int longest) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int len = tid < n ? mine.kt1 - mine.kt0 : 0;
+  int64_t sum;
+  const int at = (int)min(block_exclusive(len, s.warp_sums, sum), (int64_t)(INT_MAX / 1024));
+  if (tid <= n) s.ahead[tid] = at;  // thread n: the sum of all
+  __syncthreads();
+  const int64_t work = sum * a.n_kv;
+  float best = s.time[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  // a CTA has two pieces more often than not: a tile each to fill and drain, two for partial rows, three to join
+  const float even = (float)((work + kPlanCtas - 1) / kPlanCtas) + 2.0f + 2.0f + 3.0f;
+  if (work > INT_MAX / 2 || !(even < best)) return false;
+  // CTA c: tiles [lo, hi) of the row of all items, heads innermost; at most kRounds pieces
+  constexpr int kRounds = (kPlanExtra + 2) / kPlanCtas;
+  const int c = tid;
+  int lo = 0, hi = 0, item = 0, head = 0, rounds = 0;
+  if (c < kPlanCtas) {
+    lo = (int)(work * c / kPlanCtas);
+    hi = (int)(work * (c + 1) / kPlanCtas);
+    // an item's heads follow one another, len tiles each, from n_kv * ahead on
+    item = last_not_above(s.ahead, n, lo / a.n_kv);
+    while (item + 1 < n && s.ahead[item + 1] * a.n_kv <= lo) ++item;
+    const int il = s.ahead[item + 1] - s.ahead[item];
+    head = il > 0 ? (lo - s.ahead[item] * a.n_kv) / il : 0;
+    // how many pieces that makes
+    int pos = lo, it = item, hd = head;
+    while (pos < hi) {
+      const int l1 = s.ahead[it + 1] - s.ahead[it], end = s.ahead[it] * a.n_kv + (hd + 1) * l1;
+      if (l1 > 0) {
+        pos = min(hi, end);
+        ++rounds;
+      }
+      if (l1 == 0 || pos == end) {
+        if (l1 == 0 || ++hd == a.n_kv) {
+          hd = 0;
+          ++it;
+        }
+      }
+    }
+  }
+  // items without tiles still need their zero rows: leave those calls, and ranges of many items, to the candidates
+  const int empty = tid < n && len == 0;
+  const int most = (int)__reduce_max_sync(0xffffffffu, empty ? kRounds + 1 : rounds);
+  if (tid == 0) s.n_rows = 0;
+  __syncthreads();
+  if (lane == 0) atomicMax(&s.n_rows, most);
+  __syncthreads();
+  const int n_rounds = s.n_rows;
+  __syncthreads();
+  if (tid == 0) s.n_rows = 0;
+  if (n_rounds > kRounds) return false;
+  if (c < kPlanCtas) {
+    int pos = lo;
+    for (int r = 0; r < n_rounds; ++r) {
+      PlanPiece p{};
+      if (pos < hi) {
+        while (s.ahead[item + 1] == s.ahead[item]) ++item;
+        const int l1 = s.ahead[item + 1] - s.ahead[item], begin = s.ahead[item] * a.n_kv + head * l1, end = begin + l1;
+        const int to = min(hi, end);
+        const int b = last_not_above(s.first, a.batch + 1, item);
+        p = plan_item(a, plan_request(a, b), item - s.first[b]);
+        const int kt0 = p.kt0, slot = 2 * c + (pos > lo ? 1 : 0);
+        const bool cut = pos > begin || to < end;
+        p.n_tok |= head << 16;
+        p.kt0 = kt0 + pos - begin;
+        p.kt1 = kt0 + to - begin;
+        p.part = cut ? slot * 2 * kPlanRows : -1;
+        if (cut && pos == begin) {  // the CTA with an item's first piece enters the item
+          // its last tile, end - 1, is CTA l's for the l with work * l / G <= end - 1 < work * (l + 1) / G
+          int l = (int)((int64_t)(end - 1) * kPlanCtas / work);
+          while ((int)(work * (l + 1) / kPlanCtas) <= end - 1) ++l;
+          while ((int)(work * l / kPlanCtas) > end - 1) --l;
+          a.splits[atomicAdd(&s.n_splits, 1)] = PlanSplit{p.q_start, p.n_tok, p.part, l - c + 1};
+        }
+        pos = to;
+        if (to == end && ++head == a.n_kv) {
+          head = 0;
+          ++item;
+        }
+      }
+      a.pieces[r * kPlanCtas + ((r & 1) ? kPlanCtas - 1 - c : c)] = p;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) plan_header(a, n_rounds * kPlanCtas, s.n_splits, 0, 0, 1);
+  return true;
 }
 
 // One CTA.  Two passes over the items (their lengths; their places), an item
@@ -212,6 +322,7 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
     if (lane == 0) s.time[warp] = fits ? plan_estimate(work, count, rows, top, a.n_kv) : INFINITY;
   }
   __syncthreads();
+  if (n * a.n_kv <= kPlanCtas && plan_even(a, s, n, mine, longest)) return;
   float best = s.time[lane];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -253,20 +364,7 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    PlanHeader &h = *a.hdr;
-    h.magic = kPlanMagic;
-    h.n_tokens = a.n_tokens;
-    h.batch = a.batch;
-    h.n_q = a.n_q;
-    h.n_kv = a.n_kv;
-    h.causal = a.causal;
-    h.window = a.window;
-    h.n_pieces = (int)total;
-    h.n_splits = s.n_splits;
-    h.part_rows = s.n_rows;
-    h.dropped = dropped;
-  }
+  if (tid == 0) plan_header(a, (int)total, s.n_splits, s.n_rows, dropped, 0);
 }
 static_assert(kPlanCands == kPlanThreads / 32, "one candidate per warp");
 static_assert(kPlanBins == kPlanThreads, "one bin per thread in the scan");

@@ -267,6 +267,16 @@ def test_paged_attn_scale_and_full():
     run_paged([33, 150, 1], [100, 0, 400], 8, 2, 16, F16, causal=False)
 
 
+@pytest.mark.parametrize("new,ctx,n_q,n_kv,window", [
+    ([512], [8000], 32, 8, 0),                     # fewer items than SMs, long ones: every CTA takes an equal range
+    ([300, 40], [5000, 9000], 8, 2, 0),            # ... of items of two requests
+    ([100, 700], [3000, 2500], 16, 1, 2000),
+    ([64, 3, 65], [12000, 11000, 100], 6, 2, 0)])
+def test_paged_attn_few_long_items(new, ctx, n_q, n_kv, window):
+    run_paged(new, ctx, n_q, n_kv, 64, BF16, window=window, seed=4)
+    run_paged(new, ctx, n_q, n_kv, 16, F16, window=window, seed=5)
+
+
 def test_paged_attn_many_requests_long_and_short():
     """More work than CTAs, lengths from 1 to 6000 in one call."""
     rng = np.random.default_rng(5)
