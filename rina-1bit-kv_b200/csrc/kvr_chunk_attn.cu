@@ -52,6 +52,11 @@
 // and their V rows are zeroed in shared memory, because 0 times a NaN of a
 // neighbour would still be a NaN.
 //
+// Rows without a query (a decode step has g of them in 128) are kept at zero,
+// in Q and in P: the MMAs over them cost no time that the memory does not, but
+// with other requests' queries in them they cost power, and with it clock
+// (decode of 32 x 16384 back to back: 418 -> 387 us).
+//
 // Every wait is bounded; one that gives up sets the error word, lets the
 // copies and MMAs in flight drain and frees the tensor memory.
 #include <cuda.h>
@@ -73,6 +78,7 @@ constexpr int kCaRecords = 64;                  // pieces of a CTA kept in share
 constexpr uint32_t kCaOffRec = (kCaOffBar + kCaBars * 8 + 16 + 31) / 32 * 32;
 constexpr uint32_t kCaSmem = kCaOffRec + kCaRecords * 32;
 constexpr uint32_t kCaTmemCols = 512;
+constexpr int kCaFewTokens = 8;  // a query tile with at most so many tokens is loaded token by token
 constexpr float kLazy = 6.0f, kShift = 4.0f;
 constexpr float kLowest = -1e30f;  // maximum of a row that has seen nothing: finite, so that -inf - it is -inf
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -293,8 +299,9 @@ __device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
 
 template <int DT, bool PAGED>
 __global__ void __launch_bounds__(kCaThreads, 1)
-    chunk_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                      const __grid_constant__ CUtensorMap mv, const ChunkArgs a) {
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mq1,
+                      const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                      const ChunkArgs a) {
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t *kv_full = reinterpret_cast<uint64_t *>(sm + kCaOffBar);
   uint64_t *kv_empty = kv_full + kCaStages;
@@ -361,6 +368,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   } else if (warp == 9) {
     // ---- copies
     int fill[2] = {0, 0}, uses[2] = {0, 0};  // K and V stages, Q tiles filled so far
+    int zero_from[2] = {128, 128};           // rows of the Q tiles that hold zeros
     CaPiece c;
     bool ok = true;
     for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
@@ -395,11 +403,30 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       };
       auto load_q = [&](int t) {
         if (uses[t] > 0 && !ca_wait(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
-        if (lane == 0) {
-          const uint32_t dst = smem_u32(sm) + t * kCaTile;
-          mbar_expect_tx(&q_full[t], 2u * 128u * tpt * g);
-          ca_tma5(dst, &mq, 0, c.p.q_start + t * tpt, 0, c.head, &q_full[t]);
-          ca_tma5(dst + kCaHalf, &mq, 0, c.p.q_start + t * tpt, 1, c.head, &q_full[t]);
+        const uint32_t dst = smem_u32(sm) + t * kCaTile;
+        const int n_tok = min(tpt, c.p.n_tok - t * tpt);
+        if (n_tok <= kCaFewTokens) {  // token by token, zeros below
+          unsigned char *qs = sm + t * kCaTile;
+          const int from = n_tok * g * 8;  // 16-byte pieces of a half row
+          for (int e = from + lane; e < zero_from[t] * 8; e += 32) {
+            *reinterpret_cast<uint4 *>(qs + e * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(qs + kCaHalf + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          zero_from[t] = n_tok * g;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (lane == 0) mbar_expect_tx(&q_full[t], 2u * 128u * n_tok * g);
+          __syncwarp();
+          if (lane < 2 * n_tok) {
+            const int k = lane >> 1, half = lane & 1;
+            ca_tma5(dst + half * kCaHalf + k * g * 128, &mq1, 0, c.p.q_start + t * tpt + k, half, c.head, &q_full[t]);
+          }
+        } else {
+          zero_from[t] = 128;
+          if (lane == 0) {
+            mbar_expect_tx(&q_full[t], 2u * 128u * tpt * g);
+            ca_tma5(dst, &mq, 0, c.p.q_start + t * tpt, 0, c.head, &q_full[t]);
+            ca_tma5(dst + kCaHalf, &mq, 0, c.p.q_start + t * tpt, 1, c.head, &q_full[t]);
+          }
         }
         ++uses[t];
         return true;
@@ -540,7 +567,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int begin = window > 0 ? max(0, c.p.first_end + tok - window) : 0;
       const int end_a = causal ? min(c.p.kv_len, c.p.first_end + tok_a) : c.p.kv_len;
       const int begin_b = window > 0 ? max(0, c.p.first_end + tok_b - window) : 0;
-      float mc = kLowest, l = 0.0f;  // running maximum in log2 units, sum
+      float mc = live ? kLowest : INFINITY, l = 0.0f;  // running maximum in log2 units (rows without a query: weights 0), sum
       for (int i = 0; i < c.n; ++i, ++sn) {
         ok = __all_sync(~0u, ca_wait(&s_full[t], (unsigned)(sn & 1), abort_s));
         if (!ok) break;
@@ -643,6 +670,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           ca_fence_before();
         } else {
           if (lane == 0) ca_arrive(s_free);
+          if (i == 0) {  // no query in the warp's rows: weights 0
+            const uint32_t zero[16] = {};
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) ca_st16(p_addr + k * 16, zero);
+            ca_wait_st();
+            ca_fence_before();
+          }
           if (i > 0) {
             ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
             if (!ok) break;
@@ -814,7 +848,7 @@ struct ChunkCall {
   const void *q, *k, *v;
   int64_t q_stride;
   ChunkArgs a;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mq1, mk, mv;  // mq1: q one token at a time
 };
 
 static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float scale, const void *plan,
@@ -857,8 +891,8 @@ static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  const cudaError_t e = launch_dependent(chunk_attn_kernel<DT, PAGED>, kPlanCtas, kCaThreads, kCaSmem, st, c.mq, c.mk,
-                                         c.mv, c.a);
+  const cudaError_t e = launch_dependent(chunk_attn_kernel<DT, PAGED>, kPlanCtas, kCaThreads, kCaSmem, st, c.mq, c.mq1,
+                                         c.mk, c.mv, c.a);
   if (e != cudaSuccess) return e;
   return launch_dependent(chunk_join_kernel<DT>, kPlanCtas * 4, 256, 0, st, c.a);
 }
@@ -871,7 +905,8 @@ static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr
   const cuuint64_t qd[5] = {64, (cuuint64_t)g, (cuuint64_t)a.n_tokens, 2, (cuuint64_t)a.n_kv};
   const cuuint64_t qs[4] = {kD * 2, (cuuint64_t)c.q_stride * 2, 128, (cuuint64_t)g * kD * 2};
   const cuuint32_t qb[5] = {64, (cuuint32_t)g, (cuuint32_t)tpt, 1, 1};
-  if (!make_map(&c.mq, dtype, c.q, 5, qd, qs, qb)) return set_error(KVR_EINVAL, "%s: q has a layout TMA cannot read", fn);
+  const cuuint32_t qb1[5] = {64, (cuuint32_t)g, 1, 1, 1};
+  if (!make_map(&c.mq, dtype, c.q, 5, qd, qs, qb) || !make_map(&c.mq1, dtype, c.q, 5, qd, qs, qb1)) return set_error(KVR_EINVAL, "%s: q has a layout TMA cannot read", fn);
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e;

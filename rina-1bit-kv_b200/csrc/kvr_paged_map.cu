@@ -246,7 +246,7 @@ __device__ bool plan_even(const PlanArgs &a, PlanShared &s, int n, const PlanPie
 // lengths, not over the items.  Atomics on shared counters are made once per
 // warp and value: 700 items of one length on one counter cost more than all of
 // the rest (map of 48 prompts: 50 us with an atomic per item and candidate
-// sums over the items, PLACEHOLDER us this way).
+// sums over the items, 14.8 us this way).
 __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.n_q / a.n_kv, per = 2 * plan_tpt(a.n_q, a.n_kv);
