@@ -32,7 +32,7 @@
 // What binds a long prompt: a warpgroup's chain of a K/V tile, about 2900
 // cycles beside the other warpgroup's, and 500 more until the next S is seen,
 // against 2048 cycles of MMA for both tiles.  Tensor pipe and special function
-// unit (16 exponentials a cycle) are 61 % active each.  With the MMAs reduced to
+// unit (16 exponentials a cycle) are 70 % active each.  With the MMAs reduced to
 // one step in eight a chunk of 512 at 32256 takes 3 % less, without the
 // exponentials 7 %, without both 33 %: what is left is the issue of some 560
 // instructions a tile by one warp per scheduler and tile.  So the slow paths
@@ -80,7 +80,7 @@ constexpr uint32_t kCaSmem = kCaOffRec + kCaRecords * 32;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr int kCaFewTokens = 8;  // a query tile with at most so many tokens is loaded token by token
 constexpr float kLazy = 6.0f, kShift = 4.0f;
-constexpr float kLowest = -1e30f;  // maximum of a row that has seen nothing: finite, so that -inf - it is -inf
+constexpr float kLowest = -3e38f;  // maximum of a row that has seen nothing: finite, so that -inf - it is -inf
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 

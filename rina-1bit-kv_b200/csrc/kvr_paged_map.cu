@@ -74,7 +74,7 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, int b) {
     r.k_start = b;
   } else if (a.cu_k) {
     r.k_start = max(a.cu_k[b], 0);
-    r.kv_len = max(a.cu_k[b + 1] - r.k_start, 0);
+    r.kv_len = min(max(a.cu_k[b + 1] - r.k_start, 0), 2 * kPlanMaxLen);
   } else {
     r.k_start = lo;
     r.kv_len = r.q_len;
