@@ -489,7 +489,7 @@ KVR_API int kvr_paged_write(const void *q, const void *k, const void *v, int dty
 /* Attention of a step's query tokens over their requests' pages (a plan with
  * kv_len) or over packed prompts (a plan without, or with cu_k): q (n_tokens,
  * n_q, d) with token stride q_stride, out (n_tokens, n_q, d) contiguous of the
- * same type and 32-byte aligned, lse (n_tokens, n_q) fp32 natural log or NULL.  scale <= 0 means
+ * same type, 32-byte aligned and not q itself, lse (n_tokens, n_q) fp32 natural log or NULL.  scale <= 0 means
  * sqrt(d) (scores are divided by it).  The page size must be a multiple of 8.
  * Missing pages (entries outside [0, n_pages)) read as zeros.  Keys beyond a
  * request's length never reach its output, whatever the pool holds there.

@@ -899,6 +899,7 @@ static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
 
 static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr_stream_t stream) {
   const ChunkArgs &a = c.a;
+  KVR_REQUIRE(a.out != c.q, "%s: out must not be q (pieces of one row read q at different times)", fn);
   if (!encode_tiled()) return set_error(KVR_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", fn);
   const int g = a.n_q / a.n_kv, tpt = kPlanRows / g;
   // q as (64 channels, head of the group, token, channel half, KV head)

@@ -558,12 +558,26 @@ def _pool(k_pages, v_pages):
     return shape[0], shape[1], strides[0], strides[1]
 
 
+_INT32 = torch.int32
+
+
 def _i32(x, name, numel=None):
-    if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+    """Checks an int32 vector; returns its number of entries."""
+    n = x.numel()
+    if x.dtype is not _INT32 or x.dim() != 1 or not x.is_contiguous():
         raise TypeError(f"{name} must be a contiguous int32 vector")
-    if numel is not None and x.numel() != numel:
-        raise ValueError(f"{name} must have {numel} entries, got {x.numel()}")
-    return x
+    if numel is not None and n != numel:
+        raise ValueError(f"{name} must have {numel} entries, got {n}")
+    return n
+
+
+def _on_gpu(*tensors):
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError("kvr_b200 operators need CUDA tensors (this build has no CPU path)")
+
+
+_PLAN_BYTES: dict = {}
 
 
 class AttnPlan:
@@ -572,7 +586,13 @@ class AttnPlan:
 
     def __init__(self, n_tokens, batch, n_q, n_kv, paged, device):
         self.n_tokens, self.batch, self.n_q, self.n_kv, self.paged = n_tokens, batch, n_q, n_kv, paged
-        self.nbytes = max(call("kvr_attn_plan_bytes", n_tokens, batch, n_q, n_kv), 16)
+        key = (n_tokens, batch, n_q, n_kv)
+        nbytes = _PLAN_BYTES.get(key)
+        if nbytes is None:
+            if len(_PLAN_BYTES) > 4096:
+                _PLAN_BYTES.clear()
+            nbytes = _PLAN_BYTES[key] = max(call("kvr_attn_plan_bytes", *key), 16)
+        self.nbytes = nbytes
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
 
     def _match(self, n_tokens, n_q, paged):
@@ -618,18 +638,18 @@ def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens,
     the end of free_pages[:n_free] and are entered into block_table (B, width)
     in place.  n_tokens: the step's packed length (>= the sum of new_len; the
     rest is padding).  ctx_len, new_len and n_free are left as they are."""
-    batch = ctx_len.numel()
-    _i32(ctx_len, "ctx_len")
+    batch = _i32(ctx_len, "ctx_len")
     _i32(new_len, "new_len", batch)
-    _i32(free_pages, "free_pages")
+    n_pages = _i32(free_pages, "free_pages")
     _i32(n_free, "n_free", 1)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+    if block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise TypeError("block_table must be an int32 matrix with contiguous rows")
-    if block_table.shape[0] < batch:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {batch} requests")
+    rows, width = block_table.shape
+    if rows < batch:
+        raise ValueError(f"block_table has {rows} rows for {batch} requests")
+    _on_gpu(ctx_len, new_len, free_pages, n_free, block_table)
     dev = ctx_len.device
-    width = block_table.shape[1]
-    buf = torch.empty(2 * batch + 6 + n_tokens, dtype=torch.int32, device=dev)
+    buf = torch.empty(2 * batch + 6 + n_tokens, dtype=_INT32, device=dev)
     st = PagedStep()
     st.cu_q, st.kv_len, st.n_free, st.info, st.positions = torch.split_with_sizes(buf, (batch + 1, batch, 1, 4, n_tokens))
     st.slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
@@ -637,8 +657,8 @@ def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens,
     st.plan = AttnPlan(n_tokens, batch, n_q, n_kv, True, dev) if n_q else None
     at = buf.data_ptr()
     plan = st.plan
-    call("kvr_paged_map", ptr(ctx_len), ptr(new_len), batch, n_tokens, page, ptr(block_table),
-         max(block_table.stride(0), width), width, ptr(free_pages), free_pages.numel(), ptr(n_free), at,
+    call("kvr_paged_map", ctx_len.data_ptr(), new_len.data_ptr(), batch, n_tokens, page, block_table.data_ptr(),
+         max(block_table.stride(0), width), width, free_pages.data_ptr(), n_pages, n_free.data_ptr(), at,
          at + 4 * (batch + 1), at + 4 * (2 * batch + 6), st.slots.data_ptr(), at + 4 * (2 * batch + 1),
          at + 4 * (2 * batch + 2), n_q, n_kv, window, plan.buf.data_ptr() if plan else None,
          plan.nbytes if plan else 0, stream())
@@ -651,34 +671,40 @@ def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=
     the pools (n_pages, page, n_kv, d).  Returns the rotated q (None if q is);
     rows of tokens with slot -1 are 0."""
     n_pages, page, ps, ts = _pool(k_pages, v_pages)
-    n_tokens = k.shape[0]
+    dt = k_pages.dtype
     k, ks = _tokens(k, "k")
     v, vs = _tokens(v, "v")
-    if k.dtype != k_pages.dtype or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    n_tokens, n_kv, _ = shape = k.shape
+    if k.dtype is not dt or v.dtype is not dt or (q is not None and q.dtype is not dt):
         raise TypeError("q, k, v and the pools must share a dtype")
-    if k.shape != v.shape or k.shape[1] != k_pages.shape[2] or (q is not None and q.shape[0] != n_tokens):
+    if v.shape != shape or n_kv != k_pages.shape[2] or (q is not None and q.shape[0] != n_tokens):
         raise ValueError("q, k, v and the pools do not fit together")
-    if slots.dtype != torch.int64 or not slots.is_contiguous() or slots.numel() != n_tokens:
+    if slots.dtype is not torch.int64 or slots.numel() != n_tokens or not slots.is_contiguous():
         raise TypeError("slots must be a contiguous int64 vector, one per token")
-    qs, n_q, rs, max_pos = 0, 0, 0, 0
+    _on_gpu(k, v, k_pages, v_pages, slots)
+    qp = qo = cp = sp = pp = None
+    qs = n_q = rs = max_pos = 0
     if q is not None:
         q, qs = _tokens(q, "q")
         n_q = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(n_tokens, n_q, D, dtype=q.dtype, device=q.device)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif q_out.shape != q.shape or q_out.dtype is not dt or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous and of q's shape and dtype")
+        _on_gpu(q, q_out)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
     if cos is not None:
         _i32(positions, "positions", n_tokens)
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
             raise TypeError("the RoPE tables must be fp32")
-        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D:
+        max_pos, width = table = cos.shape
+        if sin.shape != table or width != D:
             raise ValueError(f"the RoPE tables must be (max_pos, {D})")
         cos, sin, rs = _rope_args(cos, sin)
-        max_pos = cos.shape[0]
-    call("kvr_paged_write", ptr(q), ptr(k), ptr(v), dtype_code(k), n_tokens, n_q, k.shape[1], D, qs, ks, vs, ptr(cos),
-         ptr(sin), rs, max_pos, ptr(positions) if cos is not None else None, ptr(slots), ptr(q_out), ptr(k_pages),
-         ptr(v_pages), n_pages, page, ps, ts, stream())
+        _on_gpu(positions, cos, sin)
+        cp, sp, pp = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    call("kvr_paged_write", qp, k.data_ptr(), v.data_ptr(), dtype_code(k), n_tokens, n_q, n_kv, D, qs, ks, vs, cp, sp, rs,
+         max_pos, pp, slots.data_ptr(), qo, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ps, ts, stream())
     return q_out
 
 
@@ -686,22 +712,33 @@ _ATTN_WS: dict = {}
 
 
 def _attn_workspace(device):
-    """The attention workspace of the current stream and its bytes (calls on
-    one stream do not overlap; each stream has its own).  Its size does not
-    depend on the call."""
+    """(address, bytes) of the attention workspace, and the current stream.
+    Calls on one stream do not overlap, so each stream has its own; its size
+    does not depend on the call.  A call in a graph capture on a stream without
+    one takes the device's capture workspace, allocated by the first call
+    outside of a capture: what a capture allocates is zeroed at each replay and
+    belongs to the graph."""
     s = stream()
     ws = _ATTN_WS.get((s, device))
     if ws is None:
-        nbytes = call("kvr_attn_workspace_bytes")
-        ws = _ATTN_WS[s, device] = (N.workspace(f"attn_work_{s}", nbytes, device), nbytes)
+        if torch.cuda.is_current_stream_capturing():
+            ws = _ATTN_WS.get(("capture", device))
+            if ws is None:
+                raise RuntimeError("the first attention call on a device must be made outside of a graph capture")
+        else:
+            nbytes = call("kvr_attn_workspace_bytes")
+            for key in (s, "capture"):
+                if (key, device) not in _ATTN_WS:
+                    _ATTN_WS[key, device] = (N.workspace(f"attn_work_{key}", nbytes, device), nbytes)
+            ws = _ATTN_WS[s, device]
     return ws[0].data_ptr(), ws[1], s
 
 
 def _attn_out(q, out, return_lse):
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous and of q's shape and dtype")
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() == q.data_ptr():
+        raise ValueError("out must be contiguous, of q's shape and dtype, and not q itself")
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     return out, lse
 
@@ -714,20 +751,22 @@ def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, ret
     q, qs = _tokens(q, "q")
     n_tokens, n_q, _ = q.shape
     plan._match(n_tokens, n_q, True)
-    if q.dtype != k_pages.dtype:
+    if q.dtype is not k_pages.dtype:
         raise TypeError("q and the pools must share a dtype")
     if k_pages.shape[2] != plan.n_kv:
         raise ValueError(f"the plan is for {plan.n_kv} KV heads, the pool has {k_pages.shape[2]}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+    if block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise TypeError("block_table must be an int32 matrix with contiguous rows")
-    if block_table.shape[0] < plan.batch:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {plan.batch} requests")
+    rows, width = block_table.shape
+    if rows < plan.batch:
+        raise ValueError(f"block_table has {rows} rows for {plan.batch} requests")
     out, lse = _attn_out(q, out, return_lse)
+    _on_gpu(q, k_pages, v_pages, block_table, out)
     ws, ws_bytes, s = _attn_workspace(q.device)
-    width = block_table.shape[1]
-    call("kvr_paged_attn", ptr(q), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, ptr(k_pages),
-         ptr(v_pages), n_pages, page, ps, ts, ptr(block_table), max(block_table.stride(0), width), width,
-         ptr(plan.buf), plan.nbytes, float(scale or 0.0), ptr(out), ptr(lse), ws, ws_bytes, s)
+    call("kvr_paged_attn", q.data_ptr(), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, k_pages.data_ptr(),
+         v_pages.data_ptr(), n_pages, page, ps, ts, block_table.data_ptr(), max(block_table.stride(0), width), width,
+         plan.buf.data_ptr(), plan.nbytes, float(scale or 0.0), out.data_ptr(), lse.data_ptr() if return_lse else None, ws,
+         ws_bytes, s)
     return (out, lse) if return_lse else out
 
 

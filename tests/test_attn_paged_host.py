@@ -150,6 +150,13 @@ def test_prompt_attn_refusals(kw, code, match):
     _refused("kvr_prompt_attn", _prompt_args(**kw), code, match)
 
 
+def test_output_over_the_queries_is_refused():
+    from kvr_b200 import kernels as K
+    q = torch.zeros(4, 8, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="not q itself"):
+        K._attn_out(q, q, False)
+
+
 def test_nothing_to_do_is_no_error():
     from kvr_b200 import _native as N
     N.call("kvr_paged_write", *_write_args(n=0))

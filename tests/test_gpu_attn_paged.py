@@ -452,6 +452,34 @@ def test_repeated_calls_give_the_same_bits(kind):
     K.attn_status()
 
 
+def test_capture_on_a_stream_without_a_workspace():
+    """torch's own capture stream: the graph uses the device's capture workspace."""
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(21)
+    q, k, v = torch.randn(700, 12, 128, device=DEV, generator=g).half().split([8, 2, 2], 1)
+    plan = K.attn_plan(i32([0, 700]), 700, 8, 2)
+    want = K.prompt_attn(q, k, v, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.prompt_attn(q, k, v, plan)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+
+
+def test_output_over_the_queries_is_refused():
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    q = torch.randn(6, 8, 128, device=DEV).half()
+    kv = torch.randn(6, 2, 128, device=DEV).half()
+    plan = K.attn_plan(i32([0, 6]), 6, 8, 2)
+    ws, wb, s = K._attn_workspace(q.device)
+    with pytest.raises(N.KvrError, match="must not be q"):
+        N.call("kvr_prompt_attn", N.ptr(q), N.ptr(kv), N.ptr(kv), 1, 6, 6, 1, 8, 2, 128, 1024, 256, 256, N.ptr(plan.buf),
+               plan.nbytes, 0.0, N.ptr(q), None, ws, wb, s)
+
+
 def test_plan_of_another_call_is_reported():
     from kvr_b200 import _native as N
     from kvr_b200 import kernels as K
