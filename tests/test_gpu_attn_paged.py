@@ -255,6 +255,18 @@ def test_paged_attn_ignores_what_requests_do_not_own(new, ctx, window, dtype):
     run_paged(new, ctx, 8, 2, 16, dtype, window, poison=True, pad=37)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n_q,n_kv,new", [
+    (8, 8, [15, 16, 17, 300, 8, 9]), (16, 2, [2, 3, 150, 1]), (32, 2, [1, 2, 100, 1]), (34, 2, [1, 90, 1]),
+    (48, 16, [5, 6, 200, 4, 1])])
+def test_paged_attn_items_of_about_16_rows(n_q, n_kv, new, dtype):
+    """Items with up to 16 rows (tokens x heads per KV head) take a narrower
+    product: sizes on both sides of it, after one another and cut in pieces."""
+    for seed, base in enumerate((0, 130, 9000)):
+        ctx = [base + 77 * i for i in range(len(new))]
+        run_paged(new, ctx, n_q, n_kv, 16, dtype, spread=3.0 if seed else 1.0, poison=True, seed=seed, pad=3)
+
+
 @pytest.mark.parametrize("spread", [0.0, 30.0])
 def test_paged_attn_flat_and_peaked(spread):
     """All scores equal, and scores of several hundred."""
