@@ -58,7 +58,7 @@
 // (decode of 32 x 16384 back to back: 418 -> 387 us).  For the same reason a
 // piece of at most 16 rows is multiplied as M = 64: its rows 0 .. 15 lie in the
 // same lanes of tensor memory (row r in lane r / 16 * 32 + r % 16), half the
-// rows are computed (back to back 2000 times 396 -> 370 us; a plain copy of as
+// rows are computed (back to back 2000 times 396 -> 363 us; a plain copy of as
 // many bytes takes 333 us then).
 //
 // Every wait is bounded; one that gives up sets the error word, lets the
