@@ -304,11 +304,14 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
   }
   __syncthreads();
   const int longest = s.longest, low = (1 << shift) - 1;
+  // the length an item counts as: the longest of its bin, but none longer than the longest item (which the first
+  // candidate has to leave whole: only so does its list always fit)
+  auto counted = [&](int len) { return min(len | low, longest); };
   {  // warp c: candidate c
     const int top = max(1, (longest + kPlanParts[warp] - 1) / kPlanParts[warp]);
     float work = 0.0f, count = 0.0f, rows = 0.0f;
     for (int bin = lane; bin <= longest >> shift; bin += 32) {
-      const int items = s.hist[bin], len = shift ? (bin << shift) | low : bin;
+      const int items = s.hist[bin], len = counted(bin << shift);
       if (items == 0) continue;
       const int np = max(1, (len + top - 1) / top);
       work += (float)items * len;
@@ -330,8 +333,8 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
   const int parts = kPlanParts[__ffs(__ballot_sync(0xffffffffu, s.time[lane] == best)) - 1];
   const int top = max(1, (longest + parts - 1) / parts);
   // longest pieces first: counting sort by the pieces' length (thread = bin of item lengths here)
-  auto pieces_of = [&](int len) { return max(1, ((shift ? len | low : len) + top - 1) / top); };
-  auto place_of = [&](int len, int np) { return kPlanBins - 1 - ((((shift ? len | low : len) + np - 1) / np) >> shift); };
+  auto pieces_of = [&](int len) { return max(1, (counted(len) + top - 1) / top); };
+  auto place_of = [&](int len, int np) { return kPlanBins - 1 - (((counted(len) + np - 1) / np) >> shift); };
   if (s.hist[tid]) {
     const int len = tid << shift, np = pieces_of(len);
     atomicAdd(&s.place[place_of(len, np)], s.hist[tid] * np);

@@ -1,0 +1,74 @@
+"""The paged-cache serving operators at the ends of their ranges: what a call
+must not write, and what it must refuse.  Plain 64-bit forms and tolerances as
+in test_gpu_attn_paged.py unless said."""
+import pytest
+import torch
+
+from test_gpu_attn_paged import BF16, DEV, F16, exact, i32, offsets
+
+pytestmark = pytest.mark.gpu
+
+
+def read_plan(buf):
+    """Plan buffer -> (header words, pieces (n, 8)) on the host."""
+    w = buf.cpu().view(torch.int32)
+    return w[:64].tolist(), w[64:64 + 8 * w[7].item()].view(-1, 8)
+
+
+# More items than a list has extra room for (512), all as long as the longest, in bins of more than one length: from
+# 1024 K/V tiles on.  None may be cut then, and nothing may be written behind the plan.
+@pytest.mark.parametrize("new,kv,n_q,n_kv,causal", [
+    ([1] * 600, [131072] * 600, 4, 1, True),
+    ([1] * 600, [131072 - 128] * 600, 4, 1, True),   # 1023 tiles: one length a bin
+    ([1] * 513, [262400] * 513, 8, 8, True),         # 2050 tiles, four lengths a bin
+    ([70000], [131072], 4, 1, False),
+    ([1] * 300 + [2000], [131072] * 300 + [140000], 2, 2, True)])
+def test_plan_of_many_equally_long_items_stays_in_its_buffer(new, kv, n_q, n_kv, causal):
+    from kvr_b200 import _native as N
+    n = sum(new)
+    nbytes = N.call("kvr_attn_plan_bytes", n, len(new), n_q, n_kv)
+    buf = torch.full((nbytes + (1 << 20),), 0xA5, dtype=torch.uint8, device=DEV)
+    cu, kvl = offsets(new), i32(kv)
+    N.call("kvr_attn_plan", N.ptr(cu), N.ptr(kvl), None, len(new), n, n_q, n_kv, int(causal), 0, N.ptr(buf), nbytes,
+           N.stream())
+    assert (buf[nbytes:] == 0xA5).all()
+    head, pieces = read_plan(buf)
+    per = 2 * (128 // (n_q // n_kv))
+    items = sum(-(-m // per) for m in new)
+    assert head[10] == 0 and head[11] == 0
+    assert head[7] <= items + 512 and head[8] <= 512 and head[9] * n_kv <= 75776
+    # every item's K/V tiles lie in its pieces once
+    tiles = {}
+    for q, n_tok, first, length, req, t0, t1, part in pieces.tolist():
+        tiles.setdefault((q, n_tok, first, length, req), []).append((t0, t1))
+    assert len(tiles) == items
+    for (q, n_tok, first, length, req), got in tiles.items():
+        got.sort()
+        end = min(length, first + n_tok - 1) if causal else length
+        assert got[0][0] == 0 and got[-1][1] == -(-end // 128)
+        assert all(a[1] == b[0] for a, b in zip(got, got[1:]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_paged_attn_many_requests_of_131072_keys(dtype):
+    """530 requests that share their pages.  Sums over n keys: the tensor core adds
+    n / 16 products into an fp32 accumulator, each rounded by at most 2^-23 of A,
+    beside the bound of the shorter cases."""
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(31)
+    b, n, page = 530, 131072, 64
+    k = torch.randn(n, 1, 128, device=DEV, generator=g).to(dtype)
+    ramp = torch.linspace(-1, 1, n, device=DEV)[:, None, None]  # values that tell where a key lies
+    v = (ramp + 0.1 * torch.randn(n, 1, 128, device=DEV, generator=g)).to(dtype)
+    q = torch.randn(b, 2, 128, device=DEV, generator=g).to(dtype)
+    order = torch.randperm(n // page, device=DEV, generator=g)
+    kp, vp = torch.empty(n // page, page, 1, 128, device=DEV, dtype=dtype), torch.empty(n // page, page, 1, 128, device=DEV, dtype=dtype)
+    kp[order], vp[order] = k.view(-1, page, 1, 128), v.view(-1, page, 1, 128)
+    table = order.to(torch.int32).expand(b, -1).contiguous()
+    plan = K.attn_plan(offsets([1] * b), b, 2, 1, kv_len=i32([n] * b))
+    out, lse = K.paged_attn(q, kp, vp, table, plan, return_lse=True)
+    K.attn_status()
+    want, lse_x, tol, tol_l = exact(q, k, v, causal=False)
+    tol = tol + n / 16 * 2.0 ** -23 * v.double().abs().max()
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - lse_x).abs() <= tol_l + n / 16 * 2.0 ** -23).all()
