@@ -326,7 +326,7 @@ __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
     if (lane == 0) s.time[warp] = fits ? plan_estimate(work, count, rows, top, a.n_kv) : INFINITY;
   }
   __syncthreads();
-  if (n * a.n_kv <= kPlanCtas && plan_even(a, s, n, mine, longest)) return;
+  if ((int64_t)n * a.n_kv <= kPlanCtas && plan_even(a, s, n, mine, longest)) return;
   float best = s.time[lane];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));

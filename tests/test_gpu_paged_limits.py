@@ -49,6 +49,25 @@ def test_plan_of_many_equally_long_items_stays_in_its_buffer(new, kv, n_q, n_kv,
         assert all(a[1] == b[0] for a, b in zip(got, got[1:]))
 
 
+def test_plan_of_items_times_heads_past_32_bits():
+    """2^23 items for each of 256 KV heads: far more than CTAs, whatever their
+    product is in 32 bits."""
+    from kvr_b200 import _native as N
+    n, n_q, n_kv = 1 << 24, 128 * 256, 256
+    nbytes = N.call("kvr_attn_plan_bytes", n, 1, n_q, n_kv)
+    buf = torch.full((nbytes + (1 << 20),), 0xA5, dtype=torch.uint8, device=DEV)
+    cu, kvl = i32([0, n]), i32([64])
+    N.call("kvr_attn_plan", N.ptr(cu), N.ptr(kvl), None, 1, n, n_q, n_kv, 1, 0, N.ptr(buf), nbytes, N.stream())
+    assert (buf[nbytes:] == 0xA5).all()
+    head = buf[:256].cpu().view(torch.int32).tolist()
+    assert head[7:12] == [n // 2, 0, 0, 0, 0]
+    pieces = buf[256:256 + 32 * (n // 2)].view(torch.int32).view(-1, 8)
+    starts, order = pieces[:, 0].sort()
+    assert torch.equal(starts, torch.arange(0, n, 2, dtype=torch.int32, device=DEV)) and (pieces[:, 1] == 2).all()
+    first = pieces[order, 2]
+    assert torch.equal(first, 64 - n + 1 + starts)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_paged_attn_many_requests_of_131072_keys(dtype):
     """530 requests that share their pages.  Sums over n keys: the tensor core adds
