@@ -577,6 +577,22 @@ def _on_gpu(*tensors):
             raise ValueError("kvr_b200 operators need CUDA tensors (this build has no CPU path)")
 
 
+def _table(block_table, batch):
+    """Checks a block table with a row for each of `batch` requests; returns its
+    width and row stride."""
+    if block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise TypeError("block_table must be an int32 matrix with contiguous rows")
+    rows, width = block_table.shape
+    if rows < batch:
+        raise ValueError(f"block_table has {rows} rows for {batch} requests")
+    stride = block_table.stride(0)
+    if rows == 1:  # no second row that the stride leads to
+        stride = max(stride, width)
+    elif stride < width:
+        raise ValueError("block_table: rows must not share memory (an expanded table has to be copied)")
+    return width, stride
+
+
 _PLAN_BYTES: dict = {}
 
 
@@ -642,11 +658,7 @@ def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens,
     _i32(new_len, "new_len", batch)
     n_pages = _i32(free_pages, "free_pages")
     _i32(n_free, "n_free", 1)
-    if block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-        raise TypeError("block_table must be an int32 matrix with contiguous rows")
-    rows, width = block_table.shape
-    if rows < batch:
-        raise ValueError(f"block_table has {rows} rows for {batch} requests")
+    width, stride = _table(block_table, batch)
     _on_gpu(ctx_len, new_len, free_pages, n_free, block_table)
     dev = ctx_len.device
     buf = torch.empty(2 * batch + 6 + n_tokens, dtype=_INT32, device=dev)
@@ -658,7 +670,7 @@ def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens,
     at = buf.data_ptr()
     plan = st.plan
     call("kvr_paged_map", ctx_len.data_ptr(), new_len.data_ptr(), batch, n_tokens, page, block_table.data_ptr(),
-         max(block_table.stride(0), width), width, free_pages.data_ptr(), n_pages, n_free.data_ptr(), at,
+         stride, width, free_pages.data_ptr(), n_pages, n_free.data_ptr(), at,
          at + 4 * (batch + 1), at + 4 * (2 * batch + 6), st.slots.data_ptr(), at + 4 * (2 * batch + 1),
          at + 4 * (2 * batch + 2), n_q, n_kv, window, plan.buf.data_ptr() if plan else None,
          plan.nbytes if plan else 0, stream())
@@ -755,16 +767,12 @@ def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, ret
         raise TypeError("q and the pools must share a dtype")
     if k_pages.shape[2] != plan.n_kv:
         raise ValueError(f"the plan is for {plan.n_kv} KV heads, the pool has {k_pages.shape[2]}")
-    if block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-        raise TypeError("block_table must be an int32 matrix with contiguous rows")
-    rows, width = block_table.shape
-    if rows < plan.batch:
-        raise ValueError(f"block_table has {rows} rows for {plan.batch} requests")
+    width, stride = _table(block_table, plan.batch)
     out, lse = _attn_out(q, out, return_lse)
     _on_gpu(q, k_pages, v_pages, block_table, out)
     ws, ws_bytes, s = _attn_workspace(q.device)
     call("kvr_paged_attn", q.data_ptr(), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, k_pages.data_ptr(),
-         v_pages.data_ptr(), n_pages, page, ps, ts, block_table.data_ptr(), max(block_table.stride(0), width), width,
+         v_pages.data_ptr(), n_pages, page, ps, ts, block_table.data_ptr(), stride, width,
          plan.buf.data_ptr(), plan.nbytes, float(scale or 0.0), out.data_ptr(), lse.data_ptr() if return_lse else None, ws,
          ws_bytes, s)
     return (out, lse) if return_lse else out

@@ -1,0 +1,53 @@
+"""CPU checks of the paged-cache operators and classes: what the Python calls
+hand to the native ones, what they refuse, and the host logic of PagedKVCache
+and PagedGenerator."""
+import pytest
+import torch
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.fixture
+def native(monkeypatch):
+    """The calls that would reach a GPU, recorded: name -> arguments of the last."""
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    seen, real = {}, N.call
+
+    def call(name, *args):
+        if name.endswith("_bytes"):
+            return real(name, *args)
+        seen[name] = args
+        return 0
+
+    monkeypatch.setattr(K, "call", call)
+    monkeypatch.setattr(K, "ptr", lambda t: None if t is None else t.data_ptr())
+    monkeypatch.setattr(K, "_on_gpu", lambda *t: None)
+    monkeypatch.setattr(K, "stream", lambda: 0)
+    monkeypatch.setattr(K, "_attn_workspace", lambda device: (256, 1 << 30, 0))
+    return seen
+
+
+def test_block_tables_whose_rows_share_memory_are_refused(native):
+    """A table of one row expanded to several has the stride 0: the kernels would
+    follow another stride past its storage."""
+    from kvr_b200 import kernels as K
+    pool = torch.zeros(4, 16, 2, 128, dtype=torch.float16)
+    q = torch.zeros(3, 8, 128, dtype=torch.float16)
+    plan = K.attn_plan(i32(0, 1, 2, 3), 3, 8, 2, kv_len=i32(5, 5, 5))
+    flat = torch.zeros(20, dtype=torch.int32)
+    for table in (flat[:4].expand(3, 4), flat.as_strided((3, 4), (2, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            K.paged_map(i32(5, 5, 5), i32(1, 1, 1), table, i32(0, 1, 2), i32(3), 16, 3)
+        with pytest.raises(ValueError, match="share memory"):
+            K.paged_attn(q, pool, pool, table, plan)
+    assert "kvr_paged_map" not in native and "kvr_paged_attn" not in native
+    # the stride of a view is handed on; that of a single row means nothing
+    K.paged_map(i32(5, 5, 5), i32(1, 1, 1), flat.as_strided((3, 4), (6, 1)), i32(0, 1, 2), i32(3), 16, 3)
+    assert native["kvr_paged_map"][6:8] == (6, 4)
+    K.paged_map(i32(5), i32(1), flat.as_strided((1, 4), (2, 1)), i32(0, 1, 2), i32(3), 16, 1)
+    assert native["kvr_paged_map"][6:8] == (4, 4)
+    K.paged_attn(q, pool, pool, flat.as_strided((3, 4), (6, 1)), plan)
+    assert native["kvr_paged_attn"][15:17] == (6, 4)
