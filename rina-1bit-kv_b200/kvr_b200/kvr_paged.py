@@ -82,11 +82,14 @@ class PagedKVCache:
                                f"{over} longer than max_len")
 
     def release(self, requests):
-        """Gives the pages of `requests` (a list of rows) back to the free list
-        and empties the rows; between steps only."""
+        """Gives the pages of `requests` (a list of rows; one named twice counts
+        once) back to the free list and empties the rows; between steps only."""
         if self.step is not None:
             raise RuntimeError("commit() the open step first")
-        rows = torch.tensor(list(requests), dtype=torch.int64, device=self.ctx_len.device)
+        rows = list(dict.fromkeys(int(b) for b in requests))
+        if not all(0 <= b < self.max_requests for b in rows):
+            raise ValueError(f"rows must be in [0, {self.max_requests}), got {rows}")
+        rows = torch.tensor(rows, dtype=torch.int64, device=self.ctx_len.device)
         held = (self.ctx_len[rows] + self.page - 1) // self.page
         j = torch.arange(self.block_table.shape[1], device=rows.device)
         pages = self.block_table[rows]

@@ -51,3 +51,36 @@ def test_block_tables_whose_rows_share_memory_are_refused(native):
     assert native["kvr_paged_map"][6:8] == (4, 4)
     K.paged_attn(q, pool, pool, flat.as_strided((3, 4), (6, 1)), plan)
     assert native["kvr_paged_attn"][15:17] == (6, 4)
+
+
+def held_cache():
+    """Row 0 holds pages 0, 1, row 1 pages 2, 3, 4."""
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 8, 2, 10, page=16, max_requests=3, max_len=64, device="cpu")
+    c.block_table[0, :2] = i32(0, 1)
+    c.block_table[1, :3] = i32(2, 3, 4)
+    c.ctx_len[:] = i32(17, 48, 0)
+    c.n_free.fill_(5)
+    return c
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [1, 0, 1], [0, 0, 1, 1, 2, 2]])
+def test_release_counts_a_row_once(rows):
+    c = held_cache()
+    c.release(rows)
+    n = c.n_free.item()
+    assert n == (8 if 0 not in rows else 10)
+    free = c.free_pages[:n].tolist()
+    assert len(set(free)) == n  # a page given out twice would be two requests' memory
+    held = [p for row, m in zip(c.block_table.tolist(), c.ctx_len.tolist()) for p in row[:-(-m // 16)]]
+    assert sorted(free + held) == list(range(10))
+
+
+@pytest.mark.parametrize("rows", [[3], [-1], [0, 7]])
+def test_release_refuses_rows_that_do_not_exist(rows):
+    c = held_cache()
+    with pytest.raises(ValueError, match="rows must be in"):
+        c.release(rows)
+    assert c.n_free.item() == 5 and c.ctx_len.tolist() == [17, 48, 0]
+    c.release([])
+    assert c.n_free.item() == 5
