@@ -201,6 +201,8 @@ class PagedGenerator:
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1:
             raise ValueError("every prompt needs at least one token")
+        if max(lens) > self.cos_tbl.shape[0]:
+            raise ValueError(f"a prompt of {max(lens)} tokens is longer than max_len = {self.cos_tbl.shape[0]}")
         cu = torch.tensor([0] + lens, device=self.device).cumsum(0).to(torch.int32)
         n = sum(lens)
         plan = K.attn_plan(cu, n, self.n_q, self.n_kv, window=self.cache.window)

@@ -84,3 +84,24 @@ def test_release_refuses_rows_that_do_not_exist(rows):
     assert c.n_free.item() == 5 and c.ctx_len.tolist() == [17, 48, 0]
     c.release([])
     assert c.n_free.item() == 5
+
+
+def tiny(cls="Llama", n_q=2, n_kv=1, layers=1, **kw):
+    import transformers as T
+    torch.manual_seed(0)
+    kw = {"vocab_size": 50, "hidden_size": 64, "intermediate_size": 64, "num_hidden_layers": layers,
+          "num_attention_heads": n_q, "num_key_value_heads": n_kv, "head_dim": 128, "max_position_embeddings": 64, **kw}
+    return getattr(T, cls + "ForCausalLM")(getattr(T, cls + "Config")(**kw)).half().eval()
+
+
+def generator(model=None, **kw):
+    from kvr_b200 import PagedGenerator
+    return PagedGenerator(model or tiny(), **{"n_pages": 10, "page": 16, "max_requests": 3, "max_len": 40, **kw})
+
+
+def test_score_refuses_prompts_past_the_rope_tables(native):
+    """Positions past the tables would be an index out of range on the device."""
+    gen = generator()
+    with pytest.raises(ValueError, match="longer than max_len"):
+        gen.score([[1] * 41, [2]])
+    assert not native
