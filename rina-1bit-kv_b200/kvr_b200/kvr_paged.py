@@ -146,6 +146,8 @@ class PagedGenerator:
         """One pass: new maps rows to the token ids they get (a chunk or one).
         Returns {row: logits (vocab,) fp32 after its last new token}."""
         rows = sorted(new)
+        if rows and not 0 <= rows[0] <= rows[-1] < self.cache.max_requests:
+            raise ValueError(f"rows must be in [0, {self.cache.max_requests}), got {rows}")
         lens = [len(new.get(b, ())) for b in range(self.cache.max_requests)]
         if not rows or min(lens[b] for b in rows) < 1:
             raise ValueError("every row of a step needs at least one token")
@@ -181,6 +183,8 @@ class PagedGenerator:
     @torch.no_grad()
     def generate(self, rows, max_new_tokens):
         """Greedy decoding of all rows together; returns {row: new token ids}."""
+        if len(set(rows)) < len(rows):
+            raise ValueError("a row is named twice")
         out = {b: [] for b in rows}
         for _ in range(max_new_tokens):
             for b in rows:

@@ -105,3 +105,15 @@ def test_score_refuses_prompts_past_the_rope_tables(native):
     with pytest.raises(ValueError, match="longer than max_len"):
         gen.score([[1] * 41, [2]])
     assert not native
+
+
+def test_generator_refuses_rows_that_do_not_exist_or_come_twice(native):
+    """Row -1 would read the last row's length, and that row would get its tokens."""
+    gen = generator()
+    for new in ({-1: [5], 2: [6]}, {3: [1]}, {0: [1], 7: [2]}):
+        with pytest.raises(ValueError, match="rows must be in"):
+            gen.step(new)
+    gen.last = {0: torch.zeros(50), 1: torch.zeros(50)}
+    with pytest.raises(ValueError, match="twice"):
+        gen.generate([0, 1, 0], 2)
+    assert not native
