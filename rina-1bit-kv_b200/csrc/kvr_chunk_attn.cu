@@ -221,10 +221,21 @@ __device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile 
     if (it >= kSpinLimit || *abort_s) return false;
   return true;
 }
-// All lanes go on, or none does.  (The issuing warps do without: their lanes wait converged, one instruction for
-// all, and a vote at each of their waits made a chunk of 512 at 32256 4 % slower.)
+// All lanes go on, or none does.
 __device__ __forceinline__ bool ca_wait_warp(uint64_t *bar, unsigned phase, volatile int *abort_s) {
   return __all_sync(~0u, ca_wait(bar, phase, abort_s));
+}
+// The issuing warps' wait: returns in any case, and a wait that gives up only raises the abort flag.  No lane
+// takes another path by its own outcome, so the lanes cannot part (some in a shuffle that the others have left):
+// they go on issuing, within the CTA's own memory, and leave together at the piece's end, by a vote on the flag.
+// (A vote at each wait instead made a chunk of 512 at 32256 4 % slower.)
+__device__ __forceinline__ void ca_wait_on(uint64_t *bar, unsigned phase, volatile int *abort_s, unsigned *err) {
+#pragma unroll 1
+  for (uint32_t it = 0; !mbar_try_wait(bar, phase) && !*abort_s; ++it)
+    if (it >= kSpinLimit) {
+      atomicOr(err, 1u);
+      *abort_s = 1;
+    }
 }
 // Whether the phase is complete by now (never waits).
 __device__ __forceinline__ bool ca_test(uint64_t *bar, unsigned phase) {
@@ -478,22 +489,20 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     int j = 0;               // K or V tiles consumed so far
     int seen[2] = {0, 0};    // warp 8: Q tiles, warp 10: P tiles consumed so far
     int si = 0;
-    bool ok = true;
     CaPiece c;
-    for (int r = 0; ok && ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
+    for (int r = 0; ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
+      if (__any_sync(~0u, *abort_s)) break;
       const int tiles = c.two ? 2 : 1;
       const uint32_t idesc = ca_uniform(ca_idesc<DT>(!scores, c.p.n_tok * g <= kCaFewRows ? 64 : 128));
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
-      for (int i = 0; ok && i < c.n; ++i, ++j) {
+      for (int i = 0; i < c.n; ++i, ++j) {
         const int s = ca_stage(!scores, j);
-        ok = ca_wait(&kv_full[s], (unsigned)((j / depth) & 1), abort_s);
-        if (!ok) break;
+        ca_wait_on(&kv_full[s], (unsigned)((j / depth) & 1), abort_s, a.err);
         if (scores) {
-          for (int t = 0; ok && t < tiles; ++t) {
-            if (i == 0) ok = ca_wait(&q_full[t], (unsigned)(seen[t]++ & 1), abort_s);
-            if (ok && si > 0) ok = ca_wait(s_free, (unsigned)((si - 1) & 1), abort_s);
-            if (!ok) break;
+          for (int t = 0; t < tiles; ++t) {
+            if (i == 0) ca_wait_on(&q_full[t], (unsigned)(seen[t]++ & 1), abort_s, a.err);
+            if (si > 0) ca_wait_on(s_free, (unsigned)((si - 1) & 1), abort_s, a.err);
             ++si;
             ca_fence_after();
             const uint32_t qa = ca_uniform(ca_desc_k(q_base + t * kCaTile));
@@ -521,15 +530,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
-          for (int t = 0; ok && t < tiles; ++t) {
+          for (int t = 0; t < tiles; ++t) {
             const uint32_t vb = ca_uniform(ca_desc_mn(kv_base + s * kCaTile)), add = ca_uniform(i > 0 ? 1u : 0u);
             const uint32_t pa = ca_uniform(tmem + 128 + t * 64), oa = ca_uniform(tmem + 256 + t * 128);
             const uint32_t done = ca_uniform(smem_u32(&pv_done[t]));
             // in two halves of the keys: the first weights are multiplied while the others are formed
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              ok = ca_wait(&p_full[2 * t + half], (unsigned)(seen[t] & 1), abort_s);
-              if (!ok) break;
+              ca_wait_on(&p_full[2 * t + half], (unsigned)(seen[t] & 1), abort_s, a.err);
               ca_fence_after();
               if (ca_elect()) {
 #pragma unroll
@@ -542,12 +550,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           }
         }
         __syncwarp();
-        if (ok && ca_elect()) ca_commit(smem_u32(&kv_empty[s]));
+        if (ca_elect()) ca_commit(smem_u32(&kv_empty[s]));
       }
-    }
-    if (!__all_sync(~0u, ok) && lane == 0) {
-      if (!*abort_s) atomicOr(a.err, 1u);
-      *abort_s = 1;
     }
     // every MMA, and the arrivals that its commits owe, before the tensor memory is freed and the CTA ends
     uint64_t *bar = &drained[scores ? 0 : 1];
@@ -761,6 +765,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   }
   // every role is past its last access to the tensor memory (or drained after an abort)
   ca_fence_after();
+  __syncwarp();
   if (warp == 8)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCaTmemCols));
 }
