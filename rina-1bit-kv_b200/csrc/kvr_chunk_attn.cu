@@ -897,6 +897,29 @@ static int chunk_check(const char *fn, ChunkCall &c, int dtype, int d, float sca
   return KVR_OK;
 }
 
+// Bytes of `rows` rows of n_kv or n_q heads, `stride` elements apart.
+static int64_t row_span(int64_t rows, int64_t stride, int64_t heads) { return ((rows - 1) * stride + heads * kD) * 2; }
+
+// What a call writes must not lie in what it reads: rows are finished, and stored, while other CTAs still read.
+static int chunk_check_out(const char *fn, const ChunkCall &c, int64_t k_bytes, int64_t v_bytes) {
+  const ChunkArgs &a = c.a;
+  auto meet = [](const void *p, int64_t n, const void *q, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+  };
+  const struct { const void *p; int64_t n; } w[2] = {{a.out, row_span(a.n_tokens, (int64_t)a.n_q * kD, a.n_q)},
+                                                     {a.lse, a.n_tokens * a.n_q * 4}};
+  for (const auto &o : w) {
+    if (!o.p) continue;
+    const char *name = o.p == a.out ? "out" : "lse";
+    KVR_REQUIRE(!meet(o.p, o.n, c.q, row_span(a.n_tokens, c.q_stride, a.n_q)), "%s: %s must not be q or lie in it", fn, name);
+    KVR_REQUIRE(!meet(o.p, o.n, c.k, k_bytes) && !meet(o.p, o.n, c.v, v_bytes), "%s: %s must not lie in the keys or values",
+                fn, name);
+  }
+  KVR_REQUIRE(!a.lse || !meet(w[0].p, w[0].n, w[1].p, w[1].n), "%s: out and lse overlap", fn);
+  return KVR_OK;
+}
+
 template <int DT, bool PAGED>
 static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
   static thread_local int set_dev = -1;
@@ -914,7 +937,6 @@ static cudaError_t chunk_kernels(const ChunkCall &c, int dev, cudaStream_t st) {
 
 static int chunk_launch(const char *fn, ChunkCall &c, int dtype, bool paged, kvr_stream_t stream) {
   const ChunkArgs &a = c.a;
-  KVR_REQUIRE(a.out != c.q, "%s: out must not be q (pieces of one row read q at different times)", fn);
   if (!encode_tiled()) return set_error(KVR_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", fn);
   const int g = a.n_q / a.n_kv, tpt = kPlanRows / g;
   // q as (64 channels, head of the group, token, channel half, KV head)
@@ -965,6 +987,9 @@ extern "C" int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int ba
     return set_error(KVR_ENOTSUP, "kvr_paged_attn: the page size must be a multiple of 8 tokens");
   KVR_REQUIRE(tok_stride >= (int64_t)n_kv * d && tok_stride % 8 == 0 && page_stride >= 0 && page_stride % 8 == 0,
               "kvr_paged_attn: a token's heads must be contiguous, rows 16-byte aligned");
+  const int64_t pool = row_span(n_pages, page_stride, 0) + row_span(page, tok_stride, n_kv);
+  const int bad = chunk_check_out("kvr_paged_attn", c, pool, pool);
+  if (bad) return bad;
   a.box = 128;
   while (page % a.box) a.box /= 2;
   // the pool as (64 channels, row of the page, channel half, KV head, page)
@@ -994,6 +1019,8 @@ extern "C" int kvr_prompt_attn(const void *q, const void *k, const void *v, int 
   KVR_REQUIRE(n_keys > 0 && n_keys <= kPlanMaxLen, "kvr_prompt_attn: bad key count");
   KVR_REQUIRE(k_stride >= (int64_t)n_kv * d && v_stride >= (int64_t)n_kv * d && (k_stride | v_stride) % 8 == 0,
               "kvr_prompt_attn: a token's heads must be contiguous, rows 16-byte aligned");
+  const int bad = chunk_check_out("kvr_prompt_attn", c, row_span(n_keys, k_stride, n_kv), row_span(n_keys, v_stride, n_kv));
+  if (bad) return bad;
   // k and v as (64 channels, token, channel half, KV head)
   const cuuint64_t kd[4] = {64, (cuuint64_t)n_keys, 2, (cuuint64_t)n_kv};
   const cuuint64_t ks[3] = {(cuuint64_t)k_stride * 2, 128, kD * 2}, vs[3] = {(cuuint64_t)v_stride * 2, 128, kD * 2};

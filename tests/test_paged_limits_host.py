@@ -117,3 +117,45 @@ def test_generator_refuses_rows_that_do_not_exist_or_come_twice(native):
     with pytest.raises(ValueError, match="twice"):
         gen.generate([0, 1, 0], 2)
     assert not native
+
+
+HEAP = 1 << 40  # addresses that are only compared: every call below is refused before any CUDA call
+
+
+def prompt_args(**kw):
+    """kvr_prompt_attn of 16 tokens, 8 query heads on 8: every tensor takes 32 KB, all apart."""
+    a = dict(q=HEAP, k=HEAP + (1 << 20), v=HEAP + (2 << 20), out=HEAP + (3 << 20), lse=None)
+    a.update(kw)
+    return [a["q"], a["k"], a["v"], 1, 16, 16, 2, 8, 8, 128, 1024, 1024, 1024, HEAP + (4 << 20), 1 << 15, 0.0, a["out"],
+            a["lse"], HEAP + (5 << 20), 1 << 40, None]
+
+
+def paged_args(**kw):
+    """kvr_paged_attn of 16 tokens over 4 pages of 16, 8 heads: the pools take 128 KB each."""
+    a = dict(q=HEAP, k=HEAP + (1 << 20), v=HEAP + (2 << 20), out=HEAP + (3 << 20), lse=None)
+    a.update(kw)
+    return [a["q"], 1, 16, 2, 8, 8, 128, 1024, a["k"], a["v"], 4, 16, 16384, 1024, HEAP + (6 << 20), 4, 4, HEAP + (4 << 20),
+            1 << 15, 0.0, a["out"], a["lse"], HEAP + (5 << 20), 1 << 40, None]
+
+
+@pytest.mark.parametrize("name,args,size", [("kvr_prompt_attn", prompt_args, 32768), ("kvr_paged_attn", paged_args, 131072)])
+@pytest.mark.parametrize("over", ["q", "k", "v"])
+@pytest.mark.parametrize("what", ["out", "lse"])
+def test_output_over_an_input_is_refused(name, args, size, over, what):
+    """CTAs store finished rows while others still read."""
+    from kvr_b200 import _native as N
+    at = {"q": HEAP, "k": HEAP + (1 << 20), "v": HEAP + (2 << 20)}[over]
+    size = 32768 if over == "q" else size
+    for p in (at, at + size - 512, at + 512):
+        if what == "out" and p == at + 512:
+            p = at - 512  # the end of out in the input's first row
+        with pytest.raises(N.KvrError, match="must not") as e:
+            N.call(name, *args(**{what: p}))
+        assert e.value.code == 1
+
+
+def test_output_over_the_log_sum_exps_is_refused():
+    from kvr_b200 import _native as N
+    for name, args in (("kvr_prompt_attn", prompt_args), ("kvr_paged_attn", paged_args)):
+        with pytest.raises(N.KvrError, match="overlap"):
+            N.call(name, *args(lse=HEAP + (3 << 20) + 32768 - 4))
