@@ -600,8 +600,9 @@ class AttnPlan:
     """The work list of an attention call (kvr_attn_plan), on the device, and
     the shapes it was built for."""
 
-    def __init__(self, n_tokens, batch, n_q, n_kv, paged, device):
+    def __init__(self, n_tokens, batch, n_q, n_kv, paged, device, own_keys=False):
         self.n_tokens, self.batch, self.n_q, self.n_kv, self.paged = n_tokens, batch, n_q, n_kv, paged
+        self.own_keys = own_keys  # packed keys that are the queries' own tokens
         key = (n_tokens, batch, n_q, n_kv)
         nbytes = _PLAN_BYTES.get(key)
         if nbytes is None:
@@ -633,7 +634,7 @@ def attn_plan(cu_q, n_tokens, n_q, n_kv, kv_len=None, cu_k=None, causal=True, wi
         _i32(kv_len, "kv_len", batch)
     if cu_k is not None:
         _i32(cu_k, "cu_k", batch + 1)
-    plan = AttnPlan(n_tokens, batch, n_q, n_kv, kv_len is not None, cu_q.device)
+    plan = AttnPlan(n_tokens, batch, n_q, n_kv, kv_len is not None, cu_q.device, kv_len is None and cu_k is None)
     call("kvr_attn_plan", ptr(cu_q), ptr(kv_len), ptr(cu_k), batch, n_tokens, n_q, n_kv, int(causal), window,
          ptr(plan.buf), plan.nbytes, stream())
     return plan
@@ -780,8 +781,9 @@ def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, ret
 
 def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
     """Attention over whole packed prompts: q (T, n_q, d), k and v (T_k, n_kv,
-    d), possibly strided views of one projection; `plan` from attn_plan.
-    Returns out of q's shape and dtype, or (out, lse (T, n_q) fp32)."""
+    d), possibly strided views of one projection; `plan` from attn_plan (made
+    without cu_k: k and v are of q's tokens; with it, keys that its offsets name
+    past T_k read as zeros).  Returns out of q's shape and dtype, or (out, lse (T, n_q) fp32)."""
     q, qs = _tokens(q, "q")
     k, ks = _tokens(k, "k")
     v, vs = _tokens(v, "v")
@@ -791,6 +793,8 @@ def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
         raise TypeError("q, k and v must share a dtype")
     if k.shape != v.shape or k.shape[1] != plan.n_kv:
         raise ValueError("k and v must be (tokens, n_kv, d) with the plan's n_kv")
+    if plan.own_keys and k.shape[0] != n_tokens:
+        raise ValueError(f"the plan has no cu_k: the keys must be the {n_tokens} tokens of q, got {k.shape[0]}")
     out, lse = _attn_out(q, out, return_lse)
     ws, ws_bytes, s = _attn_workspace(q.device)
     call("kvr_prompt_attn", ptr(q), ptr(k), ptr(v), dtype_code(q), n_tokens, k.shape[0], plan.batch, n_q, plan.n_kv, D,

@@ -159,3 +159,17 @@ def test_output_over_the_log_sum_exps_is_refused():
     for name, args in (("kvr_prompt_attn", prompt_args), ("kvr_paged_attn", paged_args)):
         with pytest.raises(N.KvrError, match="overlap"):
             N.call(name, *args(lse=HEAP + (3 << 20) + 32768 - 4))
+
+
+def test_prompt_keys_must_be_the_queries_tokens_without_cu_k(native):
+    """Fewer keys than tokens would be made up with zeros that take part in the softmax."""
+    from kvr_b200 import kernels as K
+    q, kv = torch.zeros(6, 8, 128, dtype=torch.float16), torch.zeros(9, 2, 128, dtype=torch.float16)
+    plan = K.attn_plan(i32(0, 2, 6), 6, 8, 2)
+    for n in (5, 7):
+        with pytest.raises(ValueError, match="no cu_k"):
+            K.prompt_attn(q, kv[:n], kv[:n], plan)
+    assert "kvr_prompt_attn" not in native
+    K.prompt_attn(q, kv[:6], kv[:6], plan)
+    K.prompt_attn(q, kv, kv, K.attn_plan(i32(0, 2, 6), 6, 8, 2, cu_k=i32(0, 4, 9)))
+    assert native["kvr_prompt_attn"][5] == 9
