@@ -706,7 +706,9 @@ def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=
             raise ValueError("q_out must be contiguous and of q's shape and dtype")
         _on_gpu(q, q_out)
         qp, qo = q.data_ptr(), q_out.data_ptr()
-    if cos is not None:
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or positions is None:
+            raise ValueError("RoPE needs both tables and positions")
         _i32(positions, "positions", n_tokens)
         if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
             raise TypeError("the RoPE tables must be fp32")

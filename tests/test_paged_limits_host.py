@@ -173,3 +173,14 @@ def test_prompt_keys_must_be_the_queries_tokens_without_cu_k(native):
     K.prompt_attn(q, kv[:6], kv[:6], plan)
     K.prompt_attn(q, kv, kv, K.attn_plan(i32(0, 2, 6), 6, 8, 2, cu_k=i32(0, 4, 9)))
     assert native["kvr_prompt_attn"][5] == 9
+
+
+def test_write_with_half_of_the_rope_arguments_is_refused(native):
+    """A sine table alone would leave q and k unrotated."""
+    from kvr_b200 import kernels as K
+    pool, x = torch.zeros(4, 16, 2, 128, dtype=torch.float16), torch.zeros(3, 2, 128, dtype=torch.float16)
+    slots, pos, tab = torch.zeros(3, dtype=torch.int64), i32(0, 1, 2), torch.zeros(8, 128)
+    for kw in (dict(sin=tab), dict(cos=tab, positions=pos), dict(sin=tab, positions=pos), dict(cos=tab, sin=tab)):
+        with pytest.raises(ValueError, match="both tables"):
+            K.paged_write(x, x, x, pool, pool, slots, **kw)
+    assert not native
