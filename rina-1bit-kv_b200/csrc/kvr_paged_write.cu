@@ -138,6 +138,20 @@ extern "C" int kvr_paged_write(const void *q, const void *k, const void *v, int 
                          reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
                          reinterpret_cast<uintptr_t>(cos_tbl) | reinterpret_cast<uintptr_t>(sin_tbl);
   KVR_REQUIRE((ptrs & 15) == 0, "kvr_paged_write: pointers must be 16-byte aligned");
+  // q_out may be q itself, row by row; nothing else that a call writes may lie in what it reads
+  auto span = [](int64_t rows, int64_t stride, int64_t heads) { return ((rows - 1) * stride + heads * kD) * 2; };
+  auto meet = [](const void *p, int64_t n, const void *o, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(o);
+    return x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+  };
+  if (q) {
+    const int64_t n = span(n_tokens, (int64_t)n_q * d, n_q), pool = span(n_pages, page_stride, 0) + span(page, tok_stride, n_kv);
+    KVR_REQUIRE((q_out == q && (n_tokens == 1 || q_stride == (int64_t)n_q * d)) || !meet(q_out, n, q, span(n_tokens, q_stride, n_q)),
+                "kvr_paged_write: q_out must be q itself, laid out alike, or apart from it");
+    KVR_REQUIRE(!meet(q_out, n, k, span(n_tokens, k_stride, n_kv)) && !meet(q_out, n, v, span(n_tokens, v_stride, n_kv)) &&
+                    !meet(q_out, n, k_pages, pool) && !meet(q_out, n, v_pages, pool),
+                "kvr_paged_write: q_out must not lie in k, v or the pages");
+  }
   PagedWriteArgs a{q, k, v, n_tokens, n_q, n_kv, q_stride, k_stride, v_stride, cos_tbl, sin_tbl, rope_stride, max_pos,
                    positions, slots, q_out, static_cast<uint16_t *>(k_pages), static_cast<uint16_t *>(v_pages),
                    n_pages * page, page, page_stride, tok_stride, 1};

@@ -91,3 +91,16 @@ def test_paged_attn_many_requests_of_131072_keys(dtype):
     tol = tol + n / 16 * 2.0 ** -23 * v.double().abs().max()
     assert ((out.double() - want).abs() <= tol).all()
     assert ((lse.double() - lse_x).abs() <= tol_l + n / 16 * 2.0 ** -23).all()
+
+
+def test_write_in_place():
+    """q_out may be q itself."""
+    from kvr_b200 import kernels as K
+    from test_gpu_attn_paged import tables
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q, k, v = (torch.randn(33, h, 128, device=DEV, generator=g).half() for h in (8, 2, 2))
+    kp, vp = torch.zeros(4, 16, 2, 128, device=DEV, dtype=F16), torch.zeros(4, 16, 2, 128, device=DEV, dtype=F16)
+    slots, pos = torch.arange(33, device=DEV), torch.arange(33, device=DEV, dtype=torch.int32)
+    want = K.paged_write(q, k, v, kp, vp, slots, pos, *tables(40))
+    got = K.paged_write(q, k, v, kp, vp, slots, pos, *tables(40), q_out=q)
+    assert got is q and torch.equal(got, want)

@@ -184,3 +184,22 @@ def test_write_with_half_of_the_rope_arguments_is_refused(native):
         with pytest.raises(ValueError, match="both tables"):
             K.paged_write(x, x, x, pool, pool, slots, **kw)
     assert not native
+
+
+def write_args(**kw):
+    """kvr_paged_write of 16 tokens, 8 query heads on 8, 4 pages of 16: tensors all apart."""
+    a = dict(q=HEAP, k=HEAP + (1 << 20), v=HEAP + (2 << 20), kp=HEAP + (3 << 20), vp=HEAP + (4 << 20), q_out=HEAP + (5 << 20),
+             qs=1024)
+    a.update(kw)
+    return [a["q"], a["k"], a["v"], 1, 16, 8, 8, 128, a["qs"], 1024, 1024, None, None, 0, 0, None, HEAP + (6 << 20), a["q_out"],
+            a["kp"], a["vp"], 4, 16, 16384, 1024, None]
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_out=HEAP + 512), dict(q_out=HEAP - 512), dict(qs=2048, q_out=HEAP), dict(q_out=HEAP + (1 << 20)),
+    dict(q_out=HEAP + (2 << 20) + 32256), dict(q_out=HEAP + (3 << 20) + 131072 - 256), dict(q_out=HEAP + (4 << 20) - 256)])
+def test_rotated_queries_over_an_input_are_refused(kw):
+    """Another warp may not have read it yet."""
+    from kvr_b200 import _native as N
+    with pytest.raises(N.KvrError, match="q_out must"):
+        N.call("kvr_paged_write", *write_args(**kw))
