@@ -21,12 +21,17 @@ from . import kernels as K
 
 
 class PagedKVCache:
+    """Up to max_requests requests of at most max_len tokens each, on n_pages
+    pages of `page` tokens a layer.  Positions stay below max_len, so RoPE tables
+    of max_len rows do; a step that would pass it is one that does not fit
+    (`check`): its tokens past max_len do not count as cached."""
+
     def __init__(self, n_layers, n_q, n_kv, n_pages, page=64, max_requests=32, max_len=32768, window=0,
                  dtype=torch.bfloat16, device="cuda"):
         if page < 8 or page % 8:
             raise ValueError("page must be a multiple of 8")
         self.n_layers, self.n_q, self.n_kv, self.page, self.window = n_layers, n_q, n_kv, page, window
-        self.n_pages, self.max_requests = n_pages, max_requests
+        self.n_pages, self.max_requests, self.max_len = n_pages, max_requests, max_len
         self.k = torch.zeros(n_layers, n_pages, page, n_kv, K.D, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         i32 = dict(dtype=torch.int32, device=device)
@@ -69,14 +74,17 @@ class PagedKVCache:
     def commit(self):
         """Ends the step: its tokens count as cached, its pages as taken."""
         st = self._open()
-        self.ctx_len.copy_(st.kv_len)
+        torch.clamp(st.kv_len, max=self.max_len, out=self.ctx_len)
         self.n_free.copy_(st.n_free)
         self.step = None
 
     def check(self):
         """Raises if the open step ran out of pages, tokens or table width
         (synchronises)."""
-        missing, cut, over, _ = self._open().info.tolist()
+        st = self._open()
+        past = (st.kv_len > self.max_len).sum(0, keepdim=True)  # the table's width is in whole pages
+        missing, cut, over, _, past = torch.cat([st.info, past]).tolist()
+        over = max(over, past)
         if missing or cut or over:
             raise RuntimeError(f"step does not fit: {missing} pages missing, {cut} requests cut at n_tokens, "
                                f"{over} longer than max_len")

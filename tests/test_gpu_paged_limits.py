@@ -104,3 +104,20 @@ def test_write_in_place():
     want = K.paged_write(q, k, v, kp, vp, slots, pos, *tables(40))
     got = K.paged_write(q, k, v, kp, vp, slots, pos, *tables(40), q_out=q)
     assert got is q and torch.equal(got, want)
+
+
+def test_generator_up_to_a_max_len_that_is_not_whole_pages():
+    from kvr_b200 import PagedGenerator
+    from test_gpu_attn_serving import prompts_of, tiny_llama, want_logits
+    m = tiny_llama()
+    gen = PagedGenerator(m, n_pages=12, page=16, max_requests=3, max_len=40, chunk=32)
+    ids = prompts_of([40])[0]
+    rows = gen.add([ids[:37]])
+    for n in (38, 39, 40):
+        got = gen.step({rows[0]: ids[n - 1:n]})[rows[0]]
+        assert torch.allclose(got, want_logits(m, ids[:n])[-1], rtol=2e-2, atol=2e-2), n
+    with pytest.raises(RuntimeError, match="longer than max_len"):
+        gen.step({rows[0]: [1]})
+    with pytest.raises(RuntimeError, match="longer than max_len"):
+        gen.step({1: ids + [2]})
+    assert torch.allclose(gen.score([ids])[0], want_logits(m, ids), rtol=2e-2, atol=2e-2)

@@ -203,3 +203,42 @@ def test_rotated_queries_over_an_input_are_refused(kw):
     from kvr_b200 import _native as N
     with pytest.raises(N.KvrError, match="q_out must"):
         N.call("kvr_paged_write", *write_args(**kw))
+
+
+@pytest.fixture
+def cpu_map(monkeypatch):
+    """kernels.paged_map by its CPU specification."""
+    from kvr_b200 import kernels as K
+    from oracle import paged_ref as R
+
+    def paged_map(ctx_len, new_len, block_table, free_pages, n_free, page, n_tokens, **kw):
+        m = R.page_map(ctx_len.tolist(), new_len.tolist(), block_table.numpy(), free_pages.tolist(), n_free.item(), page, n_tokens)
+        block_table.copy_(torch.from_numpy(m["table"]))
+        st = K.PagedStep()
+        st.cu_q, st.kv_len, st.positions, st.slots, st.info = (
+            torch.from_numpy(m[k]) for k in ("cu_q", "kv_len", "positions", "slots", "info"))
+        st.n_free, st.n_tokens, st.plan = i32(m["n_free"]), n_tokens, None
+        return st
+
+    monkeypatch.setattr(K, "paged_map", paged_map)
+
+
+def test_max_len_within_a_page(cpu_map):
+    """The table's rows hold whole pages: 48 tokens where max_len is 40."""
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 8, 2, 10, page=16, max_requests=2, max_len=40, device="cpu")
+    for new, fits in (([39, 5], True), ([1, 0], True), ([1, 3], False), ([0, 33], True), ([0, 32], False)):
+        c.begin(new, sum(new))
+        if fits:
+            before = c.ctx_len.tolist()
+            c.check()
+            c.commit()
+            assert c.ctx_len.tolist() == [a + b for a, b in zip(before, new)]
+        else:
+            with pytest.raises(RuntimeError, match="1 longer than max_len"):
+                c.check()
+            c.step = None
+    # a step committed all the same (as a captured loop does) leaves the length at max_len
+    c.begin([5, 0], 5)
+    c.commit()
+    assert c.ctx_len.tolist() == [40, 38]
