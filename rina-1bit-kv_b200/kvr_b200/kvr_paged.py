@@ -163,13 +163,13 @@ class PagedGenerator:
         st = self.cache.begin(lens, ids.numel())
         try:
             self.cache.check()
-        except RuntimeError:
-            self.cache.step = None  # nothing was written: the step can be tried again after a drop
+            h = self._layers(self.model.model.embed_tokens(ids), lambda li, q, k, v: self.cache.attend(
+                li, self.cache.write(li, q, k, v, self.cos_tbl, self.sin_tbl)))
+            ends = st.cu_q[1:].long()[torch.tensor(rows, device=self.device)] - 1
+            logits = self.model.lm_head(h[ends]).float()
+        except BaseException:
+            self.cache.step = None  # nothing counts as cached: the step can be tried again, or its rows dropped
             raise
-        h = self._layers(self.model.model.embed_tokens(ids), lambda li, q, k, v: self.cache.attend(
-            li, self.cache.write(li, q, k, v, self.cos_tbl, self.sin_tbl)))
-        ends = st.cu_q[1:].long()[torch.tensor(rows, device=self.device)] - 1
-        logits = self.model.lm_head(h[ends]).float()
         self.cache.commit()
         out = {b: logits[i] for i, b in enumerate(rows)}
         self.last.update(out)

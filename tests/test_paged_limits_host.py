@@ -242,3 +242,13 @@ def test_max_len_within_a_page(cpu_map):
     c.begin([5, 0], 5)
     c.commit()
     assert c.ctx_len.tolist() == [40, 38]
+
+
+def test_step_that_fails_in_the_model_leaves_no_open_step(cpu_map, monkeypatch):
+    from kvr_b200 import kernels as K
+    gen = generator()
+    monkeypatch.setattr(K, "paged_write", lambda *a: (_ for _ in ()).throw(RuntimeError("out of memory")))
+    with pytest.raises(RuntimeError, match="out of memory"):
+        gen.step({1: [1, 2, 3]})
+    gen.drop([1])
+    assert gen.cache.n_free.item() == 10 and gen.last == {}
