@@ -178,14 +178,19 @@ class PagedGenerator:
     @torch.no_grad()
     def add(self, prompts):
         """Takes prompts (lists of token ids) into free rows, `chunk` tokens a
-        step and prompt; returns the rows."""
+        step and prompt; returns the rows.  All of them or, where a step fails,
+        none: what was taken is given back."""
         free = [b for b in range(self.cache.max_requests) if b not in self.last]
         if len(free) < len(prompts):
             raise RuntimeError(f"{len(prompts)} prompts for {len(free)} free rows")
         rows, left = free[:len(prompts)], [list(p) for p in prompts]
-        while any(left):
-            self.step({b: left[i][:self.chunk] for i, b in enumerate(rows) if left[i]})
-            left = [p[self.chunk:] for p in left]
+        try:
+            while any(left):
+                self.step({b: left[i][:self.chunk] for i, b in enumerate(rows) if left[i]})
+                left = [p[self.chunk:] for p in left]
+        except BaseException:
+            self.drop(rows)
+            raise
         return rows
 
     @torch.no_grad()

@@ -252,3 +252,17 @@ def test_step_that_fails_in_the_model_leaves_no_open_step(cpu_map, monkeypatch):
         gen.step({1: [1, 2, 3]})
     gen.drop([1])
     assert gen.cache.n_free.item() == 10 and gen.last == {}
+
+
+def test_add_takes_all_prompts_or_none(cpu_map, monkeypatch):
+    """Prompts of 3 and 2 pages in a cache of 3: the second chunk does not fit."""
+    from kvr_b200 import kernels as K
+    monkeypatch.setattr(K, "paged_write", lambda q, *a: q)
+    monkeypatch.setattr(K, "paged_attn", lambda q, *a, **kw: q)
+    gen = generator(n_pages=3, chunk=16)
+    with pytest.raises(RuntimeError, match="does not fit"):
+        gen.add([[1] * 40, [2] * 20])
+    assert gen.cache.n_free.item() == 3 and gen.last == {} and gen.cache.ctx_len.tolist() == [0, 0, 0]
+    assert sorted(gen.cache.free_pages.tolist()) == [0, 1, 2]
+    assert gen.add([[1] * 30]) == [0]
+    assert gen.cache.n_free.item() == 1 and set(gen.last) == {0}
