@@ -180,6 +180,8 @@ class PagedGenerator:
         """Takes prompts (lists of token ids) into free rows, `chunk` tokens a
         step and prompt; returns the rows.  All of them or, where a step fails,
         none: what was taken is given back."""
+        if not all(len(p) for p in prompts):
+            raise ValueError("every prompt needs at least one token")
         free = [b for b in range(self.cache.max_requests) if b not in self.last]
         if len(free) < len(prompts):
             raise RuntimeError(f"{len(prompts)} prompts for {len(free)} free rows")

@@ -266,3 +266,12 @@ def test_add_takes_all_prompts_or_none(cpu_map, monkeypatch):
     assert sorted(gen.cache.free_pages.tolist()) == [0, 1, 2]
     assert gen.add([[1] * 30]) == [0]
     assert gen.cache.n_free.item() == 1 and set(gen.last) == {0}
+
+
+def test_add_refuses_an_empty_prompt(cpu_map):
+    """It would return a row that has no logits to go on from."""
+    gen = generator()
+    for prompts in ([[]], [[1, 2], []]):
+        with pytest.raises(ValueError, match="at least one token"):
+            gen.add(prompts)
+    assert gen.last == {} and gen.cache.n_free.item() == 10 and gen.add([]) == []
