@@ -180,12 +180,13 @@ class PagedGenerator:
         """Takes prompts (lists of token ids) into free rows, `chunk` tokens a
         step and prompt; returns the rows.  All of them or, where a step fails,
         none: what was taken is given back."""
-        if not all(len(p) for p in prompts):
+        left = [list(p) for p in prompts]
+        if not all(left):
             raise ValueError("every prompt needs at least one token")
         free = [b for b in range(self.cache.max_requests) if b not in self.last]
-        if len(free) < len(prompts):
-            raise RuntimeError(f"{len(prompts)} prompts for {len(free)} free rows")
-        rows, left = free[:len(prompts)], [list(p) for p in prompts]
+        if len(free) < len(left):
+            raise RuntimeError(f"{len(left)} prompts for {len(free)} free rows")
+        rows = free[:len(left)]
         try:
             while any(left):
                 self.step({b: left[i][:self.chunk] for i, b in enumerate(rows) if left[i]})
