@@ -113,8 +113,41 @@ class PagedKVCache:
                 f"requests={self.max_requests})")
 
 
+_MODELS = ("llama", "mistral", "qwen2", "qwen3")     # whose decoder layer `PagedGenerator._layers` is
+_ROPE = ("default", "linear", "llama3", "yarn")        # one table for sequences of every length
+_PARTS = {"q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm", "rotary_emb"}
+
+
+def _model_window(model, max_len):
+    """The model's sliding window (0: none, or none within max_len); raises
+    NotImplementedError for models with parts that PagedGenerator does not apply."""
+    cfg = model.config
+    if cfg.model_type not in _MODELS:
+        raise NotImplementedError(f"PagedGenerator serves {', '.join(_MODELS)} models, not {cfg.model_type}")
+    rope = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
+    kind = rope.get("rope_type", rope.get("type", "default"))
+    if kind not in _ROPE:
+        raise NotImplementedError(f"RoPE of type {kind} (its angles may depend on a sequence's length)")
+    for layer in model.model.layers:
+        more = {n for n, _ in layer.self_attn.named_children()} - _PARTS
+        if more:
+            raise NotImplementedError(f"attention with {', '.join(sorted(more))}")
+        if abs(getattr(layer.self_attn, "scaling", K.D ** -0.5) - K.D ** -0.5) > 1e-6:
+            raise NotImplementedError("attention scores scaled by other than 1 / sqrt(head_dim)")
+    window = (getattr(cfg, "sliding_window", None) or 0) if getattr(cfg, "use_sliding_window", True) else 0
+    if not 0 < window < max_len:
+        return 0
+    kinds = set(getattr(cfg, "layer_types", None) or ["sliding_attention"])
+    if kinds == {"full_attention"}:
+        return 0
+    if kinds != {"sliding_attention"}:
+        raise NotImplementedError("layers with and without a window (a step has one attention plan)")
+    return window
+
+
 class PagedGenerator:
-    """Many requests on one HF decoder model with an exact paged cache.
+    """Many requests on one HF decoder model (Llama, Mistral, Qwen2 or Qwen3 of
+    head_dim 128, fp16 or bf16) with an exact paged cache.
 
         gen = PagedGenerator(model, n_pages=4096, max_requests=32)
         rows = gen.add([prompt_a, prompt_b])          # prompts in chunks of `chunk` tokens
@@ -122,7 +155,9 @@ class PagedGenerator:
         gen.drop(rows)                                # their pages are free again
 
     A step takes any mix of chunks and single tokens (``step``); ``score``
-    gives the logits of whole packed prompts without a cache."""
+    gives the logits of whole packed prompts without a cache.  window: a query
+    sees the last `window` tokens only (0: as many as the model's own sliding
+    window, or all); a model's own window bounds it."""
 
     def __init__(self, model, n_pages, page=64, max_requests=32, max_len=None, window=0, chunk=2048):
         from .kvr_hook import rope_tables
@@ -133,7 +168,10 @@ class PagedGenerator:
         d = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.n_q
         if d != K.D:
             raise ValueError(f"head_dim must be {K.D}, the model has {d}")
+        if model.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"the cache holds fp16 or bf16, the model is {model.dtype}")
         max_len = max_len or cfg.max_position_embeddings
+        window = min((w for w in (window, _model_window(model, max_len)) if w > 0), default=0)
         self.cache = PagedKVCache(cfg.num_hidden_layers, self.n_q, self.n_kv, n_pages, page, max_requests, max_len, window,
                                   dtype=model.dtype, device=self.device)
         self.cos_tbl, self.sin_tbl = rope_tables(model, max_len, self.device)
@@ -145,6 +183,8 @@ class PagedGenerator:
             at = layer.self_attn
             x = layer.input_layernorm(h)
             q, k, v = (p(x).view(x.shape[0], -1, K.D) for p in (at.q_proj, at.k_proj, at.v_proj))
+            if hasattr(at, "q_norm"):  # over the channels of each head
+                q, k = at.q_norm(q), at.k_norm(k)
             h = h + at.o_proj(attend(li, q, k, v).reshape(x.shape[0], -1))
             h = h + layer.mlp(layer.post_attention_layernorm(h))
         return self.model.model.norm(h)

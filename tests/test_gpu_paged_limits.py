@@ -121,3 +121,39 @@ def test_generator_up_to_a_max_len_that_is_not_whole_pages():
     with pytest.raises(RuntimeError, match="longer than max_len"):
         gen.step({1: ids + [2]})
     assert torch.allclose(gen.score([ids])[0], want_logits(m, ids), rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("cls,kw", [
+    ("Qwen3", {}), ("Qwen2", {}), ("Llama", dict(attention_bias=True, mlp_bias=True)), ("Mistral", dict(sliding_window=20)),
+    ("Qwen3", dict(sliding_window=33, use_sliding_window=True, max_window_layers=0)),
+    ("Llama", dict(rope_parameters={"rope_type": "yarn", "factor": 4.0, "rope_theta": 1e4,
+                                    "original_max_position_embeddings": 128}))])
+def test_generator_serves_models_with_norms_biases_and_windows(cls, kw):
+    """Against the model's own forward, at the bar of the one-sequence generator's
+    test (2e-2 on logits of order one, fp16)."""
+    import transformers as T
+    from kvr_b200 import PagedGenerator
+    from test_gpu_attn_serving import prompts_of, want_logits
+    torch.manual_seed(3)
+    cfg = getattr(T, cls + "Config")(vocab_size=500, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
+                                     num_attention_heads=4, num_key_value_heads=2, head_dim=128, max_position_embeddings=512, **kw)
+    m = getattr(T, cls + "ForCausalLM")(cfg)
+    for layer in m.model.layers:  # weights that tell whether a part is applied
+        for name, w in layer.self_attn.named_parameters():
+            if "norm" in name:
+                torch.nn.init.uniform_(w, 0.5, 2.0)
+            elif name.endswith("bias"):
+                torch.nn.init.normal_(w, std=0.5)
+            else:
+                torch.nn.init.normal_(w, std=0.06)  # scores far from flat, so that windows and norms show
+    m = m.half().to(DEV).eval()
+    prompts = prompts_of([90, 1, 37])
+    gen = PagedGenerator(m, n_pages=30, page=16, max_requests=3, chunk=48)
+    rows = gen.add(prompts)
+    for b, p in zip(rows, prompts):
+        assert torch.allclose(gen.last[b], want_logits(m, p)[-1], rtol=2e-2, atol=2e-2), b
+    got = gen.step({b: [5 + b] for b in rows})
+    for b, p in zip(rows, prompts):
+        assert torch.allclose(got[b], want_logits(m, p + [5 + b])[-1], rtol=2e-2, atol=2e-2), b
+    for p, x in zip(prompts, gen.score(prompts)):
+        assert torch.allclose(x, want_logits(m, p), rtol=2e-2, atol=2e-2), len(p)

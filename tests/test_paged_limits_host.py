@@ -275,3 +275,33 @@ def test_add_refuses_an_empty_prompt(cpu_map):
         with pytest.raises(ValueError, match="at least one token"):
             gen.add(prompts)
     assert gen.last == {} and gen.cache.n_free.item() == 10 and gen.add([]) == []
+
+
+@pytest.mark.parametrize("cls,kw,match", [
+    ("Granite", dict(head_dim=None, hidden_size=256, residual_multiplier=0.5), "granite"),
+    ("Olmo2", dict(hidden_size=256, head_dim=None), "olmo2"),
+    ("Llama", dict(rope_parameters={"rope_type": "dynamic", "factor": 2.0, "rope_theta": 1e4}), "dynamic"),
+    ("Qwen2", dict(layers=2, use_sliding_window=True, sliding_window=8, max_window_layers=1, hidden_size=256), "window")])
+def test_models_with_parts_that_are_not_applied_are_refused(cls, kw, match):
+    kw = {k: v for k, v in kw.items() if v is not None}
+    m = tiny(cls, **kw)
+    with pytest.raises(NotImplementedError, match=match):
+        generator(m)
+
+
+def test_models_of_another_type_are_refused():
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        generator(tiny().float())
+
+
+@pytest.mark.parametrize("cls,kw,own,given,want", [
+    ("Llama", {}, 0, 0, 0), ("Llama", {}, 0, 7, 7), ("Mistral", dict(sliding_window=20), 20, 0, 20),
+    ("Mistral", dict(sliding_window=20), 20, 7, 7), ("Mistral", dict(sliding_window=20), 20, 30, 20),
+    ("Mistral", dict(sliding_window=40), 0, 0, 0), ("Mistral", dict(sliding_window=None), 0, 0, 0),
+    ("Qwen3", dict(sliding_window=20, use_sliding_window=False), 0, 0, 0),
+    ("Qwen3", dict(sliding_window=20, use_sliding_window=True, max_window_layers=0), 20, 0, 20)])
+def test_window_of_the_model(cls, kw, own, given, want):
+    from kvr_b200 import kvr_paged
+    m = tiny(cls, **kw)
+    assert kvr_paged._model_window(m, 40) == own
+    assert generator(m, window=given).cache.window == want
