@@ -458,15 +458,16 @@ KVR_API int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const int3
  * in request order (the k-th fresh page of the step is
  * free_pages[*n_free - 1 - k]) and are entered into block_table (batch,
  * table_width; row stride table_stride) behind the ceil(ctx/page) pages that
- * the request holds.  Writes cu_q (batch + 1), kv_len (batch) = ctx + new,
- * positions (n_tokens), slots (n_tokens) = page id * page + row, the free
- * count left, and info (4): pages missing, requests whose new tokens did not
- * fit n_tokens (the last ones are cut), requests longer than their table row,
- * 0.  Tokens without a page and padding tokens get slot -1; a missing page's
- * table entry is -1.  ctx_len, new_len and n_free are not changed, so
- * repeating a call repeats its result.  With `plan`, the causal attention
- * plan of the step (n_q, n_kv, window as kvr_attn_plan) is built in the same
- * launch. */
+ * the request holds; none is taken for what lies past a table row.  Writes
+ * cu_q (batch + 1), kv_len (batch), the keys that the request has after the
+ * step (ctx + new, or as many as its pages hold), positions (n_tokens), slots
+ * (n_tokens) = page id * page + row, the free count left, and info (4): pages
+ * missing, requests whose new tokens did not fit n_tokens (the last ones are
+ * cut), requests longer than their table row, 0.  Tokens without a page and
+ * padding tokens get slot -1; a missing page's table entry is -1.  ctx_len,
+ * new_len and n_free are not changed, so repeating a call repeats its result.
+ * With `plan`, the causal attention plan of the step (n_q, n_kv, window as
+ * kvr_attn_plan, queries at their positions) is built in the same launch. */
 KVR_API int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int batch, int64_t n_tokens, int page,
                           int32_t *block_table, int64_t table_stride, int table_width, const int32_t *free_pages,
                           int64_t n_free_cap, const int32_t *n_free, int32_t *cu_q, int32_t *kv_len,

@@ -12,21 +12,25 @@ def page_map(ctx_len, new_len, table, free_pages, n_free, page, n_tokens):
     table = np.array(table, dtype=np.int32, copy=True)
     width = table.shape[1]
     cu, kv, pos, slots = [0], [], [], []
-    taken = cut = over = 0
+    taken = beyond = cut = over = 0
     for b, c in enumerate(ctx):
         want = max(int(new_len[b]), 0)
         n = min(want, n_tokens - cu[-1])
         cut += n < want
         cu.append(cu[-1] + n)
-        kv.append(c + n)
-        fresh = {}
+        stored = c + n  # keys the request has after the step: those up to its first token without a page
+        if -(-(c + n) // page) > width:
+            over += 1
+            stored = min(stored, max(c, width * page))
         for j in range(-(-c // page), -(-(c + n) // page)):
-            fresh[j] = int(free_pages[n_free - 1 - taken]) if taken < n_free else -1
+            if j >= width:  # no page is taken for what has no table entry
+                beyond += 1
+                continue
+            table[b, j] = free_pages[n_free - 1 - taken] if taken < n_free else -1
+            if taken >= n_free:
+                stored = min(stored, j * page)
             taken += 1
-        over += -(-(c + n) // page) > width
-        for j, pg in fresh.items():
-            if j < width:
-                table[b, j] = pg
+        kv.append(stored)
         for p in range(c, c + n):
             pg = table[b, p // page] if p // page < width else -1
             pos.append(p)
@@ -35,7 +39,7 @@ def page_map(ctx_len, new_len, table, free_pages, n_free, page, n_tokens):
     slots += [-1] * (n_tokens - len(slots))
     i32 = lambda x: np.array(x, dtype=np.int32)  # noqa: E731
     return {"cu_q": i32(cu), "kv_len": i32(kv), "positions": i32(pos), "slots": np.array(slots, dtype=np.int64),
-            "table": table, "n_free": max(n_free - taken, 0), "info": i32([max(taken - n_free, 0), cut, over, 0])}
+            "table": table, "n_free": max(n_free - taken, 0), "info": i32([max(taken + beyond - n_free, 0), cut, over, 0])}
 
 
 def rope(x, cos, sin):

@@ -49,7 +49,7 @@ struct PlanHeader {  // 64 words
 struct PlanPiece {   // 8 words
   int q_start;       // first token of the item, in the packed batch
   int n_tok;         // its tokens (in an even plan: head << 16 | tokens; 0: no piece)
-  int first_end;     // keys its first token may see: kv_len - q_len + offset + 1 (causal), can be <= 0
+  int first_end;     // keys its first token may see: kv_len - q_len (or ctx) + offset + 1 (causal), can be <= 0
   int kv_len;        // keys of the request
   int k_start;       // first key of the request in packed K/V (prompt), or the request's index (pages)
   int kt0, kt1;      // K/V tiles [kt0, kt1) of the piece
@@ -83,6 +83,7 @@ struct PlanArgs {
   const int *cu_q;    // (batch + 1)
   const int *kv_len;  // (batch) or NULL
   const int *cu_k;    // (batch + 1) or NULL; both NULL: the keys are the queries' tokens
+  const int *ctx;     // (batch) keys before each request's queries, or NULL: the queries are its last tokens
   int batch, n_tokens, n_q, n_kv, causal, window;
   PlanHeader *hdr;
   PlanPiece *pieces;

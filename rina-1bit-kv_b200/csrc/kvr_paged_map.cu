@@ -6,6 +6,9 @@
 // list in request order, so page k of the step (exclusive sum of the needs
 // plus its index) is free[n_free - 1 - k] and no page needs an atomic.  Token
 // i lies at position p = ctx + i - cu[b] and in slot table[b][p/P] * P + p%P.
+// A request takes no page that its table row has no entry for, and its tokens
+// without a page are its last ones, so the keys it has after the step are the
+// first kv_len: ctx + new, or as many as its pages hold.
 //
 // One launch does all of it.  Every CTA forms the two prefix sums (tokens,
 // fresh pages) of all requests in shared memory by itself: two words per
@@ -60,6 +63,7 @@ __device__ __forceinline__ int last_not_above(const int *a, int n, int x) {
 // last request (padding: no keys, their rows come out as zeros).
 struct PlanRequest {
   int q0, q_len, kv_len, k_start;
+  int first;  // keys before its first query
 };
 __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, int b) {
   PlanRequest r;
@@ -80,6 +84,7 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, int b) {
     r.k_start = lo;
     r.kv_len = r.q_len;
   }
+  r.first = a.ctx && b < a.batch ? min(max(a.ctx[b], 0), kPlanMaxLen) : r.kv_len - r.q_len;
   return r;
 }
 
@@ -92,7 +97,7 @@ __device__ __forceinline__ PlanPiece plan_item(const PlanArgs &a, const PlanRequ
   p.kv_len = r.kv_len;
   p.k_start = r.k_start;
   p.part = -1;
-  p.first_end = a.causal ? r.kv_len - r.q_len + i * per + 1 : r.kv_len;
+  p.first_end = a.causal ? r.first + i * per + 1 : r.kv_len;
   const int64_t end = a.causal ? min((int64_t)r.kv_len, (int64_t)p.first_end + p.n_tok - 1) : r.kv_len;
   const int64_t begin = a.window > 0 ? max((int64_t)0, (int64_t)p.first_end - a.window) : 0;
   p.kt0 = (int)(begin / kPlanKeys);
@@ -397,6 +402,11 @@ struct MapArgs {
 
 // Cached tokens of request b (a length that no cache can have counts as its bound).
 __device__ __forceinline__ int map_ctx(const MapArgs &a, int b) { return min(max(a.ctx_len[b], 0), kPlanMaxLen); }
+// Fresh pages of a request that goes from ctx to kv tokens: those that its table row has entries for.
+__device__ __forceinline__ int map_fresh(const MapArgs &a, int ctx, int kv) {
+  const int P = a.page, W = a.table_width;
+  return min((kv + P - 1) / P, W) - min((ctx + P - 1) / P, W);
+}
 
 __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
   __shared__ int cu[kPlanMaxBatch + 1];
@@ -405,12 +415,12 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
     PlanShared plan;
   } s;
   __shared__ int64_t warp_sums[32];
-  __shared__ int n_cut, n_over;
+  __shared__ int n_cut, n_over, n_beyond;
   int *fresh = s.fresh;
   const int tid = threadIdx.x, nt = blockDim.x, P = a.page;
   griddep_wait();
   griddep_launch();
-  if (tid == 0) n_cut = n_over = 0;
+  if (tid == 0) n_cut = n_over = n_beyond = 0;
   const int each = (a.batch + nt - 1) / nt;
   // tokens first: requests are cut where the step's n_tokens end
   int64_t sum = 0, total;
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
     const int b = tid * each + k;
     if (b < a.batch) {
       const int ctx = map_ctx(a, b), kv = ctx + cu[b + 1] - cu[b];
-      sum += (kv + P - 1) / P - (ctx + P - 1) / P;
+      sum += map_fresh(a, ctx, kv);
     }
   }
   at = block_exclusive(sum, warp_sums, total);
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
     if (b < a.batch) {
       const int ctx = map_ctx(a, b), kv = ctx + cu[b + 1] - cu[b];
       fresh[b] = (int)at;
-      at += (kv + P - 1) / P - (ctx + P - 1) / P;
+      at += map_fresh(a, ctx, kv);
     }
   }
   if (tid == 0) fresh[a.batch] = need;
@@ -451,17 +461,24 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_map_kernel(MapArgs a) {
   const int n_free = min(max(*a.n_free, 0), a.n_free_cap);
   if (blockIdx.x == 0) {
     for (int b = tid; b < a.batch; b += nt) {
-      const int ctx = map_ctx(a, b), now = cu[b + 1] - cu[b];
+      const int ctx = map_ctx(a, b), now = cu[b + 1] - cu[b], had = (ctx + P - 1) / P, pages = (ctx + now + P - 1) / P;
       a.cu[b] = cu[b];
-      a.kv_len[b] = ctx + now;
       if (max(a.new_len[b], 0) > now) atomicAdd(&n_cut, 1);
-      if ((ctx + now + P - 1) / P > a.table_width) atomicAdd(&n_over, 1);
+      if (pages > a.table_width) {
+        atomicAdd(&n_over, 1);
+        atomicAdd(&n_beyond, pages - max(had, a.table_width));
+      }
+      const int want = map_fresh(a, ctx, ctx + now), got = min(want, max(n_free - fresh[b], 0));
+      int kv = ctx + now;
+      if (got < want || pages > a.table_width)
+        kv = (int)min((int64_t)kv, max((int64_t)ctx, (int64_t)(min(had, a.table_width) + got) * P));
+      a.kv_len[b] = kv;
     }
     __syncthreads();  // cu and kv_len are in place for the plan as well
     if (tid == 0) {
       a.cu[a.batch] = cu[a.batch];
       *a.n_free_out = max(n_free - need, 0);
-      a.info[0] = max(need - n_free, 0);
+      a.info[0] = max(need + n_beyond - n_free, 0);
       a.info[1] = n_cut;
       a.info[2] = n_over;
       a.info[3] = 0;
@@ -538,7 +555,7 @@ extern "C" int kvr_attn_plan(const int32_t *cu_q, const int32_t *kv_len, const i
   clear_error();
   KVR_REQUIRE(cu_q, "kvr_attn_plan: null pointer");
   KVR_REQUIRE(!(kv_len && cu_k), "kvr_attn_plan: give kv_len (pages) or cu_k (packed keys), not both");
-  PlanArgs a{cu_q, kv_len, cu_k, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, nullptr, 0};
+  PlanArgs a{cu_q, kv_len, cu_k, nullptr, batch, 0, n_q, n_kv, causal ? 1 : 0, 0, nullptr, nullptr, nullptr, 0};
   const int rc = plan_check("kvr_attn_plan", a, n_tokens, window, plan, plan_bytes);
   if (rc) return rc;
   const cudaError_t e = launch_dependent(attn_plan_kernel, 1, kPlanThreads, 0, as_cuda(stream), a);
@@ -564,7 +581,7 @@ extern "C" int kvr_paged_map(const int32_t *ctx_len, const int32_t *new_len, int
   KVR_REQUIRE(n_free != n_free_out, "kvr_paged_map: n_free_out must not be n_free");
   MapArgs m{};
   if (plan) {
-    m.plan = PlanArgs{cu_q, kv_len, nullptr, batch, 0, n_q, n_kv, 1, 0, nullptr, nullptr, nullptr, 0};
+    m.plan = PlanArgs{cu_q, kv_len, nullptr, ctx_len, batch, 0, n_q, n_kv, 1, 0, nullptr, nullptr, nullptr, 0};
     const int rc = plan_check("kvr_paged_map", m.plan, n_tokens, window, plan, plan_bytes);
     if (rc) return rc;
     m.with_plan = 1;

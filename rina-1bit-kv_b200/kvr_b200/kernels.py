@@ -642,7 +642,8 @@ def attn_plan(cu_q, n_tokens, n_q, n_kv, kv_len=None, cu_k=None, causal=True, wi
 
 class PagedStep:
     """What paged_map makes of a step's lengths (int32 on the device unless
-    noted): cu_q (B + 1), kv_len (B), positions (T), slots (T) int64, n_free
+    noted): cu_q (B + 1), kv_len (B) = ctx_len + new_len, or the keys that have a
+    page where pages are missing or the table row ends, positions (T), slots (T) int64, n_free
     (1) left, info (4) = [pages missing, requests cut, requests longer than
     their table row, 0], and the attention plan (None without n_q)."""
 

@@ -72,7 +72,8 @@ class PagedKVCache:
                             return_lse=return_lse)
 
     def commit(self):
-        """Ends the step: its tokens count as cached, its pages as taken."""
+        """Ends the step: its tokens (those that found a page and lie below
+        max_len) count as cached, its pages as taken."""
         st = self._open()
         torch.clamp(st.kv_len, max=self.max_len, out=self.ctx_len)
         self.n_free.copy_(st.n_free)

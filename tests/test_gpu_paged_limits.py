@@ -157,3 +157,63 @@ def test_generator_serves_models_with_norms_biases_and_windows(cls, kw):
         assert torch.allclose(got[b], want_logits(m, p + [5 + b])[-1], rtol=2e-2, atol=2e-2), b
     for p, x in zip(prompts, gen.score(prompts)):
         assert torch.allclose(x, want_logits(m, p), rtol=2e-2, atol=2e-2), len(p)
+
+
+def test_requests_without_room_keep_what_is_stored():
+    """A step that passes max_len and the free list, committed as a captured loop
+    does: no page is lost, the keys that were stored (and only they) are attended,
+    and the requests go on when pages are free again."""
+    from kvr_b200 import PagedKVCache
+    from test_gpu_attn_paged import check, exact
+    g = torch.Generator(device=DEV).manual_seed(17)
+    c = PagedKVCache(1, 8, 2, 6, page=16, max_requests=3, max_len=64, dtype=F16)
+    held = [[], [], []]  # keys and values that a request has in the cache
+
+    def step(new, stored, info):
+        x = torch.randn(sum(new), 12, 128, device=DEV, generator=g).half()
+        q, k, v = x.split([8, 2, 2], 1)
+        st = c.begin(new, sum(new))
+        out, lse = c.attend(0, c.write(0, q, k, v), return_lse=True)
+        c.commit()
+        assert st.info.tolist() == info and c.ctx_len.tolist() == stored
+        at = 0
+        for b, n in enumerate(new):
+            had = sum(len(y[0]) for y in held[b])
+            kept = stored[b] - had
+            held[b].append((k[at:at + kept], v[at:at + kept]))
+            if kept:
+                kk, vv = (torch.cat([y[i] for y in held[b]]) for i in (0, 1))
+                check(out[at:at + kept], lse[at:at + kept], exact(q[at:at + kept], kk, vv), (b, new))
+            at += n
+        assert torch.isfinite(out).all()
+        pages = [p for row, m in zip(c.block_table.tolist(), stored) for p in row[:-(-m // 16)]]
+        assert sorted(pages + c.free_pages[:c.n_free.item()].tolist()) == list(range(6))
+        return out, lse
+
+    step([30, 20, 0], [30, 20, 0], [0, 0, 0, 0])
+    out, lse = step([40, 1, 10], [64, 21, 0], [2, 0, 1, 0])
+    assert (out[41:] == 0).all() and (lse[41:] == -torch.inf).all()  # request 2 got no page: it sees nothing
+    step([1, 0, 0], [64, 21, 0], [1, 0, 1, 0])
+    c.release([0])
+    held[0] = []
+    step([0, 1, 10], [0, 22, 10], [0, 0, 0, 0])
+    step([20, 12, 6], [20, 34, 16], [0, 0, 0, 0])  # pages 2 + 3 + 1: all
+    step([0, 9, 0], [20, 43, 16], [0, 0, 0, 0])
+    step([13, 8, 0], [32, 48, 16], [2, 0, 0, 0])   # 33 and 51 tokens would take a page more each
+
+
+def test_map_plans_like_attn_plan():
+    """The step's plan and attn_plan over its lengths give the same bits."""
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(18)
+    ctx, new = [700, 0, 33, 1500], [90, 130, 0, 1]
+    table = torch.full((4, 110), -1, dtype=torch.int32, device=DEV)
+    table[:, :100] = torch.randperm(400, device=DEV, generator=g).view(4, 100).int()
+    free = torch.arange(400, 440, dtype=torch.int32, device=DEV)
+    kp, vp = (torch.randn(440, 16, 2, 128, device=DEV, generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(230, 8, 128, device=DEV, generator=g).bfloat16()
+    for window in (0, 200):
+        st = K.paged_map(i32(ctx), i32(new), table, free, i32([40]), 16, 230, n_q=8, n_kv=2, window=window)
+        plan = K.attn_plan(st.cu_q, 230, 8, 2, kv_len=st.kv_len, window=window)
+        a, b = (K.paged_attn(q, kp, vp, table, p, return_lse=True) for p in (st.plan, plan))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

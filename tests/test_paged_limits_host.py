@@ -305,3 +305,16 @@ def test_window_of_the_model(cls, kw, own, given, want):
     m = tiny(cls, **kw)
     assert kvr_paged._model_window(m, 40) == own
     assert generator(m, window=given).cache.window == want
+
+
+def test_oracle_map_counts_the_keys_that_have_pages():
+    # pages of 4, rows of 2 entries: request 0 runs past its row, request 1 past the free list, request 2 needs nothing
+    import numpy as np
+    from oracle import paged_ref as R
+    t = np.full((3, 2), -1, np.int32)
+    t[0, 0], t[2, 0] = 9, 8
+    m = R.page_map([3, 0, 2], [9, 7, 1], t, [4, 5], 2, 4, 17)
+    assert m["table"].tolist() == [[9, 5], [4, -1], [8, -1]] and m["n_free"] == 0
+    assert m["kv_len"].tolist() == [8, 4, 3] and m["cu_q"].tolist() == [0, 9, 16, 17]
+    assert m["slots"].tolist() == [39, 20, 21, 22, 23, -1, -1, -1, -1, 16, 17, 18, 19, -1, -1, -1, 34]
+    assert m["info"].tolist() == [2, 0, 1, 0]  # request 1's second page, and request 0's third
