@@ -41,6 +41,7 @@ class PagedKVCache:
         self._free = torch.arange(n_pages - 1, -2, -1, **i32)
         self.free_pages = self._free[:n_pages]
         self.n_free = torch.full((1,), n_pages, **i32)
+        self.lost = torch.zeros(4, **i32)  # what committed steps had no room for, as their info counts it
         self.step = None
 
     def begin(self, new_len, n_tokens):
@@ -75,20 +76,30 @@ class PagedKVCache:
         """Ends the step: its tokens (those that found a page and lie below
         max_len) count as cached, its pages as taken."""
         st = self._open()
+        self.lost += self._info(st)
         torch.clamp(st.kv_len, max=self.max_len, out=self.ctx_len)
         self.n_free.copy_(st.n_free)
         self.step = None
 
+    def _info(self, st):
+        """A step's info with the requests past max_len in its place of requests too long."""
+        if self.block_table.shape[1] * self.page == self.max_len:
+            return st.info
+        past = (st.kv_len > self.max_len).sum(0, keepdim=True, dtype=torch.int32)  # the table's rows are whole pages
+        return torch.cat([st.info[:2], torch.maximum(st.info[2:3], past), st.info[3:]])
+
     def check(self):
-        """Raises if the open step ran out of pages, tokens or table width
-        (synchronises)."""
-        st = self._open()
-        past = (st.kv_len > self.max_len).sum(0, keepdim=True)  # the table's width is in whole pages
-        missing, cut, over, _, past = torch.cat([st.info, past]).tolist()
-        over = max(over, past)
+        """Raises if the open step ran out of pages, tokens or table width, or,
+        between steps, if any step did that was committed since the last such
+        check (what a loop of captured steps can ask now and then).
+        Synchronises."""
+        info = self.lost if self.step is None else self._info(self.step)
+        missing, cut, over, _ = info.tolist()
         if missing or cut or over:
-            raise RuntimeError(f"step does not fit: {missing} pages missing, {cut} requests cut at n_tokens, "
-                               f"{over} longer than max_len")
+            if self.step is None:
+                self.lost.zero_()
+            raise RuntimeError(f"{'committed steps did' if self.step is None else 'step does'} not fit: {missing} pages missing, "
+                               f"{cut} requests cut at n_tokens, {over} longer than max_len")
 
     def release(self, requests):
         """Gives the pages of `requests` (a list of rows; one named twice counts

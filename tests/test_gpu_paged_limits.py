@@ -217,3 +217,41 @@ def test_map_plans_like_attn_plan():
         plan = K.attn_plan(st.cu_q, 230, 8, 2, kv_len=st.kv_len, window=window)
         a, b = (K.paged_attn(q, kp, vp, table, p, return_lse=True) for p in (st.plan, plan))
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_replayed_steps_without_room_are_reported():
+    """A captured decode step, replayed past the pages there are."""
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 8, 2, 3, page=16, max_requests=2, max_len=64, dtype=F16)
+    x = torch.randn(2, 12, 128, device=DEV).half()
+    lens = i32([1, 1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        q, k, v = x.split([8, 2, 2], 1)
+        c.begin(lens, 2)
+        out = c.attend(0, c.write(0, q, k, v))
+        c.commit()
+        return out
+
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+        for _ in range(15):
+            graph.replay()
+        c.check()
+        assert c.ctx_len.tolist() == [16, 16]
+        graph.replay()  # two pages wanted, one left
+        with pytest.raises(RuntimeError, match="1 pages missing"):
+            c.check()
+        assert c.ctx_len.tolist() == [17, 16]
+        for _ in range(3):
+            graph.replay()
+        with pytest.raises(RuntimeError, match="3 pages missing"):
+            c.check()
+        c.check()
+        assert c.ctx_len.tolist() == [20, 16]
+    torch.cuda.current_stream().wait_stream(side)

@@ -318,3 +318,33 @@ def test_oracle_map_counts_the_keys_that_have_pages():
     assert m["kv_len"].tolist() == [8, 4, 3] and m["cu_q"].tolist() == [0, 9, 16, 17]
     assert m["slots"].tolist() == [39, 20, 21, 22, 23, -1, -1, -1, -1, 16, 17, 18, 19, -1, -1, -1, 34]
     assert m["info"].tolist() == [2, 0, 1, 0]  # request 1's second page, and request 0's third
+
+
+@pytest.mark.parametrize("max_len,new,match", [
+    (40, [41, 0], "0 pages missing, 0 requests cut at n_tokens, 1 longer"), (48, [49, 0], "1 longer"), (48, [48, 30], "1 pages missing"),
+    (48, [30, 5], None)])
+def test_a_committed_step_without_room_is_reported_later(cpu_map, max_len, new, match):
+    """A loop of captured steps checks none of them on the host."""
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 8, 2, 4, page=16, max_requests=2, max_len=max_len, device="cpu")
+    c.check()
+    c.begin(new, sum(new))
+    c.commit()
+    c.begin([0, 0], 3)
+    c.check()  # the open step has nothing to report
+    c.commit()
+    if match:
+        with pytest.raises(RuntimeError, match="committed steps did not fit: .*" + match):
+            c.check()
+    c.check()  # once
+
+
+def test_a_step_cut_at_n_tokens_is_reported_later(cpu_map):
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 8, 2, 9, page=16, max_requests=3, max_len=64, device="cpu")
+    for _ in range(2):
+        c.begin([3, 3, 3], 4)
+        c.commit()
+    with pytest.raises(RuntimeError, match="4 requests cut"):
+        c.check()
+    assert c.ctx_len.tolist() == [6, 2, 0]
