@@ -496,7 +496,9 @@ KVR_API int kvr_paged_write(const void *q, const void *k, const void *v, int dty
  * request's length never reach its output, whatever the pool holds there.
  * The workspace (kvr_attn_workspace_bytes) must not be shared by calls that
  * overlap; its error word (kvr_workspace_status) reports a bounded wait that
- * gave up, or a plan that was not built for this call's shapes. */
+ * gave up, or a plan that was not built for this call's shapes or from query
+ * offsets that overlap (more of them than the list holds): such a call writes
+ * nothing. */
 KVR_API size_t kvr_attn_workspace_bytes(void);
 KVR_API int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int batch, int n_q, int n_kv, int d,
                            int64_t q_stride, const void *k_pages, const void *v_pages, int64_t n_pages, int page,
@@ -533,7 +535,7 @@ KVR_API int kvr_decode_attn_noalloc(const void *q, int q_dtype, int n_q, int n_k
 /* Synchronises `stream`, then reads and clears the error word every workspace
  * starts with: KVR_ETIMEOUT if a bounded device-side wait of an earlier call
  * using this workspace gave up, KVR_EINVAL if an attention call met a plan of
- * other shapes, else KVR_OK. */
+ * other shapes or of overlapping query offsets, else KVR_OK. */
 KVR_API int kvr_workspace_status(const void *workspace, kvr_stream_t stream);
 
 /* Test of the failure path above (no reference counterpart): one kernel

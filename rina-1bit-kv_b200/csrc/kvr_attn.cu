@@ -1745,7 +1745,8 @@ extern "C" int kvr_workspace_status(const void *workspace, kvr_stream_t stream) 
     return check_launch("kvr_workspace_status");
   if (flag) {
     cudaMemsetAsync(const_cast<void *>(workspace), 0, 4, st);
-    if (flag == kWsErrPlan) return set_error(KVR_EINVAL, "an attention plan was not built for its call's shapes");
+    if (flag == kWsErrPlan)
+      return set_error(KVR_EINVAL, "an attention plan was not for its call's shapes, or its query offsets overlap");
     return set_error(KVR_ETIMEOUT, "a bounded device-side wait gave up (flag %u)", flag);
   }
   return KVR_OK;

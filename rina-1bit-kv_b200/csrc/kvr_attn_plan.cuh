@@ -41,7 +41,7 @@ struct PlanHeader {  // 64 words
   int n_pieces;      // per head
   int n_splits;      // items cut into pieces, per head
   int part_rows;     // rows of partial results, per head
-  int dropped;       // 1: items did not fit the list (offsets that overlap)
+  int dropped;       // 1: items did not fit the list (offsets that overlap): no call runs the plan
   int even;          // 1: pieces and splits name their head
   int pad[52];
 };

@@ -318,6 +318,12 @@ __device__ __forceinline__ uint32_t ca_pack(float lo, float hi) {
   return r;
 }
 
+// Whether the plan is one for this call, with all of its items.
+__device__ __forceinline__ bool ca_plan_fits(const PlanHeader &h, const ChunkArgs &a) {
+  return h.magic == kPlanMagic && h.n_tokens == a.n_tokens && h.n_q == a.n_q && h.n_kv == a.n_kv && h.batch == a.batch &&
+         !h.dropped;
+}
+
 template <int DT, bool PAGED>
 __global__ void __launch_bounds__(kCaThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mq1,
@@ -369,8 +375,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 
   // (the CTA's first pieces go to shared memory: every role reads each of them)
   const PlanHeader &h = *a.hdr;
-  const bool fits = h.magic == kPlanMagic && h.n_tokens == a.n_tokens && h.n_q == a.n_q && h.n_kv == a.n_kv &&
-                    h.batch == a.batch;
+  const bool fits = ca_plan_fits(h, a);
   if (!fits && tid == 0) atomicOr(a.err, kWsErrPlan);
   const unsigned heads = h.even ? 1u : (unsigned)a.n_kv;  // KV heads that a list entry stands for
   const unsigned total = fits ? (unsigned)h.n_pieces * heads : 0;
@@ -780,7 +785,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
   griddep_wait();
   griddep_launch();
   const PlanHeader &h = *a.hdr;
-  if (h.magic != kPlanMagic || h.n_tokens != a.n_tokens || h.n_q != a.n_q || h.n_kv != a.n_kv || h.batch != a.batch) return;
+  if (!ca_plan_fits(h, a)) return;
   const PlanSplit *splits = plan_splits(a.hdr, a.n_tokens, a.batch, a.n_q, a.n_kv);
   const int lane = threadIdx.x & 31, g = a.n_q / a.n_kv, rows = 2 * (kPlanRows / g) * g;
   const int heads = h.even ? 1 : a.n_kv;  // KV heads that a split stands for

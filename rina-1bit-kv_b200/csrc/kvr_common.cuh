@@ -123,7 +123,7 @@ constexpr int kWsMaxRows = 4096;  // batch * n_kv
 constexpr size_t kWsSelCounters = 256;
 constexpr size_t kWsAttnCounters = kWsSelCounters + 4 * kWsMaxRows;
 constexpr size_t kWsHeader = kWsAttnCounters + 4 * kWsMaxRows;
-// Error word: 1 = a bounded wait gave up, 2 = a plan of other shapes.
+// Error word: 1 = a bounded wait gave up, 2 = a plan of other shapes, or of query offsets that overlap.
 constexpr unsigned kWsErrPlan = 2;
 
 // Optional phase timestamps for latency studies (compiled only with -DKVR_TRACE).

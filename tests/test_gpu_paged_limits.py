@@ -255,3 +255,23 @@ def test_replayed_steps_without_room_are_reported():
         c.check()
         assert c.ctx_len.tolist() == [20, 16]
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_offsets_that_overlap_past_the_list_are_reported():
+    """40 requests that all claim all tokens: the plan's list has room for some of
+    their items only.  The call leaves its output alone and says so."""
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    q = torch.randn(640, 8, 128, device=DEV).half()
+    kv = torch.randn(640, 2, 128, device=DEV).half()
+    cu = i32([640, 0] * 20 + [640])
+    plan = K.attn_plan(cu, 640, 8, 2)
+    head, _ = read_plan(plan.buf)
+    assert head[10] == 1
+    K.attn_status()
+    out = torch.full_like(q, 7)
+    K.prompt_attn(q, kv, kv, plan, out=out)
+    with pytest.raises(N.KvrError, match="offsets overlap"):
+        K.attn_status()
+    assert (out == 7).all()
+    K.attn_status()
