@@ -6,8 +6,10 @@ All tensors must live on a CUDA device; outputs are allocated here with torch
 """
 from __future__ import annotations
 
+import collections
 import contextlib
 import math
+import threading
 
 import torch
 
@@ -725,6 +727,9 @@ def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=
 
 
 _ATTN_WS: dict = {}
+# An attention call enqueues two kernels, the second of which reads what the first left in the workspace; the GIL is
+# released meanwhile.  A host thread that shares the stream must not come in between: a lock per workspace address.
+_ATTN_LOCKS: collections.defaultdict = collections.defaultdict(threading.Lock)
 
 
 def _attn_workspace(device):
@@ -775,10 +780,10 @@ def paged_attn(q, k_pages, v_pages, block_table, plan, scale=None, out=None, ret
     out, lse = _attn_out(q, out, return_lse)
     _on_gpu(q, k_pages, v_pages, block_table, out)
     ws, ws_bytes, s = _attn_workspace(q.device)
-    call("kvr_paged_attn", q.data_ptr(), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, k_pages.data_ptr(),
-         v_pages.data_ptr(), n_pages, page, ps, ts, block_table.data_ptr(), stride, width,
-         plan.buf.data_ptr(), plan.nbytes, float(scale or 0.0), out.data_ptr(), lse.data_ptr() if return_lse else None, ws,
-         ws_bytes, s)
+    with _ATTN_LOCKS[ws]:
+        call("kvr_paged_attn", q.data_ptr(), dtype_code(q), n_tokens, plan.batch, n_q, plan.n_kv, D, qs, k_pages.data_ptr(),
+             v_pages.data_ptr(), n_pages, page, ps, ts, block_table.data_ptr(), stride, width, plan.buf.data_ptr(), plan.nbytes,
+             float(scale or 0.0), out.data_ptr(), lse.data_ptr() if return_lse else None, ws, ws_bytes, s)
     return (out, lse) if return_lse else out
 
 
@@ -800,8 +805,9 @@ def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
         raise ValueError(f"the plan has no cu_k: the keys must be the {n_tokens} tokens of q, got {k.shape[0]}")
     out, lse = _attn_out(q, out, return_lse)
     ws, ws_bytes, s = _attn_workspace(q.device)
-    call("kvr_prompt_attn", ptr(q), ptr(k), ptr(v), dtype_code(q), n_tokens, k.shape[0], plan.batch, n_q, plan.n_kv, D,
-         qs, ks, vs, ptr(plan.buf), plan.nbytes, float(scale or 0.0), ptr(out), ptr(lse), ws, ws_bytes, s)
+    with _ATTN_LOCKS[ws]:
+        call("kvr_prompt_attn", ptr(q), ptr(k), ptr(v), dtype_code(q), n_tokens, k.shape[0], plan.batch, n_q, plan.n_kv, D,
+             qs, ks, vs, ptr(plan.buf), plan.nbytes, float(scale or 0.0), ptr(out), ptr(lse), ws, ws_bytes, s)
     return (out, lse) if return_lse else out
 
 

@@ -275,3 +275,32 @@ def test_offsets_that_overlap_past_the_list_are_reported():
         K.attn_status()
     assert (out == 7).all()
     K.attn_status()
+
+
+def test_host_threads_on_one_stream():
+    """Calls whose pieces are joined by a second kernel, from four threads."""
+    import threading
+    from kvr_b200 import kernels as K
+    from test_gpu_attn_paged import make_pages
+    g = torch.Generator(device=DEV).manual_seed(19)
+    jobs = []
+    for kv in ([5000], [3000, 9000], [7777], [4096, 100]):
+        kp, vp, table, _ = make_pages(g, kv, 2, 16, F16)
+        q = torch.randn(len(kv), 8, 128, device=DEV, generator=g).half()
+        plan = K.attn_plan(offsets([1] * len(kv)), len(kv), 8, 2, kv_len=i32(kv))
+        jobs.append((q, kp, vp, table, plan, K.paged_attn(q, kp, vp, table, plan)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        *args, want = jobs[k]
+        outs = [K.paged_attn(*args) for _ in range(200)]
+        wrong.extend(k for o in outs if not torch.equal(o, want))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    K.attn_status()

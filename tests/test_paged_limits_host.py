@@ -348,3 +348,42 @@ def test_a_step_cut_at_n_tokens_is_reported_later(cpu_map):
     with pytest.raises(RuntimeError, match="4 requests cut"):
         c.check()
     assert c.ctx_len.tolist() == [6, 2, 0]
+
+
+def test_host_threads_on_one_workspace_take_turns(native, monkeypatch):
+    """A call is two launches and ctypes lets other threads run meanwhile: attention,
+    attention, join, join would join the wrong rows."""
+    import threading
+    import time
+    from kvr_b200 import kernels as K
+    inside, most = [0], [0]
+    other, others = [0], [0]
+
+    def slow(name, *args):
+        if not name.endswith("_attn"):
+            return 16
+        n, m = (other, others) if args[-3] == 512 else (inside, most)
+        n[0] += 1
+        m[0] = max(m[0], n[0])
+        time.sleep(0.01)
+        n[0] -= 1
+        return 0
+
+    monkeypatch.setattr(K, "call", slow)
+    at = threading.local()
+    monkeypatch.setattr(K, "_attn_workspace", lambda device: (getattr(at, "ws", 256), 1 << 30, 0))
+    q, kv = torch.zeros(2, 8, 128, dtype=torch.float16), torch.zeros(2, 2, 128, dtype=torch.float16)
+    pool, table = torch.zeros(1, 16, 2, 128, dtype=torch.float16), torch.zeros(1, 1, dtype=torch.int32)
+    packed, paged = K.attn_plan(i32(0, 2), 2, 8, 2), K.attn_plan(i32(0, 2), 2, 8, 2, kv_len=i32(2))
+
+    def work(k):
+        at.ws = 512 if k == 4 else 256
+        for _ in range(5):
+            K.prompt_attn(q, kv, kv, packed) if k % 2 else K.paged_attn(q, pool, pool, table, paged)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(5)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert most == [1] and others == [1]
