@@ -853,6 +853,14 @@ static EncodeTiled encode_tiled() {
   return fn;
 }
 
+// The driver's calls need a context in the calling thread; a thread that has made no runtime call with a device yet
+// (its memory came from a cache) has none.
+static void bind_context() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
+}
+
 // A tensor of 16-bit values with dims[0] = 64 channels (one swizzle row);
 // strides (bytes) and boxes of the other dimensions follow.
 static bool make_map(CUtensorMap *m, int dtype, const void *base, int rank, const cuuint64_t *dims,
@@ -995,6 +1003,7 @@ extern "C" int kvr_paged_attn(const void *q, int dtype, int64_t n_tokens, int ba
   const int64_t pool = row_span(n_pages, page_stride, 0) + row_span(page, tok_stride, n_kv);
   const int bad = chunk_check_out("kvr_paged_attn", c, pool, pool);
   if (bad) return bad;
+  bind_context();
   a.box = 128;
   while (page % a.box) a.box /= 2;
   // the pool as (64 channels, row of the page, channel half, KV head, page)
@@ -1026,6 +1035,7 @@ extern "C" int kvr_prompt_attn(const void *q, const void *k, const void *v, int 
               "kvr_prompt_attn: a token's heads must be contiguous, rows 16-byte aligned");
   const int bad = chunk_check_out("kvr_prompt_attn", c, row_span(n_keys, k_stride, n_kv), row_span(n_keys, v_stride, n_kv));
   if (bad) return bad;
+  bind_context();
   // k and v as (64 channels, token, channel half, KV head)
   const cuuint64_t kd[4] = {64, (cuuint64_t)n_keys, 2, (cuuint64_t)n_kv};
   const cuuint64_t ks[3] = {(cuuint64_t)k_stride * 2, 128, kD * 2}, vs[3] = {(cuuint64_t)v_stride * 2, 128, kD * 2};

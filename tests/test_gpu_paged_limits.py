@@ -290,17 +290,39 @@ def test_host_threads_on_one_stream():
         plan = K.attn_plan(offsets([1] * len(kv)), len(kv), 8, 2, kv_len=i32(kv))
         jobs.append((q, kp, vp, table, plan, K.paged_attn(q, kp, vp, table, plan)))
     torch.cuda.synchronize()
-    wrong = []
+    wrong, done = [], []
 
     def work(k):
         *args, want = jobs[k]
         outs = [K.paged_attn(*args) for _ in range(200)]
         wrong.extend(k for o in outs if not torch.equal(o, want))
+        done.append(k)
 
     threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
     for t in threads:
         t.start()
     for t in threads:
         t.join()
-    assert not wrong
+    assert not wrong and sorted(done) == [0, 1, 2, 3]
     K.attn_status()
+
+
+@pytest.mark.parametrize("what", ["paged", "prompt"])
+def test_attention_as_a_host_threads_first_call(what):
+    """A thread whose memory comes from torch's cache has no CUDA context of its own yet."""
+    import threading
+    from kvr_b200 import kernels as K
+    q, k, v = torch.randn(40, 12, 128, device=DEV).half().split([8, 2, 2], 1)
+    if what == "prompt":
+        plan = K.attn_plan(i32([0, 40]), 40, 8, 2)
+        call = lambda: K.prompt_attn(q, k, v, plan)  # noqa: E731
+    else:
+        plan = K.attn_plan(i32([0, 40]), 40, 8, 2, kv_len=i32([40]))
+        kp, vp, table = torch.randn(3, 16, 2, 128, device=DEV).half(), torch.randn(3, 16, 2, 128, device=DEV).half(), i32([2, 0, 1])[None]
+        call = lambda: K.paged_attn(q, kp, vp, table, plan)  # noqa: E731
+    want, got = call(), []
+    call()  # its output goes back to the cache
+    t = threading.Thread(target=lambda: got.append(call()))
+    t.start()
+    t.join()
+    assert len(got) == 1 and torch.equal(got[0], want)
