@@ -727,6 +727,7 @@ def paged_write(q, k, v, k_pages, v_pages, slots, positions=None, cos=None, sin=
 
 
 _ATTN_WS: dict = {}
+_ATTN_MAKE = threading.Lock()
 # An attention call enqueues two kernels, the second of which reads what the first left in the workspace; the GIL is
 # released meanwhile.  A host thread that shares the stream must not come in between: a lock per workspace address.
 _ATTN_LOCKS: collections.defaultdict = collections.defaultdict(threading.Lock)
@@ -735,23 +736,28 @@ _ATTN_LOCKS: collections.defaultdict = collections.defaultdict(threading.Lock)
 def _attn_workspace(device):
     """(address, bytes) of the attention workspace, and the current stream.
     Calls on one stream do not overlap, so each stream has its own; its size
-    does not depend on the call.  A call in a graph capture on a stream without
-    one takes the device's capture workspace, allocated by the first call
-    outside of a capture: what a capture allocates is zeroed at each replay and
-    belongs to the graph."""
+    does not depend on the call.  Calls in a graph capture take another one, the
+    stream's second or, on a stream without (torch's own capture stream), the
+    device's (the default stream's second): a graph may be replayed on another
+    stream, beside calls on the one it was captured on.  A stream's first call
+    outside of a capture allocates both: what a capture allocates is zeroed at
+    each replay and belongs to the graph."""
     s = stream()
-    ws = _ATTN_WS.get((s, device))
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = _ATTN_WS.get((s, capturing, device))
     if ws is None:
-        if torch.cuda.is_current_stream_capturing():
-            ws = _ATTN_WS.get(("capture", device))
+        if capturing:
+            ws = _ATTN_WS.get((0, True, device))
             if ws is None:
                 raise RuntimeError("the first attention call on a device must be made outside of a graph capture")
         else:
-            nbytes = call("kvr_attn_workspace_bytes")
-            for key in (s, "capture"):
-                if (key, device) not in _ATTN_WS:
-                    _ATTN_WS[key, device] = (N.workspace(f"attn_work_{key}", nbytes, device), nbytes)
-            ws = _ATTN_WS[s, device]
+            with _ATTN_MAKE:
+                nbytes = call("kvr_attn_workspace_bytes")
+                for key in ((0, True, device), (s, True, device), (s, False, device)):
+                    if key not in _ATTN_WS:
+                        _ATTN_WS[key] = (N.workspace(f"attn_work_{key[0]}_{key[1]}", nbytes, device), nbytes)
+                torch.cuda.current_stream(device).synchronize()  # zeroed before a graph on any stream uses them
+            ws = _ATTN_WS[s, False, device]
     return ws[0].data_ptr(), ws[1], s
 
 

@@ -326,3 +326,35 @@ def test_attention_as_a_host_threads_first_call(what):
     t.start()
     t.join()
     assert len(got) == 1 and torch.equal(got[0], want)
+
+
+def test_graph_replayed_beside_calls_on_its_capture_stream():
+    """Captured on one stream, replayed on another while that one has calls of its own."""
+    from kvr_b200 import kernels as K
+    from test_gpu_attn_paged import make_pages
+    g = torch.Generator(device=DEV).manual_seed(23)
+    jobs = []
+    for kv in ([6000], [9000]):  # pieces joined through the workspace
+        kp, vp, table, _ = make_pages(g, kv, 2, 16, BF16)
+        q = torch.randn(1, 8, 128, device=DEV, generator=g).bfloat16()
+        plan = K.attn_plan(offsets([1]), 1, 8, 2, kv_len=i32(kv))
+        jobs.append((q, kp, vp, table, plan))
+    want = [K.paged_attn(*j) for j in jobs]
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (one, two):
+        s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(one):
+        K.paged_attn(*jobs[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=one):
+            outs = [K.paged_attn(*jobs[1]) for _ in range(40)]
+    two.wait_stream(one)
+    beside = []
+    for _ in range(10):
+        with torch.cuda.stream(two):
+            graph.replay()
+        with torch.cuda.stream(one):
+            beside += [K.paged_attn(*jobs[0]) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[1]) for o in outs)
+    assert all(torch.equal(o, want[0]) for o in beside)

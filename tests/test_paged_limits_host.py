@@ -387,3 +387,28 @@ def test_host_threads_on_one_workspace_take_turns(native, monkeypatch):
     for t in threads:
         t.join()
     assert most == [1] and others == [1]
+
+
+def test_captured_calls_have_a_workspace_of_their_own(monkeypatch):
+    """What a graph has baked in must not be what later calls on the stream use: the
+    graph may be replayed on another stream beside them."""
+    from types import SimpleNamespace
+    from kvr_b200 import kernels as K
+    now = {"stream": 7, "capturing": False}
+    monkeypatch.setattr(K, "_ATTN_WS", {})
+    monkeypatch.setattr(K, "stream", lambda: now["stream"])
+    monkeypatch.setattr(K.N, "workspace", lambda tag, nbytes, device: torch.zeros(1))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: SimpleNamespace(synchronize=lambda: None))
+
+    def address(stream, capturing):
+        now.update(stream=stream, capturing=capturing)
+        return K._attn_workspace("dev")[0]
+
+    with pytest.raises(RuntimeError, match="outside of a graph capture"):
+        address(7, True)
+    eager = [address(7, False), address(9, False)]
+    captured = [address(7, True), address(9, True), address(11, True)]
+    assert len(set(eager + captured)) == 5
+    assert address(12, True) == captured[2]  # streams without a call outside of captures share the device's
+    assert [address(7, False), address(9, False)] == eager and address(7, True) == captured[0]
