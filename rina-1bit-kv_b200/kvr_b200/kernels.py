@@ -818,11 +818,23 @@ def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
 
 
 def attn_status(device=None):
-    """Raises if an attention call on the current stream gave up or met a plan
-    of other shapes (synchronises the stream)."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    ws, _, s = _attn_workspace(device)
-    call("kvr_workspace_status", ws, s)
+    """Raises if an attention call on the current stream, or one in a graph replayed
+    on it, gave up or met a plan of other shapes (synchronises the stream).  It
+    reads and clears the stream's workspace and those that captures on the
+    device use."""
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    _attn_workspace(device)
+    s, first = stream(), None
+    for (of, capture, dev), ws in list(_ATTN_WS.items()):
+        if dev == device and (capture or of == s):
+            try:
+                call("kvr_workspace_status", ws[0].data_ptr(), s)
+            except N.KvrError as e:
+                first = first or e
+    if first:
+        raise first
 
 
 def kmeans(x, k=128, iters=10):

@@ -358,3 +358,33 @@ def test_graph_replayed_beside_calls_on_its_capture_stream():
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[1]) for o in outs)
     assert all(torch.equal(o, want[0]) for o in beside)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_status_covers_replayed_graphs(own_stream):
+    """A graph whose plan is of other shapes by the time it is replayed."""
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    q = torch.randn(6, 8, 128, device=DEV).half()
+    kv = torch.randn(6, 2, 128, device=DEV).half()
+    plan, other = K.attn_plan(i32([0, 6]), 6, 8, 2), K.attn_plan(i32([0, 3, 6]), 6, 8, 2)
+    keep = plan.buf[:64].clone()
+    K.prompt_attn(q, kv, kv, plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.prompt_attn(q, kv, kv, plan)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, **({"stream": side} if own_stream else {})):
+            K.prompt_attn(q, kv, kv, plan)
+        graph.replay()
+        K.attn_status()
+        plan.buf[:64].copy_(other.buf[:64])
+        graph.replay()
+        with pytest.raises(N.KvrError, match="plan"):
+            K.attn_status()
+        K.attn_status("cuda")
+        plan.buf[:64].copy_(keep)
+        graph.replay()
+        K.attn_status(torch.device("cuda"))
+    torch.cuda.current_stream().wait_stream(side)
