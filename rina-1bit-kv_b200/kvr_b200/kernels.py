@@ -764,7 +764,8 @@ def _attn_workspace(device):
 def _attn_out(q, out, return_lse):
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() == q.data_ptr():
+    elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
+          or (out.data_ptr() == q.data_ptr() and q.numel())):  # (tensors without elements have one address)
         raise ValueError("out must be contiguous, of q's shape and dtype, and not q itself")
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     return out, lse
@@ -809,6 +810,8 @@ def prompt_attn(q, k, v, plan, scale=None, out=None, return_lse=False):
         raise ValueError("k and v must be (tokens, n_kv, d) with the plan's n_kv")
     if plan.own_keys and k.shape[0] != n_tokens:
         raise ValueError(f"the plan has no cu_k: the keys must be the {n_tokens} tokens of q, got {k.shape[0]}")
+    if k.shape[0] == 0:  # no request has keys: a row that none of them sees stands for the address
+        k, v, ks, vs = q.new_zeros(1, plan.n_kv, D), q.new_zeros(1, plan.n_kv, D), plan.n_kv * D, plan.n_kv * D
     out, lse = _attn_out(q, out, return_lse)
     ws, ws_bytes, s = _attn_workspace(q.device)
     with _ATTN_LOCKS[ws]:

@@ -388,3 +388,26 @@ def test_status_covers_replayed_graphs(own_stream):
         graph.replay()
         K.attn_status(torch.device("cuda"))
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attn_of_queries_without_any_keys(causal):
+    from kvr_b200 import kernels as K
+    q, kv = torch.randn(70, 8, 128, device=DEV).half(), torch.empty(0, 2, 128, device=DEV, dtype=F16)
+    plan = K.attn_plan(i32([0, 40, 70]), 70, 8, 2, cu_k=i32([0, 0, 0]), causal=causal)
+    out, lse = K.prompt_attn(q, kv, kv, plan, return_lse=True)
+    K.attn_status()
+    assert (out == 0).all() and (lse == -torch.inf).all()
+
+
+def test_calls_without_tokens():
+    from kvr_b200 import kernels as K
+    q, kv = torch.empty(0, 8, 128, device=DEV, dtype=F16), torch.empty(0, 2, 128, device=DEV, dtype=F16)
+    out = torch.empty_like(q)
+    assert K.prompt_attn(q, kv, kv, K.attn_plan(i32([0, 0]), 0, 8, 2), out=out) is out
+    pool = torch.zeros(2, 16, 2, 128, device=DEV, dtype=F16)
+    st = K.paged_map(i32([5, 0]), i32([0, 0]), torch.zeros(2, 3, dtype=torch.int32, device=DEV), i32([1]), i32([1]), 16, 0, n_q=8, n_kv=2)
+    assert K.paged_write(q, kv, kv, pool, pool.clone(), st.slots).shape == q.shape
+    out, lse = K.paged_attn(q, pool, pool, torch.zeros(2, 3, dtype=torch.int32, device=DEV), st.plan, return_lse=True)
+    assert out.shape == q.shape and lse.shape == (0, 8) and st.kv_len.tolist() == [5, 0]
+    K.attn_status()

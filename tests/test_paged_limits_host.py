@@ -412,3 +412,12 @@ def test_captured_calls_have_a_workspace_of_their_own(monkeypatch):
     assert len(set(eager + captured)) == 5
     assert address(12, True) == captured[2]  # streams without a call outside of captures share the device's
     assert [address(7, False), address(9, False)] == eager and address(7, True) == captured[0]
+
+
+def test_calls_without_tokens_take_an_output(native):
+    from kvr_b200 import kernels as K
+    q, kv, pool = (torch.zeros(*s, 128, dtype=torch.float16) for s in ((0, 8), (0, 2), (1, 16, 2)))
+    out = torch.empty_like(q)
+    assert K.prompt_attn(q, kv, kv, K.attn_plan(i32(0, 0), 0, 8, 2), out=out) is out
+    plan = K.attn_plan(i32(0, 0), 0, 8, 2, kv_len=i32(5))
+    assert K.paged_attn(q, pool, pool, torch.zeros(1, 1, dtype=torch.int32), plan, out=out) is out
