@@ -411,3 +411,72 @@ def test_calls_without_tokens():
     out, lse = K.paged_attn(q, pool, pool, torch.zeros(2, 3, dtype=torch.int32, device=DEV), st.plan, return_lse=True)
     assert out.shape == q.shape and lse.shape == (0, 8) and st.kv_len.tolist() == [5, 0]
     K.attn_status()
+
+
+def test_log_sum_exps_merge_with_attention_over_other_keys():
+    """Keys in two caches: attention over each, merged as rows [lse, 1, out] by the
+    sequence split's merge, is attention over all.  Each part brings its own bound."""
+    from kvr_b200 import kernels as K
+    from test_gpu_attn_paged import make_pages
+    g = torch.Generator(device=DEV).manual_seed(29)
+    kv, n_q, n_kv = [333, 90, 1200], 8, 2
+    old = [200, 0, 1100]  # keys that lie elsewhere; request 1 has none there
+    q = torch.randn(3, n_q, 128, device=DEV, generator=g).half()
+    parts, keys = [], []
+    for lens in (old, [a - b for a, b in zip(kv, old)]):
+        kp, vp, table, rows = make_pages(g, lens, n_kv, 16, F16)
+        plan = K.attn_plan(offsets([1, 1, 1]), 3, n_q, n_kv, kv_len=i32(lens), causal=False)
+        parts.append(K.paged_attn(q, kp, vp, table, plan, return_lse=True))
+        keys.append([(kp[r], vp[r]) for r in rows])
+    rows = torch.stack([torch.cat([lse[..., None], torch.ones_like(lse)[..., None], out.float()], -1) for out, lse in parts])
+    got = K.lse_merge(rows.view(2, 3 * n_q, 130)).view(3, n_q, 128)
+    for b in range(3):
+        k, v = (torch.cat([part[b][i] for part in keys]) for i in (0, 1))
+        want, lse, tol, tol_l = exact(q[b:b + 1], k, v, causal=False)
+        # a part off by tol, weights off by e^(2 tol_l): the output moves by 2 tol_l of the parts' sizes
+        size = torch.stack([p[0][b:b + 1].double().abs() for p in parts]).amax(0)
+        part_tol = [exact(q[b:b + 1], *part[b], causal=False)[2] for part in keys if len(part[b][0])]
+        bound = torch.stack(part_tol).amax(0) + tol + 4 * tol_l[..., None] * size
+        assert ((got[b:b + 1].double() - want).abs() <= bound).all(), b
+
+
+def test_cache_step_against_the_keys_it_holds():
+    """Steps of chunks and single tokens: each output against the 64-bit form over
+    the rotated queries and the pages as they are, so no rotation's rounding has to
+    be allowed for; and the rotation against the CPU specification."""
+    from kvr_b200 import PagedKVCache
+    from oracle import paged_ref as R
+    from test_gpu_attn_paged import HALF_STEP, U, check, tables
+    g = torch.Generator(device=DEV).manual_seed(30)
+    cos, sin = tables(512)
+    for dtype in (F16, BF16):
+        c = PagedKVCache(1, 8, 2, 60, page=16, max_requests=3, max_len=512, dtype=dtype)
+        done = [0, 0, 0]
+        for new in ([100, 37, 0], [1, 1, 200], [260, 1, 1], [1, 0, 1]):
+            x = torch.randn(sum(new), 12, 128, device=DEV, generator=g).to(dtype)
+            q, k, v = x.split([8, 2, 2], 1)
+            st = c.begin(new, sum(new))
+            turned = c.write(0, q, k, v, cos, sin)
+            out, lse = c.attend(0, turned, return_lse=True)
+            pos = st.positions.long()
+            want = torch.from_numpy(R.rope(q.double().cpu().numpy(), *(t[pos].double().cpu().numpy() for t in (cos, sin)))).to(DEV)
+            y = torch.cat([q[..., 64:], q[..., :64]], -1)
+            tol = U[dtype] * want.abs() + 2.0 ** -22 * (q.double().abs() + y.double().abs()) + HALF_STEP[dtype]
+            assert ((turned.double() - want).abs() <= tol).all()
+            c.commit()
+            done = [a + b for a, b in zip(done, new)]
+            at = 0
+            for b, n in enumerate(new):
+                pages = c.block_table[b, :-(-done[b] // 16)].long()
+                kk, vv = (p[0][pages].reshape(-1, 2, 128)[:done[b]] for p in (c.k, c.v))
+                if n:
+                    check(out[at:at + n], lse[at:at + n], exact(turned[at:at + n], kk, vv), (dtype, new, b))
+                at += n
+        # one request once more against the CPU specification of attention
+        b, n = 1, 39
+        kk, vv = (p[0][c.block_table[b, :3].long()].reshape(-1, 2, 128)[:n].double().cpu().numpy() for p in (c.k, c.v))
+        qq = torch.randn(2, 8, 128, device=DEV, generator=g).to(dtype)
+        x_out, x_lse, _ = R.attention(qq.double().cpu().numpy(), kk, vv, 2, n)
+        mine = exact(qq, *(torch.from_numpy(t).to(DEV) for t in (kk, vv)))
+        assert (mine[0].cpu() - torch.from_numpy(x_out)).abs().max() < 1e-12
+        assert (mine[1].cpu() - torch.from_numpy(x_lse)).abs().max() < 1e-12
