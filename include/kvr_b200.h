@@ -444,8 +444,9 @@ KVR_API int kvr_peer_lse_merge(void *const *bufs, int n_ranks, int rank, const f
  * step.  Queries of request b are cu_q[b] .. cu_q[b+1] (tokens past
  * cu_q[batch] up to n_tokens are padding: output rows 0).  Keys: kv_len[b]
  * keys in pages; or packed keys cu_k[b] .. cu_k[b+1]; or, with both NULL,
- * the queries' own tokens.  The queries are the LAST tokens of their request:
- * with `causal` query i of q_len sees keys j <= kv_len - q_len + i, and with
+ * the queries' own tokens.  Output rows of tokens before cu_q[0], if any, are
+ * left alone.  The queries are the LAST tokens of their request: with `causal`
+ * query i of q_len sees keys j <= kv_len - q_len + i, and with
  * window > 0 only the last `window` of those.  A query that sees no key gets
  * output 0 and log-sum-exp -inf. */
 KVR_API size_t kvr_attn_plan_bytes(int64_t n_tokens, int batch, int n_q, int n_kv);
@@ -490,12 +491,15 @@ KVR_API int kvr_paged_write(const void *q, const void *k, const void *v, int dty
 /* Attention of a step's query tokens over their requests' pages (a plan with
  * kv_len) or over packed prompts (a plan without, or with cu_k): q (n_tokens,
  * n_q, d) with token stride q_stride, out (n_tokens, n_q, d) contiguous of the
- * same type, 32-byte aligned and not q itself, lse (n_tokens, n_q) fp32 natural log or NULL.  scale <= 0 means
+ * same type and 32-byte aligned, lse (n_tokens, n_q) fp32 natural log or NULL,
+ * neither in the memory of q, the keys or the values.  scale <= 0 means
  * sqrt(d) (scores are divided by it).  The page size must be a multiple of 8.
  * Missing pages (entries outside [0, n_pages)) read as zeros.  Keys beyond a
- * request's length never reach its output, whatever the pool holds there.
+ * request's length never reach its output, whatever the pool holds there; an
+ * infinity or NaN in V within the request may reach queries of up to 2 *
+ * floor(128 / g) tokens around that do not see the key (g query heads per KV head).
  * The workspace (kvr_attn_workspace_bytes) must not be shared by calls that
- * overlap; its error word (kvr_workspace_status) reports a bounded wait that
+ * overlap, nor by host threads that call at the same time; its error word (kvr_workspace_status) reports a bounded wait that
  * gave up, or a plan that was not built for this call's shapes or from query
  * offsets that overlap (more of them than the list holds): such a call writes
  * nothing. */

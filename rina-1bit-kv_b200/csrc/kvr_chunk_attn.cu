@@ -27,11 +27,14 @@
 // frees it, so the tensor core computes the next S while the weights of this
 // one are formed, and a tile's chain is its softmax, not softmax + two MMAs.
 // (An S per tile with P over it and S of the next keys after P V, one issuing
-// warp: 328 us for a chunk of 512 at 32256, 32/8 heads; this way 234 us.)
+// warp: 328 us for a chunk of 512 at 32256, 32/8 heads, in a graph of 12 calls;
+// this way 236 us.  Call after call, at the clock of a longer load, 275 us.)
 //
 // What binds a long prompt: a warpgroup's chain of a K/V tile, about 2900
 // cycles beside the other warpgroup's, and 500 more until the next S is seen,
-// against 2048 cycles of MMA for both tiles.  Tensor pipe and special function
+// against 2048 cycles of MMA for both tiles.  (Prompt of 16384: 1.88 ms call after
+// call, 1171 TFLOP/s, 0.71 of the burst and 0.85 of the sustained matmul rate; 1.64
+// to 1.72 ms in a graph of 12.)  Tensor pipe and special function
 // unit (16 exponentials a cycle) are 70 % active each.  With the MMAs reduced to
 // one step in eight a chunk of 512 at 32256 takes 3 % less, without the
 // exponentials 7 %, without both 33 %: what is left is the issue of some 560
@@ -48,9 +51,16 @@
 // rare after the first tiles.  Weights carry a factor 2^kShift that cancels in
 // the division: it keeps fp16 weights of 2^-18 out of the subnormals.
 //
+// What is held in fewer than 32 bits: the weights P, rounded to the tensors'
+// type because both operands of an MMA are of one 16-bit type; the sum that
+// divides them is of the unrounded ones, in fp32.  That makes the error against
+// 64 bits 1.1 to 1.4 times that of rounding the output alone (2.3e-3 for 1.7e-3
+// in bf16, 2.5e-4 for 2.0e-4 in fp16, relative in the 2-norm).
+//
 // Keys past a request's end, or before every row's window, are masked in S,
 // and their V rows are zeroed in shared memory, because 0 times a NaN of a
-// neighbour would still be a NaN.
+// neighbour would still be a NaN.  (Not so a request's own keys that some rows of
+// an item see and others do not: an infinity or NaN in such a V row reaches both.)
 //
 // Rows without a query (a decode step has g of them in 128) are kept at zero,
 // in Q and in P: the MMAs over them cost no time that the memory does not, but
@@ -62,7 +72,9 @@
 // many bytes takes 333 us then).
 //
 // Every wait is bounded; one that gives up sets the error word, lets the
-// copies and MMAs in flight drain and frees the tensor memory.
+// copies and MMAs in flight drain and frees the tensor memory.  A warp's lanes
+// give up together: by a vote at the wait, or, where a vote costs time (the
+// issuing warps), by going on to the piece's end (ca_wait_on).
 #include <cuda.h>
 
 #include "kvr_attn_plan.cuh"

@@ -16,8 +16,8 @@
 // CTA 0 then writes the per-request outputs and the attention plan, the others
 // take the tokens and fresh pages.  Tokens in fresh pages read the free list,
 // not the table that other CTAs are filling.  The work is a few hundred bytes
-// to a few MB: launch and dependent-load latency bound it (32 decode requests:
-// 4.8 us, 10 to 12 with their plan).
+// to a few MB: launch and dependent-load latency bound it (32 decode requests, in
+// a graph: 4.8 us, 12 with their plan; a call from the host takes 21).
 #include "kvr_attn_plan.cuh"
 
 namespace kvr {
@@ -251,8 +251,8 @@ __device__ bool plan_even(const PlanArgs &a, PlanShared &s, int n, const PlanPie
 // per thread; in between a warp per candidate length goes over the histogram of
 // lengths, not over the items.  Atomics on shared counters are made once per
 // warp and value: 700 items of one length on one counter cost more than all of
-// the rest (map of 48 prompts: 50 us with an atomic per item and candidate
-// sums over the items, 14.8 us this way).
+// the rest (map of 48 prompts in a graph: 50 us with an atomic per item and
+// candidate sums over the items, 14.7 us this way).
 __device__ void plan_build(const PlanArgs &a, PlanShared &s) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.n_q / a.n_kv, per = 2 * plan_tpt(a.n_q, a.n_kv);

@@ -5,8 +5,9 @@
 // of token t go to cache slot slots[t] (page slots[t] / page), q to q_out.
 //
 // The bytes bound it (32/8 heads: 24.6 KB a token): 16384 tokens in 72 us, 5.8
-// TB/s of the 6.5 that a plain copy measures; 2047 in 15 us, part of them kept in
-// L2; one token in 2 us, the time of a launch.  Eight lanes own a row:
+// TB/s of the 6.5 that a plain copy measures; in a graph 2047 (64/8 heads) in 15
+// us, part of them kept in L2, and one token in 2 us, the time of a launch (both 17
+// us as calls from the host).  Eight lanes own a row:
 // lane c holds channels 8c.. and 64+8c.., so a channel and its partner sit in
 // the same thread and a warp's loads and stores are whole 128-byte lines.  A
 // warp stays with one token and walks its rows four at a time with the
