@@ -514,6 +514,45 @@ KVR_API int kvr_prompt_attn(const void *q, const void *k, const void *v, int dty
                             int64_t v_stride, const void *plan, size_t plan_bytes, float scale, void *out,
                             float *lse, void *workspace, size_t workspace_bytes, kvr_stream_t stream);
 
+/* Reordering of a paged cache's rows, e.g. by the parents that beam search
+ * chose: place i of group g (rows[g * beams + i], a row of block_table) becomes
+ * what place parents[g * beams + i] of the group was: table entries and ctx_len
+ * in place.  A parent outside [0, beams) empties the row.  No row may be named
+ * twice.  shared (n_pages) counts the rows that hold a page beyond the first; it
+ * is brought up to date, and pages that no row holds any more go to the end of
+ * free_pages[:*n_free], in order of places and columns.  A last page that is not
+ * full stays with the parent's first child (none where a row outside of the
+ * group holds it); the others get fresh pages off the end of the list, in order of
+ * places, and copies of the page's tokens in all layers of k_pages and v_pages.  A
+ * row that finds no page keeps its full pages: its entry is -1, ctx_len ends there.
+ * info (4): pages missing, pages copied, pages given back, 0.  Pool: layers of
+ * kvr_paged_write's pools, layer_stride apart.  At most 32 beams, 4096 rows.
+ * The workspace needs no clearing and keeps nothing between calls. */
+KVR_API size_t kvr_paged_reorder_workspace_bytes(int groups, int beams, int table_width);
+KVR_API int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int table_rows, int table_width,
+                              int32_t *ctx_len, int page, int32_t *shared, int64_t n_pages, int32_t *free_pages,
+                              int64_t n_free_cap, int32_t *n_free, const int32_t *rows, const int32_t *parents,
+                              int groups, int beams, void *k_pages, void *v_pages, int dtype, int layers, int n_kv,
+                              int d, int64_t layer_stride, int64_t page_stride, int64_t tok_stride, int32_t *info,
+                              void *workspace, size_t workspace_bytes, kvr_stream_t stream);
+
+/* Beam search's choice: logits (batch * n_beams, vocab) fp32, fp16 or bf16 with
+ * row_stride elements between rows (any alignment; reads stay in 16-byte words that
+ * hold a logit of a row), cum (batch, n_beams) the beams' scores.  score(k, t) =
+ * cum[k] + logits[k, t] - logsumexp(logits[k]), compared in 64 bits.  Writes the n
+ * best of each request in order (equal ones by beam, then token): scores, beams,
+ * tokens (batch, n); and the first n_beams of them whose token is not in
+ * eos_host[0 .. n_eos) (host memory, read before the call returns): next_*
+ * (batch, n_beams).  A continuation whose score is not finite (a masked logit of
+ * -inf, a beam of score -inf, a row with a NaN or +inf) is no candidate; places
+ * without one get -inf, -1, -1.  n_beams <= n <= 128, at most 32 beams and 8 ends
+ * of sequence.  The workspace needs no clearing and keeps nothing between calls. */
+KVR_API size_t kvr_beam_select_workspace_bytes(int batch, int n_beams, int64_t vocab, int dtype, int n);
+KVR_API int kvr_beam_select(const void *logits, int dtype, int64_t row_stride, int batch, int n_beams, int64_t vocab,
+                            const float *cum, int n, const int32_t *eos_host, int n_eos, float *scores, int32_t *beams,
+                            int32_t *tokens, float *next_scores, int32_t *next_beams, int32_t *next_tokens,
+                            void *workspace, size_t workspace_bytes, kvr_stream_t stream);
+
 /* Allocation-free variant of kvr_decode_attn (no counterpart in the
  * reference).  For callers that cannot allocate device memory — a plugin
  * inside a host that owns the GPU heap, or a path where cudaMalloc would

@@ -1,0 +1,428 @@
+// Beam search's choice of continuations.
+//
+// Request b has K beams with running scores c_k and a row of V logits each:
+// score(k, t) = c_k + x_kt - lse_k, lse_k = log sum_t exp(x_kt).  The n best of
+// its K V continuations come out in order, equal scores by beam and token.
+//
+// One pass over the logits.  beam_rows_kernel: a CTA takes a segment of a row,
+// holds a running maximum and sum of exponentials per thread and a list of the
+// segment's n best logits for the CTA.  The list's last value is a threshold
+// that few logits pass: tiles in which none does cost one vote.  The first
+// threshold is the n-th largest of the threads' own maxima over the first tile
+// (at least n logits are not below it, and few more are).  Within a row the
+// order of the logits is the order of the scores, so no normaliser is needed
+// yet.  beam_merge_kernel: a CTA per request joins the sums, scores the K S n
+// listed logits and picks the n best.
+//
+// Scores are compared in 64 bits: c_k + (x - lse_k) in 32 would make different
+// logits equal and order them by token.  Sums are in 32 bits per thread (at most
+// some thousand exponentials <= 1) and joined in 64 by the second kernel.
+//
+// The logits' bytes bound the large calls, a chain of two launches the small.
+#include "kvr_common.cuh"
+
+namespace kvr {
+
+constexpr int kBsThreads = 256;
+constexpr int kBsVecs = 4;        // 16-byte loads of a thread in a tile
+constexpr int kBsMaxN = 128, kBsMaxBeams = 32, kBsMaxEos = 8;
+constexpr int kBsSlack = 64;      // entries beyond n that a list may hold before it is cut
+constexpr int kBsList = kBsMaxN + kBsSlack + 8 * kBsThreads;  // and all of a step of 8 logits a thread
+constexpr int kBsMaxCands = 8192; // of a request in the second kernel
+constexpr int kBsPicked = 1024;   // candidates that it ranks from shared memory
+
+struct BeamArgs {
+  const void *logits;
+  int64_t row_stride;  // elements
+  int rows, beams, n, splits;
+  int vocab;
+  const float *cum;
+  float2 *ml;          // (rows, splits) maximum and sum
+  uint64_t *cands;     // (rows, splits, n) keys, 0: none
+  float *scores, *next_scores;
+  int *out_beams, *tokens, *next_beams, *next_tokens;
+  int n_eos;
+  int eos[kBsMaxEos];
+};
+
+__device__ __forceinline__ float bs_exp(float x) {  // e^x for x <= 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+// Larger logits first, lower tokens first among equal ones; 0 is below every key.
+__device__ __forceinline__ uint64_t bs_key(float x, int token) {
+  return ((uint64_t)float_key(x) << 32) | (uint32_t)(0xffffffffu - (uint32_t)token);
+}
+__device__ __forceinline__ float bs_value(uint64_t key) { return key_float((uint32_t)(key >> 32)); }
+__device__ __forceinline__ int bs_token(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
+
+struct BeamShared {
+  uint64_t list[kBsList];
+  uint64_t best[kBsThreads];
+  uint64_t nth;
+  int count;
+  float m[kBsThreads / 32], s[kBsThreads / 32];
+};
+
+// The n-th largest of one key per thread (distinct unless 0), to all threads.
+__device__ __forceinline__ uint64_t bs_nth(BeamShared &sh, uint64_t mine, int n) {
+  sh.best[threadIdx.x] = mine;
+  if (threadIdx.x == 0) sh.nth = 0;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kBsThreads; i += 2) {
+    const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&sh.best[i]);
+    above += (o.x > mine) + (o.y > mine);
+  }
+  if (mine && above == n - 1) sh.nth = mine;
+  __syncthreads();
+  return sh.nth;
+}
+
+// Cuts the list to its n best, in order.
+__device__ void bs_cut(BeamShared &sh, int n) {
+  const int tid = threadIdx.x;
+  int c = sh.count;
+  if (c > kBsThreads) {  // first to those not below the n-th of the threads' own
+    uint64_t mine = 0;
+    for (int i = tid; i < c; i += kBsThreads) mine = max(mine, sh.list[i]);
+    const uint64_t low = bs_nth(sh, mine, n);
+    uint64_t keep[(kBsList + kBsThreads - 1) / kBsThreads];
+#pragma unroll
+    for (int r = 0; r < (kBsList + kBsThreads - 1) / kBsThreads; ++r) {
+      const int i = tid + r * kBsThreads;
+      keep[r] = i < c && sh.list[i] >= low ? sh.list[i] : 0;
+    }
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < (kBsList + kBsThreads - 1) / kBsThreads; ++r)
+      if (keep[r]) sh.list[atomicAdd(&sh.count, 1)] = keep[r];
+    __syncthreads();
+    c = sh.count;
+  }
+  // ranks among the rest; the sorted ones go through `best`, n of which have room
+  for (int i = tid; i < c; i += kBsThreads) {
+    const uint64_t mine = sh.list[i];
+    int above = 0;
+    for (int j = 0; j < c; ++j) above += sh.list[j] > mine;
+    if (above < n) sh.best[above] = mine;
+  }
+  __syncthreads();
+  if (tid < min(c, n)) sh.list[tid] = sh.best[tid];
+  if (tid == 0) sh.count = min(c, n);
+  __syncthreads();
+}
+
+template <int DT>
+__device__ __forceinline__ void bs_widen(const uint4 &u, float *x) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == KVR_F32) {
+      x[j] = __uint_as_float(w[j]);
+    } else if constexpr (DT == KVR_BF16) {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    }
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(BeamArgs a) {
+  constexpr int kPer = DT == KVR_F32 ? 4 : 8, kSize = 16 / kPer;  // logits of a 16-byte granule, bytes of one
+  constexpr int kTile = kBsVecs * kBsThreads;
+  __shared__ BeamShared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
+  const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
+  griddep_wait();
+  griddep_launch();
+  // The row's granules: rows need not start on one, so its first and last may hold logits of others, masked below.
+  // (Every granule read holds one of the row's at least.)
+  const char *base = static_cast<const char *>(a.logits) + (int64_t)row * a.row_stride * kSize;
+  const int head = (int)((reinterpret_cast<uintptr_t>(base) & 15) / kSize);
+  const uint4 *src = reinterpret_cast<const uint4 *>(base - head * kSize);
+  const int granules = (int)(((int64_t)head + a.vocab + kPer - 1) / kPer);
+  const int g0 = (int)((int64_t)granules * split / a.splits), g1 = (int)((int64_t)granules * (split + 1) / a.splits);
+  if (tid == 0) sh.count = 0;
+  const uint32_t pad = DT == KVR_F32 ? 0xff800000u : DT == KVR_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  uint4 next[kBsVecs];
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int v = 0; v < kBsVecs; ++v) {
+      const int g = at + v * kBsThreads + tid;
+      next[v] = g < g1 ? __ldcs(src + g) : make_uint4(pad, pad, pad, pad);
+    }
+  };
+  float m = -INFINITY, s = 0.0f, limit = -INFINITY;
+  fetch(g0);
+  for (int at = g0; at < g1; at += kTile) {
+    float x[kBsVecs * kPer];
+#pragma unroll
+    for (int v = 0; v < kBsVecs; ++v) {
+      bs_widen<DT>(next[v], x + v * kPer);
+      const int g = at + v * kBsThreads + tid, t = g * kPer - head;
+      if (g < g1 && (t < 0 || t > a.vocab - kPer)) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (t + j < 0 || t + j >= a.vocab) x[v * kPer + j] = -INFINITY;
+      }
+    }
+    if (at + kTile < g1) fetch(at + kTile);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < kBsVecs * kPer; ++i) top = fmaxf(top, x[i]);  // a NaN is passed over here, not in the sum
+    const float old = m;
+    m = fmaxf(m, top);
+    const float from = m == -INFINITY ? 0.0f : m;
+    s *= bs_exp(old - from);
+#pragma unroll
+    for (int i = 0; i < kBsVecs * kPer; ++i) s += bs_exp(x[i] - from);
+    // the list
+    const bool first = at == g0;
+    if (first) {
+      uint64_t mine = 0;
+      if (top > -INFINITY) {
+        int k = 0;
+#pragma unroll
+        for (int i = kBsVecs * kPer - 1; i >= 0; --i)
+          if (x[i] == top) k = i;
+        mine = bs_key(top, (at + k / kPer * kBsThreads + tid) * kPer - head + k % kPer);
+      }
+      const uint64_t low = bs_nth(sh, mine, n);
+      limit = low ? bs_value(low) : -INFINITY;
+    }
+    if (!__syncthreads_or(first || top > limit)) continue;
+#pragma unroll
+    for (int v = 0; v < kBsVecs; ++v) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const float y = x[v * kPer + j];
+        if (y > limit || (first && y == limit && y > -INFINITY))
+          sh.list[atomicAdd(&sh.count, 1)] = bs_key(y, (at + v * kBsThreads + tid) * kPer - head + j);
+      }
+      __syncthreads();
+      if (sh.count > n + kBsSlack) {
+        bs_cut(sh, n);
+        limit = bs_value(sh.list[n - 1]);
+      }
+      __syncthreads();  // the count is read before the next step adds to it
+    }
+    if (first && sh.count >= n) {  // later logits that equal the n-th lose to it by their token
+      bs_cut(sh, n);
+      limit = bs_value(sh.list[n - 1]);
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  bs_cut(sh, n);
+  uint64_t *out = a.cands + ((int64_t)row * a.splits + split) * n;
+  for (int i = tid; i < n; i += kBsThreads) out[i] = i < sh.count ? sh.list[i] : 0;
+  const float wm = warp_max(m);
+  s *= bs_exp(m - (wm == -INFINITY ? 0.0f : wm));
+  s = warp_sum(s);
+  if (lane == 0) {
+    sh.m[warp] = wm;
+    sh.s[warp] = s;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float bm = -INFINITY, bs = 0.0f;
+    for (int w = 0; w < kBsThreads / 32; ++w) bm = fmaxf(bm, sh.m[w]);
+    for (int w = 0; w < kBsThreads / 32; ++w) bs += sh.s[w] * bs_exp(sh.m[w] - (bm == -INFINITY ? 0.0f : bm));
+    a.ml[(int64_t)row * a.splits + split] = make_float2(bm, bs);
+  }
+}
+
+// Order of scores: a 64-bit key of the score (0: no candidate), then beam and token.
+struct BeamRank {
+  uint64_t key, id;
+};
+__device__ __forceinline__ bool bs_above(const BeamRank &x, const BeamRank &y) {
+  return x.key > y.key || (x.key == y.key && x.id < y.id);
+}
+__device__ __forceinline__ uint64_t bs_double_key(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x == 0.0 ? 0.0 : x);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double bs_key_double(uint64_t k) {
+  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
+}
+
+__global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
+  extern __shared__ BeamRank all[];  // (beams, splits, n)
+  __shared__ double lse[kBsMaxBeams];
+  __shared__ BeamRank best[kBsThreads], picked[kBsPicked], sorted[kBsMaxN], nth;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x, n = a.n, K = a.beams;
+  const int per_beam = a.splits * n, total = K * per_beam;
+  griddep_wait();
+  griddep_launch();
+  for (int k = warp; k < K; k += kBsThreads / 32) {  // a beam's sums, in 64 bits
+    const float2 *ml = a.ml + ((int64_t)b * K + k) * a.splits;
+    float m = -INFINITY;
+    for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, ml[i].x);
+    m = warp_max(m);
+    const float from = m == -INFINITY ? 0.0f : m;
+    double s = 0.0;
+    for (int i = lane; i < a.splits; i += 32) s += (double)ml[i].y * (double)expf(ml[i].x - from);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) lse[k] = (double)m + log(s);
+  }
+  if (tid == 0) {
+    count = 0;
+    nth = BeamRank{0, 0};
+  }
+  if (tid < n) sorted[tid] = BeamRank{0, 0};
+  __syncthreads();
+  BeamRank mine{0, 0};
+  for (int i = tid; i < total; i += kBsThreads) {
+    const uint64_t c = a.cands[(int64_t)b * total + i];
+    const int k = i / per_beam;
+    BeamRank r{0, 0};
+    if (c) {
+      const double score = (double)a.cum[(int64_t)b * K + k] + ((double)bs_value(c) - lse[k]);
+      if (isfinite(score)) r = BeamRank{bs_double_key(score), (uint64_t)k << 32 | (uint32_t)bs_token(c)};
+    }
+    all[i] = r;
+    if (r.key && bs_above(r, mine)) mine = r;
+  }
+  best[tid] = mine;
+  __syncthreads();
+  if (mine.key) {
+    int above = 0;
+#pragma unroll 4
+    for (int i = 0; i < kBsThreads; ++i) above += bs_above(best[i], mine);
+    if (above == n - 1) nth = mine;
+  }
+  __syncthreads();
+  const BeamRank low = nth;
+  for (int i = tid; i < total; i += kBsThreads) {
+    const BeamRank r = all[i];
+    if (r.key && !bs_above(low, r)) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kBsPicked) picked[at] = r;
+    }
+  }
+  __syncthreads();
+  // ranks: among those picked or, where they are too many for the list, among all
+  const bool few = count <= kBsPicked;
+  const BeamRank *from = few ? picked : all;
+  const int m = few ? count : total;
+  for (int i = tid; i < m; i += kBsThreads) {
+    const BeamRank r = from[i];
+    if (!r.key || bs_above(low, r)) continue;
+    int above = 0;
+    for (int j = 0; j < m; ++j) above += bs_above(from[j], r);
+    if (above < n) sorted[above] = r;
+  }
+  __syncthreads();
+  if (tid < n) {
+    const BeamRank r = sorted[tid];
+    const int64_t o = (int64_t)b * n + tid;
+    a.scores[o] = r.key ? (float)bs_key_double(r.key) : -INFINITY;
+    a.out_beams[o] = r.key ? (int)(r.id >> 32) : -1;
+    a.tokens[o] = r.key ? (int)(uint32_t)r.id : -1;
+  }
+  // the first K that do not end a sequence go on
+  if (warp == 0) {
+    int taken = 0;
+    for (int i0 = 0; i0 < n && taken < K; i0 += 32) {
+      const int i = i0 + lane;
+      const BeamRank r = i < n ? sorted[i] : BeamRank{0, 0};
+      bool on = r.key != 0;
+      for (int e = 0; e < a.n_eos; ++e) on = on && (int)(uint32_t)r.id != a.eos[e];
+      const unsigned who = __ballot_sync(0xffffffffu, on);
+      const int to = taken + __popc(who & ((1u << lane) - 1));
+      if (on && to < K) {
+        a.next_scores[(int64_t)b * K + to] = (float)bs_key_double(r.key);
+        a.next_beams[(int64_t)b * K + to] = (int)(r.id >> 32);
+        a.next_tokens[(int64_t)b * K + to] = (int)(uint32_t)r.id;
+      }
+      taken += __popc(who);
+    }
+    for (int k = taken + lane; k < K; k += 32) {
+      a.next_scores[(int64_t)b * K + k] = -INFINITY;
+      a.next_beams[(int64_t)b * K + k] = -1;
+      a.next_tokens[(int64_t)b * K + k] = -1;
+    }
+  }
+}
+
+// Segments of a row: enough CTAs for every SM to hold several at a time, none below a tile's worth of 16-byte
+// granules / 2, and no more candidates than the second kernel has room for.
+int beam_splits(int64_t rows, int beams, int n, int64_t vocab, int dtype) {
+  const int64_t granules = (vocab * (int64_t)dtype_size(dtype) + 15) / 16;
+  int64_t s = (148 * 8 + rows - 1) / rows;
+  if (s > (granules + 511) / 512) s = (granules + 511) / 512;
+  if (s > kBsMaxCands / (beams * n)) s = kBsMaxCands / (beams * n);
+  return (int)(s < 1 ? 1 : s);
+}
+
+}  // namespace kvr
+
+using namespace kvr;
+
+extern "C" size_t kvr_beam_select_workspace_bytes(int batch, int n_beams, int64_t vocab, int dtype, int n) {
+  if (batch < 1 || n_beams < 1 || n_beams > kBsMaxBeams || n < 1 || n > kBsMaxN || vocab < 1 || !valid_dtype(dtype)) return 0;
+  const int64_t rows = (int64_t)batch * n_beams;
+  return (size_t)rows * beam_splits(rows, n_beams, n, vocab, dtype) * (n + 1) * 8;
+}
+
+extern "C" int kvr_beam_select(const void *logits, int dtype, int64_t row_stride, int batch, int n_beams, int64_t vocab,
+                               const float *cum, int n, const int32_t *eos_host, int n_eos, float *scores, int32_t *beams,
+                               int32_t *tokens, float *next_scores, int32_t *next_beams, int32_t *next_tokens,
+                               void *workspace, size_t workspace_bytes, kvr_stream_t stream) {
+  clear_error();
+  KVR_REQUIRE(batch >= 0 && n_beams >= 1 && n >= n_beams && vocab >= 1 && vocab <= INT_MAX / 2 && n_eos >= 0,
+              "kvr_beam_select: bad shape");
+  if (n_beams > kBsMaxBeams || n > kBsMaxN || n_eos > kBsMaxEos)
+    return set_error(KVR_ENOTSUP, "kvr_beam_select: at most %d beams, %d candidates, %d ends of sequence", kBsMaxBeams,
+                     kBsMaxN, kBsMaxEos);
+  KVR_REQUIRE(valid_dtype(dtype), "kvr_beam_select: bad dtype");
+  if (batch == 0) return KVR_OK;
+  KVR_REQUIRE(logits && cum && scores && beams && tokens && next_scores && next_beams && next_tokens && workspace &&
+                  (!n_eos || eos_host),
+              "kvr_beam_select: null pointer");
+  const int64_t rows = (int64_t)batch * n_beams;
+  KVR_REQUIRE(row_stride >= 0 || rows == 1, "kvr_beam_select: bad row stride");
+  KVR_REQUIRE(reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) == 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "kvr_beam_select: pointers must be aligned");
+  const int splits = beam_splits(rows, n_beams, n, vocab, dtype);
+  KVR_REQUIRE(workspace_bytes >= kvr_beam_select_workspace_bytes(batch, n_beams, vocab, dtype, n),
+              "kvr_beam_select: workspace too small");
+  KVR_REQUIRE(rows * splits <= INT_MAX, "kvr_beam_select: too many rows");
+  BeamArgs a{};
+  a.logits = logits; a.row_stride = row_stride;
+  a.rows = (int)rows; a.beams = n_beams; a.n = n; a.splits = splits; a.vocab = (int)vocab;
+  a.cum = cum;
+  a.cands = static_cast<uint64_t *>(workspace);
+  a.ml = reinterpret_cast<float2 *>(a.cands + rows * splits * n);
+  a.scores = scores; a.out_beams = beams; a.tokens = tokens;
+  a.next_scores = next_scores; a.next_beams = next_beams; a.next_tokens = next_tokens;
+  a.n_eos = n_eos;
+  for (int e = 0; e < n_eos; ++e) a.eos[e] = eos_host[e];
+  const unsigned grid = (unsigned)(rows * splits);
+  cudaError_t e = launch_dependent(dtype == KVR_F32   ? beam_rows_kernel<KVR_F32>
+                                   : dtype == KVR_F16 ? beam_rows_kernel<KVR_F16>
+                                                      : beam_rows_kernel<KVR_BF16>,
+                                   grid, kBsThreads, 0, as_cuda(stream), a);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_beam_select: %s", cudaGetErrorString(e));
+  const size_t smem = (size_t)n_beams * splits * n * sizeof(BeamRank);
+  if (smem > 8 * 1024) {
+    // 48 KB without asking, of which the fixed arrays take 23
+    e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBsMaxCands * (int)sizeof(BeamRank));
+    if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_beam_select: %s", cudaGetErrorString(e));
+  }
+  e = launch_dependent(beam_merge_kernel, (unsigned)batch, kBsThreads, smem, as_cuda(stream), a);
+  if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_beam_select: %s", cudaGetErrorString(e));
+  return check_launch("kvr_beam_select");
+}

@@ -100,6 +100,11 @@ SIGNATURES = {
     "kvr_attn_workspace_bytes": (SZ, []),
     "kvr_paged_attn": (I, [P, I, I64, I, I, I, I, I64, P, P, I64, I, I64, I64, P, I64, I, P, SZ, F, P, P, P, SZ, P]),
     "kvr_prompt_attn": (I, [P, P, P, I, I64, I64, I, I, I, I, I64, I64, I64, P, SZ, F, P, P, P, SZ, P]),
+    "kvr_paged_reorder_workspace_bytes": (SZ, [I, I, I]),
+    "kvr_paged_reorder": (I, [P, I64, I, I, P, I, P, I64, P, I64, P, P, P, I, I, P, P, I, I, I, I, I64, I64, I64, P, P, SZ,
+                              P]),
+    "kvr_beam_select_workspace_bytes": (SZ, [I, I, I64, I, I]),
+    "kvr_beam_select": (I, [P, I, I64, I, I, I64, P, I, P, I, P, P, P, P, P, P, P, SZ, P]),
     "kvr_decode_attn_noalloc_max_scratch_bytes": (SZ, []),
     "kvr_decode_attn_noalloc": (I, [P, I, I, I, I, P, P, I, I, I64, I64, P, P, I, I, I64, I64, F, P, I, P]),
 }

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import collections
 import contextlib
+import ctypes as C
 import math
 import threading
 
@@ -838,6 +839,119 @@ def attn_status(device=None):
                 first = first or e
     if first:
         raise first
+
+
+# ----------------------------------------------------------- beam search --
+
+
+class BeamStep:
+    """What beam_select chose: the n best continuations of each request in order,
+    scores (B, n) fp32, beams and tokens (B, n) int32, and the first K of them that
+    do not end a sequence, next_scores, next_beams, next_tokens (B, K).  Places
+    without a continuation hold -inf, -1, -1."""
+
+    __slots__ = ("scores", "beams", "tokens", "next_scores", "next_beams", "next_tokens")
+
+
+_BEAM_WS: dict = {}
+_EOS: dict = {}
+
+
+def beam_select(logits, scores, n=None, eos=()):
+    """Beam search's choice: logits (B * K, V), or (B, K, V), of K beams of B
+    requests (rows may be strided or expanded) and the beams' scores (B, K) fp32.  A
+    continuation's score is its beam's plus the log-softmax of its logit; those that
+    are not finite (masked by -inf, of a beam of score -inf) are none.  n: how many
+    are listed of each request (K * (1 + len(eos)) where not given: enough for K to
+    go on).  eos: token ids (host integers) that end a sequence."""
+    if logits.dim() == 3:
+        logits = logits.flatten(0, 1)
+    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+        raise ValueError(f"logits must be (B * K, V) and scores (B, K), got {tuple(logits.shape)} and {tuple(scores.shape)}")
+    if scores.dtype is not torch.float32:
+        raise TypeError("scores must be fp32")
+    batch, beams = scores.shape
+    vocab = logits.shape[1]
+    if n is None:
+        n = beams * (1 + len(eos))
+    if beams < 1 or vocab < 1 or n < beams:
+        raise ValueError(f"{beams} beams, {vocab} tokens and {n} continuations: each request needs one at least, and n >= K")
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    scores = _c(scores)
+    _on_gpu(logits, scores)
+    code, dev = dtype_code(logits), logits.device
+    eos = tuple(eos)
+    ends = _EOS.get(eos)
+    if ends is None:
+        if len(_EOS) > 256:
+            _EOS.clear()
+        ends = _EOS[eos] = (C.c_int32 * max(len(eos), 1))(*eos)
+    key = (batch, beams, vocab, code, n)
+    need = _BEAM_WS.get(key)
+    if need is None:
+        if len(_BEAM_WS) > 4096:
+            _BEAM_WS.clear()
+        need = _BEAM_WS[key] = call("kvr_beam_select_workspace_bytes", *key)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    st = BeamStep()
+    f32, i32 = dict(dtype=torch.float32, device=dev), dict(dtype=_INT32, device=dev)
+    st.scores, st.next_scores = torch.empty(batch, n, **f32), torch.empty(batch, beams, **f32)
+    st.beams, st.tokens = torch.empty(batch, n, **i32), torch.empty(batch, n, **i32)
+    st.next_beams, st.next_tokens = torch.empty(batch, beams, **i32), torch.empty(batch, beams, **i32)
+    call("kvr_beam_select", logits.data_ptr(), code, logits.stride(0), batch, beams, vocab, scores.data_ptr(), n, ends,
+         len(eos), st.scores.data_ptr(), st.beams.data_ptr(), st.tokens.data_ptr(), st.next_scores.data_ptr(),
+         st.next_beams.data_ptr(), st.next_tokens.data_ptr(), ws.data_ptr(), need, stream())
+    return st
+
+
+_REORDER_WS: dict = {}
+
+
+def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parents, k_pages, v_pages):
+    """Rows of a paged cache become copies of their parents', in place: row rows[g,
+    i] of block_table and ctx_len gets what row rows[g, parents[g, i]] had (a parent
+    of -1: nothing, the row is emptied).  rows and parents (G, K) int32 on the
+    device; no row may be named twice.  shared (n_pages) int32 counts the holders of
+    each page beyond the first; free_pages[:n_free] is the list of free ones, with
+    room for all.  Full pages are shared; a last page that is not full is copied for
+    every child but the first, in the pools k_pages and v_pages ([layers,] n_pages, page,
+    n_kv, d).  Returns info (4) int32 = [pages missing, copied, given back, 0]; a row that finds no page keeps
+    its full pages."""
+    if k_pages.dim() == 5:
+        layers, ls = k_pages.shape[0], k_pages.stride(0)
+        one_k, one_v = k_pages[0], v_pages[0] if v_pages.dim() == 5 else v_pages
+        if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
+            raise ValueError("k_pages and v_pages must have one shape, type and layout")
+    else:
+        layers, ls, one_k, one_v = 1, 0, k_pages, v_pages
+    n_pages, page, ps, ts = _pool(one_k, one_v)
+    _i32(shared, "shared", n_pages)
+    cap = _i32(free_pages, "free_pages")
+    _i32(n_free, "n_free", 1)
+    n_rows = _i32(ctx_len, "ctx_len")
+    width, stride = _table(block_table, n_rows)
+    if rows.dtype is not _INT32 or parents.dtype is not _INT32 or rows.dim() != 2 or rows.shape != parents.shape:
+        raise TypeError("rows and parents must be int32 matrices of one shape (groups, beams)")
+    groups, beams = rows.shape
+    if beams < 1:
+        raise ValueError("a group needs at least one row")
+    rows, parents = _c(rows), _c(parents)
+    _on_gpu(block_table, ctx_len, shared, free_pages, n_free, rows, parents, k_pages, v_pages)
+    dev = rows.device
+    key = (groups, beams, width)
+    need = _REORDER_WS.get(key)
+    if need is None:
+        if len(_REORDER_WS) > 4096:
+            _REORDER_WS.clear()
+        need = _REORDER_WS[key] = max(call("kvr_paged_reorder_workspace_bytes", *key), 16)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    info = torch.empty(4, dtype=_INT32, device=dev)
+    call("kvr_paged_reorder", block_table.data_ptr(), stride, n_rows, width, ctx_len.data_ptr(), page, shared.data_ptr(),
+         n_pages, free_pages.data_ptr(), cap, n_free.data_ptr(), rows.data_ptr(), parents.data_ptr(), groups, beams,
+         k_pages.data_ptr(), v_pages.data_ptr(), dtype_code(k_pages), layers, one_k.shape[2], D, ls, ps, ts, info.data_ptr(),
+         ws.data_ptr(), need, stream())
+    return info
 
 
 def kmeans(x, k=128, iters=10):
