@@ -553,6 +553,26 @@ KVR_API int kvr_beam_select(const void *logits, int dtype, int64_t row_stride, i
                             int32_t *tokens, float *next_scores, int32_t *next_beams, int32_t *next_tokens,
                             void *workspace, size_t workspace_bytes, kvr_stream_t stream);
 
+/* A sparse MLP of a few tokens: z = x router^T, p = softmax(z); of each token the
+ * top_k largest p (equal ones by expert) with weights w = scale * p, or, with norm,
+ * scale * p / (sum of the chosen p); y = sum w * down_e (silu(gate_e x) * (up_e x)).
+ * fp16 or bf16 throughout, fp32 sums; h = silu(gate) * up is rounded to the type.
+ * x (n_tokens, hidden) with x_stride; router (experts, hidden); gate_up (experts,
+ * 2 * inter, hidden), the gate's rows before the up's; down (experts, hidden, inter);
+ * strides in elements, multiples of 8.  y (n_tokens, hidden) contiguous, not in x;
+ * ids, weights (n_tokens, top_k): the choice, in falling order.  A token with a NaN
+ * or infinity gives NaN, the others are not touched by it.  At most 128 tokens, 512
+ * experts, 16 of them a token; hidden and inter multiples of 8.  The workspace
+ * (256-byte aligned) needs no clearing and keeps nothing between calls; status, a
+ * word that the caller has zeroed once (16-byte aligned), is set where a bounded wait
+ * gave up (y then means nothing): kvr_workspace_status reads and clears it. */
+KVR_API size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int top_k);
+KVR_API int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hidden, int64_t x_stride, const void *router,
+                          int64_t router_stride, const void *gate_up, int64_t gu_expert_stride, int64_t gu_row_stride,
+                          const void *down, int64_t down_expert_stride, int64_t down_row_stride, int experts, int inter,
+                          int top_k, int norm, float scale, void *y, int32_t *ids, float *weights, void *workspace,
+                          size_t workspace_bytes, void *status, kvr_stream_t stream);
+
 /* Allocation-free variant of kvr_decode_attn (no counterpart in the
  * reference).  For callers that cannot allocate device memory — a plugin
  * inside a host that owns the GPU heap, or a path where cudaMalloc would

@@ -85,21 +85,24 @@ def reorder(table, ctx, shared, free, n_free, rows, parents, page):
 
 def moe(x, router, gate_up, down, top_k, norm=True, scale=1.0):
     """x (T, H), router (E, H), gate_up (E, 2 I, H), down (E, H, I) in float64 ->
-    (y (T, H), ids (T, k), weights (T, k), spread (T, H)): spread = sum of |w h d|
-    over experts and channels, what an error of the rounded h scales with."""
+    (y (T, H), ids (T, k), weights (T, k), by_h, by_sums, by_one): what errors of y
+    scale with: sum of |w d h| (a relative error of h), of |w d| times the change of h
+    by one unit of the absolute products of its gate and up sums, and of |w d|."""
     z = x @ router.T
-    z = np.where(np.isnan(z), -np.inf, z)
     ids = np.argsort(-z, axis=1, kind="stable")[:, :top_k]
-    m = z.max(1, keepdims=True)
-    e = np.exp(z - m)
+    e = np.exp(z - z.max(1, keepdims=True))
     w = np.take_along_axis(e, ids, 1)
     w = scale * w / (w.sum(1, keepdims=True) if norm else e.sum(1, keepdims=True))
     inter = gate_up.shape[1] // 2
-    y, spread = np.zeros((x.shape[0], down.shape[1])), np.zeros((x.shape[0], down.shape[1]))
+    y, by_h, by_sums, by_one = (np.zeros((x.shape[0], down.shape[1])) for _ in range(4))
     for t in range(x.shape[0]):
         for n, ex in enumerate(ids[t]):
-            gu = gate_up[ex] @ x[t]
-            h = gu[:inter] / (1 + np.exp(-gu[:inter])) * gu[inter:]
-            y[t] += w[t, n] * (down[ex] @ h)
-            spread[t] += abs(w[t, n]) * (np.abs(down[ex]) @ np.abs(h))
-    return y, ids, w, spread
+            gu, ab = gate_up[ex] @ x[t], np.abs(gate_up[ex]) @ np.abs(x[t])
+            g, u = gu[:inter], gu[inter:]
+            silu = g / (1 + np.exp(-g))
+            d = np.abs(w[t, n]) * np.abs(down[ex])
+            y[t] += w[t, n] * (down[ex] @ (silu * u))
+            by_h[t] += d @ np.abs(silu * u)
+            by_sums[t] += d @ (1.1 * ab[:inter] * np.abs(u) + np.abs(silu) * ab[inter:])  # |silu'| < 1.1
+            by_one[t] += d.sum(1)
+    return y, ids, w, by_h, by_sums, by_one

@@ -74,10 +74,9 @@
 // Every wait is bounded; one that gives up sets the error word, lets the
 // copies and MMAs in flight drain and frees the tensor memory.  A warp's lanes
 // give up together: by a vote at the wait, or, where a vote costs time (the
-// issuing warps), by going on to the piece's end (ca_wait_on).
-#include <cuda.h>
-
+// issuing warps), by going on to the piece's end (tc_wait_on).
 #include "kvr_attn_plan.cuh"
+#include "kvr_tcgen05.cuh"
 
 namespace kvr {
 
@@ -119,16 +118,9 @@ struct ChunkArgs {
 
 // ------------------------------------------------------- tcgen05 and TMA ----
 
-// Shared-memory matrix descriptors with 128-byte swizzle, as a low word to
-// which an address step >> 4 can be added (addresses stay below 2^18) and a
-// constant high word.
-// K-major (Q, K): 8-row atoms of 1 KB, 1 KB apart.
 // N x K with N contiguous (V, N = channels): atoms of 64 channels x 8 keys; 16
 // KB to the other 64 channels (low word), 1 KB to the next 8 keys.
-constexpr uint32_t kCaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t ca_desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
 __device__ __forceinline__ uint32_t ca_desc_mn(uint32_t saddr) { return (saddr >> 4) | ((kCaHalf >> 4) << 16); }
-__device__ __forceinline__ uint64_t ca_desc(uint32_t lo) { return ((uint64_t)kCaDescHi << 32) | lo; }
 // kind::f16, fp32 accumulator, M 128 or 64, N 128.
 template <int DT>
 __host__ __device__ constexpr uint32_t ca_idesc(bool b_mn, uint32_t m = 128) {
@@ -136,13 +128,6 @@ __host__ __device__ constexpr uint32_t ca_idesc(bool b_mn, uint32_t m = 128) {
          ((128u >> 3) << 17) | ((m >> 4) << 24);
 }
 
-__device__ __forceinline__ void ca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
 __device__ __forceinline__ void ca_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -150,44 +135,8 @@ __device__ __forceinline__ void ca_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// One lane of the (converged) warp, the same one every time.
-__device__ __forceinline__ bool ca_elect() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
-  return p != 0;
-}
-// A value that is the same in all lanes, in a form the compiler knows to be:
-// MMA descriptors live in uniform registers, and moving each one there from
-// per-lane registers made an MMA cost 95 to 160 cycles to issue instead of 64.
-__device__ __forceinline__ uint32_t ca_uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ void ca_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void ca_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void ca_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void ca_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void ca_ld32(uint32_t taddr, float *f) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(f);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void ca_ld16(uint32_t taddr, float *f) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(f);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
 __device__ __forceinline__ void ca_st16(uint32_t taddr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -223,32 +172,6 @@ __device__ __forceinline__ void ca_tma5(uint32_t dst, const CUtensorMap *m, int 
 
 // ---------------------------------------------------------------- waiting ----
 
-__device__ __forceinline__ void ca_bar_init(uint64_t *bar, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ bool ca_wait(uint64_t *bar, unsigned phase, volatile int *abort_s) {
-#pragma unroll 1
-  for (uint32_t it = 0; !mbar_try_wait(bar, phase); ++it)
-    if (it >= kSpinLimit || *abort_s) return false;
-  return true;
-}
-// All lanes go on, or none does.
-__device__ __forceinline__ bool ca_wait_warp(uint64_t *bar, unsigned phase, volatile int *abort_s) {
-  return __all_sync(~0u, ca_wait(bar, phase, abort_s));
-}
-// The issuing warps' wait: returns in any case, and a wait that gives up only raises the abort flag.  No lane
-// takes another path by its own outcome, so the lanes cannot part (some in a shuffle that the others have left):
-// they go on issuing, within the CTA's own memory, and leave together at the piece's end, by a vote on the flag.
-// (A vote at each wait instead made a chunk of 512 at 32256 4 % slower.)
-__device__ __forceinline__ void ca_wait_on(uint64_t *bar, unsigned phase, volatile int *abort_s, unsigned *err) {
-#pragma unroll 1
-  for (uint32_t it = 0; !mbar_try_wait(bar, phase) && !*abort_s; ++it)
-    if (it >= kSpinLimit) {
-      atomicOr(err, 1u);
-      *abort_s = 1;
-    }
-}
 // Whether the phase is complete by now (never waits).
 __device__ __forceinline__ bool ca_test(uint64_t *bar, unsigned phase) {
   uint32_t done;
@@ -259,10 +182,6 @@ __device__ __forceinline__ bool ca_test(uint64_t *bar, unsigned phase) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ void ca_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // Stage of the n-th K (or V) tile.
 __device__ __forceinline__ int ca_stage(bool v, int n) { return v ? kCaStagesK + n % kCaStagesV : n % kCaStagesK; }
 
@@ -363,24 +282,24 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   if (tid == 9 * 32) {
     *abort_s = 0;
     for (int s = 0; s < kCaStages; ++s) {
-      ca_bar_init(&kv_full[s], 1);
-      ca_bar_init(&kv_empty[s], 1);
+      tc_bar_init(&kv_full[s], 1);
+      tc_bar_init(&kv_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      ca_bar_init(&q_full[t], 1);
-      ca_bar_init(&q_empty[t], 1);
-      ca_bar_init(&s_full[t], 1);
-      ca_bar_init(&p_full[2 * t], 4);
-      ca_bar_init(&p_full[2 * t + 1], 4);
-      ca_bar_init(&drained[t], 1);
-      ca_bar_init(&pv_done[t], 1);
+      tc_bar_init(&q_full[t], 1);
+      tc_bar_init(&q_empty[t], 1);
+      tc_bar_init(&s_full[t], 1);
+      tc_bar_init(&p_full[2 * t], 4);
+      tc_bar_init(&p_full[2 * t + 1], 4);
+      tc_bar_init(&drained[t], 1);
+      tc_bar_init(&pv_done[t], 1);
     }
-    ca_bar_init(s_free, 4);
+    tc_bar_init(s_free, 4);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // barriers: for the copies and commits
-  ca_fence_before();
+  tc_fence_before();
   __syncthreads();
-  ca_fence_after();
+  tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_wait();  // what follows reads the plan, q and the cache
   griddep_launch();  // the joining kernel waits for this grid's end
@@ -423,7 +342,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       };
       auto load = [&](const CUtensorMap *m, bool v, int kt) {
         const int n = fill[v], depth = v ? kCaStagesV : kCaStagesK, s = ca_stage(v, n);
-        if (n >= depth && !ca_wait_warp(&kv_empty[s], (unsigned)((n / depth - 1) & 1), abort_s)) return false;
+        if (n >= depth && !tc_wait_warp(&kv_empty[s], (unsigned)((n / depth - 1) & 1), abort_s)) return false;
         ++fill[v];
         const uint32_t dst = smem_u32(sm) + kCaOffKv + s * kCaTile;
         if (lane == 0) mbar_expect_tx(&kv_full[s], kCaTile);
@@ -440,7 +359,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         return true;
       };
       auto load_q = [&](int t) {
-        if (uses[t] > 0 && !ca_wait_warp(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
+        if (uses[t] > 0 && !tc_wait_warp(&q_empty[t], (unsigned)((uses[t] - 1) & 1), abort_s)) return false;
         const uint32_t dst = smem_u32(sm) + t * kCaTile;
         const int n_tok = min(tpt, c.p.n_tok - t * tpt);
         if (n_tok <= kCaFewTokens) {  // token by token, zeros below
@@ -501,7 +420,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     // ---- MMAs: warp 8 the products S, warp 10 the products P V
     const uint32_t q_base = smem_u32(sm), kv_base = q_base + kCaOffKv;
     const bool scores = warp == 8;
-    const uint32_t tmem_u = ca_uniform(tmem);
+    const uint32_t tmem_u = tc_uniform(tmem);
     const int depth = scores ? kCaStagesK : kCaStagesV;
     int j = 0;               // K or V tiles consumed so far
     int seen[2] = {0, 0};    // warp 8: Q tiles, warp 10: P tiles consumed so far
@@ -510,29 +429,29 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     for (int r = 0; ca_piece(a, sm + kCaOffRec, total, heads, per, r, c); ++r) {
       if (__any_sync(~0u, *abort_s)) break;
       const int tiles = c.two ? 2 : 1;
-      const uint32_t idesc = ca_uniform(ca_idesc<DT>(!scores, c.p.n_tok * g <= kCaFewRows ? 64 : 128));
+      const uint32_t idesc = tc_uniform(ca_idesc<DT>(!scores, c.p.n_tok * g <= kCaFewRows ? 64 : 128));
       // rows of V that no query row of the piece may see
       const int before = window > 0 ? c.p.first_end - window : 0;
       for (int i = 0; i < c.n; ++i, ++j) {
         const int s = ca_stage(!scores, j);
-        ca_wait_on(&kv_full[s], (unsigned)((j / depth) & 1), abort_s, a.err);
+        tc_wait_on(&kv_full[s], (unsigned)((j / depth) & 1), abort_s, a.err);
         if (scores) {
           for (int t = 0; t < tiles; ++t) {
-            if (i == 0) ca_wait_on(&q_full[t], (unsigned)(seen[t]++ & 1), abort_s, a.err);
-            if (si > 0) ca_wait_on(s_free, (unsigned)((si - 1) & 1), abort_s, a.err);
+            if (i == 0) tc_wait_on(&q_full[t], (unsigned)(seen[t]++ & 1), abort_s, a.err);
+            if (si > 0) tc_wait_on(s_free, (unsigned)((si - 1) & 1), abort_s, a.err);
             ++si;
-            ca_fence_after();
-            const uint32_t qa = ca_uniform(ca_desc_k(q_base + t * kCaTile));
-            const uint32_t kb = ca_uniform(ca_desc_k(kv_base + s * kCaTile));
-            const uint32_t full = ca_uniform(smem_u32(&s_full[t]));
-            if (ca_elect()) {
+            tc_fence_after();
+            const uint32_t qa = tc_uniform(tc_desc_k(q_base + t * kCaTile));
+            const uint32_t kb = tc_uniform(tc_desc_k(kv_base + s * kCaTile));
+            const uint32_t full = tc_uniform(smem_u32(&s_full[t]));
+            if (tc_elect()) {
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const uint32_t o = ((k >> 2) * kCaHalf + (k & 3) * 32) >> 4;
-                ca_mma_ss(tmem_u, ca_desc(qa + o), ca_desc(kb + o), idesc, k > 0);
+                tc_mma_ss(tmem_u, tc_desc(qa + o), tc_desc(kb + o), idesc, k > 0);
               }
-              ca_commit(full);
-              if (i + 1 == c.n) ca_commit(smem_u32(&q_empty[t]));
+              tc_commit(full);
+              if (i + 1 == c.n) tc_commit(smem_u32(&q_empty[t]));
             }
           }
         } else {
@@ -548,32 +467,32 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             __syncwarp();
           }
           for (int t = 0; t < tiles; ++t) {
-            const uint32_t vb = ca_uniform(ca_desc_mn(kv_base + s * kCaTile)), add = ca_uniform(i > 0 ? 1u : 0u);
-            const uint32_t pa = ca_uniform(tmem + 128 + t * 64), oa = ca_uniform(tmem + 256 + t * 128);
-            const uint32_t done = ca_uniform(smem_u32(&pv_done[t]));
+            const uint32_t vb = tc_uniform(ca_desc_mn(kv_base + s * kCaTile)), add = tc_uniform(i > 0 ? 1u : 0u);
+            const uint32_t pa = tc_uniform(tmem + 128 + t * 64), oa = tc_uniform(tmem + 256 + t * 128);
+            const uint32_t done = tc_uniform(smem_u32(&pv_done[t]));
             // in two halves of the keys: the first weights are multiplied while the others are formed
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              ca_wait_on(&p_full[2 * t + half], (unsigned)(seen[t] & 1), abort_s, a.err);
-              ca_fence_after();
-              if (ca_elect()) {
+              tc_wait_on(&p_full[2 * t + half], (unsigned)(seen[t] & 1), abort_s, a.err);
+              tc_fence_after();
+              if (tc_elect()) {
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  ca_mma_ts(oa, pa + k * 8, ca_desc(vb + k * (2048 >> 4)), idesc, k > 0 ? 1u : add);
-                if (half) ca_commit(done);
+                  ca_mma_ts(oa, pa + k * 8, tc_desc(vb + k * (2048 >> 4)), idesc, k > 0 ? 1u : add);
+                if (half) tc_commit(done);
               }
             }
             ++seen[t];
           }
         }
         __syncwarp();
-        if (ca_elect()) ca_commit(smem_u32(&kv_empty[s]));
+        if (tc_elect()) tc_commit(smem_u32(&kv_empty[s]));
       }
     }
     // every MMA, and the arrivals that its commits owe, before the tensor memory is freed and the CTA ends
     uint64_t *bar = &drained[scores ? 0 : 1];
     __syncwarp();
-    if (ca_elect()) ca_commit(smem_u32(bar));
+    if (tc_elect()) tc_commit(smem_u32(bar));
     for (uint32_t it = 0; it < kSpinLimit && !mbar_try_wait(bar, 0);) ++it;
     __syncthreads();
   }
@@ -599,17 +518,17 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int begin_b = window > 0 ? max(0, c.p.first_end + tok_b - window) : 0;
       float mc = live ? kLowest : INFINITY, l = 0.0f;  // running maximum in log2 units (rows without a query: weights 0), sum
       for (int i = 0; i < c.n; ++i, ++sn) {
-        ok = ca_wait_warp(&s_full[t], (unsigned)(sn & 1), abort_s);
+        ok = tc_wait_warp(&s_full[t], (unsigned)(sn & 1), abort_s);
         if (!ok) break;
         if (busy) {
-          ca_fence_after();
+          tc_fence_after();
           float s[128];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ca_ld32(s_addr + k * 32, s + k * 32);
-          ca_wait_ld();
-          ca_fence_before();
+          for (int k = 0; k < 4; ++k) tc_ld32(s_addr + k * 32, s + k * 32);
+          tc_wait_ld();
+          tc_fence_before();
           __syncwarp();
-          if (lane == 0) ca_arrive(s_free);
+          if (lane == 0) tc_arrive(s_free);
           const int k0 = (c.p.kt0 + i) * 128;
           if (__builtin_expect(k0 + 128 > end_a || k0 < begin_b, 0)) {
 #pragma unroll
@@ -639,19 +558,19 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           // P V of the tile before: whether it is through is asked ahead of the place that needs to know
           bool before = i > 0, seen_pv = !before || ca_test(&pv_done[t], (unsigned)(on & 1));
           if (__builtin_expect(i > 0 && __any_sync(~0u, grow), 0)) {
-            ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
+            ok = tc_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
             if (!ok) break;
             ++on;
             before = false;
             seen_pv = true;
-            ca_fence_after();
+            tc_fence_after();
             const float f = grow ? ca_exp2(mc - top) : 1.0f;
             l *= f;
 #pragma unroll 1
             for (int k = 0; k < 8; ++k) {
               float o[16];
-              ca_ld16(o_addr + k * 16, o);
-              ca_wait_ld();
+              tc_ld16(o_addr + k * 16, o);
+              tc_wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = f == 0.0f ? 0.0f : o[e] * f;
               ca_st16(o_addr + k * 16, reinterpret_cast<const uint32_t *>(o));
@@ -677,19 +596,19 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             if (b == 31) {
               // P is free once P V of the tile before has read it
               if (!__all_sync(~0u, seen_pv)) {
-                ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
+                ok = tc_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
                 if (!ok) break;
               }
               on += before;
-              ca_fence_after();
+              tc_fence_after();
               ca_st16(p_addr, pk);
               ca_st16(p_addr + 16, pk + 16);
             }
             if (b == 47) {  // the first half's stores have had 16 pairs to land
               ca_wait_st();
-              ca_fence_before();
+              tc_fence_before();
               __syncwarp();
-              if (lane == 0) ca_arrive(&p_full[2 * t]);
+              if (lane == 0) tc_arrive(&p_full[2 * t]);
               ca_st16(p_addr + 32, pk + 32);
             }
             if (b == 63) ca_st16(p_addr + 48, pk + 48);
@@ -698,37 +617,37 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const uint64_t sum = ca_add2(ca_add2(sums[0], sums[1]), ca_add2(sums[2], sums[3]));
           l += ca_lo(sum) + ca_hi(sum);
           ca_wait_st();
-          ca_fence_before();
+          tc_fence_before();
         } else {
-          if (lane == 0) ca_arrive(s_free);
+          if (lane == 0) tc_arrive(s_free);
           if (i == 0) {  // no query in the warp's rows: weights 0
             const uint32_t zero[16] = {};
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) ca_st16(p_addr + k * 16, zero);
             ca_wait_st();
-            ca_fence_before();
+            tc_fence_before();
           }
           if (i > 0) {
-            ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
+            ok = tc_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
             if (!ok) break;
             ++on;
           }
-          if (lane == 0) ca_arrive(&p_full[2 * t]);
+          if (lane == 0) tc_arrive(&p_full[2 * t]);
         }
         __syncwarp();
-        if (lane == 0) ca_arrive(&p_full[2 * t + 1]);
+        if (lane == 0) tc_arrive(&p_full[2 * t + 1]);
       }
       if (!ok) break;
       // ---- the piece's rows
       if (c.n > 0) {
-        ok = ca_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
+        ok = tc_wait_warp(&pv_done[t], (unsigned)(on & 1), abort_s);
         if (!ok) break;
         ++on;
       }
       if (!busy) continue;
       // a row that saw a key has a weight of 2^kShift at least
       const bool none = l < 1.0f;
-      ca_fence_after();
+      tc_fence_after();
       const int64_t token = (int64_t)c.p.q_start + tok;
       const int hq = c.head * g + row - tok_in * g;
       const bool store = live && token >= 0 && token < a.n_tokens;
@@ -737,8 +656,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {
           float o[32];
-          ca_ld32(o_addr + k * 32, o);
-          ca_wait_ld();
+          tc_ld32(o_addr + k * 32, o);
+          tc_wait_ld();
           if (live) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -753,8 +672,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         for (int k = 0; k < 4; ++k) {
           float o[32];
           if (c.n > 0) {
-            ca_ld32(o_addr + k * 32, o);
-            ca_wait_ld();
+            tc_ld32(o_addr + k * 32, o);
+            tc_wait_ld();
           }
           if (store) {
 #pragma unroll
@@ -772,7 +691,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         if (store && a.lse) a.lse[token * a.n_q + hq] = none ? -INFINITY : (mc - kShift + log2f(l)) * kLn2;
       }
       // the next piece's first P V overwrites O: it waits for p_full, which this warp arrives at later
-      ca_fence_before();
+      tc_fence_before();
     }
     if (!ok && lane == 0) {
       if (!*abort_s) atomicOr(a.err, 1u);
@@ -781,7 +700,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     __syncthreads();
   }
   // every role is past its last access to the tensor memory (or drained after an abort)
-  ca_fence_after();
+  tc_fence_after();
   __syncwarp();
   if (warp == 8)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCaTmemCols));
@@ -848,41 +767,6 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
 }
 
 // ------------------------------------------------------------------- host ----
-
-typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
-
-// The driver's calls need a context in the calling thread; a thread that has made no runtime call with a device yet
-// (its memory came from a cache) has none.
-static void bind_context() {
-  static thread_local int bound = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
-}
-
-// A tensor of 16-bit values with dims[0] = 64 channels (one swizzle row);
-// strides (bytes) and boxes of the other dimensions follow.
-static bool make_map(CUtensorMap *m, int dtype, const void *base, int rank, const cuuint64_t *dims,
-                     const cuuint64_t *strides, const cuuint32_t *box) {
-  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  return encode_tiled()(m, dtype == KVR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                        (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 
 struct ChunkCall {
   const void *q, *k, *v;

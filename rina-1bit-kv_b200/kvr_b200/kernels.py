@@ -954,6 +954,89 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
     return info
 
 
+# ------------------------------------------------------------ sparse MLP --
+
+MOE_MAX_TOKENS = 128
+_MOE_WS: dict = {}
+_MOE_STATUS: dict = {}
+
+
+def _experts(w, name, shape):
+    """(E, rows, columns) with contiguous columns; its strides of experts and rows."""
+    if w.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(w.shape)}")
+    es, rs, cs = w.stride()
+    if cs != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return (es if shape[0] > 1 else shape[1] * rs), rs
+
+
+def _moe_status(device):
+    ws = _MOE_STATUS.get(device)
+    if ws is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first moe_layer call on a device must be made outside of a graph capture")
+        ws = _MOE_STATUS[device] = torch.zeros(256, dtype=torch.uint8, device=device)
+        torch.cuda.current_stream(device).synchronize()  # zeroed before a call on any stream uses it
+    return ws
+
+
+def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=None, return_routing=False):
+    """A sparse MLP of at most MOE_MAX_TOKENS tokens: x (T, H), router (E, H),
+    gate_up (E, 2 I, H) with the gate's rows first, down (E, H, I), all fp16 or all
+    bf16.  Each token goes to the top_k experts of the largest softmax(x router^T),
+    with those as weights (norm_topk: divided by their sum), times scale; an expert is
+    down(silu(gate x) * up x).  Returns y (T, H), or (y, ids (T, k) int32, weights (T, k) fp32)."""
+    if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3:
+        raise ValueError("x must be (T, H), router (E, H), gate_up (E, 2 I, H), down (E, H, I)")
+    n_tokens, hidden = x.shape
+    experts, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    if router.shape != (experts, hidden):
+        raise ValueError(f"router must be {(experts, hidden)}, got {tuple(router.shape)}")
+    ge, gr = _experts(gate_up, "gate_up", (experts, 2 * inter, hidden))
+    de, dr = _experts(down, "down", (experts, hidden, inter))
+    dt = x.dtype
+    if router.dtype is not dt or gate_up.dtype is not dt or down.dtype is not dt:
+        raise TypeError("x, router and the experts must share a dtype")
+    xs, rs = x.stride(0), router.stride(0)
+    if x.stride(1) != 1 or (n_tokens > 1 and (xs < hidden or xs % 8)) or x.data_ptr() % 16:
+        x, xs = x.clone(memory_format=torch.contiguous_format), hidden
+    if n_tokens <= 1:
+        xs = hidden
+    if router.stride(1) != 1 or (experts > 1 and (rs < hidden or rs % 8)):
+        raise ValueError("router: rows must be contiguous and 16-byte aligned")
+    if experts == 1:
+        rs = hidden
+    if out is None:
+        out = torch.empty(n_tokens, hidden, dtype=dt, device=x.device)
+    elif out.shape != (n_tokens, hidden) or out.dtype is not dt or not out.is_contiguous():
+        raise ValueError("out must be contiguous and of x's shape and dtype")
+    _on_gpu(x, router, gate_up, down, out)
+    dev = x.device
+    key = (n_tokens, hidden, inter, top_k)
+    need = _MOE_WS.get(key)
+    if need is None:
+        if len(_MOE_WS) > 4096:
+            _MOE_WS.clear()
+        need = _MOE_WS[key] = call("kvr_moe_workspace_bytes", *key)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ids = torch.empty(n_tokens, top_k, dtype=_INT32, device=dev)
+    weights = torch.empty(n_tokens, top_k, dtype=torch.float32, device=dev)
+    call("kvr_moe_layer", x.data_ptr(), dtype_code(x), n_tokens, hidden, xs, router.data_ptr(), rs, gate_up.data_ptr(), ge, gr,
+         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), ids.data_ptr(),
+         weights.data_ptr(), ws.data_ptr(), need, _moe_status(dev).data_ptr(), stream())
+    return (out, ids, weights) if return_routing else out
+
+
+def moe_status(device=None):
+    """Raises if a moe_layer call on the device gave up a wait (synchronises the
+    current stream)."""
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    call("kvr_workspace_status", _moe_status(device).data_ptr(), stream())
+
+
 def kmeans(x, k=128, iters=10):
     """Deterministic Lloyd k-means on the device: x (n, 128) -> (labels (n,)
     int32, centroids (k, 128) fp32)."""

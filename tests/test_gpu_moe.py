@@ -1,0 +1,139 @@
+"""The sparse MLP of a few tokens on the GPU against its 64-bit specification.
+
+Tolerance, with u half a step of the type (bf16 2^-8, fp16 2^-11): y is rounded (u
+|y|), h is rounded (u sum |w d h|, and in fp16 half a step of the smallest
+subnormals, 2^-25 sum |w d|), sums of H and of I products in fp32 (n 2^-23 of the
+absolute products each, rounded or cut), and 2^-20 for the router weights and the
+exponentials of silu (some steps of fp32).
+
+A weight e^z / sum e^z is off by 2^-21 of itself (exponentials, sum and division,
+some steps of fp32) and by what its logits are: a lane adds H / 32 exact products in fp32,
+so a logit is off by d <= H / 32 2^-24 sum |x r|, and the quotient by e^(2 d) - 1 <= 2.1 d."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import decode_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def inputs(T, H, I, E, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    return [t.to(DT[dtype]) for t in (n(T, H), n(E, H) * 1.3 / H ** 0.5, n(E, 2 * I, H) / H ** 0.5, n(E, H, I) / I ** 0.5)]
+
+
+def check(x, router, gu, down, k, norm=True, scale=1.0, **kw):
+    from kvr_b200 import kernels as K
+    y, ids, w = K.moe_layer(x, router, gu, down, k, norm_topk=norm, scale=scale, return_routing=True, **kw)
+    K.moe_status()
+    f = lambda t: t.double().cpu().numpy()  # noqa: E731
+    wy, wi, ww, by_h, by_sums, by_one = R.moe(f(x), f(router), f(gu), f(down), k, norm, scale)
+    assert np.array_equal(ids.cpu().numpy(), wi)
+    d = -(-x.shape[1] // 256) * 8 * 2.0 ** -24 * (np.abs(f(x)) @ np.abs(f(router)).T).max(1, keepdims=True)
+    assert (np.abs(f(w) - ww) <= (2.0 ** -21 + 2.1 * d) * ww).all()
+    u = torch.finfo(x.dtype).eps / 2
+    H, I = x.shape[1], down.shape[2]
+    tol = (u + 2.0 ** -20) * np.abs(wy) + (u + 2.0 ** -20 + 2.1 * d + I * 2.0 ** -23) * (1 + u) * by_h + H * 2.0 ** -23 * by_sums + 2.0 ** -25 * by_one
+    err = np.abs(f(y) - wy)
+    assert (err <= tol).all(), (err / tol).max()
+    assert y.dtype is x.dtype
+    return y
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,H,I,E,k", [
+    (1, 64, 16, 1, 1), (1, 8, 8, 3, 2), (2, 72, 40, 5, 3), (1, 1024, 512, 16, 2), (5, 512, 264, 60, 5), (17, 256, 104, 128, 8),
+    (64, 200, 136, 9, 9), (128, 128, 64, 4, 2), (128, 328, 72, 130, 8), (33, 1544, 1000, 12, 4), (128, 64, 32, 512, 16),
+    (16, 64, 2048, 2, 1), (100, 136, 24, 300, 1)])
+def test_layer(T, H, I, E, k, dtype):
+    check(*inputs(T, H, I, E, dtype, T + H), k)
+
+
+@pytest.mark.parametrize("norm,scale", [(False, 1.0), (True, 2.5), (False, 0.5)])
+def test_weights(norm, scale):
+    check(*inputs(9, 256, 96, 24, "bf16", 3), 4, norm, scale)
+
+
+def test_every_token_to_the_same_experts():
+    """128 tokens on two experts of 64: segments of many columns, most experts without any."""
+    x, router, gu, down = inputs(128, 256, 96, 64, "bf16", 5)
+    x[:, 0], router[:, 0] = 1.0, 0.0
+    router[7, 0] = router[40, 0] = 30.0
+    check(x, router, gu, down, 2)
+
+
+def test_equal_logits_go_to_the_lowest_experts():
+    x, router, gu, down = inputs(6, 128, 64, 20, "f16", 6)
+    router[:] = router[:1]
+    check(x, router, gu, down, 3)
+
+
+def test_strided_inputs():
+    x, router, gu, down = inputs(10, 256, 96, 8, "bf16", 7)
+    wide = torch.zeros(10, 512, dtype=x.dtype, device=DEV)
+    wide[:, 64:320] = x
+    gu2 = torch.zeros(8, 200, 264, dtype=x.dtype, device=DEV)
+    gu2[:, :192, :256] = gu
+    d2 = torch.zeros(8, 260, 104, dtype=x.dtype, device=DEV)
+    d2[:, :256, :96] = down
+    a = check(wide[:, 64:320], router, gu2[:, :192, :256], d2[:, :256, :96], 3)
+    b = check(x, router, gu, down, 3)
+    assert torch.equal(a, b)
+    odd = torch.zeros(10, 259, dtype=x.dtype, device=DEV)  # rows that TMA cannot read are copied
+    odd[:, 3:] = x
+    assert torch.equal(check(odd[:, 3:], router, gu, down, 3), b)
+
+
+def test_a_bad_token_stays_alone():
+    from kvr_b200 import kernels as K
+    x, router, gu, down = inputs(40, 256, 96, 8, "bf16", 8)
+    good, ids, w = K.moe_layer(x, router, gu, down, 2, return_routing=True)
+    x[3, 17], x[20, 5], x[39, 0] = float("nan"), float("inf"), -float("inf")
+    y, ids2, w2 = K.moe_layer(x, router, gu, down, 2, return_routing=True)
+    K.moe_status()
+    bad = torch.zeros(40, dtype=torch.bool, device=DEV)
+    bad[[3, 20, 39]] = True
+    assert y[bad].isnan().all() and w2[bad].isnan().all() and ((ids2 >= 0) & (ids2 < 8)).all()
+    assert torch.equal(y[~bad], good[~bad]) and torch.equal(ids2[~bad], ids[~bad])
+
+
+def test_repeats_and_no_tokens():
+    from kvr_b200 import kernels as K
+    a = inputs(77, 512, 200, 40, "bf16", 9)
+    first = K.moe_layer(*a, 6)
+    for _ in range(20):
+        assert torch.equal(K.moe_layer(*a, 6), first)
+    y, ids, w = K.moe_layer(a[0][:0], *a[1:], 6, return_routing=True)
+    assert y.shape == (0, 512) and ids.shape == (0, 6) and w.shape == (0, 6)
+    K.moe_status()
+
+
+def test_graph_and_streams():
+    """A captured call replayed with new inputs, beside calls on two other streams."""
+    from kvr_b200 import kernels as K
+    x, router, gu, down = inputs(24, 512, 200, 32, "f16", 10)
+    K.moe_status()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = K.moe_layer(x, router, gu, down, 4)
+    others = [inputs(t, 512, 200, 32, "f16", 10 + t) for t in (1, 128)]
+    want = [K.moe_layer(*o, 4) for o in others]
+    streams = [torch.cuda.Stream() for _ in others]
+    for seed in (1, 2, 3):
+        new = inputs(24, 512, 200, 32, "f16", seed)
+        for a, b in zip((x, router, gu, down), new):
+            a.copy_(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        got = []
+        for s, o in zip(streams, others):
+            with torch.cuda.stream(s):
+                got += [K.moe_layer(*o, 4) for _ in range(5)]
+        torch.cuda.synchronize()
+        assert torch.equal(y, K.moe_layer(*new, 4))
+        assert all(torch.equal(g, want[i // 5]) for i, g in enumerate(got))
+    K.moe_status()
