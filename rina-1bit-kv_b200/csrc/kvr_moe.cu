@@ -8,7 +8,7 @@
 // what has to be read; a token's share of the arithmetic is small.  So the weights
 // are streamed once, and the tokens ride along.  Two kernels:
 //
-// moe_route_kernel: clusters of 8 CTAs take 8 tokens; a CTA forms the logits of an
+// moe_route_kernel: clusters of 8 CTAs take 1 to 8 tokens; a CTA forms the logits of an
 // eighth of the experts, the cluster exchanges them over distributed shared memory,
 // and CTA r ranks token r's.  Logits are sums of exact products, 32-bit partial sums
 // per lane joined in 64 bits: the last expert chosen and the first left out can lie
@@ -19,22 +19,23 @@
 // little more than its weights' bytes and a few tokens leave no rows empty that memory
 // would have to fill.  Segments are an expert's tokens, at most `cols` of them.
 // Work units, taken in order from one ticket counter:
-//   gate/up  R1 rows (16 of gate, 16 of up, ...) of a segment's expert over x: h, in 16 bits
-//   down     R2 rows of Wd over h: partial rows (token, choice) in 32 bits
+//   gate/up  R1 rows (16 of gate, 16 of up, ...) of a segment's expert over x: h, in two
+//            16-bit parts
+//   down     R2 rows of Wd over both parts of h: partial rows (token, choice) in 32 bits
+//   sum      128 columns of y of some tokens: the choices of each token in their order
 // A unit waits only for units with lower tickets, which run already: no CTA has to
 // be resident for another to end.  Weights of a down unit stream in while its h is
 // still being formed, so the memory does not idle between the phases.
 //   warp 0  tickets, weight tiles by TMA (128-byte swizzle) into a ring of stages
 //   warp 1  token rows by TMA gather into the same stages
 //   warp 2  tcgen05.mma, accumulators of two units in tensor memory
-//   warps 4-7  epilogues of 32 rows each; the warp that finishes the last segment of
-//           32 rows of y adds up the choices of each token, in their order: no atomics
-//           on values.
+//   warps 4-7  epilogues of 32 rows each; sums
 //
-// What is held in fewer than 32 bits: h, rounded to the tensors' type because
-// both operands of an MMA are of one 16-bit type.  Sums, router weights and
-// partial rows are fp32.  The error against 64 bits is that of two roundings, of h and of
-// y: sqrt(2) times that of rounding y alone.
+// Both operands of an MMA are of one 16-bit type, so h has to be rounded for the
+// second product.  It goes in as two columns, h rounded and what the rounding left:
+// 16 (bf16) or 22 bits (fp16) of it, for gathers and columns that the few tokens
+// leave room for.  (Rounded once, y was 1.4 to 1.6 times as far from 64 bits as its own
+// rounding makes it.)  Sums, router weights and partial rows are fp32.
 //
 // Waits are bounded; one that gives up sets the status word, lets copies and MMAs in
 // flight end and frees the tensor memory.
@@ -48,7 +49,7 @@ constexpr int kMoSms = 148;
 
 // ------------------------------------------------------------------ router ----
 
-constexpr int kMrThreads = 256, kMrCluster = 8, kMrTokens = 8;
+constexpr int kMrThreads = 256, kMrCluster = 8, kMrMaxTokens = 8;
 
 struct RouteArgs {
   const void *x, *router;
@@ -72,108 +73,108 @@ __device__ __forceinline__ double mo_peer_double(const double *p, unsigned rank)
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
   return v;
 }
-// Larger first; NaN below everything.
-__device__ __forceinline__ bool mo_above(double x, int i, double y, int j) {
-  return x > y || (x == y && i < j) || (y != y && (x == x || i < j));
+// Order-preserving map double -> uint64; NaN below everything, never 0.
+__device__ __forceinline__ uint64_t mo_key(double z) {
+  if (z != z) return 1;
+  const uint64_t u = (uint64_t)__double_as_longlong(z == 0.0 ? 0.0 : z);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-template <int DT>
+// NT tokens a cluster: as few as the SMs have clusters for, since a CTA's time is its tokens' products.
+template <int DT, int NT>
 __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads) moe_route_kernel(RouteArgs a) {
-  __shared__ double part[kMrTokens][kMoMaxExperts / kMrCluster];  // logits of this CTA's experts
+  constexpr int kWarps = kMrThreads / 32, kEach = kMoMaxExperts / 32;
+  __shared__ double part[NT][kMoMaxExperts / kMrCluster];  // logits of this CTA's experts
+  __shared__ double slice[kWarps][NT];                     // of a warp's channels
+  __shared__ double all_s[kMoMaxExperts];                  // of this CTA's token
+  __shared__ int chosen[kMoMaxTopK];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = blockIdx.x % kMrCluster, t0 = blockIdx.x / kMrCluster * kMrTokens;
-  const int n_tok = min(kMrTokens, a.tokens - t0);
+  const int rank = blockIdx.x % kMrCluster, t0 = blockIdx.x / kMrCluster * NT;
+  const int n_tok = min(NT, a.tokens - t0);
   griddep_wait();
   griddep_launch();
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.n_counters; i += kMrThreads) a.counters[i] = 0;
-  const int per = (a.experts + kMrCluster - 1) / kMrCluster, e0 = rank * per, e1 = min(a.experts, e0 + per);
-  for (int e = e0 + warp; e < e1; e += kMrThreads / 32) {
-    float s[kMrTokens] = {};
-    for (int c = lane * 8; c < a.hidden; c += 256) {
-      float w[8];
-      load8<DT>(a.router, e * a.router_stride + c, w);
+  const int per = (a.experts + kMrCluster - 1) / kMrCluster, e0 = rank * per, n_exp = max(0, min(a.experts - e0, per));
+  // a warp takes an expert, or with few experts a part of its channels
+  const int parts = n_exp > 0 && n_exp < kWarps ? kWarps / n_exp : 1, mine = warp / parts, step = kWarps / parts;
+  for (int e = mine; e < n_exp && mine < step; e += step) {
+    float s[NT] = {};
+    const int c0 = (warp - mine * parts) * 256 + lane * 8, dc = parts * 256;
+    const void *w_row = static_cast<const uint16_t *>(a.router) + (e0 + e) * a.router_stride;
+    const void *x_row = static_cast<const uint16_t *>(a.x) + t0 * a.x_stride;
+#pragma unroll(NT == 1 ? 8 : NT == 2 ? 4 : 2)
+    for (int c = c0; c < a.hidden; c += dc) {
+      float w[8], x[NT][8];
+      load8<DT>(w_row, c, w);
 #pragma unroll
-      for (int t = 0; t < kMrTokens; ++t) {
-        if (t < n_tok) {
-          float x[8];
-          load8<DT>(a.x, (t0 + t) * a.x_stride + c, x);
+      for (int t = 0; t < NT; ++t) load8<DT>(x_row, min(t, n_tok - 1) * a.x_stride + c, x[t]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s[t] = fmaf(x[j], w[j], s[t]);
-        }
-      }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[t] = fmaf(x[t][j], w[j], s[t]);
     }
 #pragma unroll
-    for (int t = 0; t < kMrTokens; ++t) {
+    for (int t = 0; t < NT; ++t) {
       double d = s[t];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (lane == t && t < n_tok) part[t][e - e0] = d;
+      if (lane == 0) {
+        if (parts == 1) part[t][e] = d;
+        else slice[warp][t] = d;
+      }
+    }
+  }
+  if (parts > 1) {  // in the order of the channels
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * n_exp; i += kMrThreads) {
+      const int t = i / n_exp, e = i - t * n_exp;
+      double d = 0.0;
+      for (int p = 0; p < parts; ++p) d += slice[e * parts + p][t];
+      part[t][e] = d;
     }
   }
   mo_cluster_sync();
-  // CTA r: token r, by one warp; lane l holds experts l, l + 32, ...
-  if (rank < n_tok && warp == 0) {
-    constexpr int kEach = kMoMaxExperts / 32;
-    const int64_t t = t0 + rank;
-    double z[kEach];
-    float e[kEach], m = -INFINITY;
+  // CTA r: token r.  Lane l of its first warp holds experts l, l + 32, ...
+  if (rank < n_tok) {
+    for (int e = threadIdx.x; e < a.experts; e += kMrThreads) all_s[e] = mo_peer_double(&part[rank][e % per], e / per);
+    __syncthreads();
+    if (warp == 0) {
+      uint64_t key[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int x = i * 32 + lane;
-      z[i] = 0.0;
-      if (x < a.experts) {
-        z[i] = mo_peer_double(&part[rank][x % per], x / per);
-        m = fmaxf(m, (float)z[i]);
-      }
-    }
-    m = warp_max(m);
-    float all = 0.0f;
+      for (int i = 0; i < kEach; ++i) key[i] = i * 32 + lane < a.experts ? mo_key(all_s[i * 32 + lane]) : 0;
+      for (int k = 0; k < a.top_k; ++k) {  // the largest key left, the lowest expert among equal ones
+        uint64_t best = key[0];
+        int at = lane;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      e[i] = i * 32 + lane < a.experts ? expf((float)(z[i] - (double)m)) : 0.0f;
-      all += e[i];
-    }
-    all = warp_sum(all);
-    unsigned taken = 0;
-    float sum = 0.0f, mine = 0.0f;
-    int my_id = 0;
-    for (int k = 0; k < a.top_k; ++k) {
-      double best = NAN;
-      int at = INT_MAX;
-      float v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int x = i * 32 + lane;
-        if (x < a.experts && !((taken >> i) & 1) && (at == INT_MAX || mo_above(z[i], x, best, at))) {
-          best = z[i];
-          at = x;
-          v = e[i];
+        for (int i = 1; i < kEach; ++i) {
+          if (i * 32 >= a.experts) break;
+          if (key[i] > best) {
+            best = key[i];
+            at = i * 32 + lane;
+          }
         }
-      }
+        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
+        const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
+        const bool top = (unsigned)(best >> 32) == hi && (unsigned)best == lo;
+        const int e = (int)__reduce_min_sync(0xffffffffu, top ? (unsigned)at : 0xffffffffu);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double ob = __shfl_xor_sync(0xffffffffu, best, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-        if (oa != INT_MAX && (at == INT_MAX || mo_above(ob, oa, best, at))) {
-          best = ob;
-          at = oa;
-          v = ov;
-        }
+        for (int i = 0; i < kEach; ++i)
+          if (e == i * 32 + lane) key[i] = 0;
+        if (lane == 0) chosen[k] = e;
       }
-      if ((at & 31) == lane) taken |= 1u << (at >> 5);
-      sum += v;
-      if (lane == k) {
-        mine = v;
-        my_id = at;
+      __syncwarp();
+      const double m = all_s[chosen[0]];  // (a NaN only where all are)
+      float all = 0.0f;
+      for (int e = lane; e < a.experts; e += 32) all += expf((float)(all_s[e] - m));
+      all = warp_sum(all);
+      const float w = lane < a.top_k ? expf((float)(all_s[chosen[lane]] - m)) : 0.0f, sum = warp_sum(w);
+      if (lane < a.top_k) {
+        const int64_t o = (int64_t)(t0 + rank) * a.top_k + lane;
+        a.ids[o] = chosen[lane];
+        // a logit that is no number, or infinite, leaves no weight that means anything
+        a.weights[o] = all < INFINITY ? a.scale * w / (a.norm ? sum : all) : NAN;
       }
-    }
-    if (lane < a.top_k) {
-      // a logit that is no number, or infinite, leaves no weight that means anything
-      const float w = all < INFINITY ? a.scale * mine / (a.norm ? sum : all) : NAN;
-      a.ids[t * a.top_k + lane] = my_id;
-      a.weights[t * a.top_k + lane] = w;
     }
   }
   mo_cluster_sync();  // the other CTAs' logits stay until they are read
@@ -185,23 +186,24 @@ constexpr int kMoThreads = 256;
 constexpr int kMoMaxStages = 16, kMoSched = 4;
 constexpr uint32_t kMoRing = 192 * 1024;   // stages
 constexpr uint32_t kMoPad = 16 * 1024;     // an MMA reads 128 rows from a tile's start, however few of them it uses
-constexpr uint32_t kMoTmemCols = 256;      // two accumulators of 128 columns
+constexpr uint32_t kMoTmemCols = 512;      // two accumulators of up to 256 columns
 constexpr int kMoMinCols = 16;
 constexpr int kMoMaxSegs = kMoMaxExperts + kMoMaxPicks / kMoMinCols;
+constexpr int kMoSumCols = 128;            // columns of y of a sum unit
 
 struct ExpertArgs {
   int tokens, hidden, inter, experts, top_k;
   int rows1, rows2;      // rows of a gate/up and of a down unit
   int kb1, kb2;          // 64-column blocks of a stage
   int cols;              // most tokens of a segment, a multiple of 16
+  int sum_tokens;        // tokens of a sum unit
   int stages;
   uint32_t stage_bytes, a_bytes;  // of a stage; its weights' part
   const int *ids;
   const float *weights;
-  void *h;               // (tokens * top_k, inter)
+  void *h;               // (tokens * top_k, 2, inter): rounded, rest
   float *part;           // (tokens * top_k, hidden)
   void *y;
-  int64_t y_stride;
   int *counters;         // ticket; warps' parts of segments' gate/up units done; segments done of 32-row strips of y
   unsigned *err;
 };
@@ -255,23 +257,39 @@ __host__ __device__ constexpr uint32_t mo_idesc(uint32_t n) {  // kind::f16, fp3
          ((128u >> 4) << 24);
 }
 
-// Work unit u: phase (0: gate/up, 1: down), segment, tile of rows.
+// Work unit u: phase (0: gate/up, 1: down, 2: sum), segment (2: columns of y), tile of rows (2: tokens).
 struct MoUnit {
-  int down, seg, tile;
+  int phase, seg, tile;
 };
-__device__ __forceinline__ MoUnit mo_unit(const ExpertArgs &a, int u, int segs, int tiles1) {
-  const int n1 = segs * tiles1;
+struct MoPlan {
+  int segs, tiles1, tiles2, sums;  // sums: units of a column block
+  int first2, first3, units;       // first down unit, first sum unit, all
+};
+__device__ __forceinline__ MoUnit mo_unit(const MoPlan &p, int u) {
   MoUnit w;
-  w.down = u >= n1;
-  if (!w.down) {
-    w.seg = u / tiles1;
-    w.tile = u - w.seg * tiles1;
-  } else {  // tile by tile, so that choices are added up while others are still multiplied
-    u -= n1;
-    w.tile = u / segs;
-    w.seg = u - w.tile * segs;
+  if (u < p.first2) {
+    w.phase = 0;
+    w.seg = u / p.tiles1;
+    w.tile = u - w.seg * p.tiles1;
+  } else if (u < p.first3) {  // tile by tile, so that no segment's h is waited for while others' is there
+    u -= p.first2;
+    w.phase = 1;
+    w.tile = u / p.segs;
+    w.seg = u - w.tile * p.segs;
+  } else {
+    u -= p.first3;
+    w.phase = 2;
+    w.seg = u / p.sums;
+    w.tile = u - w.seg * p.sums;
   }
   return w;
+}
+// The part of a 16-bit type that a value rounds to, kept finite (the rest then holds up to as much again).
+template <int DT>
+__device__ __forceinline__ float mo_rounded(float x) {
+  const float most = DT == KVR_F16 ? 65504.0f : 3.3895313892515355e38f;
+  const float r = round_dt<DT>(x);
+  return r > most ? most : r < -most ? -most : r;
 }
 
 template <int DT>
@@ -375,44 +393,58 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     s.picks[s.first[e] + before] = (short)i;
   }
   __syncthreads();
-  const int segs = s.n_segs;
-  const int tiles1 = (a.inter + a.rows1 / 2 - 1) / (a.rows1 / 2), tiles2 = (a.hidden + a.rows2 - 1) / a.rows2;
-  const int units = segs * (tiles1 + tiles2);
+  MoPlan p;
+  p.segs = s.n_segs;
+  p.tiles1 = (a.inter + a.rows1 / 2 - 1) / (a.rows1 / 2);
+  p.tiles2 = (a.hidden + a.rows2 - 1) / a.rows2;
+  p.sums = (a.tokens + a.sum_tokens - 1) / a.sum_tokens;
+  p.first2 = p.segs * p.tiles1;
+  p.first3 = p.first2 + p.segs * p.tiles2;
+  p.units = p.first3 + (a.hidden + kMoSumCols - 1) / kMoSumCols * p.sums;
   int *ticket = a.counters, *seg_done = a.counters + 1, *strip_done = seg_done + kMoMaxSegs;
   const int blocks1 = (a.hidden + 63) / 64, blocks2 = (a.inter + 63) / 64;
   const uint32_t ring = smem_u32(sm);
 
   if (warp == 0) {
-    // ---- tickets and weights: one lane
+    // ---- tickets and weights: one lane.  Stage and phase are counted up: with it % stages and it / stages a stage
+    // took 1000 cycles to issue, more than its bytes take to arrive.
     if (lane == 0) {
-      int it = 0, q = 0;
+      int st = 0, filled = 0;
+      unsigned parity = 1;
       int next = atomicAdd(ticket, 1);
       bool ok = true;
-      while (ok) {
+      for (int q = 0; ok; ++q) {
         const int u = next;
-        if (u < units) next = atomicAdd(ticket, 1);  // asked for ahead: its answer is due a unit later
+        if (u < p.units) next = atomicAdd(ticket, 1);  // asked for ahead: its answer is due a unit later
         ok = tc_wait(&s.sched_empty[q % kMoSched], ((q / kMoSched) & 1) ^ 1, abort_s);
         if (!ok) break;
-        s.sched[q % kMoSched] = u < units ? u : -1;
+        s.sched[q % kMoSched] = u < p.units ? u : -1;
         tc_arrive(&s.sched_full[q % kMoSched]);
-        ++q;
-        if (u >= units) break;
-        const MoUnit w = mo_unit(a, u, segs, tiles1);
+        if (u >= p.units) break;
+        const MoUnit w = mo_unit(p, u);
+        if (w.phase == 2) continue;
+        const bool down = w.phase == 1;
         const int e = s.seg_expert[w.seg];
-        const int blocks = w.down ? blocks2 : blocks1, kb = w.down ? a.kb2 : a.kb1, rows = w.down ? a.rows2 : a.rows1;
-        for (int b0 = 0; b0 < blocks; b0 += kb, ++it) {
-          const int st = it % a.stages, nb = min(kb, blocks - b0);
-          if (!(ok = tc_wait(&s.empty[st], ((it / a.stages) & 1) ^ 1, abort_s))) break;
+        const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, rows = down ? a.rows2 : a.rows1;
+        const int row = down ? w.tile * rows : w.tile * rows / 2;
+        for (int b0 = 0; b0 < blocks; b0 += kb) {
+          const int nb = min(kb, blocks - b0);
+          if (!(ok = tc_wait(&s.empty[st], parity, abort_s))) break;
           mbar_expect_tx(&s.full_a[st], nb * rows * 128);
           uint32_t dst = ring + st * a.stage_bytes;
-          for (int b = b0; b < b0 + nb; ++b) {
-            if (w.down) {
-              mo_tma3(dst, &mw2, b * 64, w.tile * rows, e, &s.full_a[st]);
+          for (int c = b0 * 64; c < (b0 + nb) * 64; c += 64) {
+            if (down) {
+              mo_tma3(dst, &mw2, c, row, e, &s.full_a[st]);
               dst += rows * 128;
             } else {
               for (int r = 0; r < rows; r += 32, dst += 32 * 128)  // 16 rows of gate, the same 16 of up
-                mo_tma4(dst, &mw1, b * 64, (w.tile * rows + r) / 2, 0, e, &s.full_a[st]);
+                mo_tma4(dst, &mw1, c, row + r / 2, 0, e, &s.full_a[st]);
             }
+          }
+          filled = min(filled + 1, a.stages);
+          if (++st == a.stages) {
+            st = 0;
+            parity ^= 1;
           }
         }
       }
@@ -422,12 +454,18 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       }
       // nothing may be in flight to this CTA's memory when it ends; after an abort the last stages were not seen full
       if (*abort_s)
-        for (int i = max(0, it - a.stages); i < it; ++i)
-          mbar_wait_bounded(&s.full_a[i % a.stages], (i / a.stages) & 1, 1u << 14);
+        for (; filled > 0; --filled) {
+          if (--st < 0) {
+            st = a.stages - 1;
+            parity ^= 1;
+          }
+          mbar_wait_bounded(&s.full_a[st], parity ^ 1, 1u << 14);
+        }
     }
   } else if (warp == 1) {
-    // ---- rows of the tokens, four a copy
-    int it = 0;
+    // ---- rows of the tokens, four a copy: a lane has the same place in every stage of a unit, or two of them
+    int st = 0, filled = 0;
+    unsigned parity = 1;
     bool ok = true;
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
@@ -436,11 +474,30 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
-      const MoUnit w = mo_unit(a, u, segs, tiles1);
-      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg], quads = (n + 3) / 4;
-      if (w.down) {  // until its gate/up units are done
+      const MoUnit w = mo_unit(p, u);
+      if (w.phase == 2) continue;
+      const bool down = w.phase == 1;
+      // columns: tokens; or, of h, rounded parts and rests in turn
+      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg] * (down ? 2 : 1), quads = (n + 3) / 4;
+      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const CUtensorMap *map = down ? &mh : &mx;
+      int r[2][4], at[2], col[2], block[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int b = (i * 32 + lane) / quads, g = i * 32 + lane - b * quads;
+        block[i] = b;
+        at[i] = (b * cols + g * 4) * 128;
+        col[i] = b * 64;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = min(g * 4 + j, n - 1);  // (past the last: its row again, to no use)
+          const int pick = s.picks[first + (down ? c >> 1 : c)];
+          r[i][j] = down ? pick * 2 + (c & 1) : pick / a.top_k;
+        }
+      }
+      if (down) {  // until its gate/up units are done
         if (lane == 0)
-          for (uint32_t i = 0; mo_acquire(seg_done + w.seg) < tiles1 * (a.rows1 / 32); ++i) {
+          for (uint32_t i = 0; mo_acquire(seg_done + w.seg) < p.tiles1 * (a.rows1 / 32); ++i) {
             if (i >= kSpinLimit || *abort_s) {
               ok = false;
               break;
@@ -452,24 +509,22 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         __syncwarp();
         asm volatile("fence.proxy.async;" ::: "memory");  // h was stored, and is read by copies
       }
-      const int blocks = w.down ? blocks2 : blocks1, kb = w.down ? a.kb2 : a.kb1;
-      for (int b0 = 0; b0 < blocks; b0 += kb, ++it) {
-        const int st = it % a.stages, nb = min(kb, blocks - b0);
-        if (!(ok = tc_wait_warp(&s.empty[st], ((it / a.stages) & 1) ^ 1, abort_s))) break;
+      for (int b0 = 0; b0 < blocks; b0 += kb) {
+        const int nb = min(kb, blocks - b0);
+        if (!(ok = tc_wait_warp(&s.empty[st], parity, abort_s))) break;
         if (lane == 0) mbar_expect_tx(&s.full_b[st], nb * quads * 512);
         __syncwarp();
-        for (int i = lane; i < nb * quads; i += 32) {
-          const int b = i / quads, g = i - b * quads;
-          int r[4];
+        const uint32_t dst = ring + st * a.stage_bytes + a.a_bytes;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int pick = s.picks[first + min(g * 4 + j, n - 1)];  // (past the last: its row again, to no use)
-            r[j] = w.down ? pick : pick / a.top_k;
-          }
-          mo_gather4(ring + st * a.stage_bytes + a.a_bytes + (b * a.cols + g * 4) * 128, w.down ? &mh : &mx, (b0 + b) * 64,
-                     r[0], r[1], r[2], r[3], &s.full_b[st]);
-        }
+        for (int i = 0; i < 2; ++i)
+          if (block[i] < nb)
+            mo_gather4(dst + at[i], map, b0 * 64 + col[i], r[i][0], r[i][1], r[i][2], r[i][3], &s.full_b[st]);
         __syncwarp();
+        filled = min(filled + 1, a.stages);
+        if (++st == a.stages) {
+          st = 0;
+          parity ^= 1;
+        }
       }
     }
     if (lane == 0) {
@@ -478,13 +533,19 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         *abort_s = 1;
       }
       if (*abort_s)
-        for (int i = max(0, it - a.stages); i < it; ++i)
-          mbar_wait_bounded(&s.full_b[i % a.stages], (i / a.stages) & 1, 1u << 14);
+        for (; filled > 0; --filled) {
+          if (--st < 0) {
+            st = a.stages - 1;
+            parity ^= 1;
+          }
+          mbar_wait_bounded(&s.full_b[st], parity ^ 1, 1u << 14);
+        }
     }
     __syncwarp();
   } else if (warp == 2) {
     // ---- MMA
-    int it = 0;
+    int st = 0, n_acc = 0;
+    unsigned parity = 0;
     bool ok = true;
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
@@ -493,29 +554,39 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
-      const MoUnit w = mo_unit(a, u, segs, tiles1);
-      const int n = (s.seg_n[w.seg] + 15) / 16 * 16, rows = w.down ? a.rows2 : a.rows1;
-      const int blocks = w.down ? blocks2 : blocks1, kb = w.down ? a.kb2 : a.kb1, buf = q & 1;
-      const uint32_t idesc = tc_uniform(mo_idesc<DT>(n)), acc = tc_uniform(tmem + buf * 128);
-      tc_wait_on(&s.acc_empty[buf], ((q >> 1) & 1) ^ 1, abort_s, a.err);
-      for (int b0 = 0; b0 < blocks; b0 += kb, ++it) {
-        const int st = it % a.stages, nb = min(kb, blocks - b0);
-        tc_wait_on(&s.full_b[st], (it / a.stages) & 1, abort_s, a.err);
-        tc_wait_on(&s.full_a[st], (it / a.stages) & 1, abort_s, a.err);
+      const MoUnit w = mo_unit(p, u);
+      if (w.phase == 2) continue;
+      const bool down = w.phase == 1;
+      const int n = (s.seg_n[w.seg] * (down ? 2 : 1) + 15) / 16 * 16, rows = down ? a.rows2 : a.rows1;
+      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const int buf = n_acc & 1;
+      const uint32_t idesc = tc_uniform(mo_idesc<DT>(n)), acc = tc_uniform(tmem + buf * 256);
+      const uint32_t a_step = tc_uniform(rows * 128 >> 4), b_step = tc_uniform(cols * 128 >> 4);
+      tc_wait_on(&s.acc_empty[buf], ((n_acc >> 1) & 1) ^ 1, abort_s, a.err);
+      ++n_acc;
+      for (int b0 = 0; b0 < blocks; b0 += kb) {
+        const int nb = min(kb, blocks - b0);
+        tc_wait_on(&s.full_b[st], parity, abort_s, a.err);
+        tc_wait_on(&s.full_a[st], parity, abort_s, a.err);
         tc_fence_after();
         const uint32_t wa = tc_uniform(tc_desc_k(ring + st * a.stage_bytes));
         const uint32_t xb = tc_uniform(tc_desc_k(ring + st * a.stage_bytes + a.a_bytes));
-        const uint32_t done = tc_uniform(smem_u32(&s.empty[st]));
+        const uint32_t done = tc_uniform(smem_u32(&s.empty[st])), go = tc_uniform(b0 > 0 ? 1u : 0u);
         if (tc_elect()) {
-          for (int b = 0; b < nb; ++b) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc_mma_ss(acc, tc_desc(wa + b * (rows * 128 >> 4) + k * 2), tc_desc(xb + b * (a.cols * 128 >> 4) + k * 2), idesc,
-                        b0 + b + k > 0);
-          }
+          for (int b = 0; b < 4; ++b)
+            if (b < nb) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc_mma_ss(acc, tc_desc(wa + b * a_step + k * 2), tc_desc(xb + b * b_step + k * 2), idesc, b + k > 0 ? 1u : go);
+            }
           tc_commit(done);
         }
         __syncwarp();
+        if (++st == a.stages) {
+          st = 0;
+          parity ^= 1;
+        }
       }
       const uint32_t full = tc_uniform(smem_u32(&s.acc_full[buf]));
       if (tc_elect()) tc_commit(full);
@@ -531,32 +602,68 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     mbar_wait_bounded(&s.drained, 0);
   } else if (warp >= 4) {
     // ---- epilogues: warp w has rows 32 (w - 4) .. of a unit
-    const int part = warp - 4, row0 = part * 32;
+    const int mine = warp - 4, row0 = mine * 32;
     const uint32_t lanes = tmem + ((uint32_t)row0 << 16);
+    int n_acc = 0;
     bool ok = true;
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
       if (!ok) break;
-      const int u = s.sched[q % kMoSched], buf = q & 1;
+      const int u = s.sched[q % kMoSched];
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
-      const MoUnit w = mo_unit(a, u, segs, tiles1);
-      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg], rows = w.down ? a.rows2 : a.rows1;
-      ok = tc_wait_warp(&s.acc_full[buf], (q >> 1) & 1, abort_s);
+      const MoUnit w = mo_unit(p, u);
+      if (w.phase == 2) {
+        // 128 columns of y, four a lane, a token at a time: when all segments' rows are there
+        const int col0 = w.seg * kMoSumCols, col = col0 + lane * 4;
+        if (lane < kMoSumCols / 32 && col0 + lane * 32 < a.hidden)
+          for (uint32_t i = 0; mo_acquire(strip_done + col0 / 32 + lane) < p.segs; ++i) {
+            if (i >= kSpinLimit || *abort_s) {
+              ok = false;
+              break;
+            }
+            __nanosleep(32);
+          }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        __syncwarp();
+        if (col >= a.hidden) continue;
+        for (int t = w.tile * a.sum_tokens + mine; t < min(a.tokens, (w.tile + 1) * a.sum_tokens); t += 4) {
+          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const float *rows = a.part + (int64_t)t * a.top_k * a.hidden + col;
+#pragma unroll 8
+          for (int k = 0; k < a.top_k; ++k) {
+            const float wk = __ldg(a.weights + t * a.top_k + k);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(rows + (int64_t)k * a.hidden));
+            sum.x = fmaf(wk, v.x, sum.x);
+            sum.y = fmaf(wk, v.y, sum.y);
+            sum.z = fmaf(wk, v.z, sum.z);
+            sum.w = fmaf(wk, v.w, sum.w);
+          }
+          const uint32_t lo = (uint32_t)bits_dt<DT>(sum.x) | ((uint32_t)bits_dt<DT>(sum.y) << 16);
+          const uint32_t hi = (uint32_t)bits_dt<DT>(sum.z) | ((uint32_t)bits_dt<DT>(sum.w) << 16);
+          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.y) + (int64_t)t * a.hidden + col) = make_uint2(lo, hi);
+        }
+        continue;
+      }
+      const bool down = w.phase == 1;
+      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg], rows = down ? a.rows2 : a.rows1, buf = n_acc & 1;
+      ok = tc_wait_warp(&s.acc_full[buf], (n_acc >> 1) & 1, abort_s);
+      ++n_acc;
       if (!ok) break;
       tc_fence_after();
       if (row0 < rows) {
-        for (int c0 = 0; c0 < n; c0 += 16) {
+        for (int c0 = 0; c0 < n * (down ? 2 : 1); c0 += 16) {
           float v[16];
-          tc_ld16(lanes + buf * 128 + c0, v);
+          tc_ld16(lanes + buf * 256 + c0, v);
           tc_wait_ld();
-          if (w.down) {
+          if (down) {
             const int row = w.tile * rows + row0 + lane;
             if (row < a.hidden) {
 #pragma unroll
-              for (int c = 0; c < 16; ++c)
-                if (c0 + c < n) a.part[(int64_t)s.picks[first + c0 + c] * a.hidden + row] = v[c];
+              for (int c = 0; c < 16; c += 2)
+                if (c0 + c < 2 * n) a.part[(int64_t)s.picks[first + (c0 + c) / 2] * a.hidden + row] = v[c] + v[c + 1];
             }
           } else {
             // lane l < 16 has gate row l, lane l + 16 up row l: the lower lanes take the even tokens, the upper the odd
@@ -567,48 +674,28 @@ __global__ void __launch_bounds__(kMoThreads, 1)
               const float got = __shfl_xor_sync(0xffffffffu, upper ? v[c] : v[c + 1], 16);
               const float gate = upper ? got : v[c], up = upper ? v[c + 1] : got;
               const int col = c0 + c + (upper ? 1 : 0);
-              if (col < n && row < a.inter)
-                store_elem<DT>(a.h, (int64_t)s.picks[first + col] * a.inter + row, gate / (1.0f + expf(-gate)) * up);
+              if (col < n && row < a.inter) {
+                const float h = gate / (1.0f + expf(-gate)) * up, most = mo_rounded<DT>(h);
+                const int64_t o = (int64_t)s.picks[first + col] * 2 * a.inter + row;
+                store_elem<DT>(a.h, o, most);
+                store_elem<DT>(a.h, o + a.inter, h - most);
+              }
             }
           }
         }
       }
       tc_fence_before();
-      if (!w.down) asm volatile("fence.proxy.async;" ::: "memory");  // h is read by copies
+      if (!down) asm volatile("fence.proxy.async;" ::: "memory");  // h is read by copies
       __threadfence();
       __syncwarp();
-      if (lane == 0) tc_arrive(&s.acc_empty[buf]);
-      if (row0 >= rows) continue;
-      if (!w.down) {
-        if (lane == 0) atomicAdd(seg_done + w.seg, 1);
-        continue;
-      }
-      const int strip = (w.tile * rows + row0) / 32;
-      int done = 0;
-      if (strip * 32 < a.hidden && lane == 0) done = atomicAdd(strip_done + strip, 1) + 1;
-      if (__shfl_sync(0xffffffffu, done, 0) != segs) continue;
-      __threadfence();
-      // the last segment's 32 rows: y, the choices of each token in their order, four rows a lane
-      const int row = strip * 32 + (lane & 7) * 4;
-      if (row < a.hidden) {
-#pragma unroll 2
-        for (int t = lane >> 3; t < a.tokens; t += 4) {
-          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-          for (int k = 0; k < a.top_k; ++k) {
-            const float wk = __ldg(a.weights + t * a.top_k + k);
-            const float4 p = __ldcg(reinterpret_cast<const float4 *>(a.part + (int64_t)(t * a.top_k + k) * a.hidden + row));
-            sum.x = fmaf(wk, p.x, sum.x);
-            sum.y = fmaf(wk, p.y, sum.y);
-            sum.z = fmaf(wk, p.z, sum.z);
-            sum.w = fmaf(wk, p.w, sum.w);
-          }
-          const uint32_t lo = (uint32_t)bits_dt<DT>(sum.x) | ((uint32_t)bits_dt<DT>(sum.y) << 16);
-          const uint32_t hi = (uint32_t)bits_dt<DT>(sum.z) | ((uint32_t)bits_dt<DT>(sum.w) << 16);
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.y) + t * a.y_stride + row) = make_uint2(lo, hi);
+      if (lane == 0) {
+        tc_arrive(&s.acc_empty[buf]);
+        const int strip = (w.tile * rows + row0) / 32;
+        if (row0 < rows) {
+          if (!down) atomicAdd(seg_done + w.seg, 1);
+          else if (strip * 32 < a.hidden) atomicAdd(strip_done + strip, 1);
         }
       }
-      __syncwarp();
     }
     if (!ok && lane == 0) {
       if (!*abort_s) atomicOr(a.err, 1u);
@@ -626,7 +713,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
 
 // How a call's experts are cut, from its sizes.
 struct MoeCut {
-  int rows1, rows2, kb1, kb2, cols, stages;
+  int rows1, rows2, kb1, kb2, cols, sum_tokens, stages;
   uint32_t stage_bytes, a_bytes;
 };
 
@@ -646,14 +733,23 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   c.cols = (int)cols;
   c.rows1 = moe_rows(segs, 2 * (int64_t)inter);
   c.rows2 = moe_rows(segs, hidden);
-  auto blocks = [&](int rows) { return rows + c.cols <= 48 ? 4 : rows + c.cols <= 96 ? 2 : 1; };
-  c.kb1 = blocks(c.rows1);
-  c.kb2 = blocks(c.rows2);
-  const int a1 = c.kb1 * c.rows1, a2 = c.kb2 * c.rows2, kb = c.kb1 > c.kb2 ? c.kb1 : c.kb2;
+  // a stage of 16 to 40 KB: a stage costs its issuing warps some hundred cycles, whatever it holds
+  auto blocks = [](int rows, int cols) {
+    int kb = 4;
+    while (kb > 1 && kb * (rows + cols) * 128 > 40 * 1024) kb /= 2;
+    return kb;
+  };
+  c.kb1 = blocks(c.rows1, c.cols);
+  c.kb2 = blocks(c.rows2, 2 * c.cols);
+  const int a1 = c.kb1 * c.rows1, a2 = c.kb2 * c.rows2, b1 = c.kb1 * c.cols, b2 = c.kb2 * 2 * c.cols;
   c.a_bytes = (uint32_t)(a1 > a2 ? a1 : a2) * 128;
-  c.stage_bytes = c.a_bytes + (uint32_t)kb * c.cols * 128;
+  c.stage_bytes = c.a_bytes + (uint32_t)(b1 > b2 ? b1 : b2) * 128;
   c.stages = (int)(kMoRing / c.stage_bytes);
   if (c.stages > kMoMaxStages) c.stages = kMoMaxStages;
+  // sum units for every SM where there are as many tokens
+  const int64_t strips = (hidden + kMoSumCols - 1) / kMoSumCols;
+  c.sum_tokens = 4;
+  while (c.sum_tokens < 16 && strips * ((tokens + c.sum_tokens - 1) / c.sum_tokens) > 2 * kMoSms) c.sum_tokens *= 2;
   return c;
 }
 
@@ -671,8 +767,10 @@ static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUt
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  const unsigned groups = (unsigned)((r.tokens + kMrTokens - 1) / kMrTokens);
-  const cudaError_t e = launch_dependent(moe_route_kernel<DT>, groups * kMrCluster, kMrThreads, 0, st, r);
+  int nt = 1;
+  while (nt < kMrMaxTokens && (r.tokens + nt - 1) / nt * kMrCluster > kMoSms) nt *= 2;
+  auto route = nt == 1 ? moe_route_kernel<DT, 1> : nt == 2 ? moe_route_kernel<DT, 2> : nt == 4 ? moe_route_kernel<DT, 4> : moe_route_kernel<DT, 8>;
+  const cudaError_t e = launch_dependent(route, (unsigned)((r.tokens + nt - 1) / nt * kMrCluster), kMrThreads, 0, st, r);
   if (e != cudaSuccess) return e;
   return launch_dependent(moe_experts_kernel<DT>, kMoSms, kMoThreads, kSmem, st, m[0], m[1], m[2], m[3], x);
 }
@@ -684,7 +782,7 @@ using namespace kvr;
 extern "C" size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int top_k) {
   if (n_tokens < 1 || n_tokens > kMoMaxTokens || hidden < 1 || inter < 1 || top_k < 1 || top_k > kMoMaxTopK) return 0;
   const size_t picks = (size_t)n_tokens * top_k;
-  return align_up(moe_counters(hidden) * 4, 256) + align_up(picks * inter * 2, 256) + picks * hidden * 4;
+  return align_up(moe_counters(hidden) * 4, 256) + align_up(picks * inter * 4, 256) + picks * hidden * 4;
 }
 
 extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hidden, int64_t x_stride, const void *router,
@@ -732,16 +830,16 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   r.counters = reinterpret_cast<int *>(ws); r.n_counters = (int)moe_counters(hidden);
   ExpertArgs a{};
   a.tokens = (int)n_tokens; a.hidden = hidden; a.inter = inter; a.experts = experts; a.top_k = top_k;
-  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.stages = c.stages;
+  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
   a.stage_bytes = c.stage_bytes; a.a_bytes = c.a_bytes;
   a.ids = ids; a.weights = weights;
   a.h = ws + align_up(moe_counters(hidden) * 4, 256);
-  a.part = reinterpret_cast<float *>(static_cast<char *>(a.h) + align_up((size_t)picks * inter * 2, 256));
-  a.y = y; a.y_stride = hidden;
+  a.part = reinterpret_cast<float *>(static_cast<char *>(a.h) + align_up((size_t)picks * inter * 4, 256));
+  a.y = y;
   a.counters = r.counters; a.err = static_cast<unsigned *>(status);
   CUtensorMap m[4];
   const cuuint64_t xd[2] = {(cuuint64_t)hidden, (cuuint64_t)n_tokens}, xs[1] = {(cuuint64_t)(n_tokens > 1 ? x_stride : hidden) * 2};
-  const cuuint64_t hd[2] = {(cuuint64_t)inter, (cuuint64_t)picks}, hs[1] = {(cuuint64_t)inter * 2};
+  const cuuint64_t hd[2] = {(cuuint64_t)inter, (cuuint64_t)picks * 2}, hs[1] = {(cuuint64_t)inter * 2};
   const cuuint64_t gd[4] = {(cuuint64_t)hidden, (cuuint64_t)inter, 2, (cuuint64_t)experts};
   const cuuint64_t gs[3] = {(cuuint64_t)gu_row_stride * 2, (cuuint64_t)gu_row_stride * inter * 2, (cuuint64_t)gu_expert_stride * 2};
   const cuuint64_t dd[3] = {(cuuint64_t)inter, (cuuint64_t)hidden, (cuuint64_t)experts};
