@@ -218,38 +218,47 @@ struct MoShared {
   int warp_sums[2][kMoThreads / 32];
   int seg_expert[kMoMaxSegs];
   short seg_first[kMoMaxSegs], seg_n[kMoMaxSegs];
-  unsigned mask[kMoMaxExperts][kMoMaxTokens / 32];  // tokens of each expert
   short first[kMoMaxExperts];
   short picks[kMoMaxPicks];  // token * top_k + choice, by expert
 };
 
-__device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint64_t *bar) {
+__device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
       "[%6];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void mo_tma3(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint64_t *bar) {
+__device__ __forceinline__ void mo_tma3(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
       "[%5];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
 // 64 columns of four rows.
 __device__ __forceinline__ void mo_gather4(uint32_t dst, const CUtensorMap *m, int c0, int r0, int r1, int r2, int r3,
-                                           uint64_t *bar) {
+                                           uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
       "%4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+      "l"(m), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ int mo_acquire(const int *p) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+// After an abort: waits (not for long) for the copies of the last `filled` stages before stage `st`.
+__device__ __forceinline__ void mo_drain(uint64_t *full, int st, unsigned parity, int filled, int stages) {
+  for (; filled > 0; --filled) {
+    if (--st < 0) {
+      st = stages - 1;
+      parity ^= 1;
+    }
+    mbar_wait_bounded(&full[st], parity ^ 1, 1u << 14);
+  }
 }
 template <int DT>
 __host__ __device__ constexpr uint32_t mo_idesc(uint32_t n) {  // kind::f16, fp32 accumulator, M 128
@@ -322,7 +331,9 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     }
     tc_bar_init(&s.drained, 1);
   }
-  for (int i = tid; i < kMoMaxExperts * (kMoMaxTokens / 32); i += kMoThreads) (&s.mask[0][0])[i] = 0;
+  // tokens of each expert, a bit each; where the stages will be
+  unsigned (*mask)[kMoMaxTokens / 32] = reinterpret_cast<unsigned (*)[kMoMaxTokens / 32]>(sm);
+  for (int i = tid; i < kMoMaxExperts * (kMoMaxTokens / 32); i += kMoThreads) (&mask[0][0])[i] = 0;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // barriers: for the copies and commits
   tc_fence_before();
   __syncthreads();
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   const int picks = a.tokens * a.top_k;
   for (int i = tid; i < picks; i += kMoThreads) {
     const int t = i / a.top_k;
-    atomicOr(&s.mask[a.ids[i]][t >> 5], 1u << (t & 31));
+    atomicOr(&mask[a.ids[i]][t >> 5], 1u << (t & 31));
   }
   __syncthreads();
   {
@@ -346,7 +357,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       const int e = tid * kEach + j;
       n[j] = 0;
 #pragma unroll
-      for (int w = 0; w < kMoMaxTokens / 32; ++w) n[j] += __popc(s.mask[e][w]);
+      for (int w = 0; w < kMoMaxTokens / 32; ++w) n[j] += __popc(mask[e][w]);
       sum_n += n[j];
       sum_s += (n[j] + a.cols - 1) / a.cols;
     }
@@ -388,10 +399,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   for (int i = tid; i < picks; i += kMoThreads) {
     const int t = i / a.top_k, e = a.ids[i];
     int before = 0;
-    for (int w = 0; w < (t >> 5); ++w) before += __popc(s.mask[e][w]);
-    before += __popc(s.mask[e][t >> 5] & ((1u << (t & 31)) - 1));
+    for (int w = 0; w < (t >> 5); ++w) before += __popc(mask[e][w]);
+    before += __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1));
     s.picks[s.first[e] + before] = (short)i;
   }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies will write where the bits were
   __syncthreads();
   MoPlan p;
   p.segs = s.n_segs;
@@ -406,71 +418,74 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   const uint32_t ring = smem_u32(sm);
 
   if (warp == 0) {
-    // ---- tickets and weights: one lane.  Stage and phase are counted up: with it % stages and it / stages a stage
-    // took 1000 cycles to issue, more than its bytes take to arrive.
-    if (lane == 0) {
-      int st = 0, filled = 0;
-      unsigned parity = 1;
-      int next = atomicAdd(ticket, 1);
-      bool ok = true;
-      for (int q = 0; ok; ++q) {
-        const int u = next;
-        if (u < p.units) next = atomicAdd(ticket, 1);  // asked for ahead: its answer is due a unit later
-        ok = tc_wait(&s.sched_empty[q % kMoSched], ((q / kMoSched) & 1) ^ 1, abort_s);
-        if (!ok) break;
+    // ---- tickets and weights.  The whole warp walks, one lane issues: a copy's operands lie in uniform registers, and
+    // only of values that come from a shuffle or from the launch does the compiler know that they may (copies issued by
+    // lane 0 alone, with its own ticket's numbers: 320 cycles each, not 60).  Stage and phase are counted up: divisions
+    // made a stage cost more than its bytes take to arrive.
+    int st = 0, filled = 0;
+    unsigned parity = 1;
+    int next = 0;
+    if (lane == 0) next = atomicAdd(ticket, 1);
+    bool ok = true;
+    for (int q = 0; ok; ++q) {
+      const int u = (int)tc_uniform(next);
+      if (lane == 0 && u < p.units) next = atomicAdd(ticket, 1);  // asked for ahead: its answer is due a unit later
+      ok = tc_wait_warp(&s.sched_empty[q % kMoSched], ((q / kMoSched) & 1) ^ 1, abort_s);
+      if (!ok) break;
+      if (lane == 0) {
         s.sched[q % kMoSched] = u < p.units ? u : -1;
         tc_arrive(&s.sched_full[q % kMoSched]);
-        if (u >= p.units) break;
-        const MoUnit w = mo_unit(p, u);
-        if (w.phase == 2) continue;
-        const bool down = w.phase == 1;
-        const int e = s.seg_expert[w.seg];
-        const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, rows = down ? a.rows2 : a.rows1;
-        const int row = down ? w.tile * rows : w.tile * rows / 2;
-        for (int b0 = 0; b0 < blocks; b0 += kb) {
-          const int nb = min(kb, blocks - b0);
-          if (!(ok = tc_wait(&s.empty[st], parity, abort_s))) break;
+      }
+      __syncwarp();
+      if (u >= p.units) break;
+      const MoUnit w = mo_unit(p, u);
+      if (w.phase == 2) continue;
+      const bool down = w.phase == 1;
+      const int e = (int)tc_uniform(s.seg_expert[w.seg]);
+      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, rows = down ? a.rows2 : a.rows1;
+      const int row = down ? w.tile * rows : w.tile * rows / 2;
+      for (int b0 = 0; b0 < blocks; b0 += kb) {
+        const int nb = min(kb, blocks - b0);
+        if (!(ok = tc_wait_warp(&s.empty[st], parity, abort_s))) break;
+        uint32_t dst = tc_uniform(ring + st * a.stage_bytes);
+        const uint32_t full = tc_uniform(smem_u32(&s.full_a[st]));
+        if (tc_elect()) {
           mbar_expect_tx(&s.full_a[st], nb * rows * 128);
-          uint32_t dst = ring + st * a.stage_bytes;
           for (int c = b0 * 64; c < (b0 + nb) * 64; c += 64) {
             if (down) {
-              mo_tma3(dst, &mw2, c, row, e, &s.full_a[st]);
+              mo_tma3(dst, &mw2, c, row, e, full);
               dst += rows * 128;
             } else {
               for (int r = 0; r < rows; r += 32, dst += 32 * 128)  // 16 rows of gate, the same 16 of up
-                mo_tma4(dst, &mw1, c, row + r / 2, 0, e, &s.full_a[st]);
+                mo_tma4(dst, &mw1, c, row + r / 2, 0, e, full);
             }
           }
-          filled = min(filled + 1, a.stages);
-          if (++st == a.stages) {
-            st = 0;
-            parity ^= 1;
-          }
+        }
+        __syncwarp();
+        filled = min(filled + 1, a.stages);
+        if (++st == a.stages) {
+          st = 0;
+          parity ^= 1;
         }
       }
-      if (!ok) {
-        if (!*abort_s) atomicOr(a.err, 1u);
-        *abort_s = 1;
-      }
-      // nothing may be in flight to this CTA's memory when it ends; after an abort the last stages were not seen full
-      if (*abort_s)
-        for (; filled > 0; --filled) {
-          if (--st < 0) {
-            st = a.stages - 1;
-            parity ^= 1;
-          }
-          mbar_wait_bounded(&s.full_a[st], parity ^ 1, 1u << 14);
-        }
     }
+    if (!ok && lane == 0) {
+      if (!*abort_s) atomicOr(a.err, 1u);
+      *abort_s = 1;
+    }
+    __syncwarp();
+    // nothing may be in flight to this CTA's memory when it ends; after an abort the last stages were not seen full
+    if (*abort_s) mo_drain(s.full_a, st, parity, filled, a.stages);
   } else if (warp == 1) {
     // ---- rows of the tokens, four a copy: a lane has the same place in every stage of a unit, or two of them
+    // (all copies from one lane, with rows shuffled to it: a third slower)
     int st = 0, filled = 0;
     unsigned parity = 1;
     bool ok = true;
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
       if (!ok) break;
-      const int u = s.sched[q % kMoSched];
+      const int u = (int)tc_uniform(s.sched[q % kMoSched]);
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
@@ -478,16 +493,15 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (w.phase == 2) continue;
       const bool down = w.phase == 1;
       // columns: tokens; or, of h, rounded parts and rests in turn
-      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg] * (down ? 2 : 1), quads = (n + 3) / 4;
+      const int first = s.seg_first[w.seg], n = (int)tc_uniform(s.seg_n[w.seg] * (down ? 2 : 1)), quads = (n + 3) / 4;
       const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
       const CUtensorMap *map = down ? &mh : &mx;
-      int r[2][4], at[2], col[2], block[2];
+      int r[2][4], at[2], block[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int b = (i * 32 + lane) / quads, g = i * 32 + lane - b * quads;
-        block[i] = b;
-        at[i] = (b * cols + g * 4) * 128;
-        col[i] = b * 64;
+        block[i] = (i * 32 + lane) / quads;
+        const int g = i * 32 + lane - block[i] * quads;
+        at[i] = (block[i] * cols + g * 4) * 128;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = min(g * 4 + j, n - 1);  // (past the last: its row again, to no use)
@@ -514,11 +528,10 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         if (!(ok = tc_wait_warp(&s.empty[st], parity, abort_s))) break;
         if (lane == 0) mbar_expect_tx(&s.full_b[st], nb * quads * 512);
         __syncwarp();
-        const uint32_t dst = ring + st * a.stage_bytes + a.a_bytes;
+        const uint32_t dst = ring + st * a.stage_bytes + a.a_bytes, full = smem_u32(&s.full_b[st]);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (block[i] < nb)
-            mo_gather4(dst + at[i], map, b0 * 64 + col[i], r[i][0], r[i][1], r[i][2], r[i][3], &s.full_b[st]);
+          if (block[i] < nb) mo_gather4(dst + at[i], map, (b0 + block[i]) * 64, r[i][0], r[i][1], r[i][2], r[i][3], full);
         __syncwarp();
         filled = min(filled + 1, a.stages);
         if (++st == a.stages) {
@@ -527,21 +540,12 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         }
       }
     }
-    if (lane == 0) {
-      if (!ok) {
-        if (!*abort_s) atomicOr(a.err, 1u);
-        *abort_s = 1;
-      }
-      if (*abort_s)
-        for (; filled > 0; --filled) {
-          if (--st < 0) {
-            st = a.stages - 1;
-            parity ^= 1;
-          }
-          mbar_wait_bounded(&s.full_b[st], parity ^ 1, 1u << 14);
-        }
+    if (!ok && lane == 0) {
+      if (!*abort_s) atomicOr(a.err, 1u);
+      *abort_s = 1;
     }
     __syncwarp();
+    if (*abort_s) mo_drain(s.full_b, st, parity, filled, a.stages);
   } else if (warp == 2) {
     // ---- MMA
     int st = 0, n_acc = 0;
@@ -550,7 +554,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
       if (!ok) break;
-      const int u = s.sched[q % kMoSched];
+      const int u = (int)tc_uniform(s.sched[q % kMoSched]);
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
