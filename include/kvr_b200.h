@@ -566,7 +566,7 @@ KVR_API int kvr_beam_select(const void *logits, int dtype, int64_t row_stride, i
  * (256-byte aligned) needs no clearing and keeps nothing between calls; status, a
  * word that the caller has zeroed once (16-byte aligned), is set where a bounded wait
  * gave up (y then means nothing): kvr_workspace_status reads and clears it. */
-KVR_API size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int top_k);
+KVR_API size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int experts, int top_k);
 KVR_API int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hidden, int64_t x_stride, const void *router,
                           int64_t router_stride, const void *gate_up, int64_t gu_expert_stride, int64_t gu_row_stride,
                           const void *down, int64_t down_expert_stride, int64_t down_row_stride, int experts, int inter,

@@ -21,8 +21,9 @@
 // Work units, taken in order from one ticket counter:
 //   gate/up  R1 rows (16 of gate, 16 of up, ...) of a segment's expert over x: h, in two
 //            16-bit parts
-//   down     R2 rows of Wd over both parts of h: partial rows (token, choice) in 32 bits
-//   sum      128 columns of y of some tokens: the choices of each token in their order
+//   down     R2 rows of Wd over a share of both parts of h: partial rows (token, choice,
+//            share) in 32 bits
+//   sum      128 columns of y of some tokens: choices and shares of each token in order
 // A unit waits only for units with lower tickets, which run already: no CTA has to
 // be resident for another to end.  Weights of a down unit stream in while its h is
 // still being formed, so the memory does not idle between the phases.
@@ -49,7 +50,7 @@ constexpr int kMoSms = 148;
 
 // ------------------------------------------------------------------ router ----
 
-constexpr int kMrThreads = 256, kMrCluster = 8, kMrMaxTokens = 8;
+constexpr int kMrThreads = 256, kMrCluster = 8, kMrMaxTokens = 8, kMrExperts = 4;
 
 struct RouteArgs {
   const void *x, *router;
@@ -80,12 +81,28 @@ __device__ __forceinline__ uint64_t mo_key(double z) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
+template <int DT>
+__device__ __forceinline__ void mo_widen(const uint4 &u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == KVR_BF16) {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    }
+  }
+}
+
 // NT tokens a cluster: as few as the SMs have clusters for, since a CTA's time is its tokens' products.
 template <int DT, int NT>
-__global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads) moe_route_kernel(RouteArgs a) {
+__global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads, 1) moe_route_kernel(RouteArgs a) {
   constexpr int kWarps = kMrThreads / 32, kEach = kMoMaxExperts / 32;
   __shared__ double part[NT][kMoMaxExperts / kMrCluster];  // logits of this CTA's experts
-  __shared__ double slice[kWarps][NT];                     // of a warp's channels
+  __shared__ double slice[kWarps][NT][kMrExperts];         // of a warp's channels
   __shared__ double all_s[kMoMaxExperts];                  // of this CTA's token
   __shared__ int chosen[kMoMaxTopK];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -96,41 +113,57 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads)
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.n_counters; i += kMrThreads) a.counters[i] = 0;
   const int per = (a.experts + kMrCluster - 1) / kMrCluster, e0 = rank * per, n_exp = max(0, min(a.experts - e0, per));
-  // a warp takes an expert, or with few experts a part of its channels
-  const int parts = n_exp > 0 && n_exp < kWarps ? kWarps / n_exp : 1, mine = warp / parts, step = kWarps / parts;
-  for (int e = mine; e < n_exp && mine < step; e += step) {
-    float s[NT] = {};
-    const int c0 = (warp - mine * parts) * 256 + lane * 8, dc = parts * 256;
-    const void *w_row = static_cast<const uint16_t *>(a.router) + (e0 + e) * a.router_stride;
-    const void *x_row = static_cast<const uint16_t *>(a.x) + t0 * a.x_stride;
-#pragma unroll(NT == 1 ? 8 : NT == 2 ? 4 : 2)
+  // A warp takes four experts over a part of the channels: what it loads of x serves four, of the router NT.
+  const int groups = (n_exp + kMrExperts - 1) / kMrExperts, parts = groups > 0 && groups < kWarps ? kWarps / groups : 1;
+  for (int g = warp / parts; g < groups; g += kWarps / parts) {
+    float s[NT][kMrExperts] = {};
+    const int c0 = warp % parts * 256 + lane * 8, dc = parts * 256;
+    const uint16_t *w_row = static_cast<const uint16_t *>(a.router) + (e0 + g * kMrExperts) * a.router_stride;
+    const uint16_t *x_row = static_cast<const uint16_t *>(a.x) + t0 * a.x_stride;
+    int64_t w_off[kMrExperts], x_off[NT];  // (experts and tokens past the last: the last again, to no use)
+#pragma unroll
+    for (int e = 0; e < kMrExperts; ++e) w_off[e] = min(e, n_exp - 1 - g * kMrExperts) * a.router_stride;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x_off[t] = min(t, n_tok - 1) * a.x_stride;
+#pragma unroll(NT == 1 ? 4 : NT == 8 ? 1 : 2)
     for (int c = c0; c < a.hidden; c += dc) {
-      float w[8], x[NT][8];
-      load8<DT>(w_row, c, w);
+      uint4 w[kMrExperts], x[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) load8<DT>(x_row, min(t, n_tok - 1) * a.x_stride + c, x[t]);
+      for (int e = 0; e < kMrExperts; ++e) w[e] = __ldg(reinterpret_cast<const uint4 *>(w_row + w_off[e] + c));
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) x[t] = __ldg(reinterpret_cast<const uint4 *>(x_row + x_off[t] + c));
+      float wf[kMrExperts][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[t] = fmaf(x[t][j], w[j], s[t]);
-    }
+      for (int e = 0; e < kMrExperts; ++e) mo_widen<DT>(w[e], wf[e]);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      double d = s[t];
+      for (int t = 0; t < NT; ++t) {
+        float xf[8];
+        mo_widen<DT>(x[t], xf);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (lane == 0) {
-        if (parts == 1) part[t][e] = d;
-        else slice[warp][t] = d;
+        for (int e = 0; e < kMrExperts; ++e)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[t][e] = fmaf(xf[j], wf[e][j], s[t][e]);
       }
     }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < kMrExperts; ++e) {
+        double d = s[t][e];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (lane == 0) {
+          if (parts > 1) slice[warp][t][e] = d;
+          else if (g * kMrExperts + e < n_exp) part[t][g * kMrExperts + e] = d;
+        }
+      }
   }
   if (parts > 1) {  // in the order of the channels
     __syncthreads();
     for (int i = threadIdx.x; i < NT * n_exp; i += kMrThreads) {
       const int t = i / n_exp, e = i - t * n_exp;
       double d = 0.0;
-      for (int p = 0; p < parts; ++p) d += slice[e * parts + p][t];
+      for (int q = 0; q < parts; ++q) d += slice[e / kMrExperts * parts + q][t][e % kMrExperts];
       part[t][e] = d;
     }
   }
@@ -196,13 +229,14 @@ struct ExpertArgs {
   int rows1, rows2;      // rows of a gate/up and of a down unit
   int kb1, kb2;          // 64-column blocks of a stage
   int cols;              // most tokens of a segment, a multiple of 16
+  int shares;            // of an expert's inner channels in down units
   int sum_tokens;        // tokens of a sum unit
   int stages;
   uint32_t stage_bytes, a_bytes;  // of a stage; its weights' part
   const int *ids;
   const float *weights;
   void *h;               // (tokens * top_k, 2, inter): rounded, rest
-  float *part;           // (tokens * top_k, hidden)
+  float *part;           // (tokens * top_k, shares, hidden)
   void *y;
   int *counters;         // ticket; warps' parts of segments' gate/up units done; segments done of 32-row strips of y
   unsigned *err;
@@ -266,25 +300,33 @@ __host__ __device__ constexpr uint32_t mo_idesc(uint32_t n) {  // kind::f16, fp3
          ((128u >> 4) << 24);
 }
 
-// Work unit u: phase (0: gate/up, 1: down, 2: sum), segment (2: columns of y), tile of rows (2: tokens).
+// Work unit u: phase (0: gate/up, 1: down, 2: sum), segment (2: columns of y), tile of rows (2: tokens), and the
+// 64-column blocks [b0, b1) of the weights.
 struct MoUnit {
-  int phase, seg, tile;
+  int phase, seg, tile, share, b0, b1;
 };
 struct MoPlan {
   int segs, tiles1, tiles2, sums;  // sums: units of a column block
   int first2, first3, units;       // first down unit, first sum unit, all
+  int blocks1, blocks2, shares;
 };
 __device__ __forceinline__ MoUnit mo_unit(const MoPlan &p, int u) {
   MoUnit w;
+  w.share = w.b0 = w.b1 = 0;
   if (u < p.first2) {
     w.phase = 0;
     w.seg = u / p.tiles1;
     w.tile = u - w.seg * p.tiles1;
-  } else if (u < p.first3) {  // tile by tile, so that no segment's h is waited for while others' is there
+    w.b1 = p.blocks1;
+  } else if (u < p.first3) {
     u -= p.first2;
     w.phase = 1;
-    w.tile = u / p.segs;
-    w.seg = u - w.tile * p.segs;
+    const int t = u / p.shares;
+    w.share = u - t * p.shares;
+    w.seg = t / p.tiles2;
+    w.tile = t - w.seg * p.tiles2;
+    w.b0 = p.blocks2 * w.share / p.shares;
+    w.b1 = p.blocks2 * (w.share + 1) / p.shares;
   } else {
     u -= p.first3;
     w.phase = 2;
@@ -343,11 +385,17 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   griddep_launch();
 
   // picks by expert, and segments.  Every CTA makes the same lists: a bit per (expert, token), counts and prefix sums.
+  constexpr int kIds = kMoMaxPicks / kMoThreads;
   const int picks = a.tokens * a.top_k;
-  for (int i = tid; i < picks; i += kMoThreads) {
-    const int t = i / a.top_k;
-    atomicOr(&mask[a.ids[i]][t >> 5], 1u << (t & 31));
-  }
+  int id[kIds];
+#pragma unroll
+  for (int j = 0; j < kIds; ++j) id[j] = tid + j * kMoThreads < picks ? a.ids[tid + j * kMoThreads] : -1;
+#pragma unroll
+  for (int j = 0; j < kIds; ++j)
+    if (id[j] >= 0) {
+      const int t = (tid + j * kMoThreads) / a.top_k;
+      atomicOr(&mask[id[j]][t >> 5], 1u << (t & 31));
+    }
   __syncthreads();
   {
     constexpr int kEach = kMoMaxExperts / kMoThreads;
@@ -396,13 +444,14 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     if (tid == kMoThreads - 1) s.n_segs = at_s;
   }
   __syncthreads();
-  for (int i = tid; i < picks; i += kMoThreads) {
-    const int t = i / a.top_k, e = a.ids[i];
-    int before = 0;
-    for (int w = 0; w < (t >> 5); ++w) before += __popc(mask[e][w]);
-    before += __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1));
-    s.picks[s.first[e] + before] = (short)i;
-  }
+#pragma unroll
+  for (int j = 0; j < kIds; ++j)
+    if (id[j] >= 0) {
+      const int i = tid + j * kMoThreads, t = i / a.top_k, e = id[j];
+      int before = __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1));
+      for (int w = 0; w < (t >> 5); ++w) before += __popc(mask[e][w]);
+      s.picks[s.first[e] + before] = (short)i;
+    }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies will write where the bits were
   __syncthreads();
   MoPlan p;
@@ -411,10 +460,12 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   p.tiles2 = (a.hidden + a.rows2 - 1) / a.rows2;
   p.sums = (a.tokens + a.sum_tokens - 1) / a.sum_tokens;
   p.first2 = p.segs * p.tiles1;
-  p.first3 = p.first2 + p.segs * p.tiles2;
+  p.blocks1 = (a.hidden + 63) / 64;
+  p.blocks2 = (a.inter + 63) / 64;
+  p.shares = a.shares;
+  p.first3 = p.first2 + p.segs * p.tiles2 * a.shares;
   p.units = p.first3 + (a.hidden + kMoSumCols - 1) / kMoSumCols * p.sums;
   int *ticket = a.counters, *seg_done = a.counters + 1, *strip_done = seg_done + kMoMaxSegs;
-  const int blocks1 = (a.hidden + 63) / 64, blocks2 = (a.inter + 63) / 64;
   const uint32_t ring = smem_u32(sm);
 
   if (warp == 0) {
@@ -442,11 +493,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (w.phase == 2) continue;
       const bool down = w.phase == 1;
       const int e = (int)tc_uniform(s.seg_expert[w.seg]);
-      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, rows = down ? a.rows2 : a.rows1;
+      const int kb = down ? a.kb2 : a.kb1, rows = down ? a.rows2 : a.rows1;
       const int row = down ? w.tile * rows : w.tile * rows / 2;
-      for (int b0 = 0; b0 < blocks; b0 += kb) {
-        const int nb = min(kb, blocks - b0);
-        if (!(ok = tc_wait_warp(&s.empty[st], parity, abort_s))) break;
+      for (int b0 = w.b0; b0 < w.b1; b0 += kb) {
+        const int nb = min(kb, w.b1 - b0);
+        tc_wait_on(&s.empty[st], parity, abort_s, a.err);
         uint32_t dst = tc_uniform(ring + st * a.stage_bytes);
         const uint32_t full = tc_uniform(smem_u32(&s.full_a[st]));
         if (tc_elect()) {
@@ -468,6 +519,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           parity ^= 1;
         }
       }
+      ok = __all_sync(0xffffffffu, !*abort_s);
     }
     if (!ok && lane == 0) {
       if (!*abort_s) atomicOr(a.err, 1u);
@@ -494,7 +546,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       const bool down = w.phase == 1;
       // columns: tokens; or, of h, rounded parts and rests in turn
       const int first = s.seg_first[w.seg], n = (int)tc_uniform(s.seg_n[w.seg] * (down ? 2 : 1)), quads = (n + 3) / 4;
-      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const int kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
       const CUtensorMap *map = down ? &mh : &mx;
       int r[2][4], at[2], block[2];
 #pragma unroll
@@ -523,9 +575,9 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         __syncwarp();
         asm volatile("fence.proxy.async;" ::: "memory");  // h was stored, and is read by copies
       }
-      for (int b0 = 0; b0 < blocks; b0 += kb) {
-        const int nb = min(kb, blocks - b0);
-        if (!(ok = tc_wait_warp(&s.empty[st], parity, abort_s))) break;
+      for (int b0 = w.b0; b0 < w.b1; b0 += kb) {
+        const int nb = min(kb, w.b1 - b0);
+        tc_wait_on(&s.empty[st], parity, abort_s, a.err);
         if (lane == 0) mbar_expect_tx(&s.full_b[st], nb * quads * 512);
         __syncwarp();
         const uint32_t dst = ring + st * a.stage_bytes + a.a_bytes, full = smem_u32(&s.full_b[st]);
@@ -539,6 +591,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           parity ^= 1;
         }
       }
+      ok = __all_sync(0xffffffffu, !*abort_s);
     }
     if (!ok && lane == 0) {
       if (!*abort_s) atomicOr(a.err, 1u);
@@ -562,20 +615,20 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (w.phase == 2) continue;
       const bool down = w.phase == 1;
       const int n = (s.seg_n[w.seg] * (down ? 2 : 1) + 15) / 16 * 16, rows = down ? a.rows2 : a.rows1;
-      const int blocks = down ? blocks2 : blocks1, kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const int kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
       const int buf = n_acc & 1;
       const uint32_t idesc = tc_uniform(mo_idesc<DT>(n)), acc = tc_uniform(tmem + buf * 256);
       const uint32_t a_step = tc_uniform(rows * 128 >> 4), b_step = tc_uniform(cols * 128 >> 4);
       tc_wait_on(&s.acc_empty[buf], ((n_acc >> 1) & 1) ^ 1, abort_s, a.err);
       ++n_acc;
-      for (int b0 = 0; b0 < blocks; b0 += kb) {
-        const int nb = min(kb, blocks - b0);
+      for (int b0 = w.b0; b0 < w.b1; b0 += kb) {
+        const int nb = min(kb, w.b1 - b0);
         tc_wait_on(&s.full_b[st], parity, abort_s, a.err);
         tc_wait_on(&s.full_a[st], parity, abort_s, a.err);
         tc_fence_after();
         const uint32_t wa = tc_uniform(tc_desc_k(ring + st * a.stage_bytes));
         const uint32_t xb = tc_uniform(tc_desc_k(ring + st * a.stage_bytes + a.a_bytes));
-        const uint32_t done = tc_uniform(smem_u32(&s.empty[st])), go = tc_uniform(b0 > 0 ? 1u : 0u);
+        const uint32_t done = tc_uniform(smem_u32(&s.empty[st])), go = tc_uniform(b0 > w.b0 ? 1u : 0u);
         if (tc_elect()) {
 #pragma unroll
           for (int b = 0; b < 4; ++b)
@@ -622,7 +675,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         // 128 columns of y, four a lane, a token at a time: when all segments' rows are there
         const int col0 = w.seg * kMoSumCols, col = col0 + lane * 4;
         if (lane < kMoSumCols / 32 && col0 + lane * 32 < a.hidden)
-          for (uint32_t i = 0; mo_acquire(strip_done + col0 / 32 + lane) < p.segs; ++i) {
+          for (uint32_t i = 0; mo_acquire(strip_done + col0 / 32 + lane) < p.segs * p.shares; ++i) {
             if (i >= kSpinLimit || *abort_s) {
               ok = false;
               break;
@@ -635,10 +688,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         if (col >= a.hidden) continue;
         for (int t = w.tile * a.sum_tokens + mine; t < min(a.tokens, (w.tile + 1) * a.sum_tokens); t += 4) {
           float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          const float *rows = a.part + (int64_t)t * a.top_k * a.hidden + col;
+          const int parts = a.top_k * a.shares;
+          const float *rows = a.part + (int64_t)t * parts * a.hidden + col;
 #pragma unroll 8
-          for (int k = 0; k < a.top_k; ++k) {
-            const float wk = __ldg(a.weights + t * a.top_k + k);
+          for (int k = 0; k < parts; ++k) {
+            const float wk = __ldg(a.weights + t * a.top_k + k / a.shares);
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(rows + (int64_t)k * a.hidden));
             sum.x = fmaf(wk, v.x, sum.x);
             sum.y = fmaf(wk, v.y, sum.y);
@@ -667,7 +721,8 @@ __global__ void __launch_bounds__(kMoThreads, 1)
             if (row < a.hidden) {
 #pragma unroll
               for (int c = 0; c < 16; c += 2)
-                if (c0 + c < 2 * n) a.part[(int64_t)s.picks[first + (c0 + c) / 2] * a.hidden + row] = v[c] + v[c + 1];
+                if (c0 + c < 2 * n)
+                  a.part[((int64_t)s.picks[first + (c0 + c) / 2] * a.shares + w.share) * a.hidden + row] = v[c] + v[c + 1];
             }
           } else {
             // lane l < 16 has gate row l, lane l + 16 up row l: the lower lanes take the even tokens, the upper the odd
@@ -717,15 +772,23 @@ __global__ void __launch_bounds__(kMoThreads, 1)
 
 // How a call's experts are cut, from its sizes.
 struct MoeCut {
-  int rows1, rows2, kb1, kb2, cols, sum_tokens, stages;
+  int rows1, rows2, kb1, kb2, cols, shares, sum_tokens, stages;
   uint32_t stage_bytes, a_bytes;
 };
 
-// Rows of a unit: as many as leave every SM several units, so that none waits long for the last.
+// Rows of a gate/up unit: the least time of the fullest SM, by whole units.  A unit's time is that of its bytes, but not
+// below that of 64 rows: issuing a stage of 32 takes as long.
 static int moe_rows(int64_t segs, int64_t rows) {
-  for (int r = 128; r > 32; r /= 2)
-    if (segs * ((rows + r - 1) / r) >= kMoSms * 6) return r;
-  return 32;
+  int best = 32;
+  int64_t least = INT64_MAX;
+  for (int r = 32; r <= 128; r += 32) {
+    const int64_t units = segs * ((rows + r - 1) / r), t = (units + kMoSms - 1) / kMoSms * ((r < 64 ? 64 : r) + 4);
+    if (t < least) {
+      least = t;
+      best = r;
+    }
+  }
+  return best;
 }
 
 static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int top_k) {
@@ -736,7 +799,12 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   if (cols > (tokens + 15) / 16 * 16) cols = (tokens + 15) / 16 * 16;
   c.cols = (int)cols;
   c.rows1 = moe_rows(segs, 2 * (int64_t)inter);
-  c.rows2 = moe_rows(segs, hidden);
+  // down units are of 128 rows, and a share of the inner channels (256 at least) so that every SM has some units: partial
+  // rows are summed in any case
+  c.rows2 = hidden > 96 ? 128 : (hidden + 31) / 32 * 32;
+  const int64_t tiles2 = segs * ((hidden + c.rows2 - 1) / c.rows2);
+  c.shares = 1;
+  while (c.shares < 8 && tiles2 * c.shares < 4 * kMoSms && inter / (c.shares + 1) >= 256) ++c.shares;
   // a stage of 16 to 40 KB: a stage costs its issuing warps some hundred cycles, whatever it holds
   auto blocks = [](int rows, int cols) {
     int kb = 4;
@@ -783,10 +851,12 @@ static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUt
 
 using namespace kvr;
 
-extern "C" size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int top_k) {
-  if (n_tokens < 1 || n_tokens > kMoMaxTokens || hidden < 1 || inter < 1 || top_k < 1 || top_k > kMoMaxTopK) return 0;
+extern "C" size_t kvr_moe_workspace_bytes(int64_t n_tokens, int hidden, int inter, int experts, int top_k) {
+  if (n_tokens < 1 || n_tokens > kMoMaxTokens || hidden < 1 || inter < 1 || experts < 1 || top_k < 1 || top_k > kMoMaxTopK)
+    return 0;
   const size_t picks = (size_t)n_tokens * top_k;
-  return align_up(moe_counters(hidden) * 4, 256) + align_up(picks * inter * 4, 256) + picks * hidden * 4;
+  return align_up(moe_counters(hidden) * 4, 256) + align_up(picks * inter * 4, 256) +
+         picks * moe_cut(n_tokens, hidden, inter, experts, top_k).shares * hidden * 4;
 }
 
 extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hidden, int64_t x_stride, const void *router,
@@ -816,7 +886,8 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
                          reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(status);
   KVR_REQUIRE((ptrs & 15) == 0 && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
               "kvr_moe_layer: pointers must be 16-byte aligned, the workspace 256-byte");
-  KVR_REQUIRE(workspace_bytes >= kvr_moe_workspace_bytes(n_tokens, hidden, inter, top_k), "kvr_moe_layer: workspace too small");
+  KVR_REQUIRE(workspace_bytes >= kvr_moe_workspace_bytes(n_tokens, hidden, inter, experts, top_k),
+              "kvr_moe_layer: workspace too small");
   {  // rows of y are stored while other CTAs still read x
     const uintptr_t p = reinterpret_cast<uintptr_t>(x), q = reinterpret_cast<uintptr_t>(y);
     const uintptr_t n = ((n_tokens - 1) * x_stride + hidden) * 2, m = n_tokens * (uintptr_t)hidden * 2;
@@ -834,7 +905,7 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   r.counters = reinterpret_cast<int *>(ws); r.n_counters = (int)moe_counters(hidden);
   ExpertArgs a{};
   a.tokens = (int)n_tokens; a.hidden = hidden; a.inter = inter; a.experts = experts; a.top_k = top_k;
-  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
+  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
   a.stage_bytes = c.stage_bytes; a.a_bytes = c.a_bytes;
   a.ids = ids; a.weights = weights;
   a.h = ws + align_up(moe_counters(hidden) * 4, 256);

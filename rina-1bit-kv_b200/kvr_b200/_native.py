@@ -105,7 +105,7 @@ SIGNATURES = {
                               P]),
     "kvr_beam_select_workspace_bytes": (SZ, [I, I, I64, I, I]),
     "kvr_beam_select": (I, [P, I, I64, I, I, I64, P, I, P, I, P, P, P, P, P, P, P, SZ, P]),
-    "kvr_moe_workspace_bytes": (SZ, [I64, I, I, I]),
+    "kvr_moe_workspace_bytes": (SZ, [I64, I, I, I, I]),
     "kvr_moe_layer": (I, [P, I, I64, I, I64, P, I64, P, I64, I64, P, I64, I64, I, I, I, I, F, P, P, P, P, SZ, P, P]),
     "kvr_decode_attn_noalloc_max_scratch_bytes": (SZ, []),
     "kvr_decode_attn_noalloc": (I, [P, I, I, I, I, P, P, I, I, I64, I64, P, P, I, I, I64, I64, F, P, I, P]),

@@ -1013,7 +1013,7 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         raise ValueError("out must be contiguous and of x's shape and dtype")
     _on_gpu(x, router, gate_up, down, out)
     dev = x.device
-    key = (n_tokens, hidden, inter, top_k)
+    key = (n_tokens, hidden, inter, experts, top_k)
     need = _MOE_WS.get(key)
     if need is None:
         if len(_MOE_WS) > 4096:
