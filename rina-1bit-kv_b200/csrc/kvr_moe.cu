@@ -125,7 +125,7 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
     for (int e = 0; e < kMrExperts; ++e) w_off[e] = min(e, n_exp - 1 - g * kMrExperts) * a.router_stride;
 #pragma unroll
     for (int t = 0; t < NT; ++t) x_off[t] = min(t, n_tok - 1) * a.x_stride;
-#pragma unroll(NT == 1 ? 4 : NT == 8 ? 1 : 2)
+#pragma unroll(NT == 1 ? 4 : 2)
     for (int c = c0; c < a.hidden; c += dc) {
       uint4 w[kMrExperts], x[NT];
 #pragma unroll
@@ -383,6 +383,9 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   const uint32_t tmem = s.tmem;
   griddep_wait();  // what follows reads the routing
   griddep_launch();
+  int *ticket = a.counters, *seg_done = a.counters + 1, *strip_done = seg_done + kMoMaxSegs;
+  int next = 0;  // (the first ticket, asked for while the lists are made)
+  if (tid == 0) next = atomicAdd(ticket, 1);
 
   // picks by expert, and segments.  Every CTA makes the same lists: a bit per (expert, token), counts and prefix sums.
   constexpr int kIds = kMoMaxPicks / kMoThreads;
@@ -465,7 +468,6 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   p.shares = a.shares;
   p.first3 = p.first2 + p.segs * p.tiles2 * a.shares;
   p.units = p.first3 + (a.hidden + kMoSumCols - 1) / kMoSumCols * p.sums;
-  int *ticket = a.counters, *seg_done = a.counters + 1, *strip_done = seg_done + kMoMaxSegs;
   const uint32_t ring = smem_u32(sm);
 
   if (warp == 0) {
@@ -475,8 +477,6 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     // made a stage cost more than its bytes take to arrive.
     int st = 0, filled = 0;
     unsigned parity = 1;
-    int next = 0;
-    if (lane == 0) next = atomicAdd(ticket, 1);
     bool ok = true;
     for (int q = 0; ok; ++q) {
       const int u = (int)tc_uniform(next);
@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   } else if (warp == 1) {
     // ---- rows of the tokens, four a copy: a lane has the same place in every stage of a unit, or two of them
     // (all copies from one lane, with rows shuffled to it: a third slower)
-    int st = 0, filled = 0;
-    unsigned parity = 1;
+    int st = 0, filled = 0, known = -1;
+    unsigned parity = 1, done = 0;  // segments 32 known .. whose h is there, a bit each
     bool ok = true;
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
@@ -561,16 +561,19 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           r[i][j] = down ? pick * 2 + (c & 1) : pick / a.top_k;
         }
       }
-      if (down) {  // until its gate/up units are done
-        if (lane == 0)
-          for (uint32_t i = 0; mo_acquire(seg_done + w.seg) < p.tiles1 * (a.rows1 / 32); ++i) {
-            if (i >= kSpinLimit || *abort_s) {
-              ok = false;
-              break;
-            }
-            __nanosleep(32);
+      if (down && (w.seg / 32 != known || !((done >> (w.seg & 31)) & 1))) {
+        // until its gate/up units are done: a lane looks at a segment, so that the next units' need not be asked for again
+        known = w.seg / 32;
+        const int mine = known * 32 + lane;
+        for (uint32_t i = 0;; ++i) {
+          done = __ballot_sync(0xffffffffu, mine < p.segs && mo_acquire(seg_done + mine) >= p.tiles1 * (a.rows1 / 32));
+          if ((done >> (w.seg & 31)) & 1) break;
+          if (__any_sync(0xffffffffu, i >= kSpinLimit || *abort_s)) {
+            ok = false;
+            break;
           }
-        ok = __all_sync(0xffffffffu, ok);
+          __nanosleep(32);
+        }
         if (!ok) break;
         __syncwarp();
         asm volatile("fence.proxy.async;" ::: "memory");  // h was stored, and is read by copies
@@ -686,22 +689,32 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         if (!ok) break;
         __syncwarp();
         if (col >= a.hidden) continue;
-        for (int t = w.tile * a.sum_tokens + mine; t < min(a.tokens, (w.tile + 1) * a.sum_tokens); t += 4) {
-          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          const int parts = a.top_k * a.shares;
+        const int parts = a.top_k * a.shares, t1 = min(a.tokens, (w.tile + 1) * a.sum_tokens);
+        for (int t = w.tile * a.sum_tokens + mine * 2; t < t1; t += 8) {  // two tokens, for the loads in flight
+          float4 sum[2] = {};
           const float *rows = a.part + (int64_t)t * parts * a.hidden + col;
+          const int64_t other = t + 1 < t1 ? (int64_t)parts * a.hidden : 0;
+          const float *w0 = a.weights + t * a.top_k, *w1 = w0 + (t + 1 < t1 ? a.top_k : 0);
 #pragma unroll 8
           for (int k = 0; k < parts; ++k) {
-            const float wk = __ldg(a.weights + t * a.top_k + k / a.shares);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(rows + (int64_t)k * a.hidden));
-            sum.x = fmaf(wk, v.x, sum.x);
-            sum.y = fmaf(wk, v.y, sum.y);
-            sum.z = fmaf(wk, v.z, sum.z);
-            sum.w = fmaf(wk, v.w, sum.w);
+            const float wk[2] = {__ldg(w0 + k / a.shares), __ldg(w1 + k / a.shares)};
+            const float4 v[2] = {__ldcg(reinterpret_cast<const float4 *>(rows + (int64_t)k * a.hidden)),
+                                 __ldcg(reinterpret_cast<const float4 *>(rows + other + (int64_t)k * a.hidden))};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              sum[i].x = fmaf(wk[i], v[i].x, sum[i].x);
+              sum[i].y = fmaf(wk[i], v[i].y, sum[i].y);
+              sum[i].z = fmaf(wk[i], v[i].z, sum[i].z);
+              sum[i].w = fmaf(wk[i], v[i].w, sum[i].w);
+            }
           }
-          const uint32_t lo = (uint32_t)bits_dt<DT>(sum.x) | ((uint32_t)bits_dt<DT>(sum.y) << 16);
-          const uint32_t hi = (uint32_t)bits_dt<DT>(sum.z) | ((uint32_t)bits_dt<DT>(sum.w) << 16);
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.y) + (int64_t)t * a.hidden + col) = make_uint2(lo, hi);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = (uint32_t)bits_dt<DT>(sum[i].x) | ((uint32_t)bits_dt<DT>(sum[i].y) << 16);
+            const uint32_t hi = (uint32_t)bits_dt<DT>(sum[i].z) | ((uint32_t)bits_dt<DT>(sum[i].w) << 16);
+            if (t + i < t1)
+              *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.y) + (int64_t)(t + i) * a.hidden + col) = make_uint2(lo, hi);
+          }
         }
         continue;
       }
@@ -744,11 +757,10 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         }
       }
       tc_fence_before();
-      if (!down) asm volatile("fence.proxy.async;" ::: "memory");  // h is read by copies
-      __threadfence();
       __syncwarp();
       if (lane == 0) {
         tc_arrive(&s.acc_empty[buf]);
+        __threadfence();  // the warp's rows, before they are counted
         const int strip = (w.tile * rows + row0) / 32;
         if (row0 < rows) {
           if (!down) atomicAdd(seg_done + w.seg, 1);
@@ -820,7 +832,7 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   if (c.stages > kMoMaxStages) c.stages = kMoMaxStages;
   // sum units for every SM where there are as many tokens
   const int64_t strips = (hidden + kMoSumCols - 1) / kMoSumCols;
-  c.sum_tokens = 4;
+  c.sum_tokens = 8;
   while (c.sum_tokens < 16 && strips * ((tokens + c.sum_tokens - 1) / c.sum_tokens) > 2 * kMoSms) c.sum_tokens *= 2;
   return c;
 }
