@@ -217,7 +217,7 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
 
 constexpr int kMoThreads = 256;
 constexpr int kMoMaxStages = 16, kMoSched = 4;
-constexpr uint32_t kMoRing = 192 * 1024;   // stages
+constexpr uint32_t kMoRing = 176 * 1024;   // stages (more would keep the next call's router off the SM until this one ends)
 constexpr uint32_t kMoPad = 16 * 1024;     // an MMA reads 128 rows from a tile's start, however few of them it uses
 constexpr uint32_t kMoTmemCols = 512;      // two accumulators of up to 256 columns
 constexpr int kMoMinCols = 16;
@@ -254,6 +254,7 @@ struct MoShared {
   short seg_first[kMoMaxSegs], seg_n[kMoMaxSegs];
   short first[kMoMaxExperts];
   short picks[kMoMaxPicks];  // token * top_k + choice, by expert
+  float weights[kMoMaxPicks];
 };
 
 __device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -278,6 +279,12 @@ __device__ __forceinline__ void mo_gather4(uint32_t dst, const CUtensorMap *m, i
       "%4, %5, %6}], [%7];" ::"r"(dst),
       "l"(m), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
       : "memory");
+}
+__device__ __forceinline__ void mo_ld4(uint32_t taddr, float *f) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(f);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr));
 }
 __device__ __forceinline__ int mo_acquire(const int *p) {
   int v;
@@ -392,7 +399,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   const int picks = a.tokens * a.top_k;
   int id[kIds];
 #pragma unroll
-  for (int j = 0; j < kIds; ++j) id[j] = tid + j * kMoThreads < picks ? a.ids[tid + j * kMoThreads] : -1;
+  for (int j = 0; j < kIds; ++j) {
+    const int i = tid + j * kMoThreads;
+    id[j] = i < picks ? a.ids[i] : -1;
+    if (i < picks) s.weights[i] = a.weights[i];
+  }
 #pragma unroll
   for (int j = 0; j < kIds; ++j)
     if (id[j] >= 0) {
@@ -689,23 +700,20 @@ __global__ void __launch_bounds__(kMoThreads, 1)
         if (!ok) break;
         __syncwarp();
         if (col >= a.hidden) continue;
-        const int parts = a.top_k * a.shares, t1 = min(a.tokens, (w.tile + 1) * a.sum_tokens);
+        const int parts = a.top_k * p.shares, t1 = min(a.tokens, (w.tile + 1) * a.sum_tokens);
         for (int t = w.tile * a.sum_tokens + mine * 2; t < t1; t += 8) {  // two tokens, for the loads in flight
           float4 sum[2] = {};
           const float *rows = a.part + (int64_t)t * parts * a.hidden + col;
           const int64_t other = t + 1 < t1 ? (int64_t)parts * a.hidden : 0;
-          const float *w0 = a.weights + t * a.top_k, *w1 = w0 + (t + 1 < t1 ? a.top_k : 0);
-#pragma unroll 8
-          for (int k = 0; k < parts; ++k) {
-            const float wk[2] = {__ldg(w0 + k / a.shares), __ldg(w1 + k / a.shares)};
-            const float4 v[2] = {__ldcg(reinterpret_cast<const float4 *>(rows + (int64_t)k * a.hidden)),
-                                 __ldcg(reinterpret_cast<const float4 *>(rows + other + (int64_t)k * a.hidden))};
+#pragma unroll 4
+          for (int k = 0; k < parts; ++k, rows += a.hidden) {
+            const float4 v[2] = {__ldcg(reinterpret_cast<const float4 *>(rows)), __ldcg(reinterpret_cast<const float4 *>(rows + other))};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              sum[i].x = fmaf(wk[i], v[i].x, sum[i].x);
-              sum[i].y = fmaf(wk[i], v[i].y, sum[i].y);
-              sum[i].z = fmaf(wk[i], v[i].z, sum[i].z);
-              sum[i].w = fmaf(wk[i], v[i].w, sum[i].w);
+              sum[i].x += v[i].x;
+              sum[i].y += v[i].y;
+              sum[i].z += v[i].z;
+              sum[i].w += v[i].w;
             }
           }
 #pragma unroll
@@ -725,24 +733,28 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (!ok) break;
       tc_fence_after();
       if (row0 < rows) {
-        for (int c0 = 0; c0 < n * (down ? 2 : 1); c0 += 16) {
-          float v[16];
-          tc_ld16(lanes + buf * 256 + c0, v);
+        // four columns at a time, rolled: a launch meets this code cold, and 16 at a time took 2 us longer to fetch
+#pragma unroll 1
+        for (int c0 = 0; c0 < n * (down ? 2 : 1); c0 += 4) {
+          float v[4];
+          mo_ld4(lanes + buf * 256 + c0, v);
           tc_wait_ld();
           if (down) {
             const int row = w.tile * rows + row0 + lane;
             if (row < a.hidden) {
 #pragma unroll
-              for (int c = 0; c < 16; c += 2)
-                if (c0 + c < 2 * n)
-                  a.part[((int64_t)s.picks[first + (c0 + c) / 2] * a.shares + w.share) * a.hidden + row] = v[c] + v[c + 1];
+              for (int c = 0; c < 4; c += 2)
+                if (c0 + c < 2 * n) {
+                  const int pick = s.picks[first + (c0 + c) / 2];
+                  a.part[((int64_t)pick * p.shares + w.share) * a.hidden + row] = s.weights[pick] * (v[c] + v[c + 1]);
+                }
             }
           } else {
             // lane l < 16 has gate row l, lane l + 16 up row l: the lower lanes take the even tokens, the upper the odd
             const int row = (w.tile * rows + row0) / 2 + (lane & 15);
             const bool upper = lane >= 16;
 #pragma unroll
-            for (int c = 0; c < 16; c += 2) {
+            for (int c = 0; c < 4; c += 2) {
               const float got = __shfl_xor_sync(0xffffffffu, upper ? v[c] : v[c + 1], 16);
               const float gate = upper ? got : v[c], up = upper ? v[c + 1] : got;
               const int col = c0 + c + (upper ? 1 : 0);
@@ -811,12 +823,19 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   if (cols > (tokens + 15) / 16 * 16) cols = (tokens + 15) / 16 * 16;
   c.cols = (int)cols;
   c.rows1 = moe_rows(segs, 2 * (int64_t)inter);
-  // down units are of 128 rows, and a share of the inner channels (256 at least) so that every SM has some units: partial
-  // rows are summed in any case
+  // Down units are of 128 rows and a share of the inner channels, since partial rows are summed in any case: as many
+  // shares as make the fullest SM's time least, a unit costing about two 64-column blocks besides its own.
   c.rows2 = hidden > 96 ? 128 : (hidden + 31) / 32 * 32;
-  const int64_t tiles2 = segs * ((hidden + c.rows2 - 1) / c.rows2);
+  const int64_t tiles2 = segs * ((hidden + c.rows2 - 1) / c.rows2), blocks2 = (inter + 63) / 64;
   c.shares = 1;
-  while (c.shares < 8 && tiles2 * c.shares < 4 * kMoSms && inter / (c.shares + 1) >= 256) ++c.shares;
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= 8 && n <= blocks2; ++n) {
+    const int64_t t = (tiles2 * n + kMoSms - 1) / kMoSms * ((blocks2 + n - 1) / n + 2);
+    if (t < least) {
+      least = t;
+      c.shares = n;
+    }
+  }
   // a stage of 16 to 40 KB: a stage costs its issuing warps some hundred cycles, whatever it holds
   auto blocks = [](int rows, int cols) {
     int kb = 4;
