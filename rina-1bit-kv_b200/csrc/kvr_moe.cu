@@ -257,18 +257,20 @@ struct MoShared {
   float weights[kMoMaxPicks];
 };
 
-__device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar) {
+__device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar,
+                                        uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, "
+      "%4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ void mo_tma3(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint32_t bar) {
+__device__ __forceinline__ void mo_tma3(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint32_t bar,
+                                        uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-      "[%5];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, "
+      "%4}], [%5], %6;" ::"r"(dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy)
       : "memory");
 }
 // 64 columns of four rows.
@@ -485,7 +487,10 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     // ---- tickets and weights.  The whole warp walks, one lane issues: a copy's operands lie in uniform registers, and
     // only of values that come from a shuffle or from the launch does the compiler know that they may (copies issued by
     // lane 0 alone, with its own ticket's numbers: 320 cycles each, not 60).  Stage and phase are counted up: divisions
-    // made a stage cost more than its bytes take to arrive.
+    // made a stage cost more than its bytes take to arrive.  Weights are read once: first to leave L2, which h and the
+    // partial rows need.
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     int st = 0, filled = 0;
     unsigned parity = 1;
     bool ok = true;
@@ -515,11 +520,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           mbar_expect_tx(&s.full_a[st], nb * rows * 128);
           for (int c = b0 * 64; c < (b0 + nb) * 64; c += 64) {
             if (down) {
-              mo_tma3(dst, &mw2, c, row, e, full);
+              mo_tma3(dst, &mw2, c, row, e, full, policy);
               dst += rows * 128;
             } else {
               for (int r = 0; r < rows; r += 32, dst += 32 * 128)  // 16 rows of gate, the same 16 of up
-                mo_tma4(dst, &mw1, c, row + r / 2, 0, e, full);
+                mo_tma4(dst, &mw1, c, row + r / 2, 0, e, full, policy);
             }
           }
         }
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           float4 sum[2] = {};
           const float *rows = a.part + (int64_t)t * parts * a.hidden + col;
           const int64_t other = t + 1 < t1 ? (int64_t)parts * a.hidden : 0;
-#pragma unroll 4
+#pragma unroll 8
           for (int k = 0; k < parts; ++k, rows += a.hidden) {
             const float4 v[2] = {__ldcg(reinterpret_cast<const float4 *>(rows)), __ldcg(reinterpret_cast<const float4 *>(rows + other))};
 #pragma unroll
