@@ -5,29 +5,37 @@
 // its K V continuations come out in order, equal scores by beam and token.
 //
 // One pass over the logits.  beam_rows_kernel: a CTA takes a segment of a row,
-// holds a running maximum and sum of exponentials per thread and a list of the
-// segment's n best logits for the CTA.  The list's last value is a threshold
-// that few logits pass: tiles in which none does cost one vote.  The first
-// threshold is the n-th largest of the threads' own maxima over the first tile
-// (at least n logits are not below it, and few more are).  Within a row the
-// order of the logits is the order of the scores, so no normaliser is needed
-// yet.  beam_merge_kernel: a CTA per request joins the sums, scores the K S n
-// listed logits and picks the n best.
+// holds a running maximum and sum of exponentials per thread and, for the CTA, a
+// list of the segment's best logits.  The list's n-th is a threshold that few logits
+// pass: 16 a tile at first, then n times the logarithm of the tiles in all.  Threads
+// add what passes without waiting for one another; all warps meet only to cut the
+// list to n.  The first threshold comes from the threads' own maxima over the first
+// tile.  Within a row the order of the logits is the order of the scores, so no
+// normaliser is needed yet.  beam_merge_kernel: a CTA per request joins the sums,
+// scores the K S n listed logits and picks the n best.
 //
 // Scores are compared in 64 bits: c_k + (x - lse_k) in 32 would make different
 // logits equal and order them by token.  Sums are in 32 bits per thread (at most
 // some thousand exponentials <= 1) and joined in 64 by the second kernel.
 //
-// The logits' bytes bound the large calls, a chain of two launches the small.
+// What binds: 512 rows of 128256 in fp32, 56 us (4.7 TB/s; a kernel that only
+// reads them with as many CTAs takes 47): some 200 instructions a warp and tile of 512
+// logits, and 3 us at either end of a segment when nothing streams.  Rows in several
+// segments fill the SMs where rows are few, and pay those ends each (1184 CTAs for 512
+// rows: 65 us).  Tried: words of all rows in equal shares, 62 us; copies two tiles
+// ahead, 64 us (fewer CTAs have room).  One request of 4 beams and 32000 tokens: 9.8 us,
+// a chain of two launches and their barriers.
+#include <cfloat>
+
 #include "kvr_common.cuh"
 
 namespace kvr {
 
-constexpr int kBsThreads = 256;
-constexpr int kBsVecs = 4;        // 16-byte loads of a thread in a tile
+constexpr int kBsThreads = 256, kBsRowThreads = 256;  // of the second kernel, of the first
+constexpr int kBsTile = 16;       // logits of a thread in a tile
 constexpr int kBsMaxN = 128, kBsMaxBeams = 32, kBsMaxEos = 8;
-constexpr int kBsSlack = 64;      // entries beyond n that a list may hold before it is cut
-constexpr int kBsList = kBsMaxN + kBsSlack + 8 * kBsThreads;  // and all of a step of 8 logits a thread
+constexpr int kBsSlack = 32;      // entries beyond n that a list holds before it is cut
+constexpr int kBsList = kBsMaxN + kBsSlack + kBsTile * kBsRowThreads;  // and all of a tile
 constexpr int kBsMaxCands = 8192; // of a request in the second kernel
 constexpr int kBsPicked = 1024;   // candidates that it ranks from shared memory
 
@@ -45,6 +53,11 @@ struct BeamArgs {
   int eos[kBsMaxEos];
 };
 
+__device__ __forceinline__ float bs_max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ float bs_exp(float x) {  // e^x for x <= 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
@@ -59,20 +72,29 @@ __device__ __forceinline__ int bs_token(uint64_t key) { return (int)(0xffffffffu
 
 struct BeamShared {
   uint64_t list[kBsList];
-  uint64_t best[kBsThreads];
+  uint64_t best[kBsRowThreads];
   uint64_t nth;
   int count;
-  float m[kBsThreads / 32], s[kBsThreads / 32];
+  float m[kBsRowThreads / 32], s[kBsRowThreads / 32];
 };
 
-// The n-th largest of one key per thread (distinct unless 0), to all threads.
+// How many maxima the n-th largest is taken of, for a threshold that n values at least are not below: four times n (of
+// fewer, more values lie above it), all threads' at most.
+__device__ __forceinline__ int bs_groups(int n) {
+  int m = 32;
+  while (m < 4 * n && m < kBsThreads) m *= 2;
+  return m;
+}
+
+// The n-th largest of one key per thread (distinct unless 0), to all of the CTA's.
 __device__ __forceinline__ uint64_t bs_nth(BeamShared &sh, uint64_t mine, int n) {
-  sh.best[threadIdx.x] = mine;
-  if (threadIdx.x == 0) sh.nth = 0;
+  const int tid = threadIdx.x;
+  sh.best[tid] = mine;
+  if (tid == 0) sh.nth = 0;
   __syncthreads();
   int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < kBsThreads; i += 2) {
+#pragma unroll 4
+  for (int i = 0; i < kBsRowThreads; i += 2) {
     const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&sh.best[i]);
     above += (o.x > mine) + (o.y > mine);
   }
@@ -81,33 +103,28 @@ __device__ __forceinline__ uint64_t bs_nth(BeamShared &sh, uint64_t mine, int n)
   return sh.nth;
 }
 
-// Cuts the list to its n best, in order.
-__device__ void bs_cut(BeamShared &sh, int n) {
+// Cuts the list to its n best, in order.  All threads, between barriers.
+__device__ __noinline__ void bs_cut(BeamShared &sh, int n) {
   const int tid = threadIdx.x;
   int c = sh.count;
-  if (c > kBsThreads) {  // first to those not below the n-th of the threads' own
+  if (c > kBsRowThreads) {  // first to those not below the n-th of the threads' own, moved to the front
     uint64_t mine = 0;
-    for (int i = tid; i < c; i += kBsThreads) mine = max(mine, sh.list[i]);
+    for (int i = tid; i < c; i += kBsRowThreads) mine = max(mine, sh.list[i]);
     const uint64_t low = bs_nth(sh, mine, n);
-    uint64_t keep[(kBsList + kBsThreads - 1) / kBsThreads];
-#pragma unroll
-    for (int r = 0; r < (kBsList + kBsThreads - 1) / kBsThreads; ++r) {
-      const int i = tid + r * kBsThreads;
-      keep[r] = i < c && sh.list[i] >= low ? sh.list[i] : 0;
-    }
-    __syncthreads();
     if (tid == 0) sh.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < (kBsList + kBsThreads - 1) / kBsThreads; ++r)
-      if (keep[r]) sh.list[atomicAdd(&sh.count, 1)] = keep[r];
+    for (int i0 = 0; i0 < c; i0 += kBsRowThreads) {
+      const uint64_t key = i0 + tid < c ? sh.list[i0 + tid] : 0;
+      __syncthreads();  // a place is written when it has been read
+      if (key && key >= low) sh.list[atomicAdd(&sh.count, 1)] = key;
+    }
     __syncthreads();
     c = sh.count;
   }
   // ranks among the rest; the sorted ones go through `best`, n of which have room
-  for (int i = tid; i < c; i += kBsThreads) {
+  for (int i = tid; i < c; i += kBsRowThreads) {
     const uint64_t mine = sh.list[i];
     int above = 0;
+#pragma unroll 4
     for (int j = 0; j < c; ++j) above += sh.list[j] > mine;
     if (above < n) sh.best[above] = mine;
   }
@@ -135,15 +152,52 @@ __device__ __forceinline__ void bs_widen(const uint4 &u, float *x) {
   }
 }
 
+// Sum of e^(x - from), two at a time in the packed instructions.
+__device__ __forceinline__ float bs_sum(const float (&x)[kBsTile], float from) {
+  uint64_t acc = 0, neg, log2e;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(neg) : "f"(-from));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(log2e) : "f"(1.4426950408889634f));
+#pragma unroll
+  for (int i = 0; i < kBsTile; i += 2) {
+    uint64_t d;
+    float lo, hi;
+    // the difference first: as one fma of x, log2(e) and the scaled maximum, the maximum's rounding would be an error of
+    // every term
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 t, t, %3;\n\tmul.rn.f32x2 %0, t, %4;\n\t}"
+        : "=l"(d)
+        : "f"(x[i]), "f"(x[i + 1]), "l"(neg), "l"(log2e));
+    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %2;\n\tex2.approx.ftz.f32 %0, a;\n\tex2.approx.ftz.f32 %1, b;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "l"(d));
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(acc) : "f"(lo), "f"(hi));
+  }
+  return __uint_as_float((uint32_t)acc) + __uint_as_float((uint32_t)(acc >> 32));
+}
+
+// A value that n logits of the tile's are not below, of the threads' maxima: the least of what the warps' k-th largest are,
+// k warps' worth of n.  (The n-th largest of all threads' maxima is nearer, and takes a microsecond more.)
+__device__ __forceinline__ float bs_first_limit(BeamShared &sh, float top, int n, int full_warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int k = (n + full_warps - 1) / full_warps;
+  unsigned key = top > -INFINITY ? float_key(top) : 0, kth = 0;
+  for (int i = 0; i < k && k <= 32; ++i) {
+    kth = __reduce_max_sync(0xffffffffu, key);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, key == kth)) - 1) key = 0;
+  }
+  if (lane == 0) sh.m[warp] = kth ? key_float(kth) : -INFINITY;
+  __syncthreads();
+  float low = sh.m[0];
+  for (int w = 1; w < full_warps; ++w) low = fminf(low, sh.m[w]);
+  return fmaxf(low, -FLT_MAX);
+}
+
 template <int DT>
-__global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kBsRowThreads, 1024 / kBsRowThreads) beam_rows_kernel(BeamArgs a) {
   constexpr int kPer = DT == KVR_F32 ? 4 : 8, kSize = 16 / kPer;  // logits of a 16-byte granule, bytes of one
-  constexpr int kTile = kBsVecs * kBsThreads;
+  constexpr int kVecs = kBsTile / kPer, kTile = kVecs * kBsRowThreads;
   __shared__ BeamShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
   const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
-  griddep_wait();
-  griddep_launch();
   // The row's granules: rows need not start on one, so its first and last may hold logits of others, masked below.
   // (Every granule read holds one of the row's at least.)
   const char *base = static_cast<const char *>(a.logits) + (int64_t)row * a.row_stride * kSize;
@@ -152,79 +206,99 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(BeamArgs a) {
   const int granules = (int)(((int64_t)head + a.vocab + kPer - 1) / kPer);
   const int g0 = (int)((int64_t)granules * split / a.splits), g1 = (int)((int64_t)granules * (split + 1) / a.splits);
   if (tid == 0) sh.count = 0;
+  griddep_wait();
+  griddep_launch();
   const uint32_t pad = DT == KVR_F32 ? 0xff800000u : DT == KVR_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
-  uint4 next[kBsVecs];
-  auto fetch = [&](int at) {
+  // (fp32: the next tile's words; 16 bits: two tiles', as many)
+  constexpr int kAhead = 4 / kVecs;
+  uint4 next[kAhead][kVecs];
+  auto fetch = [&](uint4 (&to)[kVecs], int at) {
 #pragma unroll
-    for (int v = 0; v < kBsVecs; ++v) {
-      const int g = at + v * kBsThreads + tid;
-      next[v] = g < g1 ? __ldcs(src + g) : make_uint4(pad, pad, pad, pad);
+    for (int v = 0; v < kVecs; ++v) {
+      const int g = at + v * kBsRowThreads + tid;
+      to[v] = g < g1 ? __ldcs(src + g) : make_uint4(pad, pad, pad, pad);
     }
   };
-  float m = -INFINITY, s = 0.0f, limit = -INFINITY;
-  fetch(g0);
-  for (int at = g0; at < g1; at += kTile) {
-    float x[kBsVecs * kPer];
-#pragma unroll
-    for (int v = 0; v < kBsVecs; ++v) {
-      bs_widen<DT>(next[v], x + v * kPer);
-      const int g = at + v * kBsThreads + tid, t = g * kPer - head;
-      if (g < g1 && (t < 0 || t > a.vocab - kPer)) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (t + j < 0 || t + j >= a.vocab) x[v * kPer + j] = -INFINITY;
-      }
-    }
-    if (at + kTile < g1) fetch(at + kTile);
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < kBsVecs * kPer; ++i) top = fmaxf(top, x[i]);  // a NaN is passed over here, not in the sum
-    const float old = m;
-    m = fmaxf(m, top);
-    const float from = m == -INFINITY ? 0.0f : m;
-    s *= bs_exp(old - from);
-#pragma unroll
-    for (int i = 0; i < kBsVecs * kPer; ++i) s += bs_exp(x[i] - from);
-    // the list
-    const bool first = at == g0;
-    if (first) {
-      uint64_t mine = 0;
-      if (top > -INFINITY) {
-        int k = 0;
-#pragma unroll
-        for (int i = kBsVecs * kPer - 1; i >= 0; --i)
-          if (x[i] == top) k = i;
-        mine = bs_key(top, (at + k / kPer * kBsThreads + tid) * kPer - head + k % kPer);
-      }
-      const uint64_t low = bs_nth(sh, mine, n);
-      limit = low ? bs_value(low) : -INFINITY;
-    }
-    if (!__syncthreads_or(first || top > limit)) continue;
-#pragma unroll
-    for (int v = 0; v < kBsVecs; ++v) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float y = x[v * kPer + j];
-        if (y > limit || (first && y == limit && y > -INFINITY))
-          sh.list[atomicAdd(&sh.count, 1)] = bs_key(y, (at + v * kBsThreads + tid) * kPer - head + j);
-      }
-      __syncthreads();
-      if (sh.count > n + kBsSlack) {
-        bs_cut(sh, n);
-        limit = bs_value(sh.list[n - 1]);
-      }
-      __syncthreads();  // the count is read before the next step adds to it
-    }
-    if (first && sh.count >= n) {  // later logits that equal the n-th lose to it by their token
-      bs_cut(sh, n);
+  float m = -INFINITY, s = 0.0f;
+  // what a logit has to be above, or equal to with a lower token (warps are not at the same tile: a list's last entry may
+  // be of a later one)
+  float limit = -FLT_MAX;  // (so that -inf is below it)
+  int limit_token = INT_MAX;
+  // All warps cut the list and take over its limit; true when all of them are done.  They meet only for that: a warp that
+  // starts a tile with too many entries in the list comes here, and so does one that is done, so each of the others adds
+  // one tile at most, for which the list has room.  (A barrier a tile: 62 us for 512 rows of 128256, and most of a warp's
+  // time at it.)
+  auto meet = [&](bool done) {
+    const bool all = __syncthreads_and(done);
+    bs_cut(sh, n);
+    if (sh.count == n) {
       limit = bs_value(sh.list[n - 1]);
-      __syncthreads();
+      limit_token = bs_token(sh.list[n - 1]);
     }
+    __syncthreads();  // the count is read before any warp adds to it
+    return all;
+  };
+  auto tile = [&](uint4 (&from)[kVecs], int at, bool first) {
+    float x[kBsTile], tops[kBsTile / 4], top;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) bs_widen<DT>(from[v], x + v * kPer);
+    auto token = [&](int i) { return (at + i / kPer * kBsRowThreads + tid) * kPer - head + i % kPer; };
+    if (first || at + kTile >= g1) {
+#pragma unroll
+      for (int i = 0; i < kBsTile; ++i)
+        if (token(i) < 0 || token(i) >= a.vocab) x[i] = -INFINITY;
+    }
+    if (at + kAhead * kTile < g1) fetch(from, at + kAhead * kTile);
+#pragma unroll
+    for (int q = 0; q < kBsTile / 4; ++q) {  // (a NaN is passed over here, not in the sum)
+      tops[q] = bs_max3(x[4 * q], x[4 * q + 1], fmaxf(x[4 * q + 2], x[4 * q + 3]));
+    }
+    top = bs_max3(tops[0], tops[1], fmaxf(tops[2], tops[3]));
+    if (top > m) {  // (rare after the first tiles)
+      s *= bs_exp(m - top);
+      m = top;
+    }
+    s += bs_sum(x, m == -INFINITY ? 0.0f : m);
+    if (first) {
+      limit = bs_first_limit(sh, top, n, max(1, min(kBsRowThreads, g1 - g0) / 32));
+    }
+    if (top >= limit) {
+      unsigned which = 0;
+#pragma unroll
+      for (int i = 0; i < kBsTile; ++i) which |= (x[i] >= limit ? 1u : 0u) << i;
+#pragma unroll 1
+      for (; which; which &= which - 1) {
+        const int i = __ffs(which) - 1, t = token(i);
+        float y[kBsTile];
+#pragma unroll
+        for (int j = 0; j < kBsTile; ++j) y[j] = x[j];
+#pragma unroll
+        for (int o = kBsTile / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int j = 0; j < o; ++j) y[j] = i & o ? y[j + o] : y[j];
+        if (y[0] > limit || t < limit_token) sh.list[atomicAdd(&sh.count, 1)] = bs_key(y[0], t);
+      }
+    }
+    __syncwarp();
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d)
+    if (g0 + d * kTile < g1) fetch(next[d], g0 + d * kTile);
+  tile(next[0], g0, true);
+  meet(false);
+  for (int at = g0 + kTile; at < g1; at += kAhead * kTile) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+      if (at + d * kTile < g1) {
+        if (__any_sync(0xffffffffu, *static_cast<volatile int *>(&sh.count) > n + kBsSlack)) meet(false);
+        tile(next[(d + 1) % kAhead], at + d * kTile, false);
+      }
   }
-  __syncthreads();
-  bs_cut(sh, n);
+  __syncwarp();
+  while (!meet(true)) {
+  }
   uint64_t *out = a.cands + ((int64_t)row * a.splits + split) * n;
-  for (int i = tid; i < n; i += kBsThreads) out[i] = i < sh.count ? sh.list[i] : 0;
+  for (int i = tid; i < n; i += kBsRowThreads) out[i] = i < sh.count ? sh.list[i] : 0;
   const float wm = warp_max(m);
   s *= bs_exp(m - (wm == -INFINITY ? 0.0f : wm));
   s = warp_sum(s);
@@ -235,8 +309,8 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_rows_kernel(BeamArgs a) {
   __syncthreads();
   if (tid == 0) {
     float bm = -INFINITY, bs = 0.0f;
-    for (int w = 0; w < kBsThreads / 32; ++w) bm = fmaxf(bm, sh.m[w]);
-    for (int w = 0; w < kBsThreads / 32; ++w) bs += sh.s[w] * bs_exp(sh.m[w] - (bm == -INFINITY ? 0.0f : bm));
+    for (int w = 0; w < kBsRowThreads / 32; ++w) bm = fmaxf(bm, sh.m[w]);
+    for (int w = 0; w < kBsRowThreads / 32; ++w) bs += sh.s[w] * bs_exp(sh.m[w] - (bm == -INFINITY ? 0.0f : bm));
     a.ml[(int64_t)row * a.splits + split] = make_float2(bm, bs);
   }
 }
@@ -262,9 +336,19 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
   __shared__ BeamRank best[kBsThreads], picked[kBsPicked], sorted[kBsMaxN], nth;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x, n = a.n, K = a.beams;
-  const int per_beam = a.splits * n, total = K * per_beam;
+  const int per_beam = a.splits * n, total = K * per_beam, groups = bs_groups(n);
+  if (tid == 0) {
+    count = 0;
+    nth = BeamRank{0, 0};
+  }
+  if (tid < n) sorted[tid] = BeamRank{0, 0};
   griddep_wait();
   griddep_launch();
+  constexpr int kAhead = 4;  // candidates that a thread asks for while the sums are joined
+  const uint64_t *cands = a.cands + (int64_t)b * total;
+  uint64_t ahead[kAhead];
+#pragma unroll
+  for (int r = 0; r < kAhead; ++r) ahead[r] = tid + r * kBsThreads < total ? cands[tid + r * kBsThreads] : 0;
   for (int k = warp; k < K; k += kBsThreads / 32) {  // a beam's sums, in 64 bits
     const float2 *ml = a.ml + ((int64_t)b * K + k) * a.splits;
     float m = -INFINITY;
@@ -277,15 +361,9 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) lse[k] = (double)m + log(s);
   }
-  if (tid == 0) {
-    count = 0;
-    nth = BeamRank{0, 0};
-  }
-  if (tid < n) sorted[tid] = BeamRank{0, 0};
   __syncthreads();
   BeamRank mine{0, 0};
-  for (int i = tid; i < total; i += kBsThreads) {
-    const uint64_t c = a.cands[(int64_t)b * total + i];
+  auto enter = [&](int i, uint64_t c) {
     const int k = i / per_beam;
     BeamRank r{0, 0};
     if (c) {
@@ -294,27 +372,41 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
     }
     all[i] = r;
     if (r.key && bs_above(r, mine)) mine = r;
-  }
-  best[tid] = mine;
-  __syncthreads();
-  if (mine.key) {
-    int above = 0;
+  };
+#pragma unroll
+  for (int r = 0; r < kAhead; ++r)
+    if (tid + r * kBsThreads < total) enter(tid + r * kBsThreads, ahead[r]);
+  for (int i = tid + kAhead * kBsThreads; i < total; i += kBsThreads) enter(i, cands[i]);
+  // a threshold, where there are many: the n-th largest of groups' maxima
+  if (total > kBsThreads / 2) {
+    const int each = kBsThreads / groups;
+    for (int o = 1; o < each; o <<= 1) {
+      const BeamRank r{__shfl_xor_sync(0xffffffffu, mine.key, o), __shfl_xor_sync(0xffffffffu, mine.id, o)};
+      if (r.key && (!mine.key || bs_above(r, mine))) mine = r;
+    }
+    if (tid % each == 0) best[tid / each] = mine;
+    __syncthreads();
+    if (tid < groups) {
+      mine = best[tid];
+      int above = 0;
 #pragma unroll 4
-    for (int i = 0; i < kBsThreads; ++i) above += bs_above(best[i], mine);
-    if (above == n - 1) nth = mine;
-  }
-  __syncthreads();
-  const BeamRank low = nth;
-  for (int i = tid; i < total; i += kBsThreads) {
-    const BeamRank r = all[i];
-    if (r.key && !bs_above(low, r)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kBsPicked) picked[at] = r;
+      for (int i = 0; i < groups; ++i) above += bs_above(best[i], mine);
+      if (mine.key && above == n - 1) nth = mine;
+    }
+    __syncthreads();
+    const BeamRank low = nth;
+    for (int i = tid; i < total; i += kBsThreads) {
+      const BeamRank r = all[i];
+      if (r.key && !bs_above(low, r)) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kBsPicked) picked[at] = r;
+      }
     }
   }
   __syncthreads();
+  const BeamRank low = nth;
   // ranks: among those picked or, where they are too many for the list, among all
-  const bool few = count <= kBsPicked;
+  const bool few = total > kBsThreads / 2 && count <= kBsPicked;
   const BeamRank *from = few ? picked : all;
   const int m = few ? count : total;
   for (int i = tid; i < m; i += kBsThreads) {
@@ -361,7 +453,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
 // granules / 2, and no more candidates than the second kernel has room for.
 int beam_splits(int64_t rows, int beams, int n, int64_t vocab, int dtype) {
   const int64_t granules = (vocab * (int64_t)dtype_size(dtype) + 15) / 16;
-  int64_t s = (148 * 8 + rows - 1) / rows;
+  int64_t s = (148 * 3 + rows - 1) / rows;
   if (s > (granules + 511) / 512) s = (granules + 511) / 512;
   if (s > kBsMaxCands / (beams * n)) s = kBsMaxCands / (beams * n);
   return (int)(s < 1 ? 1 : s);
@@ -414,7 +506,7 @@ extern "C" int kvr_beam_select(const void *logits, int dtype, int64_t row_stride
   cudaError_t e = launch_dependent(dtype == KVR_F32   ? beam_rows_kernel<KVR_F32>
                                    : dtype == KVR_F16 ? beam_rows_kernel<KVR_F16>
                                                       : beam_rows_kernel<KVR_BF16>,
-                                   grid, kBsThreads, 0, as_cuda(stream), a);
+                                   grid, kBsRowThreads, 0, as_cuda(stream), a);
   if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_beam_select: %s", cudaGetErrorString(e));
   const size_t smem = (size_t)n_beams * splits * n * sizeof(BeamRank);
   if (smem > 8 * 1024) {
