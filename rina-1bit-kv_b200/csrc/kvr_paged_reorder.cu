@@ -10,24 +10,28 @@
 // A page holds tokens [j P, (j + 1) P) of a sequence, so it stands in column j
 // of every row that holds it, and columns do not meet.  paged_reorder_kernel: one
 // cluster of 8 CTAs; a warp takes 32 columns of a group, a column per lane:
-//   1  counts: + for the page that a row gets, - for the one that it loses;
-//   2  a page with a count below 0 has no holder left.  Rows of several groups may
-//      have lost it: the lowest place (row, column) claims it, by a minimum;
-//   3  claims won per row and 32 columns, their prefix sums;
-//   4  claimed pages to the end of the free list, in order of rows and columns,
-//      and the rows' new entries;
-//   5  (CTA 0, a thread per row) last pages: who copies, fresh pages off the end
-//      of the list, lengths.
-// No result depends on the order of atomics.  Tables and counts are small and lie
-// in L2: the chain of phases bounds it.  copy_pages_kernel then copies the tokens
-// of the listed pages in all layers, K and V, 16 bytes a lane; HBM bounds that.
+//   1  the column's pages: holders in the group before and after.  Where the group
+//      has all of a page's holders, its new count, or that it is free, is settled
+//      at once.  Counts of pages with holders outside go up and down by atomics;
+//   -  only if a group gave up such a page altogether: whether others did too, which
+//      the lowest place (row, column) then claims, by a minimum;
+//   2  (after the cluster has met) free pages counted per row, their prefix sums, the
+//      pages to the end of the free list in order of rows and columns, new entries;
+//   3  (after it has met again; CTA 0, a thread per row) last pages: who copies, fresh
+//      pages off the end of the list, lengths.
+// No result depends on the order of atomics.  copy_pages_kernel then copies the
+// tokens of the listed pages in all layers, K and V, 16 bytes a lane.
+//
+// What binds: tables and counts are small and lie in L2, so the first kernel is a
+// chain of dependent loads and two meetings; HBM binds the copies.
 #include "kvr_attn_plan.cuh"
 
 namespace kvr {
 
-constexpr int kPrCluster = 8, kPrThreads = 512, kPrWarps = kPrThreads / 32;
+constexpr int kPrCluster = 8, kPrThreads = 1024, kPrWarps = kPrThreads / 32;
 constexpr int kPrMaxBeams = 32, kPrMaxRows = 4096;
-constexpr int kPrStepTokens = 8;  // tokens that a warp copies at a time
+constexpr int kPrStepTokens = 8;     // tokens that a warp copies at a time
+constexpr int kPrSmem = 216 * 1024;  // places of the rows, and entries of as many units as fit
 
 struct ReorderArgs {
   int *table;
@@ -42,15 +46,30 @@ struct ReorderArgs {
   int *n_free;
   const int *rows, *parents;
   int groups, beams;
+  int slots;    // units of a warp whose entries stay in shared memory
   int *info;
-  int *counts;  // (groups * beams, blocks of 32 columns) scratch
+  int *counts;  // (groups * beams, blocks of 32 columns) scratch: pages given back
+  unsigned *given;  // (units, 32) scratch: places of the group whose page a lane gives back, a bit each
   int4 *copies; // (groups * beams) scratch: from page, to page, tokens
   int *n_copies;
+};
+
+// What is known of a place (a row of a group) before the call.
+struct PrPlace {
+  int row, parent;  // table row; place of its parent in the group; -1: none
+  int len, last;    // its tokens; the page that its parent's last tokens lie in, -1: none, or a full one
 };
 
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int pr_peer(const int *p, unsigned rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
 }
 
 // Sum of v over the CTA's lower threads; `total` over all.
@@ -66,7 +85,7 @@ __device__ __forceinline__ int pr_exclusive(int v, int *warp_sums, int &total) {
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int s = lane < kPrWarps ? warp_sums[lane] : 0;
+    int s = warp_sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, s, o);
@@ -78,125 +97,178 @@ __device__ __forceinline__ int pr_exclusive(int v, int *warp_sums, int &total) {
   total = warp_sums[31];
   return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
-
-__device__ __forceinline__ int pr_row(const ReorderArgs &a, int i) {  // table row of place i, -1: none
-  const int r = a.rows[i];
-  return r >= 0 && r < a.table_rows ? r : -1;
-}
-__device__ __forceinline__ int pr_len(const ReorderArgs &a, int i) {  // its tokens before the call
-  const int r = pr_row(a, i);
-  return r < 0 ? 0 : (int)min((int64_t)max(__ldcg(a.ctx + r), 0), (int64_t)a.width * a.page);
-}
-__device__ __forceinline__ int pr_parent(const ReorderArgs &a, int i) {  // place of its parent, -1: none
-  const int p = a.parents[i];
-  return p >= 0 && p < a.beams ? i / a.beams * a.beams + p : -1;
-}
+static_assert(kPrWarps == 32, "one sum per lane");
 
 __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads) paged_reorder_kernel(ReorderArgs a) {
-  extern __shared__ int old_s[];  // (warps, beams, 32): a unit's old entries
-  __shared__ int parent_s[kPrWarps][kPrMaxBeams], row_s[kPrWarps][kPrMaxBeams], held_s[kPrWarps][kPrMaxBeams];
-  __shared__ int warp_sums[32], longest;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int warp_sums[32], longest, disputed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, n = a.groups * K;
+  PrPlace *place = reinterpret_cast<PrPlace *>(smem);  // (n)
+  int *ahead = reinterpret_cast<int *>(place + n);     // (n) pages given back by the places before
+  int *entries = ahead + n;                            // (warps, slots, K, 32)
+  if (tid == 0) longest = disputed = 0;
   griddep_wait();
   griddep_launch();
-  if (tid == 0) longest = 0;
   __syncthreads();
   int most = 0;
-  for (int i = tid; i < n; i += kPrThreads) most = max(most, (pr_len(a, i) + a.page - 1) / a.page);
-  most = warp_max_int(most);
-  if (lane == 0) atomicMax(&longest, most);
+  for (int i = tid; i < n; i += kPrThreads) {
+    const int r = a.rows[i], p = a.parents[i];
+    PrPlace x;
+    x.row = r >= 0 && r < a.table_rows ? r : -1;
+    x.parent = x.row >= 0 && p >= 0 && p < K ? p : -1;
+    x.len = x.row < 0 ? 0 : (int)min((int64_t)max(__ldcg(a.ctx + x.row), 0), (int64_t)a.width * a.page);
+    x.last = -1;
+    place[i] = x;
+    most = max(most, (x.len + a.page - 1) / a.page);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0 && most > 0) atomicMax(&longest, most);
   __syncthreads();
   const int blocks = (longest + 31) / 32, units = a.groups * blocks, all_warps = kPrCluster * kPrWarps;
-  // unit u of this warp: group, columns.  CTA first, so that few units spread over the cluster's SMs
+  auto held = [&](int i) { return (place[i].len + a.page - 1) / a.page; };
+  auto entry = [&](int i, int j) {  // page of place i in column j before the call, -1: none
+    int e = -1;
+    if (j < held(i)) e = a.table[place[i].row * a.table_stride + j];
+    return e >= 0 && e < a.n_pages ? e : -1;
+  };
+  // unit u of this warp: group, 32 columns.  CTA first, so that few units spread over the cluster's SMs
   const int me = warp * kPrCluster + (int)blockIdx.x;
-  int *old = old_s + warp * K * 32;
-  auto load = [&](int u) {
+  const bool kept = units <= all_warps * a.slots;  // all units' entries stay in shared memory
+  auto load = [&](int u, int nth, bool again) {
+    int *old = entries + (warp * a.slots + (kept ? nth : 0)) * K * 32 + lane;
+    if (kept && again) return old;
     const int g = u / blocks, j = (u - g * blocks) * 32 + lane;
-    __syncwarp();
-    if (lane < K) {
-      const int i = g * K + lane;
-      const int r = pr_row(a, i), p = pr_parent(a, i);
-      row_s[warp][lane] = r;
-      held_s[warp][lane] = (pr_len(a, i) + a.page - 1) / a.page;
-      parent_s[warp][lane] = r < 0 || p < 0 ? -1 : p - g * K;
-    }
-    __syncwarp();
 #pragma unroll 8
-    for (int i = 0; i < K; ++i) {
-      int e = -1;
-      if (j < held_s[warp][i]) e = a.table[row_s[warp][i] * a.table_stride + j];
-      old[i * 32 + lane] = e >= 0 && e < a.n_pages ? e : -1;
-    }
-    // (a lane reads back only what it wrote)
+    for (int i = 0; i < K; ++i) old[i * 32] = entry(g * K + i, j);  // (a lane reads back only what it wrote)
+    return old;
   };
-  auto fresh = [&](int i) {  // what place i of the unit gets
-    const int p = parent_s[warp][i];
-    return p < 0 ? -1 : old[p * 32 + lane];
-  };
-  const bool once = units <= all_warps;  // a warp's only unit stays in shared memory
-  for (int u = me; u < units; u += all_warps) {
-    load(u);
-    for (int i = 0; i < K; ++i) {
-      const int had = old[i * 32 + lane], gets = fresh(i);
-      if (had == gets) continue;
-      if (gets >= 0) atomicAdd(a.shared + gets, 1);
-      if (had >= 0) atomicSub(a.shared + had, 1);
-    }
-  }
-  cluster_sync();
-  // place of an entry; the claims lie below every count
+  auto parent_of = [&](int u, int i) { return place[u / blocks * K + i].parent; };
+  // places of entries; the claims lie below every count
   auto claim = [&](int u, int i) {
     const int g = u / blocks;
     return INT_MIN + (g * K + i) * (blocks * 32) + (u - g * blocks) * 32 + lane;
   };
-  for (int u = me; u < units; u += all_warps) {
-    if (!once) load(u);
-    for (int i = 0; i < K; ++i) {
-      const int had = old[i * 32 + lane];
-      if (had >= 0 && had != fresh(i) && __ldcg(a.shared + had) < 0) atomicMin(a.shared + had, claim(u, i));
-    }
-  }
-  cluster_sync();
-  for (int u = me; u < units; u += all_warps) {
-    if (!once) load(u);
+  auto count = [&](int u, unsigned given) {
     const int g = u / blocks;
     for (int i = 0; i < K; ++i) {
-      const int had = old[i * 32 + lane];
-      const bool won = had >= 0 && had != fresh(i) && __ldcg(a.shared + had) == claim(u, i);
-      const unsigned who = __ballot_sync(0xffffffffu, won);
+      const unsigned who = __ballot_sync(0xffffffffu, (given >> i) & 1);
       if (lane == 0) a.counts[(int64_t)(g * K + i) * blocks + u - g * blocks] = __popc(who);
     }
+  };
+  // the page of place i, if it is the first of the group to hold it: holders before and after
+  auto holders = [&](const int *old, int u, int i, int &before, int &after) {
+    const int page = old[i * 32];
+    before = after = 0;
+    if (page < 0) return false;
+    for (int o = 0; o < K; ++o) {
+      if (old[o * 32] == page) {
+        if (o < i) return false;
+        ++before;
+      }
+      const int p = parent_of(u, o);
+      after += p >= 0 && old[p * 32] == page;
+    }
+    return true;
+  };
+  for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
+    const int *old = load(u, nth, false);
+    bool changed = false;
+    for (int i = 0; i < K; ++i) {
+      const int p = parent_of(u, i);
+      changed |= old[i * 32] != (p < 0 ? -1 : old[p * 32]);
+    }
+    unsigned given = 0;
+    for (int i = 0; i < K && changed; ++i) {
+      int before, after;
+      if (!holders(old, u, i, before, after) || before == after) continue;
+      int *c = a.shared + old[i * 32];
+      if (__ldcg(c) < before) {  // (no holder but this group's)
+        *c = max(after - 1, 0);
+        if (after == 0) given |= 1u << i;
+      } else {
+        atomicAdd(c, after - before);
+        if (after == 0) disputed = 1;
+      }
+    }
+    a.given[u * 32 + lane] = given;
+    count(u, given);
   }
+  if (blockIdx.x == 0)  // before any entry is written: the pages that rows will have to copy
+    for (int i = tid; i < n; i += kPrThreads) {
+      const int p = place[i].parent;
+      if (p < 0) continue;
+      const int from = i / K * K + p, len = place[from].len;
+      if (len % a.page) place[i].last = entry(from, (len - 1) / a.page);
+    }
   cluster_sync();
-  const int n_free = min(max(*a.n_free, 0), a.n_free_cap);
-  int gone = 0;
-  if (blockIdx.x == 0) {  // prefix sums of the counts, in place
-    const int64_t entries = (int64_t)n * blocks, each = (entries + kPrThreads - 1) / kPrThreads;
+  int any = 0;
+  for (int c = 0; c < kPrCluster; ++c) any |= pr_peer(&disputed, c);
+  if (any) {
+    for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
+      const int *old = load(u, nth, true);
+      for (int i = 0; i < K; ++i) {
+        int before, after;
+        if (!holders(old, u, i, before, after) || after > 0) continue;
+        int *c = a.shared + old[i * 32];
+        if (__ldcg(c) < 0) atomicMin(c, claim(u, i));
+      }
+    }
+    cluster_sync();
+    for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
+      const int *old = load(u, nth, true);
+      unsigned given = a.given[u * 32 + lane];
+      for (int i = 0; i < K; ++i) {
+        int before, after;
+        if (!holders(old, u, i, before, after) || after > 0) continue;
+        int *c = a.shared + old[i * 32];
+        if (__ldcg(c) == claim(u, i)) {
+          given |= 1u << i;
+          *c = 0;
+        }
+      }
+      a.given[u * 32 + lane] = given;
+      count(u, given);
+    }
+    cluster_sync();
+  }
+  // pages given back by each row, and by those before it
+  for (int i = warp; i < n; i += kPrWarps) {
     int sum = 0;
-    for (int64_t k = tid * each; k < min((tid + 1) * each, entries); ++k) sum += __ldcg(a.counts + k);
+    for (int b = lane; b < blocks; b += 32) sum += __ldcg(a.counts + (int64_t)i * blocks + b);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) ahead[i] = sum;
+  }
+  __syncthreads();
+  int gone;
+  {
+    const int each = (n + kPrThreads - 1) / kPrThreads;
+    int sum = 0;
+    for (int i = tid * each; i < min((tid + 1) * each, n); ++i) sum += ahead[i];
     int at = pr_exclusive(sum, warp_sums, gone);
-    for (int64_t k = tid * each; k < min((tid + 1) * each, entries); ++k) {
-      const int c = __ldcg(a.counts + k);
-      a.counts[k] = at;
+    for (int i = tid * each; i < min((tid + 1) * each, n); ++i) {
+      const int c = ahead[i];
+      ahead[i] = at;
       at += c;
     }
   }
-  cluster_sync();
-  for (int u = me; u < units; u += all_warps) {
-    if (!once) load(u);
-    const int g = u / blocks, j = (u - g * blocks) * 32 + lane;
+  const int n_free = min(max(__ldcg(a.n_free), 0), a.n_free_cap);
+  __syncthreads();
+  for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
+    const int *old = load(u, nth, true);
+    const int g = u / blocks, b = u - g * blocks, j = b * 32 + lane;
+    const unsigned given = a.given[u * 32 + lane], anyone = __reduce_or_sync(0xffffffffu, given);
     for (int i = 0; i < K; ++i) {
-      const int had = old[i * 32 + lane], gets = fresh(i);
-      const bool won = had >= 0 && had != gets && __ldcg(a.shared + had) == claim(u, i);
-      const unsigned who = __ballot_sync(0xffffffffu, won);
-      if (won) {
-        const int64_t at = (int64_t)n_free + __ldcg(a.counts + (int64_t)(g * K + i) * blocks + u - g * blocks) +
-                           __popc(who & ((1u << lane) - 1));
-        if (at < a.n_free_cap) a.free_pages[at] = had;
-        a.shared[had] = 0;
+      const int at_i = g * K + i;
+      if ((anyone >> i) & 1) {
+        int before = 0;  // the row's in columns before this unit's
+        for (int c = lane; c < b; c += 32) before += __ldcg(a.counts + (int64_t)at_i * blocks + c);
+        before = __reduce_add_sync(0xffffffffu, before);
+        const unsigned who = __ballot_sync(0xffffffffu, (given >> i) & 1);
+        const int64_t at = (int64_t)n_free + ahead[at_i] + before + __popc(who & ((1u << lane) - 1));
+        if (((given >> i) & 1) && at < a.n_free_cap) a.free_pages[at] = old[i * 32];
       }
-      const int r = row_s[warp][i], p = parent_s[warp][i];
-      if (r >= 0 && had != gets && j < max(held_s[warp][i], p < 0 ? 0 : held_s[warp][p]))
+      const int r = place[at_i].row, p = place[at_i].parent, gets = p < 0 ? -1 : old[p * 32];
+      if (r >= 0 && old[i * 32] != gets && j < max(held(at_i), p < 0 ? 0 : held(g * K + p)))
         a.table[r * a.table_stride + j] = gets;
     }
   }
@@ -205,42 +277,32 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads)
   // last pages, a thread per row
   const int left = (int)min((int64_t)n_free + gone, (int64_t)a.n_free_cap);
   int done = 0, missing = 0;
-  const int step = kPrThreads / K * K;  // whole groups: lengths are read before any of the group is written
-  for (int i0 = 0; i0 < n; i0 += step) {
+  for (int i0 = 0; i0 < n; i0 += kPrThreads) {
     const int i = i0 + tid;
-    const bool in = tid < step && i < n;
-    const int parent = in ? pr_parent(a, i) : -1, r = in ? pr_row(a, i) : -1;
-    const int now = parent >= 0 && r >= 0 ? pr_len(a, parent) : 0;
-    const int col = (now - 1) / a.page;
-    int copy = 0, page = -1;
-    if (now % a.page) {
-      page = __ldcg(a.table + r * a.table_stride + col);
-      if (page >= 0 && page < a.n_pages) {
-        int before = 0, same = 0;  // children of the parent
-        const int g = i / K * K;
-        for (int o = g; o < g + K; ++o) {
-          const int is = pr_parent(a, o) == parent && pr_row(a, o) >= 0;
-          same += is;
-          before += is && o < i;
-        }
-        copy = before > 0 || __ldcg(a.shared + page) + 1 > same;  // (or a row outside of the group holds it)
+    const PrPlace x = i < n ? place[i] : PrPlace{-1, -1, 0, -1};
+    const int g = i / K * K, now = x.parent >= 0 ? place[g + x.parent].len : 0;
+    int copy = 0;
+    if (x.last >= 0) {
+      int before = 0, same = 0;  // children of the parent
+      for (int o = g; o < g + K; ++o) {
+        const int is = place[o].parent == x.parent;
+        same += is;
+        before += is && o < i;
       }
+      copy = before > 0 || __ldcg(a.shared + x.last) + 1 > same;  // (or a row outside of the group holds it)
     }
     int sum;
     const int k = done + pr_exclusive(copy, warp_sums, sum);
     done += sum;
-    __syncthreads();  // lengths, counts and entries of these rows are read
+    __syncthreads();  // counts are read
     if (copy) {
-      const int to = k < left ? a.free_pages[left - 1 - k] : -1;
-      atomicSub(a.shared + page, 1);
-      a.table[r * a.table_stride + col] = to;
-      if (to >= 0) a.copies[k] = make_int4(page, to, now % a.page, 0);
-      if (to < 0) {
-        ++missing;
-        a.ctx[r] = col * a.page;
-      }
+      const int to = k < left ? __ldcg(a.free_pages + left - 1 - k) : -1, col = (now - 1) / a.page;
+      atomicSub(a.shared + x.last, 1);
+      a.table[x.row * a.table_stride + col] = to;
+      if (to >= 0) a.copies[k] = make_int4(x.last, to, now % a.page, 0);
+      else ++missing;
     }
-    if (r >= 0 && !(copy && k >= left)) a.ctx[r] = now;
+    if (x.row >= 0) a.ctx[x.row] = copy && k >= left ? now / a.page * a.page : now;
     __syncthreads();
   }
   int all_missing;
@@ -304,8 +366,8 @@ using namespace kvr;
 
 extern "C" size_t kvr_paged_reorder_workspace_bytes(int groups, int beams, int table_width) {
   if (groups < 1 || beams < 1 || beams > kPrMaxBeams || table_width < 1) return 0;
-  const size_t n = (size_t)groups * beams;
-  return n * sizeof(int4) + 16 + n * ((table_width + 31) / 32) * sizeof(int);
+  const size_t n = (size_t)groups * beams, blocks = (table_width + 31) / 32;
+  return n * sizeof(int4) + 16 + (n * blocks + (size_t)groups * blocks * 32) * sizeof(int);
 }
 
 extern "C" int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int table_rows, int table_width,
@@ -350,14 +412,21 @@ extern "C" int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int
   a.copies = static_cast<int4 *>(workspace);
   a.n_copies = reinterpret_cast<int *>(a.copies + (size_t)groups * beams);
   a.counts = a.n_copies + 4;
+  a.given = reinterpret_cast<unsigned *>(a.counts + (size_t)groups * beams * ((table_width + 31) / 32));
   if (groups == 0) {
     const cudaError_t z = cudaMemsetAsync(info, 0, 16, as_cuda(stream));
     return z == cudaSuccess ? KVR_OK : set_error(KVR_ECUDA, "kvr_paged_reorder: %s", cudaGetErrorString(z));
   }
-  const size_t smem = (size_t)kPrWarps * beams * 32 * sizeof(int);
+  // entries of as many units as a row of the table can make, where they fit
+  const size_t places = (size_t)groups * beams * (sizeof(PrPlace) + sizeof(int)), unit = (size_t)kPrWarps * beams * 32 * sizeof(int);
+  const int64_t warps = kPrCluster * kPrWarps, most = ((int64_t)groups * ((table_width + 31) / 32) + warps - 1) / warps;
+  a.slots = (int)((kPrSmem - places) / unit);
+  if (a.slots > most) a.slots = (int)most;
+  static_assert((size_t)kPrMaxRows * (sizeof(PrPlace) + sizeof(int)) + (size_t)kPrWarps * 32 * kPrMaxBeams * sizeof(int) <= kPrSmem,
+                "a unit of a warp at least");
+  const size_t smem = places + a.slots * unit;
   if (smem > 40 * 1024) {
-    const cudaError_t s = cudaFuncSetAttribute(paged_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kPrWarps * kPrMaxBeams * 32 * (int)sizeof(int));
+    const cudaError_t s = cudaFuncSetAttribute(paged_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrSmem);
     if (s != cudaSuccess) return set_error(KVR_ECUDA, "kvr_paged_reorder: %s", cudaGetErrorString(s));
   }
   cudaError_t e = launch_dependent(paged_reorder_kernel, kPrCluster, kPrThreads, smem, as_cuda(stream), a);
