@@ -12,9 +12,10 @@
 // cluster of 8 CTAs; a warp takes 32 columns of a group, a column per lane:
 //   1  the column's pages: holders in the group before and after.  Where the group
 //      has all of a page's holders, its new count, or that it is free, is settled
-//      at once.  Counts of pages with holders outside go up and down by atomics;
-//   -  only if a group gave up such a page altogether: whether others did too, which
-//      the lowest place (row, column) then claims, by a minimum;
+//      at once.  Counts of pages with holders outside go up and down by atomics, with a
+//      mark, so that another group does not take what is left for all there was;
+//   -  only if there were such pages: the marks go, and a page without a holder is
+//      claimed by the lowest place (row, column) that gave it up, by a minimum;
 //   2  (after the cluster has met) free pages counted per row, their prefix sums, the
 //      pages to the end of the free list in order of rows and columns, new entries;
 //   3  (after it has met again; CTA 0, a thread per row) last pages: who copies, fresh
@@ -31,6 +32,8 @@ namespace kvr {
 constexpr int kPrCluster = 8, kPrThreads = 1024, kPrWarps = kPrThreads / 32;
 constexpr int kPrMaxBeams = 32, kPrMaxRows = 4096;
 constexpr int kPrStepTokens = 8;     // tokens that a warp copies at a time
+constexpr int kPrMark = 1 << 18;     // on counts of pages with holders outside of a group: above all counts
+constexpr int kPrMaxTable = 1 << 16; // rows of a table
 constexpr int kPrSmem = 216 * 1024;  // places of the rows, and entries of as many units as fit
 
 struct ReorderArgs {
@@ -99,7 +102,7 @@ __device__ __forceinline__ int pr_exclusive(int v, int *warp_sums, int &total) {
 }
 static_assert(kPrWarps == 32, "one sum per lane");
 
-__global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads) paged_reorder_kernel(ReorderArgs a) {
+__global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads, 1) paged_reorder_kernel(ReorderArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int warp_sums[32], longest, disputed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, n = a.groups * K;
@@ -125,24 +128,34 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads)
   if (lane == 0 && most > 0) atomicMax(&longest, most);
   __syncthreads();
   const int blocks = (longest + 31) / 32, units = a.groups * blocks, all_warps = kPrCluster * kPrWarps;
-  auto held = [&](int i) { return (place[i].len + a.page - 1) / a.page; };
-  auto entry = [&](int i, int j) {  // page of place i in column j before the call, -1: none
-    int e = -1;
-    if (j < held(i)) e = a.table[place[i].row * a.table_stride + j];
-    return e >= 0 && e < a.n_pages ? e : -1;
-  };
   // unit u of this warp: group, 32 columns.  CTA first, so that few units spread over the cluster's SMs
   const int me = warp * kPrCluster + (int)blockIdx.x;
   const bool kept = units <= all_warps * a.slots;  // all units' entries stay in shared memory
+  struct Place {
+    int row, parent, held;
+  };
+  auto place_of = [&](int u) {  // lane i: place i of the unit's group, and its pages
+    Place x{-1, -1, 0};
+    if (lane < K) {
+      const PrPlace p = place[u / blocks * K + lane];
+      x = Place{p.row, p.parent, (p.len + a.page - 1) / a.page};
+    }
+    return x;
+  };
   auto load = [&](int u, int nth, bool again) {
     int *old = entries + (warp * a.slots + (kept ? nth : 0)) * K * 32 + lane;
     if (kept && again) return old;
-    const int g = u / blocks, j = (u - g * blocks) * 32 + lane;
+    const int j = (u - u / blocks * blocks) * 32 + lane;
+    const Place x = place_of(u);
 #pragma unroll 8
-    for (int i = 0; i < K; ++i) old[i * 32] = entry(g * K + i, j);  // (a lane reads back only what it wrote)
+    for (int i = 0; i < K; ++i) {  // (a lane reads back only what it wrote)
+      const int r = __shfl_sync(0xffffffffu, x.row, i), h = __shfl_sync(0xffffffffu, x.held, i);
+      int e = -1;
+      if (j < h) e = a.table[r * a.table_stride + j];
+      old[i * 32] = e >= 0 && e < a.n_pages ? e : -1;
+    }
     return old;
   };
-  auto parent_of = [&](int u, int i) { return place[u / blocks * K + i].parent; };
   // places of entries; the claims lie below every count
   auto claim = [&](int u, int i) {
     const int g = u / blocks;
@@ -155,40 +168,54 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads)
       if (lane == 0) a.counts[(int64_t)(g * K + i) * blocks + u - g * blocks] = __popc(who);
     }
   };
-  // the page of place i, if it is the first of the group to hold it: holders before and after
-  auto holders = [&](const int *old, int u, int i, int &before, int &after) {
+  // Of the column's page at place i: whether the group's holders change and i is the first of them; how many they are.
+  // All lanes together (the parents come from the lanes).
+  auto changes = [&](const int *old, int parent, int i, int &before, int &after) {
     const int page = old[i * 32];
+    bool first = page >= 0;
     before = after = 0;
-    if (page < 0) return false;
+#pragma unroll 4
     for (int o = 0; o < K; ++o) {
-      if (old[o * 32] == page) {
-        if (o < i) return false;
-        ++before;
-      }
-      const int p = parent_of(u, o);
+      const bool same = old[o * 32] == page;
+      first &= !(same && o < i);
+      before += same;
+      const int p = __shfl_sync(0xffffffffu, parent, o);
       after += p >= 0 && old[p * 32] == page;
     }
-    return true;
+    return first && before != after;
   };
   for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
     const int *old = load(u, nth, false);
-    bool changed = false;
+    const int parent = place_of(u).parent;
+    bool differs = false;
     for (int i = 0; i < K; ++i) {
-      const int p = parent_of(u, i);
-      changed |= old[i * 32] != (p < 0 ? -1 : old[p * 32]);
+      const int p = __shfl_sync(0xffffffffu, parent, i);
+      differs |= old[i * 32] != (p < 0 ? -1 : old[p * 32]);
     }
     unsigned given = 0;
-    for (int i = 0; i < K && changed; ++i) {
-      int before, after;
-      if (!holders(old, u, i, before, after) || before == after) continue;
-      int *c = a.shared + old[i * 32];
-      if (__ldcg(c) < before) {  // (no holder but this group's)
-        *c = max(after - 1, 0);
-        if (after == 0) given |= 1u << i;
-      } else {
-        atomicAdd(c, after - before);
-        if (after == 0) disputed = 1;
+    if (__any_sync(0xffffffffu, differs)) {
+      for (int i0 = 0; i0 < K; i0 += 4) {  // four counts' loads at a time
+        int before[4], after[4], c[4];
+        bool is[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          is[q] = i0 + q < K && changes(old, parent, i0 + q, before[q], after[q]);
+          c[q] = is[q] ? __ldcg(a.shared + old[(i0 + q) * 32]) : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (!is[q]) continue;
+          int *to = a.shared + old[(i0 + q) * 32];
+          if (c[q] < before[q]) {  // (no holder but this group's)
+            *to = max(after[q] - 1, 0);
+            if (after[q] == 0) given |= 1u << (i0 + q);
+          } else {
+            atomicAdd(to, after[q] - before[q] + kPrMark);
+            disputed = 1;
+          }
+        }
       }
+      __syncwarp();
     }
     a.given[u * 32 + lane] = given;
     count(u, given);
@@ -198,38 +225,36 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads)
       const int p = place[i].parent;
       if (p < 0) continue;
       const int from = i / K * K + p, len = place[from].len;
-      if (len % a.page) place[i].last = entry(from, (len - 1) / a.page);
+      if (len % a.page == 0) continue;
+      const int page = a.table[place[from].row * a.table_stride + (len - 1) / a.page];
+      if (page >= 0 && page < a.n_pages) place[i].last = page;
     }
   cluster_sync();
   int any = 0;
   for (int c = 0; c < kPrCluster; ++c) any |= pr_peer(&disputed, c);
   if (any) {
-    for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
-      const int *old = load(u, nth, true);
-      for (int i = 0; i < K; ++i) {
-        int before, after;
-        if (!holders(old, u, i, before, after) || after > 0) continue;
-        int *c = a.shared + old[i * 32];
-        if (__ldcg(c) < 0) atomicMin(c, claim(u, i));
-      }
-    }
-    cluster_sync();
-    for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
-      const int *old = load(u, nth, true);
-      unsigned given = a.given[u * 32 + lane];
-      for (int i = 0; i < K; ++i) {
-        int before, after;
-        if (!holders(old, u, i, before, after) || after > 0) continue;
-        int *c = a.shared + old[i * 32];
-        if (__ldcg(c) == claim(u, i)) {
-          given |= 1u << i;
-          *c = 0;
+    // what the first pass did with atomics, again: pass 0 takes the marks off, 1 claims, 2 sees whose claim it was
+    for (int pass = 0; pass < 3; ++pass) {
+      for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
+        const int *old = load(u, nth, true);
+        const int parent = place_of(u).parent;
+        unsigned given = a.given[u * 32 + lane];
+        for (int i = 0; i < K; ++i) {
+          int before, after;
+          const bool is = changes(old, parent, i, before, after);
+          int *c = a.shared + max(old[i * 32], 0);
+          if (is && pass == 0 && __ldcg(c) >= kPrMark / 2) atomicSub(c, kPrMark);
+          if (is && pass == 1 && after == 0 && __ldcg(c) < 0) atomicMin(c, claim(u, i));
+          if (is && pass == 2 && after == 0 && __ldcg(c) == claim(u, i)) {
+            given |= 1u << i;
+            *c = 0;
+          }
         }
+        a.given[u * 32 + lane] = given;
+        if (pass == 2) count(u, given);
       }
-      a.given[u * 32 + lane] = given;
-      count(u, given);
+      cluster_sync();
     }
-    cluster_sync();
   }
   // pages given back by each row, and by those before it
   for (int i = warp; i < n; i += kPrWarps) {
@@ -256,20 +281,22 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads)
   for (int u = me, nth = 0; u < units; u += all_warps, ++nth) {
     const int *old = load(u, nth, true);
     const int g = u / blocks, b = u - g * blocks, j = b * 32 + lane;
+    const Place x = place_of(u);
     const unsigned given = a.given[u * 32 + lane], anyone = __reduce_or_sync(0xffffffffu, given);
     for (int i = 0; i < K; ++i) {
-      const int at_i = g * K + i;
       if ((anyone >> i) & 1) {
+        const int64_t at_i = g * K + i;
         int before = 0;  // the row's in columns before this unit's
-        for (int c = lane; c < b; c += 32) before += __ldcg(a.counts + (int64_t)at_i * blocks + c);
+        for (int c = lane; c < b; c += 32) before += __ldcg(a.counts + at_i * blocks + c);
         before = __reduce_add_sync(0xffffffffu, before);
         const unsigned who = __ballot_sync(0xffffffffu, (given >> i) & 1);
         const int64_t at = (int64_t)n_free + ahead[at_i] + before + __popc(who & ((1u << lane) - 1));
         if (((given >> i) & 1) && at < a.n_free_cap) a.free_pages[at] = old[i * 32];
       }
-      const int r = place[at_i].row, p = place[at_i].parent, gets = p < 0 ? -1 : old[p * 32];
-      if (r >= 0 && old[i * 32] != gets && j < max(held(at_i), p < 0 ? 0 : held(g * K + p)))
-        a.table[r * a.table_stride + j] = gets;
+      const int r = __shfl_sync(0xffffffffu, x.row, i), p = __shfl_sync(0xffffffffu, x.parent, i);
+      const int had_n = __shfl_sync(0xffffffffu, x.held, i), gets_n = __shfl_sync(0xffffffffu, x.held, max(p, 0));
+      const int gets = p < 0 ? -1 : old[p * 32];
+      if (r >= 0 && old[i * 32] != gets && j < max(had_n, p < 0 ? 0 : gets_n)) a.table[r * a.table_stride + j] = gets;
     }
   }
   cluster_sync();
@@ -384,6 +411,7 @@ extern "C" int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int
   KVR_REQUIRE(block_table && ctx_len && shared && (rows || !groups) && (parents || !groups) && workspace,
               "kvr_paged_reorder: null pointer");
   KVR_REQUIRE(page >= 1 && page <= (1 << 20), "kvr_paged_reorder: bad page size");
+  if (table_rows > kPrMaxTable) return set_error(KVR_ENOTSUP, "kvr_paged_reorder: at most %d table rows", kPrMaxTable);
   KVR_REQUIRE(table_rows >= 1 && table_width >= 1 && (table_stride >= table_width || table_rows == 1),
               "kvr_paged_reorder: bad block table shape");
   KVR_REQUIRE((int64_t)groups * beams * align_up(table_width, 32) < (1 << 30), "kvr_paged_reorder: the rows are too long");
