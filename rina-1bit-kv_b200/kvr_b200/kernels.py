@@ -580,6 +580,15 @@ def _on_gpu(*tensors):
             raise ValueError("kvr_b200 operators need CUDA tensors (this build has no CPU path)")
 
 
+def _on_current_gpu(*tensors):
+    """What a call reads and writes lies where its stream is."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != here:
+            raise ValueError(f"kvr_b200 operators need CUDA tensors on the current device (cuda:{here}; this build has no CPU "
+                             f"path), got one on {t.device}")
+
+
 def _table(block_table, batch):
     """Checks a block table with a row for each of `batch` requests; returns its
     width and row stride."""
@@ -879,7 +888,7 @@ def beam_select(logits, scores, n=None, eos=()):
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
     scores = _c(scores)
-    _on_gpu(logits, scores)
+    _on_current_gpu(logits, scores)
     code, dev = dtype_code(logits), logits.device
     eos = tuple(eos)
     ends = _EOS.get(eos)
@@ -918,14 +927,18 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
     every child but the first, in the pools k_pages and v_pages ([layers,] n_pages, page,
     n_kv, d).  Returns info (4) int32 = [pages missing, copied, given back, 0]; a row that finds no page keeps
     its full pages."""
-    if k_pages.dim() == 5:
-        layers, ls = k_pages.shape[0], k_pages.stride(0)
-        one_k, one_v = k_pages[0], v_pages[0] if v_pages.dim() == 5 else v_pages
-        if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
-            raise ValueError("k_pages and v_pages must have one shape, type and layout")
-    else:
-        layers, ls, one_k, one_v = 1, 0, k_pages, v_pages
-    n_pages, page, ps, ts = _pool(one_k, one_v)
+    shape, strides = k_pages.shape, k_pages.stride()
+    layers, ls = 1, 0
+    if len(shape) == 5:
+        layers, ls, shape, strides = shape[0], strides[0], shape[1:], strides[1:]
+    if len(shape) != 4 or shape[3] != D or layers < 1:
+        raise ValueError(f"k_pages must be ([layers,] pages, page, heads, {D}), got {tuple(k_pages.shape)}")
+    if strides[3] != 1 or (shape[2] > 1 and strides[2] != D):
+        raise ValueError("k_pages: a token's heads must be contiguous")
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.stride() != k_pages.stride():
+        raise ValueError("k_pages and v_pages must have one shape, type and layout")
+    n_pages, page, n_kv, _ = shape
+    ps, ts = strides[0], strides[1]
     _i32(shared, "shared", n_pages)
     cap = _i32(free_pages, "free_pages")
     _i32(n_free, "n_free", 1)
@@ -937,7 +950,7 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
     if beams < 1:
         raise ValueError("a group needs at least one row")
     rows, parents = _c(rows), _c(parents)
-    _on_gpu(block_table, ctx_len, shared, free_pages, n_free, rows, parents, k_pages, v_pages)
+    _on_current_gpu(block_table, ctx_len, shared, free_pages, n_free, rows, parents, k_pages, v_pages)
     dev = rows.device
     key = (groups, beams, width)
     need = _REORDER_WS.get(key)
@@ -949,7 +962,7 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
     info = torch.empty(4, dtype=_INT32, device=dev)
     call("kvr_paged_reorder", block_table.data_ptr(), stride, n_rows, width, ctx_len.data_ptr(), page, shared.data_ptr(),
          n_pages, free_pages.data_ptr(), cap, n_free.data_ptr(), rows.data_ptr(), parents.data_ptr(), groups, beams,
-         k_pages.data_ptr(), v_pages.data_ptr(), dtype_code(k_pages), layers, one_k.shape[2], D, ls, ps, ts, info.data_ptr(),
+         k_pages.data_ptr(), v_pages.data_ptr(), dtype_code(k_pages), layers, n_kv, D, ls, ps, ts, info.data_ptr(),
          ws.data_ptr(), need, stream())
     return info
 
@@ -1011,7 +1024,7 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         out = torch.empty(n_tokens, hidden, dtype=dt, device=x.device)
     elif out.shape != (n_tokens, hidden) or out.dtype is not dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and of x's shape and dtype")
-    _on_gpu(x, router, gate_up, down, out)
+    _on_current_gpu(x, router, gate_up, down, out)
     dev = x.device
     key = (n_tokens, hidden, inter, experts, top_k)
     need = _MOE_WS.get(key)

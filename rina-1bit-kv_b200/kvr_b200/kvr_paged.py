@@ -13,7 +13,9 @@ order:
     cache.commit()                              # the new tokens count as cached
 
 Nothing reads a length on the host, so a step of fixed n_tokens can be captured
-in a CUDA graph.
+in a CUDA graph.  Between steps ``cache.reorder(rows, parents)`` makes rows the
+continuations of others (beams of one request, samples of one prompt): they share
+full pages.
 """
 import torch
 
@@ -41,6 +43,8 @@ class PagedKVCache:
         self._free = torch.arange(n_pages - 1, -2, -1, **i32)
         self.free_pages = self._free[:n_pages]
         self.n_free = torch.full((1,), n_pages, **i32)
+        self.shared = torch.zeros(n_pages, **i32)  # rows that hold a page, beyond the first
+        self._sharing = False
         self.lost = torch.zeros(4, **i32)  # what committed steps had no room for, as their info counts it
         self.step = None
 
@@ -101,6 +105,37 @@ class PagedKVCache:
             raise RuntimeError(f"{'committed steps did' if self.step is None else 'step does'} not fit: {missing} pages missing, "
                                f"{cut} requests cut at n_tokens, {over} longer than max_len")
 
+    def reorder(self, rows, parents):
+        """Between steps: rows rows[g][i] become the continuations of rows
+        rows[g][parents[g][i]] of their group (a parent of -1: the row is emptied).
+        Lists, checked here, or int32 tensors (groups, beams) on the device, which
+        must not name a row twice.  Returns kernels.paged_reorder's info; a row that
+        finds no page for its copy of a last page that is not full keeps the full
+        ones, and `check` says so."""
+        if self.step is not None:
+            raise RuntimeError("commit() the open step first")
+        dev = self.ctx_len.device
+        if not torch.is_tensor(rows):
+            rows = [[int(b) for b in g] for g in rows]
+            flat = [b for g in rows for b in g]
+            if len({len(g) for g in rows}) > 1 or not flat:
+                raise ValueError("groups must have one number of rows, one at least")
+            if len(set(flat)) < len(flat):
+                raise ValueError("a row is named twice")
+            if not all(0 <= b < self.max_requests for b in flat):
+                raise ValueError(f"rows must be in [0, {self.max_requests}), got {rows}")
+            rows = torch.tensor(rows, dtype=torch.int32, device=dev)
+        if not torch.is_tensor(parents):
+            parents = [[int(p) for p in g] for g in parents]
+            if any(not -1 <= p < rows.shape[1] for g in parents for p in g):
+                raise ValueError(f"parents must be places of the group, or -1, got {parents}")
+            parents = torch.tensor(parents, dtype=torch.int32, device=dev)
+        info = K.paged_reorder(self.block_table, self.ctx_len, self.shared, self.free_pages, self.n_free, rows, parents,
+                               self.k, self.v)
+        self._sharing = True
+        self.lost[:1] += info[:1]
+        return info
+
     def release(self, requests):
         """Gives the pages of `requests` (a list of rows; one named twice counts
         once) back to the free list and empties the rows; between steps only."""
@@ -109,6 +144,9 @@ class PagedKVCache:
         rows = list(dict.fromkeys(int(b) for b in requests))
         if not all(0 <= b < self.max_requests for b in rows):
             raise ValueError(f"rows must be in [0, {self.max_requests}), got {rows}")
+        if self._sharing and rows:  # pages that other rows hold too stay theirs
+            self.reorder([[b] for b in rows], [[-1]] * len(rows))
+            return
         rows = torch.tensor(rows, dtype=torch.int64, device=self.ctx_len.device)
         held = (self.ctx_len[rows] + self.page - 1) // self.page
         j = torch.arange(self.block_table.shape[1], device=rows.device)
@@ -125,7 +163,7 @@ class PagedKVCache:
                 f"requests={self.max_requests})")
 
 
-_MODELS = ("llama", "mistral", "qwen2", "qwen3")     # whose decoder layer `PagedGenerator._layers` is
+_MODELS = ("llama", "mistral", "qwen2", "qwen3", "qwen3_moe")  # whose decoder layer `PagedGenerator._layers` is
 _ROPE = ("default", "linear", "llama3", "yarn")        # one table for sequences of every length
 _PARTS = {"q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm", "rotary_emb"}
 
@@ -141,6 +179,8 @@ def _model_window(model, max_len):
     if kind not in _ROPE:
         raise NotImplementedError(f"RoPE of type {kind} (its angles may depend on a sequence's length)")
     for layer in model.model.layers:
+        if _sparse(layer.mlp) and cfg.hidden_act != "silu":
+            raise NotImplementedError(f"experts with {cfg.hidden_act}")
         more = {n for n, _ in layer.self_attn.named_children()} - _PARTS
         if more:
             raise NotImplementedError(f"attention with {', '.join(sorted(more))}")
@@ -157,16 +197,35 @@ def _model_window(model, max_len):
     return window
 
 
+def _sparse(mlp):
+    """Whether a decoder layer's MLP is a router and experts that kernels.moe_layer
+    computes; raises NotImplementedError for one that has other parts."""
+    if not hasattr(mlp, "experts"):
+        return False
+    more = {n for n, _ in mlp.named_children()} - {"gate", "experts"}
+    if more:
+        raise NotImplementedError(f"a sparse MLP with {', '.join(sorted(more))}")
+    gate, experts = mlp.gate, mlp.experts
+    names = {n for n, _ in experts.named_parameters()} | {f"gate.{n}" for n, _ in gate.named_parameters()}
+    if names != {"gate_up_proj", "down_proj", "gate.weight"} or not hasattr(gate, "top_k"):
+        raise NotImplementedError(f"a sparse MLP of {', '.join(sorted(names))}")
+    e, h = gate.weight.shape
+    if experts.gate_up_proj.shape[::2] != (e, h) or experts.down_proj.shape[:2] != (e, h):
+        raise NotImplementedError("experts whose weights are laid out otherwise")
+    return True
+
+
 class PagedGenerator:
-    """Many requests on one HF decoder model (Llama, Mistral, Qwen2 or Qwen3 of
-    head_dim 128, fp16 or bf16) with an exact paged cache.
+    """Many requests on one HF decoder model (Llama, Mistral, Qwen2 or Qwen3, dense or
+    with sparse MLPs, of head_dim 128, fp16 or bf16) with an exact paged cache.
 
         gen = PagedGenerator(model, n_pages=4096, max_requests=32)
         rows = gen.add([prompt_a, prompt_b])          # prompts in chunks of `chunk` tokens
         tokens = gen.generate(rows, max_new_tokens=64)
         gen.drop(rows)                                # their pages are free again
 
-    A step takes any mix of chunks and single tokens (``step``); ``score``
+    ``beam_search`` continues prompts by beams, which share the pages of what they
+    have in common.  A step takes any mix of chunks and single tokens (``step``); ``score``
     gives the logits of whole packed prompts without a cache.  window: a query
     sees the last `window` tokens only (0: as many as the model's own sliding
     window, or all); a model's own window bounds it."""
@@ -198,8 +257,21 @@ class PagedGenerator:
             if hasattr(at, "q_norm"):  # over the channels of each head
                 q, k = at.q_norm(q), at.k_norm(k)
             h = h + at.o_proj(attend(li, q, k, v).reshape(x.shape[0], -1))
-            h = h + layer.mlp(layer.post_attention_layernorm(h))
+            h = h + self._mlp(layer.mlp, layer.post_attention_layernorm(h))
         return self.model.model.norm(h)
+
+    @staticmethod
+    def _mlp(mlp, x):
+        """A layer's MLP over packed rows: a sparse one of a few tokens in one call,
+        of more by the model's own module."""
+        if not hasattr(mlp, "experts"):
+            return mlp(x)
+        experts = mlp.experts
+        if x.shape[0] <= K.MOE_MAX_TOKENS and x.shape[1] % 8 == 0 and experts.down_proj.shape[2] % 8 == 0:
+            return K.moe_layer(x, mlp.gate.weight, experts.gate_up_proj, experts.down_proj, mlp.gate.top_k,
+                               norm_topk=bool(getattr(mlp.gate, "norm_topk_prob", True)))
+        y = mlp(x[None])
+        return (y[0] if isinstance(y, tuple) else y)[0]
 
     @torch.no_grad()
     def step(self, new):
@@ -259,6 +331,75 @@ class PagedGenerator:
                 out[b].append(int(self.last[b].argmax()))
             self.step({b: out[b][-1:] for b in rows})
         return out
+
+    @torch.no_grad()
+    def beam_search(self, prompts, n_beams, max_new_tokens, eos=(), length_penalty=1.0):
+        """Continues each prompt by beam search over n_beams beams; returns for each
+        prompt its best continuations, at most n_beams, best first, as (tokens, score):
+        score is the sum of the tokens' log-probabilities over their number to the
+        power of length_penalty.  eos: a token id, or several, that end a sequence.  A
+        prompt is done when it has n_beams ended sequences that its beams, at their
+        present length, do not beat.  It takes n_beams free rows a prompt, and gives
+        them back."""
+        eos = (eos,) if isinstance(eos, int) else tuple(eos)
+        prompts = [list(p) for p in prompts]
+        if n_beams < 1 or max_new_tokens < 1:
+            raise ValueError("n_beams and max_new_tokens must be 1 at least")
+        free = [b for b in range(self.cache.max_requests) if b not in self.last]
+        if len(free) < n_beams * len(prompts):
+            raise RuntimeError(f"{len(prompts)} prompts of {n_beams} beams for {len(free)} free rows")
+        if not prompts:
+            return []
+        first = self.add(prompts)
+        rest = iter(b for b in free if b not in first)
+        rows = [[b] + [next(rest) for _ in range(n_beams - 1)] for b in first]
+        try:
+            return self._beams(rows, max_new_tokens, eos, length_penalty)
+        finally:
+            self.drop([b for g in rows for b in g])
+
+    def _reorder(self, rows, parents):
+        self.cache.reorder(rows, parents)
+        self.cache.check()  # a beam without a page for its copy would go on from a shorter text
+
+    def _beams(self, rows, max_new_tokens, eos, length_penalty):
+        n, k = len(rows), len(rows[0])
+        logits = torch.stack([self.last[g[0]] for g in rows])[:, None].expand(n, k, -1)  # all beams see the prompt's
+        scores = torch.full((n, k), -float("inf"), device=self.device)
+        scores[:, 0] = 0.0
+        self._reorder(rows, [[0] * k] * n)
+        seqs = [[[] for _ in range(k)] for _ in range(n)]
+        ended = [[] for _ in range(n)]  # (score, tokens)
+        live = set(range(n))
+        for t in range(1, max_new_tokens + 1):
+            st = K.beam_select(logits, scores, eos=eos)
+            cand = [x.tolist() for x in (st.scores, st.beams, st.tokens)]
+            nexts = [x.tolist() for x in (st.next_scores, st.next_beams, st.next_tokens)]
+            for g in list(live):
+                for s, b, tok in list(zip(cand[0][g], cand[1][g], cand[2][g]))[:k]:
+                    if b >= 0 and tok in eos:
+                        ended[g].append((s / t ** length_penalty, seqs[g][b] + [tok]))
+                ended[g] = sorted(ended[g], key=lambda e: -e[0])[:k]
+                seqs[g] = [seqs[g][b] + [tok] if b >= 0 else [] for b, tok in zip(nexts[1][g], nexts[2][g])]
+                best = max(nexts[0][g])
+                if best == -float("inf") or (len(ended[g]) == k and ended[g][-1][0] >= best / t ** length_penalty):
+                    live.discard(g)
+                    if len(ended[g]) == k:
+                        nexts[0][g] = [-float("inf")] * k
+            if not live or t == max_new_tokens:
+                break
+            scores = st.next_scores
+            self._reorder(rows, [nexts[1][g] if g in live else [-1] * k for g in range(n)])
+            out = self.step({rows[g][i]: [nexts[2][g][i]] for g in sorted(live) for i in range(k) if nexts[1][g][i] >= 0})
+            empty = next(iter(out.values()))  # (of beams that there are not: their scores are -inf)
+            logits = torch.stack([out.get(b, empty) for g in rows for b in g])
+            if len(live) < n:
+                scores = scores.clone()
+                scores[[g for g in range(n) if g not in live]] = -float("inf")
+        for g in range(n):  # beams that have not ended, as they are
+            ended[g] += [(s / max(len(q), 1) ** length_penalty, q) for s, q in zip(nexts[0][g], seqs[g]) if s > -float("inf")]
+            ended[g] = sorted(ended[g], key=lambda e: -e[0])[:k]
+        return [[(q, s) for s, q in e] for e in ended]
 
     def drop(self, rows):
         """Ends requests: their pages and rows are free again."""
