@@ -365,6 +365,9 @@ __global__ void __launch_bounds__(kMoThreads, 1)
                  "r"(kMoTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (tid == 32) {
+    for (const CUtensorMap *m : {&mx, &mw1, &mh, &mw2}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
   if (tid == 0) {
     s.abort_s = 0;
     for (int i = 0; i < a.stages; ++i) {
@@ -924,11 +927,16 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
               "kvr_moe_layer: pointers must be 16-byte aligned, the workspace 256-byte");
   KVR_REQUIRE(workspace_bytes >= kvr_moe_workspace_bytes(n_tokens, hidden, inter, experts, top_k),
               "kvr_moe_layer: workspace too small");
-  {  // rows of y are stored while other CTAs still read x
-    const uintptr_t p = reinterpret_cast<uintptr_t>(x), q = reinterpret_cast<uintptr_t>(y);
-    const uintptr_t n = ((n_tokens - 1) * x_stride + hidden) * 2, m = n_tokens * (uintptr_t)hidden * 2;
-    KVR_REQUIRE(p + n <= q || q + m <= p, "kvr_moe_layer: y must not lie in x");
-  }
+  // rows of y are stored while other CTAs still read
+  auto meets = [&](const void *in, int64_t elements) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(in), q = reinterpret_cast<uintptr_t>(y);
+    return p < q + (uintptr_t)n_tokens * hidden * 2 && q < p + (uintptr_t)elements * 2;
+  };
+  KVR_REQUIRE(!meets(x, (n_tokens - 1) * x_stride + hidden), "kvr_moe_layer: y must not lie in x");
+  KVR_REQUIRE(!meets(router, (experts - 1) * router_stride + hidden) &&
+                  !meets(gate_up, (experts - 1) * gu_expert_stride + (2 * (int64_t)inter - 1) * gu_row_stride + hidden) &&
+                  !meets(down, (experts - 1) * down_expert_stride + (hidden - 1) * down_row_stride + inter),
+              "kvr_moe_layer: y must not lie in the weights");
   if (!encode_tiled()) return set_error(KVR_ECUDA, "kvr_moe_layer: the driver has no cuTensorMapEncodeTiled");
   bind_context();
   const MoeCut c = moe_cut(n_tokens, hidden, inter, experts, top_k);

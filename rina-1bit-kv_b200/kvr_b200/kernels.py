@@ -895,6 +895,8 @@ def beam_select(logits, scores, n=None, eos=()):
     if ends is None:
         if len(_EOS) > 256:
             _EOS.clear()
+        if not all(0 <= t < 1 << 31 for t in eos):
+            raise ValueError(f"eos must be token ids, got {eos}")
         ends = _EOS[eos] = (C.c_int32 * max(len(eos), 1))(*eos)
     key = (batch, beams, vocab, code, n)
     need = _BEAM_WS.get(key)

@@ -210,7 +210,8 @@ def _sparse(mlp):
     if names != {"gate_up_proj", "down_proj", "gate.weight"} or not hasattr(gate, "top_k"):
         raise NotImplementedError(f"a sparse MLP of {', '.join(sorted(names))}")
     e, h = gate.weight.shape
-    if experts.gate_up_proj.shape[::2] != (e, h) or experts.down_proj.shape[:2] != (e, h):
+    if (experts.gate_up_proj.shape[::2] != (e, h) or experts.down_proj.shape[:2] != (e, h)
+            or getattr(experts, "is_transposed", False) or not getattr(experts, "has_gate", True)):
         raise NotImplementedError("experts whose weights are laid out otherwise")
     return True
 

@@ -55,7 +55,8 @@ def test_select_hands_on_strides_and_ends(native):
 def test_select_refusals(native):
     from kvr_b200 import kernels as K
     x, s = torch.zeros(6, 50), torch.zeros(2, 3)
-    for bad in (dict(logits=x[:5]), dict(scores=torch.zeros(6)), dict(n=2), dict(logits=x[:, :0]), dict(logits=torch.zeros(50))):
+    for bad in (dict(logits=x[:5]), dict(scores=torch.zeros(6)), dict(n=2), dict(logits=x[:, :0]), dict(logits=torch.zeros(50)),
+                dict(eos=(1 << 31,)), dict(eos=[-1])):
         with pytest.raises(ValueError):
             K.beam_select(**{"logits": x, "scores": s, **bad})
     with pytest.raises(TypeError):
@@ -223,8 +224,8 @@ def moe_call(**kw):
 @pytest.mark.parametrize("kw,match", [
     (dict(T=129), "at most"), (dict(E=513), "at most"), (dict(E=32, k=17), "at most"), (dict(k=5), "shape"), (dict(k=0), "shape"),
     (dict(dtype=0), "fp16"), (dict(H=60, xs=64), "multiples of 8"), (dict(I=20), "multiples of 8"), (dict(x=None), "null"), (dict(status=None), "null"),
-    (dict(xs=32), "share"), (dict(ge=47 * 64), "share"), (dict(dr=16), "share"), (dict(xs=68), "aligned"), (dict(down=PTR + 8), "aligned"),
-    (dict(ws=PTR + 16), "aligned"), (dict(ws_bytes=64), "workspace"), (dict(y=PTR + 64), "lie in x"), (dict(H=1 << 17, xs=1 << 17, rs=1 << 17,
+    (dict(xs=32), "share"), (dict(ge=40 * 64), "share"), (dict(dr=16), "share"), (dict(xs=68), "aligned"), (dict(down=PTR + 8), "aligned"),
+    (dict(ws=PTR + 16), "aligned"), (dict(ws_bytes=64), "workspace"), (dict(y=PTR + 64), "lie in x"), (dict(y=1 << 20, gu=(1 << 20) - 512), "weights"), (dict(y=1 << 20, router=(1 << 20) + 128), "weights"), (dict(H=1 << 17, xs=1 << 17, rs=1 << 17,
                                                                                                               gr=1 << 17, ge=1 << 24), "too large")])
 def test_moe_c_refusals(kw, match):
     from kvr_b200._native import KvrError
