@@ -904,15 +904,20 @@ def beam_select(logits, scores, n=None, eos=()):
         if len(_BEAM_WS) > 4096:
             _BEAM_WS.clear()
         need = _BEAM_WS[key] = call("kvr_beam_select_workspace_bytes", *key)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    # outputs and workspace in one allocation, in this order: scores, next_scores, beams, tokens, next_beams, next_tokens
+    m, k = batch * n, batch * beams
+    at = (3 * (m + k) + 3) // 4 * 4
+    buf = torch.empty(at + need // 4, dtype=_INT32, device=dev)
     st = BeamStep()
-    f32, i32 = dict(dtype=torch.float32, device=dev), dict(dtype=_INT32, device=dev)
-    st.scores, st.next_scores = torch.empty(batch, n, **f32), torch.empty(batch, beams, **f32)
-    st.beams, st.tokens = torch.empty(batch, n, **i32), torch.empty(batch, n, **i32)
-    st.next_beams, st.next_tokens = torch.empty(batch, beams, **i32), torch.empty(batch, beams, **i32)
+    f, listed, kept = buf.view(torch.float32), (n, 1), (beams, 1)
+    st.scores, st.next_scores = f.as_strided((batch, n), listed, 0), f.as_strided((batch, beams), kept, m)
+    st.beams, st.tokens = buf.as_strided((batch, n), listed, m + k), buf.as_strided((batch, n), listed, 2 * m + k)
+    st.next_beams = buf.as_strided((batch, beams), kept, 3 * m + k)
+    st.next_tokens = buf.as_strided((batch, beams), kept, 3 * m + 2 * k)
+    p = buf.data_ptr()
     call("kvr_beam_select", logits.data_ptr(), code, logits.stride(0), batch, beams, vocab, scores.data_ptr(), n, ends,
-         len(eos), st.scores.data_ptr(), st.beams.data_ptr(), st.tokens.data_ptr(), st.next_scores.data_ptr(),
-         st.next_beams.data_ptr(), st.next_tokens.data_ptr(), ws.data_ptr(), need, stream())
+         len(eos), p, p + 4 * (m + k), p + 4 * (2 * m + k), p + 4 * m, p + 4 * (3 * m + k), p + 4 * (3 * m + 2 * k),
+         p + 4 * at, need, stream())
     return st
 
 
@@ -1034,13 +1039,18 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         if len(_MOE_WS) > 4096:
             _MOE_WS.clear()
         need = _MOE_WS[key] = call("kvr_moe_workspace_bytes", *key)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    ids = torch.empty(n_tokens, top_k, dtype=_INT32, device=dev)
-    weights = torch.empty(n_tokens, top_k, dtype=torch.float32, device=dev)
+    # workspace (256-byte aligned, as allocations are), then ids and weights
+    picks, at = n_tokens * top_k, (need + 3) // 4
+    buf = torch.empty(at + 2 * picks, dtype=_INT32, device=dev)
+    p = buf.data_ptr()
     call("kvr_moe_layer", x.data_ptr(), dtype_code(x), n_tokens, hidden, xs, router.data_ptr(), rs, gate_up.data_ptr(), ge, gr,
-         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), ids.data_ptr(),
-         weights.data_ptr(), ws.data_ptr(), need, _moe_status(dev).data_ptr(), stream())
-    return (out, ids, weights) if return_routing else out
+         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), p + 4 * at, p + 4 * (at + picks),
+         p, need, _moe_status(dev).data_ptr(), stream())
+    if not return_routing:
+        return out
+    one = (top_k, 1)
+    return (out, buf.as_strided((n_tokens, top_k), one, at),
+            buf.view(torch.float32).as_strided((n_tokens, top_k), one, at + picks))
 
 
 def moe_status(device=None):
