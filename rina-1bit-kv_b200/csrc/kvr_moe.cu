@@ -97,13 +97,15 @@ __device__ __forceinline__ void mo_widen(const uint4 &u, float (&x)[8]) {
   }
 }
 
-// NT tokens a cluster: as few as the SMs have clusters for, since a CTA's time is its tokens' products.
+// NT tokens a cluster: as few as the SMs have clusters for, since a CTA's time is its tokens' products.  (From four on,
+// registers for two CTAs an SM: 16 clusters of 8 do not fit the GPCs one CTA an SM, and the last one came 13 us late.)
 template <int DT, int NT>
-__global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads, 1) moe_route_kernel(RouteArgs a) {
-  constexpr int kWarps = kMrThreads / 32, kEach = kMoMaxExperts / 32;
+__global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads, NT < 4 ? 1 : 2) moe_route_kernel(RouteArgs a) {
+  constexpr int kWarps = kMrThreads / 32;
   __shared__ double part[NT][kMoMaxExperts / kMrCluster];  // logits of this CTA's experts
   __shared__ double slice[kWarps][NT][kMrExperts];         // of a warp's channels
   __shared__ double all_s[kMoMaxExperts];                  // of this CTA's token
+  __shared__ __align__(16) uint64_t key_s[kMoMaxExperts];
   __shared__ int chosen[kMoMaxTopK];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = blockIdx.x % kMrCluster, t0 = blockIdx.x / kMrCluster * NT;
@@ -145,18 +147,36 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
           for (int j = 0; j < 8; ++j) s[t][e] = fmaf(xf[j], wf[e][j], s[t][e]);
       }
     }
+    // The lanes' sums, in 64 bits: at each step a lane hands half of its values on and adds up the other half, so that
+    // in the end it has one (or, of the last steps, all lanes the same).
+    constexpr int kValues = NT * kMrExperts;
+    double v[kValues];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < kMrExperts; ++e) {
-        double d = s[t][e];
+      for (int e = 0; e < kMrExperts; ++e) v[t * kMrExperts + e] = s[t][e];
+    int which = 0, n = kValues;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        if (lane == 0) {
-          if (parts > 1) slice[warp][t][e] = d;
-          else if (g * kMrExperts + e < n_exp) part[t][g * kMrExperts + e] = d;
-        }
+    for (int o = 16; o > 0; o >>= 1) {
+      const bool upper = lane & o;
+      if (n > 1) {
+        n >>= 1;
+        which = which * 2 + upper;
+#pragma unroll
+        for (int j = 0; j < kValues / 2; ++j)
+          if (j < n) {
+            const double send = upper ? v[j] : v[j + n];
+            v[j] = (upper ? v[j + n] : v[j]) + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
       }
+    }
+    if ((lane & (32 / kValues - 1)) == 0) {
+      const int t = which / kMrExperts, e = which % kMrExperts;
+      if (parts > 1) slice[warp][t][e] = v[0];
+      else if (g * kMrExperts + e < n_exp) part[t][g * kMrExperts + e] = v[0];
+    }
   }
   if (parts > 1) {  // in the order of the channels
     __syncthreads();
@@ -168,35 +188,27 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
     }
   }
   mo_cluster_sync();
-  // CTA r: token r.  Lane l of its first warp holds experts l, l + 32, ...
+  // CTA r: token r.  An expert's rank is the number of those above it: larger logits, lower experts among equal ones.
   if (rank < n_tok) {
-    for (int e = threadIdx.x; e < a.experts; e += kMrThreads) all_s[e] = mo_peer_double(&part[rank][e % per], e / per);
+    const int even = (a.experts + 1) / 2 * 2;
+    for (int e = threadIdx.x; e < even; e += kMrThreads) {
+      const double z = e < a.experts ? mo_peer_double(&part[rank][e % per], e / per) : 0.0;
+      all_s[e] = z;
+      key_s[e] = e < a.experts ? mo_key(z) : 0;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += kMrThreads) {
+      const uint64_t mine = key_s[e];
+      int above = 0;
+#pragma unroll 4
+      for (int o = 0; o < even; o += 2) {
+        const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&key_s[o]);
+        above += (k.x > mine || (k.x == mine && o < e)) + (k.y > mine || (k.y == mine && o + 1 < e));
+      }
+      if (above < a.top_k) chosen[above] = e;
+    }
     __syncthreads();
     if (warp == 0) {
-      uint64_t key[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) key[i] = i * 32 + lane < a.experts ? mo_key(all_s[i * 32 + lane]) : 0;
-      for (int k = 0; k < a.top_k; ++k) {  // the largest key left, the lowest expert among equal ones
-        uint64_t best = key[0];
-        int at = lane;
-#pragma unroll
-        for (int i = 1; i < kEach; ++i) {
-          if (i * 32 >= a.experts) break;
-          if (key[i] > best) {
-            best = key[i];
-            at = i * 32 + lane;
-          }
-        }
-        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
-        const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
-        const bool top = (unsigned)(best >> 32) == hi && (unsigned)best == lo;
-        const int e = (int)__reduce_min_sync(0xffffffffu, top ? (unsigned)at : 0xffffffffu);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-          if (e == i * 32 + lane) key[i] = 0;
-        if (lane == 0) chosen[k] = e;
-      }
-      __syncwarp();
       const double m = all_s[chosen[0]];  // (a NaN only where all are)
       float all = 0.0f;
       for (int e = lane; e < a.experts; e += 32) all += expf((float)(all_s[e] - m));
