@@ -41,7 +41,8 @@ def check_select(logits, cum, n=None, eos=(), given=None):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("B,k,V,pad", [(1, 1, 1, 0), (1, 4, 32000, 0), (3, 5, 50257, 0), (2, 3, 1009, 7), (1, 32, 2049, 1),
-                                       (7, 2, 7, 1), (40, 8, 4100, 0), (1, 1, 200001, 0)])
+                                       (7, 2, 7, 1), (40, 8, 4100, 0), (1, 1, 200001, 0),
+                                       (700, 1, 300, 0), (3, 31, 16, 3)])
 def test_select(dtype, B, k, V, pad):
     g = torch.Generator(device=DEV).manual_seed(V + k)
     wide = (3 * torch.randn(B * k, V + pad, device=DEV, generator=g)).to(DT[dtype])
@@ -222,6 +223,15 @@ def test_reorder_without_pages(spare):
     page = 16
     w = check_reorder(make_cache(1, 4, [[100, 0, 0, 0]], page, 5, spare=spare), np.zeros((1, 4), int), page)
     assert w["info"][0] == 3 - spare
+
+
+@pytest.mark.parametrize("groups,beams", [(128, 32), (4096, 1), (819, 5)])
+def test_reorder_most_rows(groups, beams):
+    page = 8
+    rng = np.random.default_rng(groups)
+    lens = [[int(rng.integers(0, 5 * page))] * beams for _ in range(groups)]
+    cache = make_cache(groups, beams, lens, page, groups, spare=groups * beams // 2, n_kv=1, layers=1)
+    check_reorder(cache, rng.integers(-1, beams, (groups, beams)), page)
 
 
 @pytest.mark.parametrize("beams", [3, 8])

@@ -193,3 +193,108 @@ def test_beam_search_without_pages_gives_all_back():
     assert gen.cache.n_free.item() == 8 and not gen.last and gen.cache.ctx_len.eq(0).all()
     gen.cache.check()  # (what was lost has been told)
     assert len(gen.beam_search(prompts_of([30]), 2, 3)[0]) == 2
+
+
+class Step:
+    """A decode step of two requests of three beams as one chain on the device: pages, writes, attention, a sparse MLP,
+    logits, selection, reordering.  Nothing is read on the host, so it can be captured."""
+
+    G, K, H, LAYERS = 2, 3, 256, 2
+
+    def __init__(self):
+        from kvr_b200 import PagedKVCache
+        g = torch.Generator(device=DEV).manual_seed(1)
+        n = lambda *s: (torch.randn(*s, device=DEV, generator=g) / s[-1] ** 0.5).half()  # noqa: E731
+        self.emb = n(500, self.H) * 16
+        self.o = [n(self.H, 4 * 128) for _ in range(self.LAYERS)]
+        self.moe = [(n(10, self.H) * 2, n(10, 2 * 72, self.H), n(10, self.H, 72)) for _ in range(self.LAYERS)]
+        self.qkv = [n(8 * 128, self.H) for _ in range(self.LAYERS)]
+        a = torch.outer(torch.arange(256, device=DEV).float(), 10000.0 ** (-torch.arange(0, 128, 2, device=DEV).float() / 128))
+        self.cos, self.sin = torch.cat([a.cos()] * 2, 1), torch.cat([a.sin()] * 2, 1)
+        self.cache = PagedKVCache(self.LAYERS, 4, 2, 80, page=8, max_requests=self.G * self.K, max_len=256, dtype=torch.float16)
+        i32 = dict(dtype=torch.int32, device=DEV)
+        self.rows = torch.tensor([[4, 0, 2], [1, 5, 3]], **i32)
+        self.new = torch.ones(self.G * self.K, **i32)
+        self.tokens = torch.tensor([[7] * 3, [9] * 3], **i32)   # by beam
+        self.scores = torch.tensor([[0.0] + [-float("inf")] * 2] * 2, device=DEV)
+        self.by_row = torch.empty(self.G * self.K, **i32)
+
+    def __call__(self):
+        from kvr_b200 import kernels as K
+        c = self.cache
+        # (a beam without a token goes on with token 0: its score keeps it out)
+        self.by_row[self.rows.view(-1).long()] = self.tokens.clamp(min=0).view(-1)
+        h = self.emb[self.by_row.long()]
+        c.begin(self.new, self.G * self.K)
+        for i in range(self.LAYERS):
+            q, k, v = (h @ self.qkv[i].t()).view(-1, 8, 128).split([4, 2, 2], 1)
+            q = c.write(i, q, k, v, self.cos, self.sin)
+            h = h + c.attend(i, q).view(-1, 4 * 128) @ self.o[i].t()
+            x = torch.nn.functional.rms_norm(h, (self.H,))
+            h = h + K.moe_layer(x, *self.moe[i], 3)
+        c.commit()
+        logits = (torch.nn.functional.rms_norm(h, (self.H,)) @ self.emb.t())[self.rows.view(-1).long()]
+        st = K.beam_select(logits, self.scores)
+        c.reorder(self.rows, st.next_beams)
+        self.tokens.copy_(st.next_tokens)
+        self.scores.copy_(st.next_scores)
+
+
+def test_whole_step_in_a_graph():
+    from kvr_b200 import kernels as K
+    eager, captured = Step(), Step()
+    for s in (eager, captured):
+        s()  # (and what a first call sets up)
+        s()
+    state = lambda s: [s.tokens, s.scores, s.cache.block_table, s.cache.ctx_len, s.cache.shared, s.cache.n_free, s.cache.free_pages,  # noqa: E731
+                       s.cache.k, s.cache.v]
+    keep = [t.clone() for t in state(captured)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured()
+    for t, b in zip(state(captured), keep):
+        t.copy_(b)
+    for i in range(40):
+        eager()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(state(eager), state(captured))), i
+    eager.cache.check()
+    K.moe_status()
+    K.attn_status()
+    assert eager.cache.ctx_len.eq(42).all() and eager.scores.isfinite().all()
+    held = {p for r in eager.cache.block_table.tolist() for p in r[:6]}
+    free = eager.cache.free_pages[:eager.cache.n_free.item()].tolist()
+    assert sorted(held | set(free)) == list(range(80)) and len(free) + len(held) == 80
+    assert eager.cache.shared.sum().item() == 6 * 6 - len(held)
+
+
+def test_host_threads_at_once():
+    """Threads on one stream and on streams of their own: every call has its own workspace."""
+    import threading
+
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(2)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=g).half()  # noqa: E731
+    w = (n(16, 256), n(16, 192, 256) / 16, n(16, 256, 96) / 10)
+    xs, logits = [n(t, 256) for t in (1, 5, 40, 128)], [n(6, 5000 + 900 * i) for i in range(4)]
+    scores = -torch.rand(2, 3, device=DEV, generator=g)
+    want = [(K.moe_layer(x, *w, 4), K.beam_select(z, scores, eos=(1,)).tokens) for x, z in zip(xs, logits)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(60):
+                y, t = K.moe_layer(xs[i], *w, 4), K.beam_select(logits[i], scores, eos=(1,)).tokens
+                if not (torch.equal(y, want[i][0]) and torch.equal(t, want[i][1])):
+                    bad.append(i)
+
+    for streams in ([torch.cuda.current_stream()] * 4, [torch.cuda.Stream() for _ in range(4)]):
+        threads = [threading.Thread(target=work, args=(i, s)) for i, s in enumerate(streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    torch.cuda.synchronize()
+    K.moe_status()
+    assert not bad

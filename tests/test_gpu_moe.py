@@ -137,3 +137,17 @@ def test_graph_and_streams():
         assert torch.equal(y, K.moe_layer(*new, 4))
         assert all(torch.equal(g, want[i // 5]) for i, g in enumerate(got))
     K.moe_status()
+
+
+def test_a_wait_that_ran_out_is_reported():
+    """The status word that the waits set, set by the self-test's wait: reported once, then calls go on."""
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    a = inputs(3, 64, 16, 4, "f16", 11)
+    want = K.moe_layer(*a, 2)
+    K.moe_status()
+    N.call("kvr_selftest_bounded_wait", K._moe_status(a[0].device).data_ptr(), 1000, N.stream())
+    with pytest.raises(N.KvrError, match="gave up"):
+        K.moe_status()
+    K.moe_status()
+    assert torch.equal(K.moe_layer(*a, 2), want)
