@@ -197,15 +197,19 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
       key_s[e] = e < a.experts ? mo_key(z) : 0;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += kMrThreads) {
-      const uint64_t mine = key_s[e];
+    int each = 1;  // threads that share an expert's count
+    while (each < 32 && a.experts * each * 2 <= kMrThreads) each *= 2;
+    for (int e0 = 0; e0 < a.experts; e0 += kMrThreads / each) {
+      const int e = e0 + threadIdx.x / each;
+      const uint64_t mine = e < a.experts ? key_s[e] : 0;
       int above = 0;
 #pragma unroll 4
-      for (int o = 0; o < even; o += 2) {
+      for (int o = threadIdx.x % each * 2; o < even; o += 2 * each) {
         const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&key_s[o]);
         above += (k.x > mine || (k.x == mine && o < e)) + (k.y > mine || (k.y == mine && o + 1 < e));
       }
-      if (above < a.top_k) chosen[above] = e;
+      for (int o = 1; o < each; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+      if (e < a.experts && threadIdx.x % each == 0 && above < a.top_k) chosen[above] = e;
     }
     __syncthreads();
     if (warp == 0) {
@@ -229,7 +233,7 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
 
 constexpr int kMoThreads = 256;
 constexpr int kMoMaxStages = 16, kMoSched = 4;
-constexpr uint32_t kMoRing = 176 * 1024;   // stages (more would keep the next call's router off the SM until this one ends)
+constexpr uint32_t kMoRing = 180 * 1024;   // stages (more would keep the next call's router off the SM until this one ends)
 constexpr uint32_t kMoPad = 16 * 1024;     // an MMA reads 128 rows from a tile's start, however few of them it uses
 constexpr uint32_t kMoTmemCols = 512;      // two accumulators of up to 256 columns
 constexpr int kMoMinCols = 16;
@@ -240,7 +244,7 @@ struct ExpertArgs {
   int tokens, hidden, inter, experts, top_k;
   int rows1, rows2;      // rows of a gate/up and of a down unit
   int kb1, kb2;          // 64-column blocks of a stage
-  int cols;              // most tokens of a segment, a multiple of 16
+  int cols, cols2;       // columns of a gate/up unit (most tokens of a segment) and of a down unit, multiples of 16
   int shares;            // of an expert's inner channels in down units
   int sum_tokens;        // tokens of a sum unit
   int stages;
@@ -411,78 +415,106 @@ __global__ void __launch_bounds__(kMoThreads, 1)
   int next = 0;  // (the first ticket, asked for while the lists are made)
   if (tid == 0) next = atomicAdd(ticket, 1);
 
-  // picks by expert, and segments.  Every CTA makes the same lists: a bit per (expert, token), counts and prefix sums.
-  constexpr int kIds = kMoMaxPicks / kMoThreads;
+  // picks by expert, and segments.  Every CTA makes the same lists.
   const int picks = a.tokens * a.top_k;
-  int id[kIds];
+  if (picks <= 32) {  // by one warp, a pick per lane
+    if (warp == 0) {
+      const int id = lane < picks ? a.ids[lane] : -1;
+      if (lane < picks) s.weights[lane] = a.weights[lane];
+      const unsigned same = __match_any_sync(0xffffffffu, id);  // picks of the lane's expert
+      const int lead = __ffs(same) - 1, n = id >= 0 && lead == lane ? __popc(same) : 0, n_s = (n + a.cols - 1) / a.cols;
+      int at_n = n, at_s = n_s;
 #pragma unroll
-  for (int j = 0; j < kIds; ++j) {
-    const int i = tid + j * kMoThreads;
-    id[j] = i < picks ? a.ids[i] : -1;
-    if (i < picks) s.weights[i] = a.weights[i];
-  }
-#pragma unroll
-  for (int j = 0; j < kIds; ++j)
-    if (id[j] >= 0) {
-      const int t = (tid + j * kMoThreads) / a.top_k;
-      atomicOr(&mask[id[j]][t >> 5], 1u << (t & 31));
-    }
-  __syncthreads();
-  {
-    constexpr int kEach = kMoMaxExperts / kMoThreads;
-    int n[kEach], sum_n = 0, sum_s = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int e = tid * kEach + j;
-      n[j] = 0;
-#pragma unroll
-      for (int w = 0; w < kMoMaxTokens / 32; ++w) n[j] += __popc(mask[e][w]);
-      sum_n += n[j];
-      sum_s += (n[j] + a.cols - 1) / a.cols;
-    }
-    int at_n = sum_n, at_s = sum_s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int yn = __shfl_up_sync(0xffffffffu, at_n, o), ys = __shfl_up_sync(0xffffffffu, at_s, o);
-      if (lane >= o) {
-        at_n += yn;
-        at_s += ys;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int yn = __shfl_up_sync(0xffffffffu, at_n, o), ys = __shfl_up_sync(0xffffffffu, at_s, o);
+        if (lane >= o) {
+          at_n += yn;
+          at_s += ys;
+        }
       }
+      if (lane == 31) s.n_segs = at_s;
+      at_n -= n;
+      at_s -= n_s;
+      for (int c = 0; c < n; c += a.cols, ++at_s) {
+        s.seg_expert[at_s] = id;
+        s.seg_first[at_s] = (short)(at_n + c);
+        s.seg_n[at_s] = (short)min(a.cols, n - c);
+      }
+      const int first = __shfl_sync(0xffffffffu, at_n, lead);
+      if (id >= 0) s.picks[first + __popc(same & ((1u << lane) - 1))] = (short)lane;
     }
-    if (lane == 31) {
-      s.warp_sums[0][warp] = at_n;
-      s.warp_sums[1][warp] = at_s;
+  } else {  // a bit per (expert, token), counts and prefix sums
+    constexpr int kIds = kMoMaxPicks / kMoThreads;
+    int id[kIds];
+#pragma unroll
+    for (int j = 0; j < kIds; ++j) {
+      const int i = tid + j * kMoThreads;
+      id[j] = i < picks ? a.ids[i] : -1;
+      if (i < picks) s.weights[i] = a.weights[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kIds; ++j)
+      if (id[j] >= 0) {
+        const int t = (tid + j * kMoThreads) / a.top_k;
+        atomicOr(&mask[id[j]][t >> 5], 1u << (t & 31));
+      }
+    __syncthreads();
+    {
+      constexpr int kEach = kMoMaxExperts / kMoThreads;
+      int n[kEach], sum_n = 0, sum_s = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int e = tid * kEach + j;
+        n[j] = 0;
+#pragma unroll
+        for (int w = 0; w < kMoMaxTokens / 32; ++w) n[j] += __popc(mask[e][w]);
+        sum_n += n[j];
+        sum_s += (n[j] + a.cols - 1) / a.cols;
+      }
+      int at_n = sum_n, at_s = sum_s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int yn = __shfl_up_sync(0xffffffffu, at_n, o), ys = __shfl_up_sync(0xffffffffu, at_s, o);
+        if (lane >= o) {
+          at_n += yn;
+          at_s += ys;
+        }
+      }
+      if (lane == 31) {
+        s.warp_sums[0][warp] = at_n;
+        s.warp_sums[1][warp] = at_s;
+      }
+      __syncthreads();
+      at_n -= sum_n;
+      at_s -= sum_s;
+      for (int w = 0; w < warp; ++w) {
+        at_n += s.warp_sums[0][w];
+        at_s += s.warp_sums[1][w];
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int e = tid * kEach + j;
+        s.first[e] = (short)at_n;
+        for (int c = 0; c < n[j]; c += a.cols) {
+          s.seg_expert[at_s] = e;
+          s.seg_first[at_s] = (short)(at_n + c);
+          s.seg_n[at_s] = (short)min(a.cols, n[j] - c);
+          ++at_s;
+        }
+        at_n += n[j];
+      }
+      if (tid == kMoThreads - 1) s.n_segs = at_s;
     }
     __syncthreads();
-    at_n -= sum_n;
-    at_s -= sum_s;
-    for (int w = 0; w < warp; ++w) {
-      at_n += s.warp_sums[0][w];
-      at_s += s.warp_sums[1][w];
-    }
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int e = tid * kEach + j;
-      s.first[e] = (short)at_n;
-      for (int c = 0; c < n[j]; c += a.cols) {
-        s.seg_expert[at_s] = e;
-        s.seg_first[at_s] = (short)(at_n + c);
-        s.seg_n[at_s] = (short)min(a.cols, n[j] - c);
-        ++at_s;
+    for (int j = 0; j < kIds; ++j)
+      if (id[j] >= 0) {
+        const int i = tid + j * kMoThreads, t = i / a.top_k, e = id[j];
+        int before = __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1));
+        for (int w = 0; w < (t >> 5); ++w) before += __popc(mask[e][w]);
+        s.picks[s.first[e] + before] = (short)i;
       }
-      at_n += n[j];
-    }
-    if (tid == kMoThreads - 1) s.n_segs = at_s;
   }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kIds; ++j)
-    if (id[j] >= 0) {
-      const int i = tid + j * kMoThreads, t = i / a.top_k, e = id[j];
-      int before = __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1));
-      for (int w = 0; w < (t >> 5); ++w) before += __popc(mask[e][w]);
-      s.picks[s.first[e] + before] = (short)i;
-    }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies will write where the bits were
   __syncthreads();
   MoPlan p;
@@ -577,7 +609,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       const bool down = w.phase == 1;
       // columns: tokens; or, of h, rounded parts and rests in turn
       const int first = s.seg_first[w.seg], n = (int)tc_uniform(s.seg_n[w.seg] * (down ? 2 : 1)), quads = (n + 3) / 4;
-      const int kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const int kb = down ? a.kb2 : a.kb1, cols = down ? a.cols2 : a.cols;
       const CUtensorMap *map = down ? &mh : &mx;
       int r[2][4], at[2], block[2];
 #pragma unroll
@@ -649,7 +681,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (w.phase == 2) continue;
       const bool down = w.phase == 1;
       const int n = (s.seg_n[w.seg] * (down ? 2 : 1) + 15) / 16 * 16, rows = down ? a.rows2 : a.rows1;
-      const int kb = down ? a.kb2 : a.kb1, cols = down ? 2 * a.cols : a.cols;
+      const int kb = down ? a.kb2 : a.kb1, cols = down ? a.cols2 : a.cols;
       const int buf = n_acc & 1;
       const uint32_t idesc = tc_uniform(mo_idesc<DT>(n)), acc = tc_uniform(tmem + buf * 256);
       const uint32_t a_step = tc_uniform(rows * 128 >> 4), b_step = tc_uniform(cols * 128 >> 4);
@@ -816,7 +848,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
 
 // How a call's experts are cut, from its sizes.
 struct MoeCut {
-  int rows1, rows2, kb1, kb2, cols, shares, sum_tokens, stages;
+  int rows1, rows2, kb1, kb2, cols, cols2, shares, sum_tokens, stages;
   uint32_t stage_bytes, a_bytes;
 };
 
@@ -842,6 +874,7 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   int64_t cols = (2 * picks / experts + 16 + 15) / 16 * 16;
   if (cols > (tokens + 15) / 16 * 16) cols = (tokens + 15) / 16 * 16;
   c.cols = (int)cols;
+  c.cols2 = (int)(2 * cols < (2 * tokens + 15) / 16 * 16 ? 2 * cols : (2 * tokens + 15) / 16 * 16);  // h in two parts
   c.rows1 = moe_rows(segs, 2 * (int64_t)inter);
   // Down units are of 128 rows and a share of the inner channels, since partial rows are summed in any case: as many
   // shares as make the fullest SM's time least, a unit costing about two 64-column blocks besides its own.
@@ -863,8 +896,8 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
     return kb;
   };
   c.kb1 = blocks(c.rows1, c.cols);
-  c.kb2 = blocks(c.rows2, 2 * c.cols);
-  const int a1 = c.kb1 * c.rows1, a2 = c.kb2 * c.rows2, b1 = c.kb1 * c.cols, b2 = c.kb2 * 2 * c.cols;
+  c.kb2 = blocks(c.rows2, c.cols2);
+  const int a1 = c.kb1 * c.rows1, a2 = c.kb2 * c.rows2, b1 = c.kb1 * c.cols, b2 = c.kb2 * c.cols2;
   c.a_bytes = (uint32_t)(a1 > a2 ? a1 : a2) * 128;
   c.stage_bytes = c.a_bytes + (uint32_t)(b1 > b2 ? b1 : b2) * 128;
   c.stages = (int)(kMoRing / c.stage_bytes);
@@ -961,7 +994,7 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   r.counters = reinterpret_cast<int *>(ws); r.n_counters = (int)moe_counters(hidden);
   ExpertArgs a{};
   a.tokens = (int)n_tokens; a.hidden = hidden; a.inter = inter; a.experts = experts; a.top_k = top_k;
-  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
+  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.cols2 = c.cols2; a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
   a.stage_bytes = c.stage_bytes; a.a_bytes = c.a_bytes;
   a.ids = ids; a.weights = weights;
   a.h = ws + align_up(moe_counters(hidden) * 4, 256);
