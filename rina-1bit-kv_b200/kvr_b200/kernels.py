@@ -976,7 +976,7 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
 
 # ------------------------------------------------------------ sparse MLP --
 
-MOE_MAX_TOKENS = 128
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 128, 512, 16
 _MOE_WS: dict = {}
 _MOE_STATUS: dict = {}
 

@@ -264,13 +264,15 @@ class PagedGenerator:
     @staticmethod
     def _mlp(mlp, x):
         """A layer's MLP over packed rows: a sparse one of a few tokens in one call,
-        of more by the model's own module."""
+        of more, or of a shape or type that the call does not take, by the model's own module."""
         if not hasattr(mlp, "experts"):
             return mlp(x)
-        experts = mlp.experts
-        if x.shape[0] <= K.MOE_MAX_TOKENS and x.shape[1] % 8 == 0 and experts.down_proj.shape[2] % 8 == 0:
-            return K.moe_layer(x, mlp.gate.weight, experts.gate_up_proj, experts.down_proj, mlp.gate.top_k,
-                               norm_topk=bool(getattr(mlp.gate, "norm_topk_prob", True)))
+        gate, experts = mlp.gate, mlp.experts
+        n, hidden, inter = experts.down_proj.shape
+        if (x.shape[0] <= K.MOE_MAX_TOKENS and n <= K.MOE_MAX_EXPERTS and gate.top_k <= K.MOE_MAX_TOP_K
+                and hidden % 8 == 0 and inter % 8 == 0 and gate.weight.dtype is x.dtype):
+            return K.moe_layer(x, gate.weight, experts.gate_up_proj, experts.down_proj, gate.top_k,
+                               norm_topk=bool(getattr(gate, "norm_topk_prob", True)))
         y = mlp(x[None])
         return (y[0] if isinstance(y, tuple) else y)[0]
 

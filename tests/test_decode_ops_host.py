@@ -384,3 +384,27 @@ def test_beam_search_refusals_and_cleanup(monkeypatch):
     with pytest.raises(RuntimeError, match="not fit"):
         gen.beam_search([[1], [2]], 2, 3)
     assert not gen.last and not any(gen.cache.text)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,inter,router,own", [
+    (1, 4, 2, 16, 8, torch.bfloat16, True), (128, 512, 16, 16, 8, torch.bfloat16, True),
+    (129, 4, 2, 16, 8, torch.bfloat16, False), (2, 513, 2, 16, 8, torch.bfloat16, False), (2, 32, 17, 16, 8, torch.bfloat16, False),
+    (2, 4, 2, 20, 8, torch.bfloat16, False), (2, 4, 2, 16, 12, torch.bfloat16, False), (2, 4, 2, 16, 8, torch.float32, False)])
+def test_sparse_mlps_that_the_call_does_not_take_stay_the_models(native, tokens, experts, top_k, hidden, inter, router, own):
+    from kvr_b200.kvr_paged import PagedGenerator
+
+    class Sparse(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            zeros = lambda *s, dtype=torch.bfloat16: torch.nn.Parameter(torch.zeros(*s, dtype=dtype), requires_grad=False)
+            self.gate, self.experts = torch.nn.Module(), torch.nn.Module()
+            self.gate.weight, self.gate.top_k = zeros(experts, hidden, dtype=router), top_k
+            self.experts.gate_up_proj = zeros(experts, 2 * inter, hidden)
+            self.experts.down_proj = zeros(experts, hidden, inter)
+
+        def forward(self, x):
+            return x + 1
+
+    y = PagedGenerator._mlp(Sparse(), torch.zeros(tokens, hidden, dtype=torch.bfloat16))
+    assert y.shape == (tokens, hidden) and ("kvr_moe_layer" in native) == own
+    assert own or bool((y == 1).all())
