@@ -27,6 +27,7 @@
  *   modules/kvr_window.py:43-69, kvr_hook.py:274-282,
  *   modules/kvr_triton.py:42-104     (attention)       -> kvr_decode_attn
  *   (no reference counterpart: the 1-bit sd1 codec)    -> kvr_sd1_*, kvr_transform, kvr_lse_merge
+ *   (none either: decoding by beams, sparse MLPs)      -> kvr_beam_select, kvr_paged_reorder, kvr_moe_layer
  */
 #ifndef KVR_B200_H
 #define KVR_B200_H

@@ -38,6 +38,12 @@
 // leave room for.  (Rounded once, y was 1.4 to 1.6 times as far from 64 bits as its own
 // rounding makes it.)  Sums, router weights and partial rows are fp32.
 //
+// What binds: HBM where the weights are many.  128 tokens over 128 experts of 4096 x 1408
+// (4.4 GB): 690 us, 6.4 TB/s, 0.98 of a plain copy; 32 over 8 of 8192 wide hidden
+// layers 463.  One token, 8 of 128 experts of 2048 x 768 (75 MB, 12 us of reading): 28 us, the rest
+// a chain of round trips: logits and ranks (4), lists (1), a first tile's way from memory (2),
+// h through a counter and L2 (3), last products, partial rows and sums (6).
+//
 // Waits are bounded; one that gives up sets the status word, lets copies and MMAs in
 // flight end and frees the tensor memory.
 #include "kvr_tcgen05.cuh"
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
 
   // picks by expert, and segments.  Every CTA makes the same lists.
   const int picks = a.tokens * a.top_k;
-  if (picks <= 32) {  // by one warp, a pick per lane
+  if (picks <= 32) {  // by one warp, a pick per lane: no bits, no meetings (a token of 128 experts 28.2 -> 27.4 us)
     if (warp == 0) {
       const int id = lane < picks ? a.ids[lane] : -1;
       if (lane < picks) s.weights[lane] = a.weights[lane];
@@ -994,7 +1000,8 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   r.counters = reinterpret_cast<int *>(ws); r.n_counters = (int)moe_counters(hidden);
   ExpertArgs a{};
   a.tokens = (int)n_tokens; a.hidden = hidden; a.inter = inter; a.experts = experts; a.top_k = top_k;
-  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.cols2 = c.cols2; a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
+  a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.cols2 = c.cols2;
+  a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
   a.stage_bytes = c.stage_bytes; a.a_bytes = c.a_bytes;
   a.ids = ids; a.weights = weights;
   a.h = ws + align_up(moe_counters(hidden) * 4, 256);
