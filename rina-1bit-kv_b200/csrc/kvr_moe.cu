@@ -28,7 +28,7 @@
 // be resident for another to end.  Weights of a down unit stream in while its h is
 // still being formed, so the memory does not idle between the phases.
 //   warp 0  tickets, weight tiles by TMA (128-byte swizzle) into a ring of stages
-//   warp 1  token rows by TMA gather into the same stages
+//   warps 1, 3  token rows into the same stages, 16 bytes a lane, swizzled by hand
 //   warp 2  tcgen05.mma, accumulators of two units in tensor memory
 //   warps 4-7  epilogues of 32 rows each; sums
 //
@@ -255,6 +255,8 @@ struct ExpertArgs {
   int sum_tokens;        // tokens of a sum unit
   int stages;
   uint32_t stage_bytes, a_bytes;  // of a stage; its weights' part
+  const void *x;
+  int64_t x_stride;
   const int *ids;
   const float *weights;
   void *h;               // (tokens * top_k, 2, inter): rounded, rest
@@ -277,6 +279,7 @@ struct MoShared {
   short first[kMoMaxExperts];
   short picks[kMoMaxPicks];  // token * top_k + choice, by expert
   float weights[kMoMaxPicks];
+  short rows[2][2 * kMoMaxTokens];  // of x or h, of the unit that a copying warp is at
 };
 
 __device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar,
@@ -295,14 +298,9 @@ __device__ __forceinline__ void mo_tma3(uint32_t dst, const CUtensorMap *m, int 
       "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy)
       : "memory");
 }
-// 64 columns of four rows.
-__device__ __forceinline__ void mo_gather4(uint32_t dst, const CUtensorMap *m, int c0, int r0, int r1, int r2, int r3,
-                                           uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-      : "memory");
+// 16 bytes (zeros where !there) past L1.
+__device__ __forceinline__ void mo_copy16(uint32_t dst, const char *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void mo_ld4(uint32_t taddr, float *f) {
   uint32_t *r = reinterpret_cast<uint32_t *>(f);
@@ -376,8 +374,7 @@ __device__ __forceinline__ float mo_rounded(float x) {
 
 template <int DT>
 __global__ void __launch_bounds__(kMoThreads, 1)
-    moe_experts_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw1,
-                       const __grid_constant__ CUtensorMap mh, const __grid_constant__ CUtensorMap mw2, const ExpertArgs a) {
+    moe_experts_kernel(const __grid_constant__ CUtensorMap mw1, const __grid_constant__ CUtensorMap mw2, const ExpertArgs a) {
   extern __shared__ __align__(1024) unsigned char sm[];
   MoShared &s = *reinterpret_cast<MoShared *>(sm + kMoRing + kMoPad);
   volatile int *abort_s = &s.abort_s;
@@ -388,13 +385,13 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == 32) {
-    for (const CUtensorMap *m : {&mx, &mw1, &mh, &mw2}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    for (const CUtensorMap *m : {&mw1, &mw2}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   if (tid == 0) {
     s.abort_s = 0;
     for (int i = 0; i < a.stages; ++i) {
       tc_bar_init(&s.full_a[i], 1);
-      tc_bar_init(&s.full_b[i], 1);
+      tc_bar_init(&s.full_b[i], 32);  // a copying warp's lanes
       tc_bar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -403,7 +400,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     }
     for (int i = 0; i < kMoSched; ++i) {
       tc_bar_init(&s.sched_full[i], 1);
-      tc_bar_init(&s.sched_empty[i], 6);  // copies of tokens, MMA, four epilogue warps
+      tc_bar_init(&s.sched_empty[i], 7);  // two copying warps, MMA, four epilogue warps
     }
     tc_bar_init(&s.drained, 1);
   }
@@ -597,16 +594,22 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     __syncwarp();
     // nothing may be in flight to this CTA's memory when it ends; after an abort the last stages were not seen full
     if (*abort_s) mo_drain(s.full_a, st, parity, filled, a.stages);
-  } else if (warp == 1) {
-    // ---- rows of the tokens, four a copy: a lane has the same place in every stage of a unit, or two of them
-    // (all copies from one lane, with rows shuffled to it: a third slower)
-    int st = 0, filled = 0, known = -1;
+  } else if (warp == 1 || warp == 3) {
+    // ---- rows of the tokens: the warps take stages by turns, a lane 16 bytes of a row at a time.  A lane's arrival follows
+    // its copies, so neither warp waits for them.  (TMA gathers of four rows, a lane each: 100 cycles a gather, which 16
+    // tokens an expert already notice.  Both warps at every stage, handing it on when its copies are there: their work
+    // on a stage took longer than its weights.)
+    const int half = warp >> 1, chunk = lane & 7, sub = lane >> 3;
+    short *from = s.rows[half];
+    int st = 0, turn = half, known = -1;
     unsigned parity = 1, done = 0;  // segments 32 known .. whose h is there, a bit each
     bool ok = true;
+    // places of rows 8 i + sub and 8 i + 4 + sub, swizzled
+    const uint32_t at0 = a.a_bytes + sub * 128 + ((chunk ^ sub) << 4), at1 = a.a_bytes + (sub + 4) * 128 + ((chunk ^ (sub + 4)) << 4);
     for (int q = 0; ok; ++q) {
       ok = tc_wait_warp(&s.sched_full[q % kMoSched], (q / kMoSched) & 1, abort_s);
       if (!ok) break;
-      const int u = (int)tc_uniform(s.sched[q % kMoSched]);
+      const int u = s.sched[q % kMoSched];
       __syncwarp();
       if (lane == 0) tc_arrive(&s.sched_empty[q % kMoSched]);
       if (u < 0) break;
@@ -614,28 +617,21 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       if (w.phase == 2) continue;
       const bool down = w.phase == 1;
       // columns: tokens; or, of h, rounded parts and rests in turn
-      const int first = s.seg_first[w.seg], n = (int)tc_uniform(s.seg_n[w.seg] * (down ? 2 : 1)), quads = (n + 3) / 4;
-      const int kb = down ? a.kb2 : a.kb1, cols = down ? a.cols2 : a.cols;
-      const CUtensorMap *map = down ? &mh : &mx;
-      int r[2][4], at[2], block[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        block[i] = (i * 32 + lane) / quads;
-        const int g = i * 32 + lane - block[i] * quads;
-        at[i] = (block[i] * cols + g * 4) * 128;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = min(g * 4 + j, n - 1);  // (past the last: its row again, to no use)
-          const int pick = s.picks[first + (down ? c >> 1 : c)];
-          r[i][j] = down ? pick * 2 + (c & 1) : pick / a.top_k;
-        }
+      const int first = s.seg_first[w.seg], n = s.seg_n[w.seg] * (down ? 2 : 1), quads = (n + 3) / 4;
+      const int kb = down ? a.kb2 : a.kb1, cols = down ? a.cols2 : a.cols, width = down ? a.inter : a.hidden;
+      const char *base = static_cast<const char *>(down ? a.h : a.x) + chunk * 16;
+      const int64_t pitch = down ? (int64_t)a.inter * 2 : a.x_stride * 2;
+      for (int i = lane; i < quads * 4; i += 32) {
+        const int c = min(i, n - 1);  // (past the last: its row again, to no use)
+        const int pick = s.picks[first + (down ? c >> 1 : c)];
+        from[i] = (short)(down ? pick * 2 + (c & 1) : pick / a.top_k);
       }
       if (down && (w.seg / 32 != known || !((done >> (w.seg & 31)) & 1))) {
         // until its gate/up units are done: a lane looks at a segment, so that the next units' need not be asked for again
         known = w.seg / 32;
-        const int mine = known * 32 + lane;
+        const int look = known * 32 + lane;
         for (uint32_t i = 0;; ++i) {
-          done = __ballot_sync(0xffffffffu, mine < p.segs && mo_acquire(seg_done + mine) >= p.tiles1 * (a.rows1 / 32));
+          done = __ballot_sync(0xffffffffu, look < p.segs && mo_acquire(seg_done + look) >= p.tiles1 * (a.rows1 / 32));
           if ((done >> (w.seg & 31)) & 1) break;
           if (__any_sync(0xffffffffu, i >= kSpinLimit || *abort_s)) {
             ok = false;
@@ -644,33 +640,37 @@ __global__ void __launch_bounds__(kMoThreads, 1)
           __nanosleep(32);
         }
         if (!ok) break;
-        __syncwarp();
-        asm volatile("fence.proxy.async;" ::: "memory");  // h was stored, and is read by copies
       }
+      __syncwarp();
       for (int b0 = w.b0; b0 < w.b1; b0 += kb) {
-        const int nb = min(kb, w.b1 - b0);
-        tc_wait_on(&s.empty[st], parity, abort_s, a.err);
-        if (lane == 0) mbar_expect_tx(&s.full_b[st], nb * quads * 512);
-        __syncwarp();
-        const uint32_t dst = ring + st * a.stage_bytes + a.a_bytes, full = smem_u32(&s.full_b[st]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (block[i] < nb) mo_gather4(dst + at[i], map, (b0 + block[i]) * 64, r[i][0], r[i][1], r[i][2], r[i][3], full);
-        __syncwarp();
-        filled = min(filled + 1, a.stages);
+        if (turn == 0) {
+          const int nb = min(kb, w.b1 - b0);
+          tc_wait_on(&s.empty[st], parity, abort_s, a.err);
+          for (int b = 0; b < nb; ++b) {
+            const int col = (b0 + b) * 64;
+            const bool there = col + chunk * 8 < width;
+            const char *src = base + (there ? col * 2 : 0);
+            const uint32_t dst = ring + st * a.stage_bytes + b * cols * 128;
+#pragma unroll 4
+            for (int i = 0; i < quads; ++i)
+              mo_copy16(dst + (i >> 1) * 1024 + (i & 1 ? at1 : at0), src + from[i * 4 + sub] * pitch, there);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full_b[st])) : "memory");
+        }
+        turn ^= 1;
         if (++st == a.stages) {
           st = 0;
           parity ^= 1;
         }
       }
+      __syncwarp();
       ok = __all_sync(0xffffffffu, !*abort_s);
     }
     if (!ok && lane == 0) {
       if (!*abort_s) atomicOr(a.err, 1u);
       *abort_s = 1;
     }
-    __syncwarp();
-    if (*abort_s) mo_drain(s.full_b, st, parity, filled, a.stages);
+    cp_async_wait<0>();
   } else if (warp == 2) {
     // ---- MMA
     int st = 0, n_acc = 0;
@@ -696,6 +696,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       for (int b0 = w.b0; b0 < w.b1; b0 += kb) {
         const int nb = min(kb, w.b1 - b0);
         tc_wait_on(&s.full_b[st], parity, abort_s, a.err);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // rows stored by lanes' copies, read by MMAs
         tc_wait_on(&s.full_a[st], parity, abort_s, a.err);
         tc_fence_after();
         const uint32_t wa = tc_uniform(tc_desc_k(ring + st * a.stage_bytes));
@@ -918,7 +919,7 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
 static size_t moe_counters(int hidden) { return 1 + kMoMaxSegs + (size_t)(hidden + 31) / 32; }
 
 template <int DT>
-static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUtensorMap (&m)[4], cudaStream_t st) {
+static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUtensorMap (&m)[2], cudaStream_t st) {
   constexpr int kSmem = kMoRing + kMoPad + (int)sizeof(MoShared);
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
   static thread_local int set_dev = -1;
@@ -934,7 +935,7 @@ static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUt
   auto route = nt == 1 ? moe_route_kernel<DT, 1> : nt == 2 ? moe_route_kernel<DT, 2> : nt == 4 ? moe_route_kernel<DT, 4> : moe_route_kernel<DT, 8>;
   const cudaError_t e = launch_dependent(route, (unsigned)((r.tokens + nt - 1) / nt * kMrCluster), kMrThreads, 0, st, r);
   if (e != cudaSuccess) return e;
-  return launch_dependent(moe_experts_kernel<DT>, kMoSms, kMoThreads, kSmem, st, m[0], m[1], m[2], m[3], x);
+  return launch_dependent(moe_experts_kernel<DT>, kMoSms, kMoThreads, kSmem, st, m[0], m[1], x);
 }
 
 }  // namespace kvr
@@ -1003,21 +1004,19 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   a.rows1 = c.rows1; a.rows2 = c.rows2; a.kb1 = c.kb1; a.kb2 = c.kb2; a.cols = c.cols; a.cols2 = c.cols2;
   a.shares = c.shares; a.sum_tokens = c.sum_tokens; a.stages = c.stages;
   a.stage_bytes = c.stage_bytes; a.a_bytes = c.a_bytes;
+  a.x = x; a.x_stride = n_tokens > 1 ? x_stride : hidden;
   a.ids = ids; a.weights = weights;
   a.h = ws + align_up(moe_counters(hidden) * 4, 256);
   a.part = reinterpret_cast<float *>(static_cast<char *>(a.h) + align_up((size_t)picks * inter * 4, 256));
   a.y = y;
   a.counters = r.counters; a.err = static_cast<unsigned *>(status);
-  CUtensorMap m[4];
-  const cuuint64_t xd[2] = {(cuuint64_t)hidden, (cuuint64_t)n_tokens}, xs[1] = {(cuuint64_t)(n_tokens > 1 ? x_stride : hidden) * 2};
-  const cuuint64_t hd[2] = {(cuuint64_t)inter, (cuuint64_t)picks * 2}, hs[1] = {(cuuint64_t)inter * 2};
+  CUtensorMap m[2];
   const cuuint64_t gd[4] = {(cuuint64_t)hidden, (cuuint64_t)inter, 2, (cuuint64_t)experts};
   const cuuint64_t gs[3] = {(cuuint64_t)gu_row_stride * 2, (cuuint64_t)gu_row_stride * inter * 2, (cuuint64_t)gu_expert_stride * 2};
   const cuuint64_t dd[3] = {(cuuint64_t)inter, (cuuint64_t)hidden, (cuuint64_t)experts};
   const cuuint64_t ds[2] = {(cuuint64_t)down_row_stride * 2, (cuuint64_t)down_expert_stride * 2};
-  const cuuint32_t row[2] = {64, 1}, gb[4] = {64, 16, 2, 1}, db[3] = {64, (cuuint32_t)c.rows2, 1};
-  if (!make_map(&m[0], dtype, x, 2, xd, xs, row) || !make_map(&m[1], dtype, gate_up, 4, gd, gs, gb) ||
-      !make_map(&m[2], dtype, a.h, 2, hd, hs, row) || !make_map(&m[3], dtype, down, 3, dd, ds, db))
+  const cuuint32_t gb[4] = {64, 16, 2, 1}, db[3] = {64, (cuuint32_t)c.rows2, 1};
+  if (!make_map(&m[0], dtype, gate_up, 4, gd, gs, gb) || !make_map(&m[1], dtype, down, 3, dd, ds, db))
     return set_error(KVR_EINVAL, "kvr_moe_layer: a layout that TMA cannot read");
   const cudaError_t e = dtype == KVR_F16 ? moe_launch<KVR_F16>(r, a, m, as_cuda(stream)) : moe_launch<KVR_BF16>(r, a, m, as_cuda(stream));
   if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_moe_layer: %s", cudaGetErrorString(e));
