@@ -279,7 +279,7 @@ struct MoShared {
   short first[kMoMaxExperts];
   short picks[kMoMaxPicks];  // token * top_k + choice, by expert
   float weights[kMoMaxPicks];
-  short rows[2][2 * kMoMaxTokens];  // of x or h, of the unit that a copying warp is at
+  uint32_t rows[2][2 * kMoMaxTokens];  // where x's or h's are, in 16 bytes, of the unit that a copying warp is at
 };
 
 __device__ __forceinline__ void mo_tma4(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint32_t bar,
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kMoThreads, 1)
     // tokens an expert already notice.  Both warps at every stage, handing it on when its copies are there: their work
     // on a stage took longer than its weights.)
     const int half = warp >> 1, chunk = lane & 7, sub = lane >> 3;
-    short *from = s.rows[half];
+    uint32_t *from = s.rows[half];
     int st = 0, turn = half, known = -1;
     unsigned parity = 1, done = 0;  // segments 32 known .. whose h is there, a bit each
     bool ok = true;
@@ -620,11 +620,11 @@ __global__ void __launch_bounds__(kMoThreads, 1)
       const int first = s.seg_first[w.seg], n = s.seg_n[w.seg] * (down ? 2 : 1), quads = (n + 3) / 4;
       const int kb = down ? a.kb2 : a.kb1, cols = down ? a.cols2 : a.cols, width = down ? a.inter : a.hidden;
       const char *base = static_cast<const char *>(down ? a.h : a.x) + chunk * 16;
-      const int64_t pitch = down ? (int64_t)a.inter * 2 : a.x_stride * 2;
+      const uint32_t pitch = (down ? a.inter : (int)a.x_stride) / 8;
       for (int i = lane; i < quads * 4; i += 32) {
         const int c = min(i, n - 1);  // (past the last: its row again, to no use)
         const int pick = s.picks[first + (down ? c >> 1 : c)];
-        from[i] = (short)(down ? pick * 2 + (c & 1) : pick / a.top_k);
+        from[i] = (down ? pick * 2 + (c & 1) : pick / a.top_k) * pitch;
       }
       if (down && (w.seg / 32 != known || !((done >> (w.seg & 31)) & 1))) {
         // until its gate/up units are done: a lane looks at a segment, so that the next units' need not be asked for again
@@ -650,10 +650,18 @@ __global__ void __launch_bounds__(kMoThreads, 1)
             const int col = (b0 + b) * 64;
             const bool there = col + chunk * 8 < width;
             const char *src = base + (there ? col * 2 : 0);
-            const uint32_t dst = ring + st * a.stage_bytes + b * cols * 128;
-#pragma unroll 4
-            for (int i = 0; i < quads; ++i)
-              mo_copy16(dst + (i >> 1) * 1024 + (i & 1 ? at1 : at0), src + from[i * 4 + sub] * pitch, there);
+            uint32_t dst = ring + st * a.stage_bytes + b * cols * 128;
+            const uint32_t *f = from + sub;
+            int i = 0;
+            for (; i + 8 <= quads; i += 8, f += 32, dst += 4096) {
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = f[j * 4];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) mo_copy16(dst + (j & 1 ? at1 : at0) + j / 2 * 1024, src + (uint64_t)o[j] * 16, there);
+            }
+            for (; i < quads; ++i, f += 4)
+              mo_copy16(dst + (i & 1 ? at1 : at0) + (i & 7) / 2 * 1024, src + (uint64_t)*f * 16, there);
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full_b[st])) : "memory");
         }
@@ -964,6 +972,7 @@ extern "C" int kvr_moe_layer(const void *x, int dtype, int64_t n_tokens, int hid
   if (dtype != KVR_F16 && dtype != KVR_BF16) return set_error(KVR_ENOTSUP, "kvr_moe_layer: fp16 or bf16");
   if (hidden % 8 || inter % 8) return set_error(KVR_ENOTSUP, "kvr_moe_layer: hidden and inter must be multiples of 8");
   if (hidden > 1 << 16 || inter > 1 << 20) return set_error(KVR_ENOTSUP, "kvr_moe_layer: hidden or inter too large");
+  if (n_tokens > 1 && x_stride > 1 << 28) return set_error(KVR_ENOTSUP, "kvr_moe_layer: x's rows lie too far apart");
   if (n_tokens == 0) return KVR_OK;
   KVR_REQUIRE(x && router && gate_up && down && y && ids && weights && workspace && status, "kvr_moe_layer: null pointer");
   KVR_REQUIRE((x_stride >= hidden || n_tokens == 1) && router_stride >= hidden && gu_row_stride >= hidden &&
