@@ -239,8 +239,7 @@ __global__ void __cluster_dims__(kMrCluster, 1, 1) __launch_bounds__(kMrThreads,
 
 constexpr int kMoThreads = 256;
 constexpr int kMoMaxStages = 16, kMoSched = 4;
-constexpr uint32_t kMoRing = 180 * 1024;   // stages (more would keep the next call's router off the SM until this one ends)
-constexpr uint32_t kMoPad = 16 * 1024;     // an MMA reads 128 rows from a tile's start, however few of them it uses
+constexpr uint32_t kMoRing = 204 * 1024;   // stages, and what an MMA reads past the last: 128 rows from a tile's start
 constexpr uint32_t kMoTmemCols = 512;      // two accumulators of up to 256 columns
 constexpr int kMoMinCols = 16;
 constexpr int kMoMaxSegs = kMoMaxExperts + kMoMaxPicks / kMoMinCols;
@@ -376,7 +375,7 @@ template <int DT>
 __global__ void __launch_bounds__(kMoThreads, 1)
     moe_experts_kernel(const __grid_constant__ CUtensorMap mw1, const __grid_constant__ CUtensorMap mw2, const ExpertArgs a) {
   extern __shared__ __align__(1024) unsigned char sm[];
-  MoShared &s = *reinterpret_cast<MoShared *>(sm + kMoRing + kMoPad);
+  MoShared &s = *reinterpret_cast<MoShared *>(sm + kMoRing);
   volatile int *abort_s = &s.abort_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == 2) {
@@ -653,15 +652,15 @@ __global__ void __launch_bounds__(kMoThreads, 1)
             uint32_t dst = ring + st * a.stage_bytes + b * cols * 128;
             const uint32_t *f = from + sub;
             int i = 0;
-            for (; i + 8 <= quads; i += 8, f += 32, dst += 4096) {
-              uint32_t o[8];
+            for (; i + 4 <= quads; i += 4, f += 16, dst += 2048) {
+              uint32_t o[4];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = f[j * 4];
+              for (int j = 0; j < 4; ++j) o[j] = f[j * 4];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) mo_copy16(dst + (j & 1 ? at1 : at0) + j / 2 * 1024, src + (uint64_t)o[j] * 16, there);
+              for (int j = 0; j < 4; ++j) mo_copy16(dst + (j & 1 ? at1 : at0) + j / 2 * 1024, src + (uint64_t)o[j] * 16, there);
             }
             for (; i < quads; ++i, f += 4)
-              mo_copy16(dst + (i & 1 ? at1 : at0) + (i & 7) / 2 * 1024, src + (uint64_t)*f * 16, there);
+              mo_copy16(dst + (i & 1 ? at1 : at0) + (i & 3) / 2 * 1024, src + (uint64_t)*f * 16, there);
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full_b[st])) : "memory");
         }
@@ -915,7 +914,13 @@ static MoeCut moe_cut(int64_t tokens, int hidden, int inter, int experts, int to
   const int a1 = c.kb1 * c.rows1, a2 = c.kb2 * c.rows2, b1 = c.kb1 * c.cols, b2 = c.kb2 * c.cols2;
   c.a_bytes = (uint32_t)(a1 > a2 ? a1 : a2) * 128;
   c.stage_bytes = c.a_bytes + (uint32_t)(b1 > b2 ? b1 : b2) * 128;
-  c.stages = (int)(kMoRing / c.stage_bytes);
+  // an MMA reads 128 rows, however few of them a tile has: past its stage, where the tile is short
+  auto past = [&](int kb, int rows) {
+    const uint32_t end = (uint32_t)(kb - 1) * rows * 128 + 128 * 128;
+    return end > c.stage_bytes ? end - c.stage_bytes : 0u;
+  };
+  const uint32_t p1 = past(c.kb1, c.rows1), p2 = past(c.kb2, c.rows2);
+  c.stages = (int)((kMoRing - (p1 > p2 ? p1 : p2)) / c.stage_bytes);
   if (c.stages > kMoMaxStages) c.stages = kMoMaxStages;
   // sum units for every SM where there are as many tokens
   const int64_t strips = (hidden + kMoSumCols - 1) / kMoSumCols;
@@ -928,7 +933,7 @@ static size_t moe_counters(int hidden) { return 1 + kMoMaxSegs + (size_t)(hidden
 
 template <int DT>
 static cudaError_t moe_launch(const RouteArgs &r, const ExpertArgs &x, const CUtensorMap (&m)[2], cudaStream_t st) {
-  constexpr int kSmem = kMoRing + kMoPad + (int)sizeof(MoShared);
+  constexpr int kSmem = kMoRing + (int)sizeof(MoShared);
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
   static thread_local int set_dev = -1;
   int dev = 0;
