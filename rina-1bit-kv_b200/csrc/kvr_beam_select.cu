@@ -70,7 +70,7 @@ __device__ __forceinline__ uint64_t bs_key(float x, int token) {
 __device__ __forceinline__ float bs_value(uint64_t key) { return key_float((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int bs_token(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-struct BeamShared {
+struct __align__(16) BeamShared {
   uint64_t list[kBsList];
   uint64_t best[kBsRowThreads];
   uint64_t nth;
@@ -125,7 +125,11 @@ __device__ __noinline__ void bs_cut(BeamShared &sh, int n) {
     const uint64_t mine = sh.list[i];
     int above = 0;
 #pragma unroll 4
-    for (int j = 0; j < c; ++j) above += sh.list[j] > mine;
+    for (int j = 0; j + 1 < c; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&sh.list[j]);
+      above += (o.x > mine) + (o.y > mine);
+    }
+    if (c & 1) above += sh.list[c - 1] > mine;
     if (above < n) sh.best[above] = mine;
   }
   __syncthreads();
@@ -286,16 +290,18 @@ __global__ void __launch_bounds__(kBsRowThreads, 1024 / kBsRowThreads) beam_rows
     if (g0 + d * kTile < g1) fetch(next[d], g0 + d * kTile);
   tile(next[0], g0, true);
   meet(false);
-  for (int at = g0 + kTile; at < g1; at += kAhead * kTile) {
+  if (g0 + kTile < g1) {
+    for (int at = g0 + kTile; at < g1; at += kAhead * kTile) {
 #pragma unroll
-    for (int d = 0; d < kAhead; ++d)
-      if (at + d * kTile < g1) {
-        if (__any_sync(0xffffffffu, *static_cast<volatile int *>(&sh.count) > n + kBsSlack)) meet(false);
-        tile(next[(d + 1) % kAhead], at + d * kTile, false);
-      }
-  }
-  __syncwarp();
-  while (!meet(true)) {
+      for (int d = 0; d < kAhead; ++d)
+        if (at + d * kTile < g1) {
+          if (__any_sync(0xffffffffu, *static_cast<volatile int *>(&sh.count) > n + kBsSlack)) meet(false);
+          tile(next[(d + 1) % kAhead], at + d * kTile, false);
+        }
+    }
+    __syncwarp();
+    while (!meet(true)) {
+    }
   }
   uint64_t *out = a.cands + ((int64_t)row * a.splits + split) * n;
   for (int i = tid; i < n; i += kBsRowThreads) out[i] = i < sh.count ? sh.list[i] : 0;
