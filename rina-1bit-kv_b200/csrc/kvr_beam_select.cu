@@ -212,6 +212,14 @@ __global__ void __launch_bounds__(kBsRowThreads, 1024 / kBsRowThreads) beam_rows
   if (tid == 0) sh.count = 0;
   griddep_wait();
   griddep_launch();
+  uint64_t *out = a.cands + ((int64_t)row * a.splits + split) * n;
+  // A beam that there is not (a first step has one of K, a request that has ended none): its row is not read.  (24 requests
+  // of 8 beams, one each, 128256 logits in fp16: 22.5 -> 13.7 us.)
+  if (!isfinite(a.cum[row])) {
+    for (int i = tid; i < n; i += kBsRowThreads) out[i] = 0;
+    if (tid == 0) a.ml[(int64_t)row * a.splits + split] = make_float2(0.0f, 1.0f);
+    return;
+  }
   const uint32_t pad = DT == KVR_F32 ? 0xff800000u : DT == KVR_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
   // (fp32: the next tile's words; 16 bits: two tiles', as many)
   constexpr int kAhead = 4 / kVecs;
@@ -303,7 +311,6 @@ __global__ void __launch_bounds__(kBsRowThreads, 1024 / kBsRowThreads) beam_rows
     while (!meet(true)) {
     }
   }
-  uint64_t *out = a.cands + ((int64_t)row * a.splits + split) * n;
   for (int i = tid; i < n; i += kBsRowThreads) out[i] = i < sh.count ? sh.list[i] : 0;
   const float wm = warp_max(m);
   s *= bs_exp(m - (wm == -INFINITY ? 0.0f : wm));

@@ -111,6 +111,24 @@ def test_select_first_step_from_one_row():
     check_select(same.expand(4, -1).contiguous(), cum[:1], given=same.expand(4, -1))
 
 
+@pytest.mark.parametrize("V", [9, 4100, 128256])
+def test_select_beams_that_there_are_not(V):
+    """Their rows mean nothing, whatever stands in them: no candidates, and no request's other beams change."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = 2 * torch.randn(5 * 4, V, device=DEV, generator=g)
+    cum = -torch.rand(5, 4, device=DEV, generator=g)
+    inf = float("inf")
+    cum[0, 1:], cum[1, :3], cum[2, 2], cum[3] = -inf, -inf, float("nan"), -inf
+    cum[4, 0] = inf
+    dead = ~cum.isfinite().flatten()
+    plain = check_select(logits.clone(), cum)
+    for fill in (float("nan"), inf, -inf, 3e38):
+        logits[dead] = fill
+        got = check_select(logits.clone(), cum)
+        assert torch.equal(got.tokens, plain.tokens) and torch.equal(got.scores, plain.scores)
+    assert (plain.beams[3] == -1).all() and (plain.next_scores[3] == -inf).all()
+
+
 def test_select_in_a_graph_and_on_another_stream():
     from kvr_b200 import kernels as K
     g = torch.Generator(device=DEV).manual_seed(5)
