@@ -18,13 +18,13 @@
 // logits equal and order them by token.  Sums are in 32 bits per thread (at most
 // some thousand exponentials <= 1) and joined in 64 by the second kernel.
 //
-// What binds: 512 rows of 128256 in fp32, 56 us (4.7 TB/s; a kernel that only
+// What binds: 512 rows of 128256 in fp32, 51.5 us (5.1 TB/s; a kernel that only
 // reads them with as many CTAs takes 47): some 200 instructions a warp and tile of 512
 // logits, and 3 us at either end of a segment when nothing streams.  Rows in several
 // segments fill the SMs where rows are few, and pay those ends each (1184 CTAs for 512
-// rows: 65 us).  Tried: words of all rows in equal shares, 62 us; copies two tiles
-// ahead, 64 us (fewer CTAs have room).  One request of 4 beams and 32000 tokens: 9.8 us,
-// a chain of two launches and their barriers.
+// rows: 9 us more).  Tried: words of all rows in equal shares, 6 us more; copies two tiles
+// ahead, 8 us more (fewer CTAs have room).  One request of 4 beams and 32000 tokens: 7.8 us,
+// a chain of two launches and their barriers; the second kernel is 4 to 5 us of it.
 #include <cfloat>
 
 #include "kvr_common.cuh"
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kBsRowThreads, 1024 / kBsRowThreads) beam_rows
   int limit_token = INT_MAX;
   // All warps cut the list and take over its limit; true when all of them are done.  They meet only for that: a warp that
   // starts a tile with too many entries in the list comes here, and so does one that is done, so each of the others adds
-  // one tile at most, for which the list has room.  (A barrier a tile: 62 us for 512 rows of 128256, and most of a warp's
+  // one tile at most, for which the list has room.  (A barrier a tile: 6 us more for 512 rows of 128256, and most of a warp's
   // time at it.)
   auto meet = [&](bool done) {
     const bool all = __syncthreads_and(done);

@@ -34,15 +34,17 @@
 //
 // Both operands of an MMA are of one 16-bit type, so h has to be rounded for the
 // second product.  It goes in as two columns, h rounded and what the rounding left:
-// 16 (bf16) or 22 bits (fp16) of it, for gathers and columns that the few tokens
+// 16 (bf16) or 22 bits (fp16) of it, for copies and columns that the few tokens
 // leave room for.  (Rounded once, y was 1.4 to 1.6 times as far from 64 bits as its own
 // rounding makes it.)  Sums, router weights and partial rows are fp32.
 //
 // What binds: HBM where the weights are many.  128 tokens over 128 experts of 4096 x 1408
-// (4.4 GB): 690 us, 6.4 TB/s, 0.98 of a plain copy; 32 over 8 of 8192 wide hidden
-// layers 463.  One token, 8 of 128 experts of 2048 x 768 (75 MB, 12 us of reading): 28 us, the rest
-// a chain of round trips: logits and ranks (4), lists (1), a first tile's way from memory (2),
-// h through a counter and L2 (3), last products, partial rows and sums (6).
+// (4.4 GB): 664 us in a graph, 6.7 TB/s, a plain copy's rate (708 back to back for seconds, under the
+// power cap); 32 over 8 experts of 4096 x 14336 443.  One token, 8 of 128 experts of 2048 x 768 (75
+// MB, 12 us of reading): 27 us, the rest a chain of round trips: logits and ranks (4), lists
+// (1), a first tile's way from memory (2), h through a counter and L2 (3), last products, partial
+// rows and sums (6).  With many tokens an expert their rows cross L2 as often as the weights: 69 tokens over 4 of
+// 4 experts of 1128 x 13776 110 us, of which 57 are the weights'.
 //
 // Waits are bounded; one that gives up sets the status word, lets copies and MMAs in
 // flight end and frees the tensor memory.
