@@ -25,8 +25,8 @@
 //
 // What binds: tables and counts are small and lie in L2, so the first kernel is a
 // chain of dependent loads and two meetings; HBM binds the copies.  Both kernels in a graph: a
-// prompt of 1000 tokens forked 4 ways in 32 layers 17.5 us, 8 groups of 8 rows of 1300 to 2000 pages, little
-// to copy, 26; 16 groups of 4 in 32 layers, 67 MB read and as many written, 36 us (the
+// prompt of 1000 tokens forked 4 ways in 32 layers 17.4 us, 8 groups of 8 rows of 1300 to 2000 pages, little
+// to copy, 26; 16 groups of 4 in 32 layers, 67 MB read and as many written, 34 us (the
 // copies alone at a plain copy's rate: 20).
 #include "kvr_attn_plan.cuh"
 
@@ -34,7 +34,7 @@ namespace kvr {
 
 constexpr int kPrCluster = 8, kPrThreads = 1024, kPrWarps = kPrThreads / 32;
 constexpr int kPrMaxBeams = 32, kPrMaxRows = 4096;
-constexpr int kPrStepTokens = 8;     // tokens that a warp copies at a time
+constexpr int kPrCopyWords = 256;    // of 16 bytes, that a warp copies at a time
 constexpr int kPrMark = 1 << 18;     // on counts of pages with holders outside of a group: above all counts
 constexpr int kPrMaxTable = 1 << 16; // rows of a table
 constexpr int kPrSmem = 216 * 1024;  // places of the rows, and entries of as many units as fit
@@ -354,39 +354,37 @@ struct CopyArgs {
   const int *n_copies;
 };
 
+// A warp takes 256 words of 16 bytes of a page at a time, eight a lane on their way.  (Eight tokens at a time, with a
+// division a word: 450 instructions in place of 130, 1 to 2 us more a call.)
 __global__ void __launch_bounds__(256) copy_pages_kernel(CopyArgs a) {
   griddep_wait();
   griddep_launch();
-  const int lane = threadIdx.x & 31, steps = (a.page + kPrStepTokens - 1) / kPrStepTokens;
-  const int64_t warps = (int64_t)gridDim.x * 8, n = (int64_t)*a.n_copies * a.layers * 2 * steps;
-  const int row = a.n_kv * 16;  // 16-byte words of a token: 128 channels of 2 bytes a head
-  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < n; w += warps) {
-    // steps innermost: the copies of a page follow one another
-    const int step = (int)(w % steps);
-    int64_t rest = w / steps;
-    const int layer = (int)(rest % a.layers);
-    rest /= a.layers;
-    const bool v = rest & 1;
-    const int4 c = a.copies[rest >> 1];
-    const int t0 = step * kPrStepTokens, tokens = min(kPrStepTokens, c.z - t0);
-    if (tokens <= 0) continue;
-    uint16_t *pool = (v ? a.v : a.k) + layer * a.layer_stride + t0 * a.tok_stride;
+  const int lane = threadIdx.x & 31, row = a.n_kv * 16;  // words of a token: 128 channels of 2 bytes a head
+  const unsigned chunks = ((unsigned)a.page * row + kPrCopyWords - 1) / kPrCopyWords, inv = 0xffffffffu / row + 1;
+  // (a page is larger than 512 bytes, so that all of a GPU's memory is fewer chunks than 2^31)
+  const unsigned n = (unsigned)*a.n_copies * a.layers * 2 * chunks;
+  for (unsigned w = blockIdx.x * 8 + (threadIdx.x >> 5); w < n; w += gridDim.x * 8) {
+    // chunks innermost: the copies of a page follow one another
+    unsigned rest = w / chunks;
+    const int first = (w - rest * chunks) * kPrCopyWords + lane;
+    const unsigned pair = rest / a.layers, layer = rest - pair * a.layers;
+    const int4 c = a.copies[pair >> 1];
+    const int words = c.z * row;
+    uint16_t *pool = (pair & 1 ? a.v : a.k) + layer * a.layer_stride;
     const uint16_t *src = pool + c.x * a.page_stride;
     uint16_t *dst = pool + c.y * a.page_stride;
-    const int words = tokens * row;
-    for (int at = lane; at < words; at += 32 * 8) {
-      uint4 x[8];
-      int64_t off[8];
+    uint4 x[kPrCopyWords / 32];
+    auto at = [&](int i) {
+      int t = __umulhi(i, inv);  // i / row, or one more
+      t -= t * row > i;
+      return t * a.tok_stride + (i - t * row) * 8;
+    };
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = at + u * 32, t = i / row;
-        off[u] = t * a.tok_stride + (i - t * row) * 8;
-        if (i < words) x[u] = __ldcs(reinterpret_cast<const uint4 *>(src + off[u]));
-      }
+    for (int u = 0; u < kPrCopyWords / 32; ++u)
+      if (first + u * 32 < words) x[u] = __ldcs(reinterpret_cast<const uint4 *>(src + at(first + u * 32)));
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (at + u * 32 < words) *reinterpret_cast<uint4 *>(dst + off[u]) = x[u];
-    }
+    for (int u = 0; u < kPrCopyWords / 32; ++u)
+      if (first + u * 32 < words) *reinterpret_cast<uint4 *>(dst + at(first + u * 32)) = x[u];
   }
 }
 
@@ -427,6 +425,7 @@ extern "C" int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int
   KVR_REQUIRE(k_pages && v_pages, "kvr_paged_reorder: null pointer");
   KVR_REQUIRE(layers >= 1 && n_kv >= 1 && tok_stride >= (int64_t)n_kv * d && page_stride >= 0 && layer_stride >= 0,
               "kvr_paged_reorder: a token's heads must be contiguous");
+  if ((int64_t)page * n_kv >= 1 << 27) return set_error(KVR_ENOTSUP, "kvr_paged_reorder: pages of 32 GB");
   KVR_REQUIRE((layer_stride | page_stride | tok_stride) % 8 == 0 &&
                   ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
                     reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
@@ -464,9 +463,9 @@ extern "C" int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int
   if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_paged_reorder: %s", cudaGetErrorString(e));
   CopyArgs c{static_cast<uint16_t *>(k_pages), static_cast<uint16_t *>(v_pages), layers, page, n_kv,
              layer_stride, page_stride, tok_stride, a.copies, a.n_copies};
-  // at most as many warps as there can be steps of work
-  const int64_t steps = (int64_t)groups * beams * layers * 2 * ((page + kPrStepTokens - 1) / kPrStepTokens);
-  const int64_t ctas = (steps + 7) / 8;
+  // at most as many warps as there can be chunks
+  const int64_t chunks = (int64_t)groups * beams * layers * 2 * (((int64_t)page * n_kv * 16 + kPrCopyWords - 1) / kPrCopyWords);
+  const int64_t ctas = (chunks + 7) / 8;
   e = launch_dependent(copy_pages_kernel, (unsigned)(ctas > 148 * 8 ? 148 * 8 : ctas), 256, 0, as_cuda(stream), c);
   if (e != cudaSuccess) return set_error(KVR_ECUDA, "kvr_paged_reorder: %s", cudaGetErrorString(e));
   return check_launch("kvr_paged_reorder");

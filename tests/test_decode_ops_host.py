@@ -155,6 +155,12 @@ def cache():
     return PagedKVCache(1, 8, 2, 10, page=16, max_requests=4, max_len=64, device="cpu")
 
 
+def test_reorder_refuses_pages_beyond_its_arithmetic():
+    from kvr_b200._native import KvrError
+    with pytest.raises(KvrError, match="32 GB"):
+        reorder_call(page=1 << 20, n_kv=128, ts=128 * 128, ps=1 << 37, ls=1 << 42)
+
+
 def test_cache_reorder_refusals(native):
     c = cache()
     for rows, parents in (([[0, 0]], [[0, 0]]), ([[0, 1], [2]], [[0, 0], [0]]), ([[0, 4]], [[0, 0]]), ([[-1, 0]], [[0, 0]]),
