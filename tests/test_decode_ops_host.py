@@ -239,6 +239,12 @@ def test_moe_c_refusals(kw, match):
         moe_call(**kw)
 
 
+def test_moe_refuses_rows_beyond_its_arithmetic():
+    from kvr_b200._native import KvrError
+    with pytest.raises(KvrError, match="too far apart"):
+        moe_call(xs=(1 << 28) + 8)
+
+
 def test_no_tokens_is_no_call():
     assert moe_call(T=0, x=None) == 0
 

@@ -58,6 +58,21 @@ def test_weights(norm, scale):
     check(*inputs(9, 256, 96, 24, "bf16", 3), 4, norm, scale)
 
 
+@pytest.mark.parametrize("T,H,I,E,k", [(128, 1096, 520, 2, 2), (65, 520, 1032, 3, 3), (128, 2056, 72, 1, 1), (48, 1160, 776, 2, 1),
+                                       (96, 72, 1544, 4, 3), (112, 648, 392, 6, 5), (32, 2056, 1288, 8, 2)])
+def test_many_tokens_an_expert(T, H, I, E, k):
+    """Stages of every size, many rounds of the ring in both products, widths that end inside a block."""
+    check(*inputs(T, H, I, E, "bf16", T + I), k)
+
+
+def test_rows_far_apart():
+    """Rows of x whose places pass 32 bits in bytes."""
+    x, router, gu, down = inputs(128, 136, 72, 5, "bf16", 4)
+    far = torch.empty(127 * (1 << 24) + 136, dtype=x.dtype, device=DEV).as_strided((128, 136), (1 << 24, 1))
+    far.copy_(x)
+    check(far, router, gu, down, 2)
+
+
 def test_every_token_to_the_same_experts():
     """128 tokens on two experts of 64: segments of many columns, most experts without any."""
     x, router, gu, down = inputs(128, 256, 96, 64, "bf16", 5)
