@@ -330,7 +330,7 @@ def _reorder_plain(s):
     copy = part & ((rank > 0) | outside)
     nth = copy.cumsum(0) - 1
     have = nth < n_free
-    fresh = free[(n_free - 1 - nth).clamp(0, n_pages - 1)]
+    fresh = free[(n_free - 1 - nth).clamp(min=0)]
     count.index_add_(0, page[copy], -torch.ones_like(count[:1]).expand(int(copy.sum())))
     new.scatter_(1, last[:, None], torch.where(copy, torch.where(have, fresh, -1), new.gather(1, last[:, None])[:, 0])[:, None])
     moved = copy & have
