@@ -522,9 +522,9 @@ KVR_API int kvr_prompt_attn(const void *q, const void *k, const void *v, int dty
  * twice.  shared (n_pages) counts the rows that hold a page beyond the first; it
  * is brought up to date, and pages that no row holds any more go to the end of
  * free_pages[:*n_free], in order of places and columns.  A last page that is not
- * full stays with the parent's first child (none where a row outside of the
- * group holds it); the others get fresh pages off the end of the list, in order of
- * places, and copies of the page's tokens in all layers of k_pages and v_pages.  A
+ * full stays with the call's first place that it falls to (none where a row outside
+ * of the call holds it); the others get fresh pages off the end of the list, in order
+ * of places, and copies of the page's tokens in all layers of k_pages and v_pages.  A
  * row that finds no page keeps its full pages: its entry is -1, ctx_len ends there.
  * info (4): pages missing, pages copied, pages given back, 0.  Pool: layers of
  * kvr_paged_write's pools, layer_stride apart.  At most 32 beams, 4096 rows.

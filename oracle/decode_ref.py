@@ -55,13 +55,19 @@ def reorder(table, ctx, shared, free, n_free, rows, parents, page):
         free[n_free] = p
         n_free += 1
         holders[p] = 0
+    # a last page that is not full stays with the first place that gets it, if no row outside of the call has it
     want, copies, missing = [], [], 0
-    for g, i in places:
-        pages, c = now[g, i]
+    gets = {}
+    for place in places:
+        pages, c = now[place]
         if c % page and pages[-1] >= 0:
-            same = [o for o in range(len(rows[g])) if parents[g][o] == parents[g][i]]
-            if i != same[0] or holders[pages[-1]] + 1 > len(same):
-                want.append((g, i))
+            gets.setdefault(pages[-1], []).append(place)
+    for place in places:
+        pages, c = now[place]
+        if c % page and pages[-1] >= 0:
+            same = gets[pages[-1]]
+            if place != same[0] or holders[pages[-1]] + 1 > len(same):
+                want.append(place)
     for g, i in want:
         pages, c = now[g, i]
         holders[pages[-1]] -= 1

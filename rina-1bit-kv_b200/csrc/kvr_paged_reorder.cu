@@ -4,8 +4,9 @@
 // Pages are shared, not copied.  `shared[p]` counts the rows that hold page p
 // beyond the first, so a page that only one row holds, or none, has 0, and pages
 // that come off or go to the free list need no entry of their own.  A row's last page,
-// where it is not full, is written by the row's next token: the parent's first
-// child keeps it, every other child gets a fresh page with a copy of its tokens.
+// where it is not full, is written by the row's next token: the first row of the
+// call that it falls to keeps it (none, where a row outside of the call holds it), every other one
+// gets a fresh page with a copy of its tokens.
 //
 // A page holds tokens [j P, (j + 1) P) of a sequence, so it stands in column j
 // of every row that holds it, and columns do not meet.  paged_reorder_kernel: one
@@ -110,7 +111,7 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads,
   __shared__ int warp_sums[32], longest, disputed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, n = a.groups * K;
   PrPlace *place = reinterpret_cast<PrPlace *>(smem);  // (n)
-  int *ahead = reinterpret_cast<int *>(place + n);     // (n) pages given back by the places before
+  int *ahead = reinterpret_cast<int *>(place + n);     // (n) pages given back by the places before; at last, who copies
   int *entries = ahead + n;                            // (warps, slots, K, 32)
   if (tid == 0) longest = disputed = 0;
   griddep_wait();
@@ -304,27 +305,38 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads,
   }
   cluster_sync();
   if (blockIdx.x != 0) return;
-  // last pages, a thread per row
+  // last pages, a thread per row: first who copies, by counts that no place has changed yet.  The first place of the call that
+  // a page falls to keeps it, unless a row outside of the call holds it too
+  for (int i = tid; i < n; i += kPrThreads) {
+    const int last = place[i].last;
+    int copy = 0;
+    if (last >= 0) {
+      const int holders = __ldcg(a.shared + last) + 1;
+      int before, same;
+      auto look = [&](int from, int to) {
+        before = same = 0;
+        for (int o = from; o < to; ++o) {
+          const int is = place[o].last == last;
+          same += is;
+          before += is && o < i;
+        }
+      };
+      look(i / K * K, i / K * K + K);
+      if (same < holders) look(0, n);  // (never so after a beam search's step: the group has all holders)
+      copy = before > 0 || holders > same;
+    }
+    ahead[i] = copy;
+  }
+  __syncthreads();
   const int left = (int)min((int64_t)n_free + gone, (int64_t)a.n_free_cap);
   int done = 0, missing = 0;
   for (int i0 = 0; i0 < n; i0 += kPrThreads) {
     const int i = i0 + tid;
     const PrPlace x = i < n ? place[i] : PrPlace{-1, -1, 0, -1};
-    const int g = i / K * K, now = x.parent >= 0 ? place[g + x.parent].len : 0;
-    int copy = 0;
-    if (x.last >= 0) {
-      int before = 0, same = 0;  // children of the parent
-      for (int o = g; o < g + K; ++o) {
-        const int is = place[o].parent == x.parent;
-        same += is;
-        before += is && o < i;
-      }
-      copy = before > 0 || __ldcg(a.shared + x.last) + 1 > same;  // (or a row outside of the group holds it)
-    }
+    const int now = x.parent >= 0 ? place[i / K * K + x.parent].len : 0, copy = i < n ? ahead[i] : 0;
     int sum;
     const int k = done + pr_exclusive(copy, warp_sums, sum);
     done += sum;
-    __syncthreads();  // counts are read
     if (copy) {
       const int to = k < left ? __ldcg(a.free_pages + left - 1 - k) : -1, col = (now - 1) / a.page;
       atomicSub(a.shared + x.last, 1);
@@ -333,7 +345,6 @@ __global__ void __cluster_dims__(kPrCluster, 1, 1) __launch_bounds__(kPrThreads,
       else ++missing;
     }
     if (x.row >= 0) a.ctx[x.row] = copy && k >= left ? now / a.page * a.page : now;
-    __syncthreads();
   }
   int all_missing;
   pr_exclusive(missing, warp_sums, all_missing);

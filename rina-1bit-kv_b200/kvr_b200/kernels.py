@@ -931,7 +931,8 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
     device; no row may be named twice.  shared (n_pages) int32 counts the holders of
     each page beyond the first; free_pages[:n_free] is the list of free ones, with
     room for all.  Full pages are shared; a last page that is not full is copied for
-    every child but the first, in the pools k_pages and v_pages ([layers,] n_pages, page,
+    every row that it falls to but the call's first (for that too, where a row outside of the
+    call holds it), in the pools k_pages and v_pages ([layers,] n_pages, page,
     n_kv, d).  Returns info (4) int32 = [pages missing, copied, given back, 0]; a row that finds no page keeps
     its full pages."""
     shape, strides = k_pages.shape, k_pages.stride()

@@ -420,3 +420,40 @@ def test_sparse_mlps_that_the_call_does_not_take_stay_the_models(native, tokens,
     y = PagedGenerator._mlp(Sparse(), torch.zeros(tokens, hidden, dtype=torch.bfloat16))
     assert y.shape == (tokens, hidden) and ("kvr_moe_layer" in native) == own
     assert own or bool((y == 1).all())
+
+
+# ------------------------------------------- last pages that rows share --
+
+
+def whole_pool(table, ctx, shared, free, n_free, page):
+    """Each page of the pool is held or free, once; counts are what the rows hold."""
+    held = [int(p) for r, c in zip(table, ctx) for p in r[:-(-int(c) // page)] if p >= 0]
+    assert sorted(set(held) | {int(p) for p in free[:n_free]}) == list(range(len(shared))) and n_free + len(set(held)) == len(shared)
+    assert [int(x) for x in shared] == [max(held.count(p) - 1, 0) for p in range(len(shared))]
+
+
+# rows 0, 1 and 2 hold page 1, which is not full, behind page 0; row 3 has pages of its own
+SHARED_LAST = [([[0, 1, 2]], [[0, 1, 2]]), ([[0, 1, 2]], [[0, 1, 1]]), ([[2, 3, 1, 0]], [[0, 2, 2, 3]]), ([[0], [1], [2]], [[0]] * 3),
+               ([[1], [2]], [[0]] * 2), ([[0, 3], [1, 2]], [[0, 0], [1, 0]]), ([[0, 3], [1, 2]], [[1, 1], [1, 0]]),
+               ([[1, 2], [3, 0]], [[-1, 1], [0, -1]]), ([[3], [2]], [[0]] * 2)]
+
+
+def shared_last(free):
+    table = np.array([[0, 1, -1], [0, 1, -1], [0, 1, -1], [2, 3, -1]], np.int32)
+    shared = np.array([2, 2] + [0] * (2 + free), np.int32)
+    return table, np.array([20, 20, 25, 18], np.int32), shared, np.array(list(range(4, 4 + free)) + [0] * 4, np.int32), free
+
+
+@pytest.mark.parametrize("free", [0, 1, 8])
+@pytest.mark.parametrize("rows,parents", SHARED_LAST)
+def test_no_shared_last_page_is_lost(rows, parents, free):
+    """The first place that a last page of several rows falls to keeps it, unless a row outside of the call has it."""
+    table, ctx, shared, free_pages, n = shared_last(free)
+    w = R.reorder(table, ctx, shared, free_pages, n, rows, parents, 16)
+    whole_pool(w["table"], w["ctx"], w["shared"], w["free"], w["n_free"], 16)
+    last = [w["table"][r, 1] for r in range(4) if w["ctx"][r] > 16]
+    named = {r for g in rows for r in g}
+    if named >= {0, 1, 2}:
+        assert len(set(last)) == len(last)  # nobody writes where another reads
+    else:  # row 0 goes on with it: the others do not
+        assert w["table"][0, 1] == 1 and 1 not in [w["table"][r, 1] for r in named]

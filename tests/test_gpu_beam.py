@@ -312,3 +312,38 @@ def test_reorder_in_a_graph():
         other = K.paged_reorder(*eager, r, parents, k2, v2)
         assert torch.equal(info, other) and all(torch.equal(a, b) for a, b in zip(state, eager))
         assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+@pytest.mark.parametrize("free", [0, 1, 8])
+def test_reorder_last_pages_that_rows_share(free):
+    """A last page of several rows, in one group under several parents, in several groups, with a row outside of the call."""
+    from test_decode_ops_host import SHARED_LAST, shared_last, whole_pool
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for rows, parents in SHARED_LAST:
+        table, ctx, shared, free_pages, n = shared_last(free)
+        k, v = (torch.randn(2, len(shared), 16, 1, 128, device=DEV, generator=g).half() for _ in range(2))
+        w = check_reorder((table, ctx, shared, free_pages, n, np.array(rows), k, v), np.array(parents), 16)
+        whole_pool(w["table"], w["ctx"], w["shared"], w["free"], w["n_free"], 16)
+
+
+@pytest.mark.parametrize("groups,beams,free", [(3000, 1, 0), (3000, 1, 700), (3000, 1, 2000), (1024, 3, 3000), (4096, 1, 5000)])
+def test_reorder_last_pages_shared_by_distant_groups(groups, beams, free):
+    """More places than threads: what one place does to a page's count is nothing that a later one goes by."""
+    from test_decode_ops_host import whole_pool
+    rng = np.random.default_rng(groups + free)
+    rows = groups * beams + 10           # ten of them not in the call
+    pages = groups
+    of = rng.integers(0, pages, rows)    # whose last page a row has
+    n = pages + 1 + free                 # (page 0 in front of all)
+    of = np.unique(of, return_inverse=True)[1]  # each one held
+    n -= pages - (of.max() + 1)
+    table = np.full((rows, 2), -1, np.int32)
+    table[:, 0], table[:, 1] = 0, of + 1
+    shared = (np.bincount(table.reshape(-1), minlength=n) - 1).clip(min=0).astype(np.int32)
+    lists = np.concatenate([np.arange(of.max() + 2, n), np.zeros(n, np.int64)])[:n].astype(np.int32)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn(1, n, 16, 1, 128, device=DEV, generator=g).half() for _ in range(2))
+    ctx = rng.integers(17, 32, rows).astype(np.int32)
+    where = rng.permutation(rows)[:groups * beams].reshape(groups, beams)
+    w = check_reorder((table, ctx, shared, lists, n - of.max() - 2, where, k, v), rng.integers(0, beams, (groups, beams)), 16)
+    whole_pool(w["table"], w["ctx"], w["shared"], w["free"], w["n_free"], 16)
