@@ -980,6 +980,7 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 128, 512, 16
 _MOE_WS: dict = {}
 _MOE_STATUS: dict = {}
+_MOE_LOCK = threading.Lock()
 
 
 def _experts(w, name, shape):
@@ -997,8 +998,12 @@ def _moe_status(device):
     if ws is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first moe_layer call on a device must be made outside of a graph capture")
-        ws = _MOE_STATUS[device] = torch.zeros(256, dtype=torch.uint8, device=device)
-        torch.cuda.current_stream(device).synchronize()  # zeroed before a call on any stream uses it
+        with _MOE_LOCK:
+            ws = _MOE_STATUS.get(device)
+            if ws is None:
+                ws = torch.zeros(256, dtype=torch.uint8, device=device)
+                torch.cuda.current_stream(device).synchronize()  # zeroed before a call on any stream uses it
+                _MOE_STATUS[device] = ws
     return ws
 
 

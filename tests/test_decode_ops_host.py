@@ -457,3 +457,32 @@ def test_no_shared_last_page_is_lost(rows, parents, free):
         assert len(set(last)) == len(last)  # nobody writes where another reads
     else:  # row 0 goes on with it: the others do not
         assert w["table"][0, 1] == 1 and 1 not in [w["table"][r, 1] for r in named]
+
+
+# ---------------------------------------------------- the status word --
+
+
+def test_status_word_is_seen_when_it_is_zeroed(monkeypatch):
+    """Two host threads' first calls: one word for both, that none of them gets before its zeros are there."""
+    import threading
+    from kvr_b200 import kernels as K
+    entered, go, got = threading.Event(), threading.Event(), []
+
+    class Stream:
+        def synchronize(self):
+            entered.set()
+            assert go.wait(20)
+
+    monkeypatch.setattr(K, "_MOE_STATUS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    threads = [threading.Thread(target=lambda: got.append(K._moe_status(torch.device("cpu")))) for _ in range(2)]
+    threads[0].start()
+    assert entered.wait(20)
+    threads[1].start()
+    threads[1].join(0.5)
+    early = list(got)
+    go.set()
+    for t in threads:
+        t.join()
+    assert not early and got[0] is got[1] and K._moe_status(torch.device("cpu")) is got[0]
