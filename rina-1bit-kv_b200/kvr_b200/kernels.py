@@ -993,6 +993,16 @@ def _experts(w, name, shape):
     return (es if shape[0] > 1 else shape[1] * rs), rs
 
 
+def moe_status_word(device):
+    """A word of the caller's own for moe_layer's `status`: what its calls set, no
+    other caller's moe_status reads and clears.  Zeroed when this returns."""
+    device = torch.device(device)
+    word = torch.zeros(256, dtype=torch.uint8, device=device)
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()  # before a call on any stream uses it
+    return word
+
+
 def _moe_status(device):
     ws = _MOE_STATUS.get(device)
     if ws is None:
@@ -1007,12 +1017,13 @@ def _moe_status(device):
     return ws
 
 
-def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=None, return_routing=False):
+def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=None, return_routing=False, status=None):
     """A sparse MLP of at most MOE_MAX_TOKENS tokens: x (T, H), router (E, H),
     gate_up (E, 2 I, H) with the gate's rows first, down (E, H, I), all fp16 or all
     bf16.  Each token goes to the top_k experts of the largest softmax(x router^T),
     with those as weights (norm_topk: divided by their sum), times scale; an expert is
-    down(silu(gate x) * up x).  Returns y (T, H), or (y, ids (T, k) int32, weights (T, k) fp32)."""
+    down(silu(gate x) * up x).  Returns y (T, H), or (y, ids (T, k) int32, weights (T, k) fp32).
+    status: a word of moe_status_word (None: the device's, which moe_status() reads)."""
     if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3:
         raise ValueError("x must be (T, H), router (E, H), gate_up (E, 2 I, H), down (E, H, I)")
     n_tokens, hidden = x.shape
@@ -1039,6 +1050,10 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         raise ValueError("out must be contiguous and of x's shape and dtype")
     _on_current_gpu(x, router, gate_up, down, out)
     dev = x.device
+    if status is None:
+        status = _moe_status(dev)
+    elif status.dtype is not torch.uint8 or status.numel() < 4 or status.device != dev:
+        raise ValueError("status must be a word of moe_status_word on x's device")
     key = (n_tokens, hidden, inter, experts, top_k)
     need = _MOE_WS.get(key)
     if need is None:
@@ -1051,7 +1066,7 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
     p = buf.data_ptr()
     call("kvr_moe_layer", x.data_ptr(), dtype_code(x), n_tokens, hidden, xs, router.data_ptr(), rs, gate_up.data_ptr(), ge, gr,
          down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), p + 4 * at, p + 4 * (at + picks),
-         p, need, _moe_status(dev).data_ptr(), stream())
+         p, need, status.data_ptr(), stream())
     if not return_routing:
         return out
     one = (top_k, 1)
@@ -1059,13 +1074,15 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
             buf.view(torch.float32).as_strided((n_tokens, top_k), one, at + picks))
 
 
-def moe_status(device=None):
-    """Raises if a moe_layer call on the device gave up a wait (synchronises the
-    current stream)."""
-    device = torch.device("cuda" if device is None else device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    call("kvr_workspace_status", _moe_status(device).data_ptr(), stream())
+def moe_status(device=None, status=None):
+    """Raises if a moe_layer call on the device gave up a wait, or, with a word of
+    moe_status_word, one that was given it (synchronises the current stream)."""
+    if status is None:
+        device = torch.device("cuda" if device is None else device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        status = _moe_status(device)
+    call("kvr_workspace_status", status.data_ptr(), stream())
 
 
 def kmeans(x, k=128, iters=10):

@@ -231,6 +231,8 @@ class PagedGenerator:
     sees the last `window` tokens only (0: as many as the model's own sliding
     window, or all); a model's own window bounds it."""
 
+    _status = None  # of sparse MLPs: the word that a call sets whose wait gave up
+
     def __init__(self, model, n_pages, page=64, max_requests=32, max_len=None, window=0, chunk=2048):
         from .kvr_hook import rope_tables
 
@@ -247,6 +249,8 @@ class PagedGenerator:
         self.cache = PagedKVCache(cfg.num_hidden_layers, self.n_q, self.n_kv, n_pages, page, max_requests, max_len, window,
                                   dtype=model.dtype, device=self.device)
         self.cos_tbl, self.sin_tbl = rope_tables(model, max_len, self.device)
+        if any(_sparse(layer.mlp) for layer in model.model.layers):
+            self._status = K.moe_status_word(self.device)
         self.last = {}  # row -> logits (vocab,) fp32 after its last token
 
     def _layers(self, h, attend):
@@ -258,11 +262,17 @@ class PagedGenerator:
             if hasattr(at, "q_norm"):  # over the channels of each head
                 q, k = at.q_norm(q), at.k_norm(k)
             h = h + at.o_proj(attend(li, q, k, v).reshape(x.shape[0], -1))
-            h = h + self._mlp(layer.mlp, layer.post_attention_layernorm(h))
+            h = h + self._mlp(layer.mlp, layer.post_attention_layernorm(h), self._status)
         return self.model.model.norm(h)
 
+    def _check_sparse(self, n_tokens):
+        """Raises if a sparse MLP of a pass of n_tokens gave up a wait: its logits, and what it wrote into the cache, then mean
+        nothing.  Synchronises, if there was such a call."""
+        if self._status is not None and n_tokens <= K.MOE_MAX_TOKENS:
+            K.moe_status(status=self._status)
+
     @staticmethod
-    def _mlp(mlp, x):
+    def _mlp(mlp, x, status=None):
         """A layer's MLP over packed rows: a sparse one of a few tokens in one call,
         of more, or of a shape or type that the call does not take, by the model's own module."""
         if not hasattr(mlp, "experts"):
@@ -272,7 +282,7 @@ class PagedGenerator:
         if (x.shape[0] <= K.MOE_MAX_TOKENS and n <= K.MOE_MAX_EXPERTS and gate.top_k <= K.MOE_MAX_TOP_K
                 and hidden % 8 == 0 and inter % 8 == 0 and gate.weight.dtype is x.dtype):
             return K.moe_layer(x, gate.weight, experts.gate_up_proj, experts.down_proj, gate.top_k,
-                               norm_topk=bool(getattr(gate, "norm_topk_prob", True)))
+                               norm_topk=bool(getattr(gate, "norm_topk_prob", True)), status=status)
         y = mlp(x[None])
         return (y[0] if isinstance(y, tuple) else y)[0]
 
@@ -294,6 +304,7 @@ class PagedGenerator:
                 li, self.cache.write(li, q, k, v, self.cos_tbl, self.sin_tbl)))
             ends = st.cu_q[1:].long()[torch.tensor(rows, device=self.device)] - 1
             logits = self.model.lm_head(h[ends]).float()
+            self._check_sparse(ids.numel())
         except BaseException:
             self.cache.step = None  # nothing counts as cached: the step can be tried again, or its rows dropped
             raise
@@ -431,4 +442,6 @@ class PagedGenerator:
 
         h = self._layers(self.model.model.embed_tokens(torch.tensor([t for p in prompts for t in p], device=self.device)),
                          lambda li, q, k, v: K.prompt_attn(rope(q), rope(k), v, plan))
-        return list(self.model.lm_head(h).float().split(lens))
+        logits = self.model.lm_head(h).float()
+        self._check_sparse(n)
+        return list(logits.split(lens))

@@ -298,3 +298,35 @@ def test_host_threads_at_once():
     torch.cuda.synchronize()
     K.moe_status()
     assert not bad
+
+
+def test_a_sparse_mlp_that_gave_up_ends_the_step(monkeypatch):
+    """A wait that ran out (the self-test's, on the word that the call was given): the step, and what is built on it, raise
+    before anything counts as cached; it can be tried again."""
+    from kvr_b200 import PagedGenerator
+    from kvr_b200 import _native as N
+    from kvr_b200 import kernels as K
+    m = tiny("norm", seed=6)
+    gen = PagedGenerator(m, n_pages=40, page=16, max_requests=6, chunk=64)
+    (a,) = gen.add(prompts_of([30]))
+    K.moe_status()
+    kept = [gen.cache.ctx_len.clone(), gen.cache.n_free.clone(), gen.last[a].clone()]
+    real = K.moe_layer
+
+    def gave_up(x, *args, status=None, **kw):
+        y = real(x, *args, status=status, **kw)
+        word = K._moe_status(x.device) if status is None else status
+        N.call("kvr_selftest_bounded_wait", word.data_ptr(), 1000, N.stream())
+        return y
+
+    monkeypatch.setattr(K, "moe_layer", gave_up)
+    for broken in (lambda: gen.step({a: [5]}), lambda: gen.generate([a], 2), lambda: gen.beam_search(prompts_of([20, 9]), 2, 4),
+                   lambda: gen.add(prompts_of([12])), lambda: gen.score(prompts_of([40, 11]))):
+        with pytest.raises(N.KvrError, match="gave up"):
+            broken()
+        now = [gen.cache.ctx_len, gen.cache.n_free, gen.last[a]]
+        assert all(torch.equal(x, y) for x, y in zip(kept, now)) and list(gen.last) == [a] and gen.cache.step is None
+    K.moe_status()  # (nobody else's word was set)
+    monkeypatch.setattr(K, "moe_layer", real)
+    text = prompts_of([30])[0]
+    assert torch.allclose(gen.step({a: [5]})[a], want_logits(m, text + [5])[-1], rtol=BAR, atol=BAR)
