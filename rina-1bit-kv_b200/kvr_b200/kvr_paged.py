@@ -145,7 +145,11 @@ class PagedKVCache:
         if not all(0 <= b < self.max_requests for b in rows):
             raise ValueError(f"rows must be in [0, {self.max_requests}), got {rows}")
         if self._sharing and rows:  # pages that other rows hold too stay theirs
-            self.reorder([[b] for b in rows], [[-1]] * len(rows))
+            columns = -(-self.block_table.shape[1] // 32) * 32
+            most = min(K.REORDER_MAX_ROWS, max(K.REORDER_MAX_ENTRIES // columns, 1))
+            for i in range(0, len(rows), most):
+                some = rows[i:i + most]
+                self.reorder([[b] for b in some], [[-1]] * len(some))
             return
         rows = torch.tensor(rows, dtype=torch.int64, device=self.ctx_len.device)
         held = (self.ctx_len[rows] + self.page - 1) // self.page

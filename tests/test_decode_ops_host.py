@@ -486,3 +486,27 @@ def test_status_word_is_seen_when_it_is_zeroed(monkeypatch):
     for t in threads:
         t.join()
     assert not early and got[0] is got[1] and K._moe_status(torch.device("cpu")) is got[0]
+
+
+# --------------------------------------------- release where rows share --
+
+
+def test_release_of_many_rows_after_sharing(native, monkeypatch):
+    """As many rows as the cache has, of tables of any width: in calls of what one of them takes."""
+    from kvr_b200 import PagedKVCache
+    from kvr_b200 import kernels as K
+    calls = []
+    monkeypatch.setattr(K, "paged_reorder", lambda table, ctx, shared, free, n_free, rows, parents, k, v: (
+        calls.append((rows.clone(), parents.clone())), torch.zeros(4, dtype=torch.int32))[1])
+    c = PagedKVCache(1, 8, 2, 10, page=16, max_requests=9000, max_len=32, device="cpu")
+    c.reorder([[0, 1]], [[0, 0]])
+    calls.clear()
+    c.release(range(8999, -1, -1))
+    assert [r.shape[1] for r, _ in calls] == [1] * len(calls) and max(len(r) for r, _ in calls) <= 4096
+    assert torch.cat([r[:, 0] for r, _ in calls]).tolist() == list(range(8999, -1, -1))
+    assert all(p.eq(-1).all() for _, p in calls)
+    wide = PagedKVCache(1, 8, 2, 10, page=8, max_requests=1200, max_len=1 << 23, device="cpu")  # 2^20 columns
+    wide.reorder([[0, 1]], [[0, 0]])
+    calls.clear()
+    wide.release(range(1200))
+    assert sum(len(r) for r, _ in calls) == 1200 and max(len(r) for r, _ in calls) * (1 << 20) < 1 << 30

@@ -330,3 +330,24 @@ def test_a_sparse_mlp_that_gave_up_ends_the_step(monkeypatch):
     monkeypatch.setattr(K, "moe_layer", real)
     text = prompts_of([30])[0]
     assert torch.allclose(gen.step({a: [5]})[a], want_logits(m, text + [5])[-1], rtol=BAR, atol=BAR)
+
+
+def test_release_of_many_rows_that_share_pages():
+    """More rows than one reordering takes, all of them holders of one page."""
+    from kvr_b200 import PagedKVCache
+    c = PagedKVCache(1, 4, 2, 9010, page=8, max_requests=9000, max_len=24, dtype=torch.float16)
+    n = torch.arange(9000, dtype=torch.int32, device=DEV)
+    c.block_table[:, 0] = 5                  # rows forked from one prompt
+    c.block_table[:, 1] = n + 6
+    c.ctx_len.fill_(12)
+    c.shared[5] = 8999
+    c.free_pages[:10] = torch.tensor([0, 1, 2, 3, 4, 9006, 9007, 9008, 9009, 0], dtype=torch.int32)
+    c.n_free.fill_(9)
+    c.reorder([[0, 1]], [[0, 1]])            # (nothing changes)
+    c.release(range(0, 8998))
+    assert c.n_free.item() == 9 + 8998 and c.shared[5].item() == 1 and c.shared.sum().item() == 1
+    assert c.free_pages[9:9007].tolist() == list(range(6, 9004))
+    c.release([8998, 8999])
+    assert sorted(c.free_pages[:c.n_free.item()].tolist()) == list(range(9010)) and c.shared.eq(0).all()
+    assert c.ctx_len.eq(0).all() and c.block_table.eq(-1).all()
+    c.check()
