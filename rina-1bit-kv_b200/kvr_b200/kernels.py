@@ -921,7 +921,7 @@ def beam_select(logits, scores, n=None, eos=()):
     return st
 
 
-REORDER_MAX_BEAMS, REORDER_MAX_ROWS = 32, 4096
+REORDER_MAX_BEAMS, REORDER_MAX_ROWS, REORDER_MAX_TABLE = 32, 4096, 1 << 16
 REORDER_MAX_ENTRIES = (1 << 30) - 1  # of the call's rows, columns by 32
 _REORDER_WS: dict = {}
 

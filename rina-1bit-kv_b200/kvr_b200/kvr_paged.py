@@ -17,6 +17,8 @@ in a CUDA graph.  Between steps ``cache.reorder(rows, parents)`` makes rows the
 continuations of others (beams of one request, samples of one prompt): they share
 full pages.
 """
+import contextlib
+
 import torch
 
 from . import kernels as K
@@ -45,6 +47,9 @@ class PagedKVCache:
         self.n_free = torch.full((1,), n_pages, **i32)
         self.shared = torch.zeros(n_pages, **i32)  # rows that hold a page, beyond the first
         self._sharing = False
+        # whether rows can come to share pages, by `reorder` or by kernels.paged_reorder on these tensors
+        self._countable = (self.ctx_len.is_cuda and dtype in (torch.float16, torch.bfloat16) and n_layers > 0
+                           and max_requests <= K.REORDER_MAX_TABLE)
         self.lost = torch.zeros(4, **i32)  # what committed steps had no room for, as their info counts it
         self.step = None
 
@@ -144,12 +149,15 @@ class PagedKVCache:
         rows = list(dict.fromkeys(int(b) for b in requests))
         if not all(0 <= b < self.max_requests for b in rows):
             raise ValueError(f"rows must be in [0, {self.max_requests}), got {rows}")
-        if self._sharing and rows:  # pages that other rows hold too stay theirs
+        if rows and (self._sharing or self._countable):  # pages that other rows hold too stay theirs
             columns = -(-self.block_table.shape[1] // 32) * 32
             most = min(K.REORDER_MAX_ROWS, max(K.REORDER_MAX_ENTRIES // columns, 1))
-            for i in range(0, len(rows), most):
-                some = rows[i:i + most]
-                self.reorder([[b] for b in some], [[-1]] * len(some))
+            dev = self.ctx_len.device
+            with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():
+                for i in range(0, len(rows), most):
+                    some = rows[i:i + most]
+                    self.reorder([[b] for b in some], [[-1]] * len(some))
+            self.block_table[torch.tensor(rows, device=self.ctx_len.device)] = -1  # (steps that were given up leave entries behind)
             return
         rows = torch.tensor(rows, dtype=torch.int64, device=self.ctx_len.device)
         held = (self.ctx_len[rows] + self.page - 1) // self.page

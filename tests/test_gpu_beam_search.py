@@ -351,3 +351,25 @@ def test_release_of_many_rows_that_share_pages():
     assert sorted(c.free_pages[:c.n_free.item()].tolist()) == list(range(9010)) and c.shared.eq(0).all()
     assert c.ctx_len.eq(0).all() and c.block_table.eq(-1).all()
     c.check()
+
+
+def test_release_counts_holders_however_rows_came_to_share():
+    """kernels.paged_reorder on a cache's own tensors, then release: the other rows' pages stay theirs."""
+    from kvr_b200 import PagedKVCache
+    from kvr_b200 import kernels as K
+    c = PagedKVCache(2, 4, 2, 20, page=16, max_requests=4, max_len=128, dtype=torch.bfloat16)
+    c.begin([50, 0, 3, 0], 53)
+    c.commit()
+    assert c.n_free.item() == 15
+    i32 = lambda *x: torch.tensor([x], dtype=torch.int32, device=DEV)  # noqa: E731
+    K.paged_reorder(c.block_table, c.ctx_len, c.shared, c.free_pages, c.n_free, i32(0, 1, 3), i32(0, 0, 0), c.k, c.v)
+    assert c.n_free.item() == 13 and c.ctx_len.tolist() == [50, 50, 3, 50]
+    c.begin([0, 0, 9, 20], 29)               # row 3 writes a page of its own
+    c.step = None                            # and the step is given up
+    for rows, left in (([1, 2], 15), ([3], 16), ([0], 20)):
+        c.release(rows)
+        assert c.n_free.item() == left, rows
+        held = {p for r, m in zip(c.block_table.tolist(), c.ctx_len.tolist()) for p in r[:-(-m // 16)]}
+        assert sorted(held | set(c.free_pages[:left].tolist())) == list(range(20)) and len(held) == 20 - left
+        assert c.block_table[rows].eq(-1).all() and c.ctx_len[rows].eq(0).all()
+    assert c.shared.eq(0).all()
