@@ -862,6 +862,7 @@ class BeamStep:
     __slots__ = ("scores", "beams", "tokens", "next_scores", "next_beams", "next_tokens")
 
 
+BEAM_MAX_BEAMS, BEAM_MAX_N, BEAM_MAX_EOS = 32, 128, 8
 _BEAM_WS: dict = {}
 _EOS: dict = {}
 

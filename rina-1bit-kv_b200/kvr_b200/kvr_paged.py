@@ -366,11 +366,19 @@ class PagedGenerator:
         power of length_penalty.  eos: a token id, or several, that end a sequence.  A
         prompt is done when it has n_beams ended sequences that its beams, at their
         present length, do not beat.  It takes n_beams free rows a prompt, and gives
-        them back."""
-        eos = (eos,) if isinstance(eos, int) else tuple(eos)
+        them back.  At most 32 beams, 8 ends, n_beams * (1 + ends) of 128, and 4096 rows in all."""
+        eos = (eos,) if isinstance(eos, int) else tuple(dict.fromkeys(int(t) for t in eos))
         prompts = [list(p) for p in prompts]
         if n_beams < 1 or max_new_tokens < 1:
             raise ValueError("n_beams and max_new_tokens must be 1 at least")
+        # what the selection and the reordering take, before prompts are computed for nothing
+        if n_beams > K.BEAM_MAX_BEAMS or len(eos) > K.BEAM_MAX_EOS or n_beams * (1 + len(eos)) > K.BEAM_MAX_N:
+            raise ValueError(f"at most {K.BEAM_MAX_BEAMS} beams, {K.BEAM_MAX_EOS} ends of sequence and n_beams * (1 + ends) of "
+                             f"{K.BEAM_MAX_N}, got {n_beams} beams and {len(eos)} ends")
+        if not all(0 <= t < 1 << 31 for t in eos):
+            raise ValueError(f"eos must be token ids, got {eos}")
+        if n_beams * len(prompts) > K.REORDER_MAX_ROWS or self.cache.max_requests > K.REORDER_MAX_TABLE:
+            raise ValueError(f"at most {K.REORDER_MAX_ROWS} rows at a time, of a cache of at most {K.REORDER_MAX_TABLE}")
         free = [b for b in range(self.cache.max_requests) if b not in self.last]
         if len(free) < n_beams * len(prompts):
             raise RuntimeError(f"{len(prompts)} prompts of {n_beams} beams for {len(free)} free rows")

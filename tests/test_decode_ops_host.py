@@ -510,3 +510,25 @@ def test_release_of_many_rows_after_sharing(native, monkeypatch):
     calls.clear()
     wide.release(range(1200))
     assert sum(len(r) for r, _ in calls) == 1200 and max(len(r) for r, _ in calls) * (1 << 20) < 1 << 30
+
+
+# ------------------------------------------------- limits of beam search --
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(n_beams=33), "32 beams"), (dict(eos=tuple(range(9))), "8 ends"), (dict(n_beams=32, eos=(1, 2, 3, 4)), "128"),
+    (dict(n_beams=16, eos=tuple(range(8))), "128"), (dict(eos=(-1,)), "token ids"), (dict(eos=1 << 31), "token ids"),
+    (dict(prompts=[[1]] * 2049, n_beams=2), "4096")])
+def test_beam_search_refuses_before_it_computes(kw, match, monkeypatch):
+    """What the selection or the reordering would refuse is refused before the prompts are computed."""
+    gen = toy_generator(Toy(6, 1), 5000, monkeypatch)
+    gen.step = lambda new: pytest.fail("computed a step")
+    with pytest.raises(ValueError, match=match):
+        gen.beam_search(**{"prompts": [[1, 2]], "n_beams": 2, "max_new_tokens": 3, **kw})
+    assert not gen.last
+
+
+def test_beam_search_counts_an_end_once(monkeypatch):
+    gen = toy_generator(Toy(6, 3), 40, monkeypatch)
+    once = gen.beam_search([[1, 2]], 32, 2, eos=[4, 1])
+    assert gen.beam_search([[1, 2]], 32, 2, eos=[4, 1, 4, 1, 1, 4, 4, 4, 4]) == once
