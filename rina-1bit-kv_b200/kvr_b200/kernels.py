@@ -891,7 +891,7 @@ def beam_select(logits, scores, n=None, eos=()):
     scores = _c(scores)
     _on_current_gpu(logits, scores)
     code, dev = dtype_code(logits), logits.device
-    eos = tuple(eos)
+    eos = tuple(map(int, eos))  # (by value: the arrays below are kept by it)
     ends = _EOS.get(eos)
     if ends is None:
         if len(_EOS) > 256:

@@ -532,3 +532,15 @@ def test_beam_search_counts_an_end_once(monkeypatch):
     gen = toy_generator(Toy(6, 3), 40, monkeypatch)
     once = gen.beam_search([[1, 2]], 32, 2, eos=[4, 1])
     assert gen.beam_search([[1, 2]], 32, 2, eos=[4, 1, 4, 1, 1, 4, 4, 4, 4]) == once
+
+
+def test_select_takes_ends_by_value(native):
+    """Ends in objects that change between calls (an element of a tensor): each call's own values."""
+    from kvr_b200 import kernels as K
+    end = torch.tensor(5)
+    for t in (5, 9, 2):
+        end.fill_(t)
+        K.beam_select(torch.zeros(3, 50), torch.zeros(1, 3), eos=[end])
+        assert list(native["kvr_beam_select"][8]) == [t]
+    K.beam_select(torch.zeros(3, 50), torch.zeros(1, 3), eos=np.array([7, 8]))
+    assert list(native["kvr_beam_select"][8]) == [7, 8] and native["kvr_beam_select"][7] == 9
