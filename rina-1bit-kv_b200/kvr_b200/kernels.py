@@ -857,7 +857,8 @@ class BeamStep:
     """What beam_select chose: the n best continuations of each request in order,
     scores (B, n) fp32, beams and tokens (B, n) int32, and the first K of them that
     do not end a sequence, next_scores, next_beams, next_tokens (B, K).  Places
-    without a continuation hold -inf, -1, -1."""
+    without a continuation hold -inf, -1, -1.  All lie in one buffer with the call's
+    workspace (at most 128 KB a request): clone what is to be kept for long."""
 
     __slots__ = ("scores", "beams", "tokens", "next_scores", "next_beams", "next_tokens")
 
@@ -1063,18 +1064,19 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         if len(_MOE_WS) > 4096:
             _MOE_WS.clear()
         need = _MOE_WS[key] = call("kvr_moe_workspace_bytes", *key)
-    # workspace (256-byte aligned, as allocations are), then ids and weights
+    # workspace (256-byte aligned, as allocations are), then ids and weights; those that are returned have a buffer of their own
     picks, at = n_tokens * top_k, (need + 3) // 4
-    buf = torch.empty(at + 2 * picks, dtype=_INT32, device=dev)
-    p = buf.data_ptr()
+    buf = torch.empty(at + (0 if return_routing else 2 * picks), dtype=_INT32, device=dev)
+    routing, first = (torch.empty(2 * picks, dtype=_INT32, device=dev), 0) if return_routing else (buf, at)
+    p = routing.data_ptr() + 4 * first
     call("kvr_moe_layer", x.data_ptr(), dtype_code(x), n_tokens, hidden, xs, router.data_ptr(), rs, gate_up.data_ptr(), ge, gr,
-         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), p + 4 * at, p + 4 * (at + picks),
-         p, need, status.data_ptr(), stream())
+         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), p, p + 4 * picks, buf.data_ptr(),
+         need, status.data_ptr(), stream())
     if not return_routing:
         return out
     one = (top_k, 1)
-    return (out, buf.as_strided((n_tokens, top_k), one, at),
-            buf.view(torch.float32).as_strided((n_tokens, top_k), one, at + picks))
+    return (out, routing.as_strided((n_tokens, top_k), one, 0),
+            routing.view(torch.float32).as_strided((n_tokens, top_k), one, picks))
 
 
 def moe_status(device=None, status=None):

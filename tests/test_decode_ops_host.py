@@ -544,3 +544,15 @@ def test_select_takes_ends_by_value(native):
         assert list(native["kvr_beam_select"][8]) == [t]
     K.beam_select(torch.zeros(3, 50), torch.zeros(1, 3), eos=np.array([7, 8]))
     assert list(native["kvr_beam_select"][8]) == [7, 8] and native["kvr_beam_select"][7] == 9
+
+
+def test_routing_does_not_keep_the_workspace(native):
+    """ids and weights that a caller collects over layers and steps hold their own bytes, not a call's h and partial rows."""
+    from kvr_b200 import kernels as K
+    a = moe_args(T=100, H=512, I=256, E=8)
+    y, ids, w = K.moe_layer(**a, return_routing=True)
+    assert ids.shape == w.shape == (100, 2) and ids.dtype is torch.int32 and w.dtype is torch.float32
+    for t in (ids, w):
+        assert t.untyped_storage().nbytes() <= 100 * 2 * 8 + 256
+    c = native["kvr_moe_layer"]
+    assert c[19] == ids.data_ptr() and c[20] == w.data_ptr() and c[21] % 64 == 0 and c[22] > 100 * 2 * 256 * 4
