@@ -982,6 +982,7 @@ def paged_reorder(block_table, ctx_len, shared, free_pages, n_free, rows, parent
 # ------------------------------------------------------------ sparse MLP --
 
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 128, 512, 16
+MOE_MAX_HIDDEN, MOE_MAX_INTER = 1 << 16, 1 << 20
 _MOE_WS: dict = {}
 _MOE_STATUS: dict = {}
 _MOE_LOCK = threading.Lock()

@@ -228,6 +228,16 @@ def _sparse(mlp):
     return True
 
 
+def _readable(w, dtype):
+    """Whether kernels.moe_layer takes these weights: their type, 16-byte aligned rows that share no memory."""
+    if w.dtype is not dtype or w.data_ptr() % 16:
+        return False
+    if w.is_contiguous():  # (rows of a multiple of 8)
+        return True
+    st = w.stride()
+    return st[-1] == 1 and not any(s % 8 for s in st[:-1]) and all(s >= n * t for s, n, t in zip(st, w.shape[1:], st[1:]))
+
+
 class PagedGenerator:
     """Many requests on one HF decoder model (Llama, Mistral, Qwen2 or Qwen3, dense or
     with sparse MLPs, of head_dim 128, fp16 or bf16) with an exact paged cache.
@@ -292,7 +302,9 @@ class PagedGenerator:
         gate, experts = mlp.gate, mlp.experts
         n, hidden, inter = experts.down_proj.shape
         if (x.shape[0] <= K.MOE_MAX_TOKENS and n <= K.MOE_MAX_EXPERTS and gate.top_k <= K.MOE_MAX_TOP_K
-                and hidden % 8 == 0 and inter % 8 == 0 and gate.weight.dtype is x.dtype):
+                and hidden % 8 == 0 and inter % 8 == 0 and hidden <= K.MOE_MAX_HIDDEN and inter <= K.MOE_MAX_INTER
+                and x.dtype in (torch.float16, torch.bfloat16)
+                and all(_readable(w, x.dtype) for w in (gate.weight, experts.gate_up_proj, experts.down_proj))):
             return K.moe_layer(x, gate.weight, experts.gate_up_proj, experts.down_proj, gate.top_k,
                                norm_topk=bool(getattr(gate, "norm_topk_prob", True)), status=status)
         y = mlp(x[None])

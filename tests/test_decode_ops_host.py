@@ -556,3 +556,51 @@ def test_routing_does_not_keep_the_workspace(native):
         assert t.untyped_storage().nbytes() <= 100 * 2 * 8 + 256
     c = native["kvr_moe_layer"]
     assert c[19] == ids.data_ptr() and c[20] == w.data_ptr() and c[21] % 64 == 0 and c[22] > 100 * 2 * 256 * 4
+
+
+@pytest.mark.parametrize("change,own", [
+    (None, True), ("wide rows", True), ("experts fp32", False), ("down fp32", False), ("gate_up off", False), ("down off", False),
+    ("router off", False), ("router 36 apart", False), ("down transposed", False), ("experts expanded", False), ("all fp32", False)])
+def test_sparse_mlps_laid_out_otherwise_stay_the_models(native, change, own):
+    """Types, places in memory and strides that the call refuses: the model's own module, no error."""
+    from kvr_b200.kvr_paged import PagedGenerator
+    E, H, I = 4, 32, 24
+    bf = torch.bfloat16
+    off = lambda *s: torch.zeros(int(np.prod(s)) + 1, dtype=bf)[1:].view(*s)  # noqa: E731
+
+    class Sparse(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate, self.experts = torch.nn.Module(), torch.nn.Module()
+            self.gate.top_k = 2
+            gate, gu, down = torch.zeros(E, H, dtype=bf), torch.zeros(E, 2 * I, H, dtype=bf), torch.zeros(E, H, I, dtype=bf)
+            if change == "wide rows":
+                down = torch.zeros(E, H, 40, dtype=bf)[:, :, :I]
+            elif change == "experts fp32":
+                gu, down = gu.float(), down.float()
+            elif change == "all fp32":
+                gate, gu, down = gate.float(), gu.float(), down.float()
+            elif change == "down fp32":
+                down = down.float()
+            elif change == "gate_up off":
+                gu = off(E, 2 * I, H)
+            elif change == "down off":
+                down = off(E, H, I)
+            elif change == "router off":
+                gate = off(E, H)
+            elif change == "router 36 apart":
+                gate = torch.zeros(E, 36, dtype=bf)[:, :H]
+            elif change == "down transposed":
+                down = torch.zeros(E, I, H, dtype=bf).transpose(1, 2)
+            elif change == "experts expanded":
+                gu = gu[:1].expand(E, -1, -1)
+            p = lambda t: torch.nn.Parameter(t, requires_grad=False)  # noqa: E731
+            self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj = p(gate), p(gu), p(down)
+
+        def forward(self, x):
+            return x + 1
+
+    x = torch.zeros(3, H, dtype=torch.float32 if change == "all fp32" else bf)
+    y = PagedGenerator._mlp(Sparse(), x)
+    assert y.shape == (3, H) and ("kvr_moe_layer" in native) == own
+    assert own or bool((y == 1).all())
