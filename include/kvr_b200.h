@@ -544,7 +544,7 @@ KVR_API int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int ta
  * best of each request in order (equal ones by beam, then token): scores, beams,
  * tokens (batch, n); and the first n_beams of them whose token is not in
  * eos_host[0 .. n_eos) (host memory, read before the call returns): next_*
- * (batch, n_beams).  A continuation whose score is not finite (a masked logit of
+ * (batch, n_beams).  A continuation whose score is not finite in fp32 (a masked logit of
  * -inf, a beam of score -inf, a row with a NaN or +inf) is no candidate; places
  * without one get -inf, -1, -1.  n_beams <= n <= 128, at most 32 beams and 8 ends
  * of sequence.  The workspace needs no clearing and keeps nothing between calls. */

@@ -15,9 +15,10 @@ def beam_select(logits, cum, n, eos=()):
         for k in range(K):
             x = np.asarray(logits[b, k], dtype=np.float64)
             m = x.max()  # a NaN stays one
-            with np.errstate(invalid="ignore", divide="ignore"):
+            with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
                 score = float(cum[b, k]) + (x - (m + np.log(np.exp(x - m).sum())))
-            found += [(-score[t], k, t) for t in np.nonzero(np.isfinite(score))[0]]
+                there = np.isfinite(score.astype(np.float32))  # (what is returned is fp32)
+            found += [(-score[t], k, t) for t in np.nonzero(there)[0]]
         found.sort()
         on = 0
         for i, (s, k, t) in enumerate(found[:n]):

@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(BeamArgs a) {
     BeamRank r{0, 0};
     if (c) {
       const double score = (double)cum[k] + ((double)bs_value(c) - lse[k]);
-      if (isfinite(score)) r = BeamRank{bs_double_key(score), (uint64_t)k << 32 | (uint32_t)bs_token(c)};
+      if (isfinite((float)score)) r = BeamRank{bs_double_key(score), (uint64_t)k << 32 | (uint32_t)bs_token(c)};
     }
     all[i] = r;
     if (r.key && bs_above(r, mine)) mine = r;

@@ -872,7 +872,7 @@ def beam_select(logits, scores, n=None, eos=()):
     """Beam search's choice: logits (B * K, V), or (B, K, V), of K beams of B
     requests (rows may be strided or expanded) and the beams' scores (B, K) fp32.  A
     continuation's score is its beam's plus the log-softmax of its logit; those that
-    are not finite (masked by -inf, of a beam of score -inf) are none.  n: how many
+    are not finite in fp32 (masked by -inf, of a beam of score -inf) are none.  n: how many
     are listed of each request (K * (1 + len(eos)) where not given: enough for K to
     go on).  eos: token ids (host integers) that end a sequence."""
     if logits.dim() == 3:

@@ -347,3 +347,18 @@ def test_reorder_last_pages_shared_by_distant_groups(groups, beams, free):
     where = rng.permutation(rows)[:groups * beams].reshape(groups, beams)
     w = check_reorder((table, ctx, shared, lists, n - of.max() - 2, where, k, v), rng.integers(0, beams, (groups, beams)), 16)
     whole_pool(w["table"], w["ctx"], w["shared"], w["free"], w["n_free"], 16)
+
+
+def test_select_scores_beyond_fp32():
+    """A masked token of a beam that came by a masked token: a sum below all of fp32 is no continuation, in any of the outputs."""
+    low = torch.finfo(torch.float32).min
+    x = torch.full((4, 600), low, device=DEV)
+    x[:, :2] = torch.randn(4, 2, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    x[3] = 1.0
+    cum = torch.tensor([[-1.0, low], [low / 2, low]], device=DEV)
+    got = check_select(x, cum, 12, (0,))
+    assert got.scores.isfinite().eq(got.beams >= 0).all() and got.next_scores.isfinite().eq(got.next_tokens >= 0).all()
+    # request 0: two tokens of each beam, and the masked ones of beam 0; none of beam 1's masked ones
+    assert got.beams[0].tolist() == [0] * 12
+    one = check_select(x[1:2], cum[:1, 1:], 5)
+    assert one.tokens[0, 2:].tolist() == [-1] * 3 and one.scores[0, :2].isfinite().all()
