@@ -557,7 +557,8 @@ KVR_API int kvr_beam_select(const void *logits, int dtype, int64_t row_stride, i
 /* A sparse MLP of a few tokens: z = x router^T, p = softmax(z); of each token the
  * top_k largest p (equal ones by expert) with weights w = scale * p, or, with norm,
  * scale * p / (sum of the chosen p); y = sum w * down_e (silu(gate_e x) * (up_e x)).
- * fp16 or bf16 throughout, fp32 sums; h = silu(gate) * up is rounded to the type.
+ * fp16 or bf16 throughout, fp32 sums; h = silu(gate) * up goes into the second product
+ * in two parts of the type, rounded and rest (in fp16 up to twice its largest value).
  * x (n_tokens, hidden) with x_stride; router (experts, hidden); gate_up (experts,
  * 2 * inter, hidden), the gate's rows before the up's; down (experts, hidden, inter);
  * strides in elements, multiples of 8.  y (n_tokens, hidden) contiguous, not in x;

@@ -34,8 +34,8 @@
 //
 // Both operands of an MMA are of one 16-bit type, so h has to be rounded for the
 // second product.  It goes in as two columns, h rounded and what the rounding left:
-// 16 (bf16) or 22 bits (fp16) of it, for copies and columns that the few tokens
-// leave room for.  (Rounded once, y was 1.4 to 1.6 times as far from 64 bits as its own
+// 16 bits of it in bf16, in fp16 22 of an h from 1/8 up, and below that what is left to
+// the smallest step, 2^-24 (18 bits at 0.01), for copies and columns that the few tokens leave room for.  (Rounded once, y was 1.4 to 1.6 times as far from 64 bits as its own
 // rounding makes it.)  Sums, router weights and partial rows are fp32.
 //
 // What binds: HBM where the weights are many.  128 tokens over 128 experts of 4096 x 1408

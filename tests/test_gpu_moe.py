@@ -166,3 +166,66 @@ def test_a_wait_that_ran_out_is_reported():
         K.moe_status()
     K.moe_status()
     assert torch.equal(K.moe_layer(*a, 2), want)
+
+
+# ------------------------------------------------ h, in two parts of the type --
+
+
+def paired(T, H, I, E, dtype, seed, big=1.0):
+    """Inner channels in pairs: nearly the same h, opposite columns of down.  y is small against sum |w d h|, so that what h
+    loses on its way shows; positive x, gate and up keep the absolute products near the products."""
+    dt = DT[dtype]
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.rand(*s, generator=g)  # noqa: E731
+    gate, up = (0.2 + r(E, I // 2, H)) / H ** 0.5, big * (0.2 + r(E, I // 2, H)) / H ** 0.5
+    gate, up = (t.repeat_interleave(2, 1).to(dt) for t in (gate, up))
+    other = 1 + torch.finfo(dt).eps * torch.randint(1, 3, (E, I // 2, H), generator=g)  # a step or two of the type
+    up[:, 1::2] = (up[:, 1::2].float() * other).to(dt)
+    down = (torch.randn(E, H, I // 2, generator=g) / I ** 0.5).repeat_interleave(2, 2).to(dt)
+    down[:, :, 1::2] *= -1
+    # (a router of zeros: every expert has the weight 1 / E, exactly)
+    return [t.to(DEV) for t in ((0.25 + r(T, H)).to(dt), torch.zeros(E, H, dtype=dt), torch.cat([gate, up], 1), down)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,H,I,E", [(1, 16, 16, 1), (16, 16, 16, 1), (40, 24, 16, 1), (128, 16, 24, 1), (128, 64, 128, 1), (9, 16, 16, 4),
+                                     (70, 32, 200, 2)])
+def test_h_keeps_what_one_rounding_drops(T, H, I, E, dtype):
+    """The bar of the tests above, with h rounded twice in place of once: h in two parts of the type is off by u^2 |h|, and
+    in fp16, whose smallest step is 2^-24, by half of that at least.  (Weights of 1 / E: no error of the router.)"""
+    from kvr_b200 import kernels as K
+    x, router, gu, down = paired(T, H, I, E, dtype, T + H)
+    f = lambda t: t.double().cpu().numpy()  # noqa: E731
+    wy, _, _, by_h, by_sums, by_one = R.moe(f(x), f(router), f(gu), f(down), E)
+    u = torch.finfo(x.dtype).eps / 2
+    tol = (u + 2.0 ** -20) * np.abs(wy) + (u * u + 2.0 ** -20 + I * 2.0 ** -23) * (1 + u) * by_h + H * 2.0 ** -23 * by_sums
+    tol += 2.0 ** -25 * by_one if dtype == "f16" else 0.0
+    # (the bar tells: h rounded once, and all else exact, does not pass it)
+    z = np.einsum("eih,th->tei", f(gu), f(x))
+    h = z[..., :I] / (1 + np.exp(-z[..., :I])) * z[..., I:]
+    once = np.einsum("tei,ehi->th", torch.tensor(h).to(x.dtype).double().numpy(), f(down)) / E
+    assert (np.abs(once - wy) > tol).any()
+    y = f(K.moe_layer(x, router, gu, down, E))
+    K.moe_status()
+    assert (np.abs(y - wy) <= tol).all(), (np.abs(y - wy) / tol).max()
+
+
+def test_h_above_the_largest_half():
+    """fp16: an h of up to twice the type's largest value is its largest value and a rest, off by half a step of the rest."""
+    from kvr_b200 import kernels as K
+    x, router, gu, down = paired(30, 16, 16, 1, "f16", 3, big=14000.0)
+    down = (torch.randn(1, 16, 16, generator=torch.Generator().manual_seed(4)) / 256).half().to(DEV)
+    f = lambda t: t.double().cpu().numpy()  # noqa: E731
+    wy, _, _, by_h, by_sums, by_one = R.moe(f(x), f(router), f(gu), f(down), 1)
+    z = f(x) @ f(gu)[0].T
+    h = z[:, :16] / (1 + np.exp(-z[:, :16])) * z[:, 16:]
+    assert (h > 65504).mean() > 0.2 and h.max() < 131008 and np.abs(wy).max() < 65504
+    u = 2.0 ** -11
+    rest = np.maximum(u * h, h - 65504)  # at most
+    d = np.abs(f(down)[0])
+    tol = (u + 2.0 ** -20) * np.abs(wy) + (2.0 ** -20 + 16 * 2.0 ** -23) * (1 + u) * by_h + (u * rest) @ d.T + 16 * 2.0 ** -23 * by_sums
+    tol += 2.0 ** -25 * by_one
+    assert (np.abs(np.minimum(h, 65504) @ f(down)[0].T - wy) > tol).any()  # (the bar tells)
+    y = f(K.moe_layer(x, router, gu, down, 1))
+    K.moe_status()
+    assert (np.abs(y - wy) <= tol).all(), (np.abs(y - wy) / tol).max()
