@@ -373,3 +373,98 @@ def test_release_counts_holders_however_rows_came_to_share():
         assert sorted(held | set(c.free_pages[:left].tolist())) == list(range(20)) and len(held) == 20 - left
         assert c.block_table[rows].eq(-1).all() and c.ctx_len[rows].eq(0).all()
     assert c.shared.eq(0).all()
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_beam_search_keeps_what_its_logits_say(sparse):
+    """Every logit that the search used, by the text of its row, is the model's for that text; and the plain search on those
+    logits finds the same sequences.  Nothing is close but for ties: a score is off by the log-sum-exp's error and a rounding
+    to fp32 a step, 2^-21 + 2^-24 40 + 300 / 256 2^-24 < 4e-6, so where no two of the plain search's candidates lie within
+    2e-4 (12 steps, both of them, twice) the order is the same."""
+    from kvr_b200 import PagedGenerator
+    m = tiny("norm", seed=8, experts=5, top_k=5) if sparse else tiny(False, seed=8)  # (all experts: no choice is close)
+    k, steps, eos = 4, 12, 7
+    prompts = prompts_of([40, 1, 64, 133, 17, 90], 12)
+    gen = PagedGenerator(m, n_pages=90, page=16, max_requests=26, chunk=64)
+    text, seen = [[] for _ in range(26)], {}
+    step, reorder = gen.step, gen.cache.reorder
+
+    def noted_step(new):
+        out = step(new)
+        for b, ids in new.items():
+            text[b] += ids
+            seen[tuple(text[b])] = out[b].clone()
+        return out
+
+    def noted_reorder(rows, parents):
+        old = [list(t) for t in text]
+        for g, ps in zip(rows, parents):
+            for b, p in zip(g, ps):
+                text[b] = list(old[g[p]]) if p >= 0 else []
+        return reorder(rows, parents)
+
+    gen.step, gen.cache.reorder = noted_step, noted_reorder
+    got = gen.beam_search(prompts, k, steps, eos=eos)
+    compared = 0
+    for p, found in zip(prompts, got):
+        for t in [t for t in seen if t[:len(p)] == tuple(p)]:
+            # What a hidden state is off by, e of its size, goes through the rows of lm_head as the state itself does, so logits
+            # are off by e of their spread: sqrt(256) 0.2 = 3.2 here, not one.  (e: some ten roundings to fp16 on the way, each
+            # 2^-11 / sqrt(3) of an element at most, 9e-4 rms; the largest of 50 texts' 300 logits is 4.3 times that, and
+            # two such computations differ by 1.4 times that: 5.4e-3, a quarter of the bar.)
+            want = want_logits(m, list(t))[-1]
+            assert ((seen[t] - want).abs() <= BAR * (want.std() + want.abs())).all(), (seen[t] - want).abs().max()
+        beams, ended, gap = [(0.0, [])], [], math.inf
+        for t in range(1, steps + 1):
+            cand = []
+            for s, q in beams:
+                lp = seen[tuple(p + q)].double().log_softmax(-1)
+                top = lp.topk(2 * k + 1)
+                cand += [(s + v, q + [i]) for v, i in zip(top.values.tolist(), top.indices.tolist())]
+            cand.sort(key=lambda c: -c[0])
+            gap = min([gap] + [a[0] - b[0] for a, b in zip(cand[:2 * k], cand[1:2 * k + 1])])
+            if gap <= 2e-4:
+                break  # (from here on the beams may be others, whose texts nobody has seen)
+            ended = sorted(ended + [(s / t, q) for s, q in cand[:k] if q[-1] == eos], key=lambda e: -e[0])[:k]
+            beams = [(s, q) for s, q in cand if q[-1] != eos][:k]
+            if len(ended) == k and ended[-1][0] >= beams[0][0] / t:
+                beams = []
+                break
+        if gap <= 2e-4:
+            continue
+        want = sorted(ended + [(s / len(q), q) for s, q in beams], key=lambda e: -e[0])[:k]
+        gap = min([math.inf] + [a[0] - b[0] for a, b in zip(want, want[1:])])
+        if gap > 1e-5:
+            assert [q for q, _ in found] == [q for _, q in want]
+            assert all(abs(a - b) < 1e-4 for (_, a), (b, _) in zip(found, want))
+            compared += 1
+    assert compared >= 2, compared
+
+
+def test_host_threads_first_calls_at_once():
+    """As above, from the first call on (no status word, no kernel attributes of a warm-up), and a thread that raises is seen."""
+    import concurrent.futures
+
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(2)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=g).half()  # noqa: E731
+    w = (n(16, 256), n(16, 192, 256) / 16, n(16, 256, 96) / 10)
+    xs, logits = [n(t, 256) for t in (1, 5, 40, 128)], [n(6, 5000 + 900 * i) for i in range(4)]
+    scores = -torch.rand(2, 3, device=DEV, generator=g)
+    torch.cuda.synchronize()
+    K._MOE_STATUS.clear()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = [(K.moe_layer(xs[i], *w, 4), K.beam_select(logits[i], scores, eos=(1,)).tokens) for _ in range(60)]
+            torch.cuda.current_stream().synchronize()
+            return out
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        got = [f.result() for f in [pool.submit(work, i) for i in range(4)]]
+    assert len(K._MOE_STATUS) == 1
+    K.moe_status()
+    for i, runs in enumerate(got):
+        assert len(runs) == 60
+        y, t = K.moe_layer(xs[i], *w, 4), K.beam_select(logits[i], scores, eos=(1,)).tokens
+        assert all(torch.equal(a, y) and torch.equal(b, t) for a, b in runs)
