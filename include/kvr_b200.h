@@ -541,8 +541,9 @@ KVR_API int kvr_paged_reorder(int32_t *block_table, int64_t table_stride, int ta
  * row_stride elements between rows (any alignment; reads stay in 16-byte words that
  * hold a logit of a row), cum (batch, n_beams) the beams' scores.  score(k, t) =
  * cum[k] + logits[k, t] - logsumexp(logits[k]), compared in 64 bits.  Writes the n
- * best of each request in order (equal ones by beam, then token): scores, beams,
- * tokens (batch, n); and the first n_beams of them whose token is not in
+ * best of each request in order (equal ones by beam, then token; the log-sum-exp of a
+ * row is off by some 1e-6 at most, so beams whose scores lie closer may come in either
+ * order): scores, beams, tokens (batch, n); and the first n_beams of them whose token is not in
  * eos_host[0 .. n_eos) (host memory, read before the call returns): next_*
  * (batch, n_beams).  A continuation whose score is not finite in fp32 (a masked logit of
  * -inf, a beam of score -inf, a row with a NaN or +inf) is no candidate; places

@@ -16,7 +16,9 @@
 //
 // Scores are compared in 64 bits: c_k + (x - lse_k) in 32 would make different
 // logits equal and order them by token.  Sums are in 32 bits per thread (at most
-// some thousand exponentials <= 1) and joined in 64 by the second kernel.
+// some thousand exponentials <= 1) and joined in 64 by the second kernel.  (Which logits a
+// thread adds up depends on where a row lies within 16 bytes, so equal rows may have
+// sums of other last bits, and ties between their beams no order but theirs.)
 //
 // What binds: 512 rows of 128256 in fp32, 51.5 us (5.1 TB/s; a kernel that only
 // reads them with as many CTAs takes 47): some 200 instructions a warp and tile of 512

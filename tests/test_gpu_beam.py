@@ -362,3 +362,34 @@ def test_select_scores_beyond_fp32():
     assert got.beams[0].tolist() == [0] * 12
     one = check_select(x[1:2], cum[:1, 1:], 5)
     assert one.tokens[0, 2:].tolist() == [-1] * 3 and one.scores[0, :2].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k,n,eos", [(32, 64, (3,)), (32, 128, (3, 5, 9)), (32, 33, ()), (16, 32, (7,)), (31, 93, (1, 2))])
+def test_select_many_beams_of_equal_scores(k, n, eos, dtype):
+    """Beams whose scores and rows are alike: the best of all lie in all lists, at equal ranks.
+
+    Rows of 20011 logits lie at different places within 16 bytes, so the sums of equal rows are added up in different orders,
+    and each log-sum-exp may be off by lse_error on its own.  Scores that differ by less than twice that have no order by
+    the sums' accuracy: among such candidates of different beams any order is right, within a beam (one log-sum-exp) only
+    that of the logits, then the tokens."""
+    from kvr_b200 import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(k + n)
+    cum = torch.zeros(1, k, device=DEV)
+    x = (2 * torch.randn(k, 20011, device=DEV, generator=g)).to(DT[dtype])
+    check_select(x, cum, n, eos)
+    x[:] = x[:1]
+    got = K.beam_select(x, cum, n, eos)
+    lp = x[0].double().log_softmax(0)  # the score of a token, in every beam
+    order = lp.sort(descending=True, stable=True)[1]
+    beams, tokens, scores = got.beams[0].tolist(), got.tokens[0].tolist(), got.scores[0].double()
+    close = lse_error(20011) + 2.0 ** -23 * lp[order[:n]].abs().max()
+    assert len(set(zip(beams, tokens))) == n and (scores.diff() <= 0).all()
+    assert ((scores - lp[got.tokens[0].long()]).abs() <= close).all()
+    best = lp[order].repeat_interleave(k)[:n]  # each token of all beams, from the best on
+    assert ((scores - best).abs() <= 2 * close).all()
+    for b in range(k):  # a beam's own are its best, in order
+        mine = [t for o, t in zip(beams, tokens) if o == b]
+        assert mine == order[:len(mine)].tolist()
+    on = [i for i in range(n) if tokens[i] not in eos][:k]
+    assert got.next_beams[0].tolist()[:len(on)] == [beams[i] for i in on] and got.next_tokens[0].tolist()[:len(on)] == [tokens[i] for i in on]
