@@ -1065,19 +1065,21 @@ def moe_layer(x, router, gate_up, down, top_k, norm_topk=True, scale=1.0, out=No
         if len(_MOE_WS) > 4096:
             _MOE_WS.clear()
         need = _MOE_WS[key] = call("kvr_moe_workspace_bytes", *key)
-    # workspace (256-byte aligned, as allocations are), then ids and weights; those that are returned have a buffer of their own
+    # workspace (256-byte aligned, as allocations are), then ids and weights, which have their own memory if they are returned
     picks, at = n_tokens * top_k, (need + 3) // 4
-    buf = torch.empty(at + (0 if return_routing else 2 * picks), dtype=_INT32, device=dev)
-    routing, first = (torch.empty(2 * picks, dtype=_INT32, device=dev), 0) if return_routing else (buf, at)
-    p = routing.data_ptr() + 4 * first
+    if return_routing:
+        buf = torch.empty(at, dtype=_INT32, device=dev)
+        ids = torch.empty(n_tokens, top_k, dtype=_INT32, device=dev)
+        weights = torch.empty(n_tokens, top_k, dtype=torch.float32, device=dev)
+        p, pi, pw = buf.data_ptr(), ids.data_ptr(), weights.data_ptr()
+    else:
+        buf = torch.empty(at + 2 * picks, dtype=_INT32, device=dev)
+        p = buf.data_ptr()
+        pi, pw = p + 4 * at, p + 4 * (at + picks)
     call("kvr_moe_layer", x.data_ptr(), dtype_code(x), n_tokens, hidden, xs, router.data_ptr(), rs, gate_up.data_ptr(), ge, gr,
-         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), p, p + 4 * picks, buf.data_ptr(),
-         need, status.data_ptr(), stream())
-    if not return_routing:
-        return out
-    one = (top_k, 1)
-    return (out, routing.as_strided((n_tokens, top_k), one, 0),
-            routing.view(torch.float32).as_strided((n_tokens, top_k), one, picks))
+         down.data_ptr(), de, dr, experts, inter, top_k, int(norm_topk), scale, out.data_ptr(), pi, pw, p, need,
+         status.data_ptr(), stream())
+    return (out, ids, weights) if return_routing else out
 
 
 def moe_status(device=None, status=None):
