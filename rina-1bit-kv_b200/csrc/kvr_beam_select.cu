@@ -26,7 +26,8 @@
 // segments fill the SMs where rows are few, and pay those ends each (1184 CTAs for 512
 // rows: 9 us more).  Tried: words of all rows in equal shares, 6 us more; copies two tiles
 // ahead, 8 us more (fewer CTAs have room).  One request of 4 beams and 32000 tokens: 7.8 us,
-// a chain of two launches and their barriers; the second kernel is 4 to 5 us of it.
+// a chain of two launches and their barriers; the second kernel is 4 to 5 us of it.  That one is slow where very many
+// candidates pass its threshold: 32 beams of equal scores with n = 64, 4.2 ms (spread over 12 units: 38 us).
 #include <cfloat>
 
 #include "kvr_common.cuh"

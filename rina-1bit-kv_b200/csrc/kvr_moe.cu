@@ -44,7 +44,7 @@
 // MB, 12 us of reading): 27 us, the rest a chain of round trips: logits and ranks (4), lists
 // (1), a first tile's way from memory (2), h through a counter and L2 (3), last products, partial
 // rows and sums (6).  With many tokens an expert their rows cross L2 as often as the weights: 69 tokens over 4 of
-// 4 experts of 1128 x 13776 110 us, of which 57 are the weights'.
+// 4 experts of 1128 x 13776 110 us, of which 57 are the weights'; 128 over 6 of 8 of 720 x 888 63, of 5.
 //
 // Waits are bounded; one that gives up sets the status word, lets copies and MMAs in
 // flight end and frees the tensor memory.

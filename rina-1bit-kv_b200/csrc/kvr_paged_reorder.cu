@@ -26,8 +26,8 @@
 //
 // What binds: tables and counts are small and lie in L2, so the first kernel is a
 // chain of dependent loads and two meetings; HBM binds the copies.  Both kernels in a graph: a
-// prompt of 1000 tokens forked 4 ways in 32 layers 17.3 us, 8 groups of 8 rows of 1300 to 2000 pages, little
-// to copy, 26; 16 groups of 4 in 32 layers, 67 MB read and as many written, 34 us (the
+// prompt of 1000 tokens forked 4 ways in 32 layers 17 us, 8 groups of 8 rows of 1300 to 2000 pages, little
+// to copy, 25; 16 groups of 4 in 32 layers, 67 MB read and as many written, 36 us (the
 // copies alone at a plain copy's rate: 20).
 #include "kvr_attn_plan.cuh"
 
