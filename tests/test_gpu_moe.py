@@ -229,3 +229,9 @@ def test_h_above_the_largest_half():
     y = f(K.moe_layer(x, router, gu, down, 1))
     K.moe_status()
     assert (np.abs(y - wy) <= tol).all(), (np.abs(y - wy) / tol).max()
+
+
+@pytest.mark.parametrize("T,H,I,E,k", [(1, 65536, 8, 2, 1), (70, 65536, 16, 3, 2), (2, 8, 131072, 2, 2), (128, 8, 8, 512, 16), (128, 40, 24, 16, 16),
+                                       (3, 32768, 64, 4, 4), (1, 24, 1048576, 1, 1), (128, 104, 56, 1, 1)])
+def test_the_largest_and_the_smallest_sizes(T, H, I, E, k):
+    check(*inputs(T, H, I, E, "bf16", T + H), k)
